@@ -47,7 +47,8 @@ typedef enum sfe_status {
   SFE_AUDIO_TOO_LONG = 4
 } sfe_status;
 
-typedef enum sfe_dtype { SFE_F32 = 0, SFE_BF16 = 1 } sfe_dtype;
+/* Features are SFE_F32 or SFE_BF16; SFE_F16 is a type of the model operators. */
+typedef enum sfe_dtype { SFE_F32 = 0, SFE_BF16 = 1, SFE_F16 = 2 } sfe_dtype;
 
 /* Input sample formats.  Integer PCM is decoded in the kernel exactly as the
  * reference's WAV reader does (examples/transcribe_wav.rs:342-348,
@@ -259,6 +260,138 @@ int sfe_extract_chunks_streamed(sfe_ctx* ctx, const float* host_recording, int64
 int sfe_extract_chunks_streamed_pcm(sfe_ctx* ctx, const void* host_recording, int32_t pcm_format,
                                     int32_t bits_per_sample, int64_t len, const sfe_chunk* tasks, int32_t n,
                                     int32_t out_dtype, void* out, int64_t* frame_offsets, int64_t window_samples);
+
+/* ---- model operators ------------------------------------------------------
+ *
+ * What an encoder-decoder runs behind the features (the models themselves are
+ * closed in the reference, src/model.rs): attention over the packed sequences of
+ * a ragged batch, rotary positions, the norms around a block, and a step of beam
+ * search.  Tensors are device memory; offsets are host memory, read before the
+ * call returns.  Every call is asynchronous on `stream` and ordered after the
+ * context's earlier calls, except while `stream` is being captured into a
+ * graph: there its order is the graph's, and replays have to be ordered with the
+ * context's other calls by the caller.  Arguments are checked before any device
+ * work; a refused call returns SFE_INVALID_ARG and does nothing. */
+
+/* A tensor [rows][heads][channels]: strides in elements, channels contiguous. */
+typedef struct sfe_heads {
+  void* data;
+  int64_t row_stride;
+  int64_t head_stride;
+} sfe_heads;
+
+/* Attention over n packed sequences with grouped heads.  Sequence s has the
+ * queries [q_offsets[s], q_offsets[s + 1]) and the keys [k_offsets[s],
+ * k_offsets[s + 1]) (host arrays of n + 1; lengths may be 0).  Query head h reads kv head
+ * h / (heads / kv_heads).  Queries and keys are aligned at their ends: query i of
+ * Lq sees the keys j of Lk with i + Lk - Lq - left <= j <= i + Lk - Lq + right; a
+ * negative left or right sets no bound (causal: left -1, right 0; all: -1, -1).
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j over the visible keys, zero where
+ * none is visible.  Keys that are not visible contribute nothing, whatever
+ * their values.
+ * A plan holds the sequences' division into tiles, and the partial results of
+ * tiles that are cut along their keys; one plan serves every layer over the same
+ * lengths, on any stream, and can be captured (its making cannot).  Free it
+ * before its context, and after the graphs that hold it.  head_dim is a multiple of 8,
+ * at most 128. */
+typedef struct sfe_attn_plan sfe_attn_plan;
+int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_offsets, int32_t n, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, int64_t left, int64_t right, void* stream,
+                       sfe_attn_plan** out);
+void sfe_attention_plan_free(sfe_attn_plan* plan);
+
+/* q, out: [q_offsets[n]][heads][head_dim]; k, v: [k_offsets[n]][kv_heads]
+ * [head_dim], of dtype SFE_BF16 or SFE_F16, 16-byte aligned (data and
+ * strides), rows less than 2^23 elements apart.  key_mask: a byte for each
+ * key row, 0 hides it from every query (NULL: none hidden).  scale > 0.  out must
+ * not overlap the inputs. */
+int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
+                  const uint8_t* key_mask, float scale, const sfe_heads* out, void* stream);
+
+/* Rotary positions.  A pair of channels (a, b) of the first rotary_dim of each
+ * head turns by angle = position * f_p, f_p = base^(-2p / rotary_dim) as scaled:
+ *   a' = magnitude (a cos - b sin),  b' = magnitude (b cos + a sin);
+ * pairs are (p, p + rotary_dim / 2) (SFE_ROTARY_HALF) or (2p, 2p + 1)
+ * (SFE_ROTARY_INTERLEAVED).  Scalings for long contexts, factor >= 1:
+ *   LINEAR  f / factor
+ *   BASE    base * factor^(rotary_dim / (rotary_dim - 2)) as the base
+ *   PARTS   f ((1 - keep) / factor + keep), keep = (original_length f / 2 pi -
+ *           low) / (high - low) limited to [0, 1].
+ * The table is plain host memory of the caller. */
+typedef enum sfe_rotary_layout { SFE_ROTARY_HALF = 0, SFE_ROTARY_INTERLEAVED = 1 } sfe_rotary_layout;
+typedef enum sfe_rotary_scaling {
+  SFE_ROTARY_UNSCALED = 0,
+  SFE_ROTARY_LINEAR = 1,
+  SFE_ROTARY_BASE = 2,
+  SFE_ROTARY_PARTS = 3
+} sfe_rotary_scaling;
+typedef struct sfe_rotary_table {
+  int32_t rotary_dim; /* even, at most 256 */
+  int32_t layout;
+  float magnitude;
+  int32_t reserved;
+  uint64_t step[128]; /* turns a position, as a fraction of 2^64 */
+} sfe_rotary_table;
+int sfe_rotary_init(sfe_rotary_table* table, int32_t rotary_dim, int32_t layout, double base, int32_t scaling,
+                    double factor, double original_length, double low, double high, double magnitude);
+
+/* Rotates q [rows][q_heads][head_dim] into q_out and k [rows][k_heads]
+ * [head_dim] into k_out (either may have 0 heads), row r by positions[r] (device
+ * memory; any 32-bit value).  Channels past rotary_dim are copied.  inverse: by
+ * the negative angle (also the gradient).  SFE_F32, SFE_BF16 or SFE_F16.  An output
+ * may be its input's own view (in place); other overlaps are refused. */
+int sfe_rotary(sfe_ctx* ctx, const sfe_rotary_table* table, int32_t inverse, int32_t dtype, const int32_t* positions,
+               int64_t rows, int32_t head_dim, int32_t q_heads, const sfe_heads* q, const sfe_heads* q_out,
+               int32_t k_heads, const sfe_heads* k, const sfe_heads* k_out, void* stream);
+
+/* Norms before and after a block with the block's gate and residual scale:
+ *   h = N_post(block); h *= gate (or sigmoid(gate)); residual_out = residual +
+ *   scale * h; norm_out = N_pre(residual_out, before it is rounded)
+ * N: SFE_NORM_LAYER (v - mean) / sqrt(var + eps) * weight + bias, SFE_NORM_RMS
+ * v / sqrt(mean v^2 + eps) * weight, SFE_NORM_NONE.  residual, residual_out:
+ * [rows][width] of stream_dtype; block, gate, norm_out: of block_dtype
+ * (stream_dtype is SFE_F32 or block_dtype); weights and biases are f32, a bias may be
+ * NULL.  Row strides in elements; gate_row 0 is one gate for all rows, gate NULL
+ * none.  residual_out may be residual, norm_out may be block. */
+typedef enum sfe_norm { SFE_NORM_NONE = 0, SFE_NORM_LAYER = 1, SFE_NORM_RMS = 2 } sfe_norm;
+typedef struct sfe_residual {
+  int32_t stream_dtype, block_dtype;
+  int64_t rows;
+  int32_t width; /* at most 16384 */
+  int32_t post, pre;
+  int32_t gate_sigmoid;
+  float scale, eps;
+  const void *residual, *block, *gate;
+  void *residual_out, *norm_out;
+  int64_t residual_row, block_row, gate_row, residual_out_row, norm_out_row;
+  const float *post_weight, *post_bias, *pre_weight, *pre_bias;
+} sfe_residual;
+int sfe_residual_norm(sfe_ctx* ctx, const sfe_residual* args, void* stream);
+
+/* A step of beam search over logits [streams * beams][vocab] (rows row_stride
+ * elements apart): for each stream the `beams` best of its beams * vocab candidates
+ *   scores[w] + logit[w][t] - log sum_t exp(logit[w][t]),
+ * best first, ties to the lowest (w, t).  A beam with finished[w] != 0 (NULL: none)
+ * has the one candidate (scores[w], end_token) and its logits are not read.
+ * Totals of -inf or NaN are no candidates (a stream's first step gives all beams but
+ * one the score -inf); a place without a candidate gets score -inf, token -1 and
+ * parent its own place.  out_finished (may be NULL): the parent was finished or the
+ * token is end_token (-1: no such token).  1 to 32 beams. */
+int sfe_beam_select(sfe_ctx* ctx, int32_t dtype, const void* logits, int64_t row_stride, int32_t streams, int32_t beams,
+                    int32_t vocab, const float* scores, const uint8_t* finished, int32_t end_token, float* out_scores,
+                    int32_t* parents, int32_t* tokens, uint8_t* out_finished, void* stream);
+
+/* Reorders beam states to their parents: out[o][b * beams + w] = in[o][b * beams +
+ * parents[b * beams + w]] for states [outer][streams * beams][inner_bytes].  out may be in
+ * (in place).  A parent outside [0, beams) leaves the place its own state. */
+typedef struct sfe_beam_state {
+  const void* in;
+  void* out;
+  int64_t outer;
+  int64_t inner_bytes;
+} sfe_beam_state;
+int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int32_t beams, const sfe_beam_state* states,
+                     int32_t n, void* stream);
 
 /* ---- tuning and instrumentation (no reference counterpart) ----------- */
 

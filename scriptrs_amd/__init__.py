@@ -15,3 +15,4 @@ from .long_form import (  # noqa: F401
 from .vad import (  # noqa: F401
     VAD_CONTEXT_SAMPLES, VAD_INPUT_SAMPLES, VAD_WINDOW_SAMPLES, SileroVadFramer, vad_num_windows,
 )
+from .model_ops import AttentionPlan, ModelOps, RotaryTable  # noqa: F401

@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SFE_LIBRARY") or os.path.join(_HERE, "libscriptrs_fe.so")
 
 SFE_OK, SFE_EMPTY_AUDIO, SFE_INVALID_ARG, SFE_HIP_ERROR, SFE_AUDIO_TOO_LONG = 0, 1, 2, 3, 4
-SFE_F32, SFE_BF16 = 0, 1
+SFE_F32, SFE_BF16, SFE_F16 = 0, 1, 2
 SFE_PCM_F32, SFE_PCM_I16, SFE_PCM_I32 = 0, 1, 2
 
 # Every symbol include/scriptrs_fe.h declares.
@@ -25,6 +25,8 @@ EXPORTS = (
     "sfe_extract_chunks_padded", "sfe_extract_chunks_streamed", "sfe_extract_chunks_streamed_pcm",
     "sfe_set_frame_sharing", "sfe_set_timing", "sfe_get_timing", "sfe_vad_num_windows", "sfe_vad_frames", "sfe_extract_chunks_noalloc",
     "sfe_debug_allocation_count", "sfe_debug_mel_schedule", "sfe_debug_stamps",
+    "sfe_attention_plan", "sfe_attention_plan_free", "sfe_attention", "sfe_rotary_init", "sfe_rotary",
+    "sfe_residual_norm", "sfe_beam_select", "sfe_beam_reorder",
 )
 
 
@@ -44,6 +46,32 @@ class SfeOverlapConfig(ctypes.Structure):
 class SfeChunk(ctypes.Structure):
     _fields_ = [("audio_start", ctypes.c_int64), ("audio_end", ctypes.c_int64),
                 ("global_sample_offset", ctypes.c_int64), ("context_samples", ctypes.c_int64)]
+
+
+class SfeHeads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class SfeRotaryTable(ctypes.Structure):
+    _fields_ = [("rotary_dim", ctypes.c_int32), ("layout", ctypes.c_int32), ("magnitude", ctypes.c_float),
+                ("reserved", ctypes.c_int32), ("step", ctypes.c_uint64 * 128)]
+
+
+class SfeResidual(ctypes.Structure):
+    _fields_ = [("stream_dtype", ctypes.c_int32), ("block_dtype", ctypes.c_int32), ("rows", ctypes.c_int64),
+                ("width", ctypes.c_int32), ("post", ctypes.c_int32), ("pre", ctypes.c_int32),
+                ("gate_sigmoid", ctypes.c_int32), ("scale", ctypes.c_float), ("eps", ctypes.c_float),
+                ("residual", ctypes.c_void_p), ("block", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("residual_out", ctypes.c_void_p), ("norm_out", ctypes.c_void_p),
+                ("residual_row", ctypes.c_int64), ("block_row", ctypes.c_int64), ("gate_row", ctypes.c_int64),
+                ("residual_out_row", ctypes.c_int64), ("norm_out_row", ctypes.c_int64),
+                ("post_weight", ctypes.c_void_p), ("post_bias", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p),
+                ("pre_bias", ctypes.c_void_p)]
+
+
+class SfeBeamState(ctypes.Structure):
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("outer", ctypes.c_int64),
+                ("inner_bytes", ctypes.c_int64)]
 
 
 _lib = None
@@ -97,6 +125,16 @@ def lib() -> ctypes.CDLL:
         "sfe_debug_allocation_count": (i64, []),
         "sfe_debug_mel_schedule": (ctypes.c_int, [P(SfeConfig)]),
         "sfe_debug_stamps": (ctypes.c_int, [vp, i64]),
+        "sfe_attention_plan": (ctypes.c_int, [vp, i64p, i64p, i32, i32, i32, i32, i64, i64, vp, P(vp)]),
+        "sfe_attention_plan_free": (None, [vp]),
+        "sfe_attention": (ctypes.c_int, [vp, i32, P(SfeHeads), P(SfeHeads), P(SfeHeads), vp, ctypes.c_float,
+                                         P(SfeHeads), vp]),
+        "sfe_rotary_init": (ctypes.c_int, [P(SfeRotaryTable), i32, i32, ctypes.c_double, i32] + [ctypes.c_double] * 5),
+        "sfe_rotary": (ctypes.c_int, [vp, P(SfeRotaryTable), i32, i32, vp, i64, i32, i32, P(SfeHeads), P(SfeHeads),
+                                      i32, P(SfeHeads), P(SfeHeads), vp]),
+        "sfe_residual_norm": (ctypes.c_int, [vp, P(SfeResidual), vp]),
+        "sfe_beam_select": (ctypes.c_int, [vp, i32, vp, i64, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp]),
+        "sfe_beam_reorder": (ctypes.c_int, [vp, vp, i32, i32, P(SfeBeamState), i32, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)

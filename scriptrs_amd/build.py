@@ -39,6 +39,12 @@ SOURCES = [
     ("sfe_norm_shift.hip", ["-x", "hip"]),
     ("sfe_vad.hip", ["-x", "hip"]),
     ("sfe_noalloc.hip", ["-x", "hip"]),
+    ("sfe_attn.hip", ["-x", "hip"]),
+    ("sfe_rotary.hip", ["-x", "hip"]),
+    ("sfe_residual.hip", ["-x", "hip"]),
+    ("sfe_beam.hip", ["-x", "hip"]),
+    ("sfe_attn_plan.cpp", ["-x", "hip"]),
+    ("sfe_ops.cpp", ["-x", "hip"]),
     # bit-exact table construction: every f32/f64 op rounded separately
     ("sfe_tables.cpp", ["-x", "hip", "-ffp-contract=off"]),
     ("sfe_share.cpp", ["-x", "hip"]),

@@ -1,0 +1,715 @@
+// Attention over packed sequences with grouped heads.
+//
+// For query i of a sequence of Lq queries and Lk keys, head h reading kv head
+// h / group:  o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j that i
+// sees: i + Lk - Lq - left <= j <= i + Lk - Lq + right and not masked; zero if
+// there is none.  One pass over the keys with a running reference exponent and
+// sum: with x_j = scale log2(e) q_i . k_j and any reference m, the weights are
+// 2^(x_j - m) / sum 2^(x_j - m).  m follows the running maximum only when that
+// rises 15 above it, to 7 below the new maximum, so most steps rescale nothing;
+// weights stay below 2^15 (f16 holds 65504) and weights down to 2^-17 of the
+// largest keep all their bits in f16 (bf16 has the range anyway).  Scores, m,
+// sums and outputs are f32; a weight is rounded to the inputs' type for the
+// product with v, whose inputs are of that type too (an error of 2^-9 of
+// each term in bf16, as in v itself).
+//
+// Both products are matrix instructions on transposed tiles: S^T = K Q^T gives
+// each lane the scores of one query, so the softmax is within lanes (but for
+// one exchange when m moves), and S^T's register order is an operand order of
+// the second product O^T = V^T P^T once V's rows are read in the same order
+// (the transposing LDS read): the weights never leave their registers.
+//
+// K and V steps go from memory into LDS directly (buffer loads with an LDS
+// destination) while the step before is computed on.  Rows past a sequence's
+// end and hidden rows take an offset past the buffer's range, which the
+// hardware answers with zeros: neither is read, so NaN or infinity there
+// reaches nothing.  LDS rows hold their 16-byte chunks in an order permuted by
+// the row (K: any chunk of 16 rows on distinct banks; V: 4 rows x 64 bytes).
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sfe_ops.hpp"
+
+namespace sfe {
+namespace {
+
+typedef __bf16 Bf;
+typedef _Float16 Hf;
+typedef float F2 __attribute__((ext_vector_type(2)));
+typedef float F4 __attribute__((ext_vector_type(4)));
+typedef float F16 __attribute__((ext_vector_type(16)));
+typedef int I4 __attribute__((ext_vector_type(4)));
+typedef short S4 __attribute__((ext_vector_type(4)));
+typedef short S8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct Mat;
+template <>
+struct Mat<Bf> {
+  typedef Bf V8 __attribute__((ext_vector_type(8)));
+  typedef Bf V2 __attribute__((ext_vector_type(2)));
+  static __device__ F16 m32(V8 a, V8 b, F16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ F4 m16(V8 a, V8 b, F4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static constexpr uint32_t kExp = 0x7f807f80, kCarry = 0x00800080, kOne = 0x3f80;
+};
+template <>
+struct Mat<Hf> {
+  typedef Hf V8 __attribute__((ext_vector_type(8)));
+  typedef Hf V2 __attribute__((ext_vector_type(2)));
+  static __device__ F16 m32(V8 a, V8 b, F16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static __device__ F4 m16(V8 a, V8 b, F4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static constexpr uint32_t kExp = 0x7c007c00, kCarry = 0x04000400, kOne = 0x3c00;
+};
+
+constexpr float kNever = -1e30f;  // reference exponent before the first visible key
+constexpr float kRise = 15.0f;    // the reference moves when a score passes it by this much
+constexpr float kBelow = 7.0f;    // ... to this much below the maximum
+constexpr uint32_t kOutside = 0x80000000u;  // an offset past every buffer's range
+constexpr int kBufWord3 = 0x00020000;
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+
+// A row range as a raw buffer: rows [row, end) of a tensor of one head, as far
+// as 32-bit offsets reach.
+__device__ __forceinline__ I4 row_buffer(const AttnTensor& t, int64_t row, int64_t rows, int head, int dim_bytes) {
+  const char* p = t.data + row * t.row + (int64_t)head * t.head;
+  const int64_t bytes = rows <= 0 ? 0 : (rows - 1) * t.row + dim_bytes;
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  I4 r;
+  r.x = __builtin_amdgcn_readfirstlane((int)(uint32_t)u);
+  r.y = __builtin_amdgcn_readfirstlane((int)((uint32_t)(u >> 32) & 0xffffu));
+  r.z = __builtin_amdgcn_readfirstlane((int)(bytes < 0x7fffff00 ? bytes : 0x7fffff00));
+  r.w = kBufWord3;
+  return r;
+}
+
+// 16 bytes a lane from buffer offset `off` (a lane's own) into LDS at `lds` +
+// 16 * lane.  Completion is waited for with vmcnt.
+__device__ __forceinline__ void load_lds(I4 buf, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf)
+               : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::V8 read_k(uint32_t lds) {
+  return __builtin_bit_cast(typename Mat<T>::V8, *(const __attribute__((address_space(3))) S8*)(uintptr_t)lds);
+}
+// Two transposed reads: 4 + 4 rows of V of this lane's column.
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::V8 read_v(uint32_t lo, uint32_t hi) {
+  typedef __attribute__((address_space(3))) S4* P;
+  const S4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)lo);
+  const S4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)hi);
+  return __builtin_bit_cast(typename Mat<T>::V8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The larger (sum) of this lane's value and that of the lane 32 away.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// Keys that query `pos` of a sequence sees, [*lo, *hi] (empty: *hi < *lo).
+__device__ __forceinline__ void visible(const AttnArgs& a, int pos, int lq, int lk, int* lo, int* hi) {
+  const int64_t at = (int64_t)pos + lk - lq;
+  const int64_t l = a.left == kAttnNoBound ? 0 : at - a.left, h = a.right == kAttnNoBound ? lk - 1 : at + a.right;
+  *lo = (int)(l < 0 ? 0 : (l > lk ? lk : l));
+  *hi = (int)(h < -1 ? -1 : (h > lk - 1 ? lk - 1 : h));
+}
+
+// Bits [lo, hi] of a word, both taken relative to its first key.
+__device__ __forceinline__ uint64_t span_bits(int lo, int hi) {
+  lo = lo < 0 ? 0 : lo;
+  hi = hi > 63 ? 63 : hi;
+  return hi < lo ? 0 : (~0ull >> (63 - hi)) & (~0ull << lo);
+}
+
+// Which unit a workgroup takes: consecutive workgroups go to the 8 XCDs in
+// turn, so each XCD gets a contiguous share of the units, and the tiles that
+// read one sequence's keys find them in one L2.
+__device__ __forceinline__ int unit_of_block(int units) {
+  const int per = (units + 7) / 8;
+  const int u = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+  return (int)(blockIdx.x / 8) < per && u < units ? u : -1;
+}
+
+// Whether any of a V operand's 8 values is infinite or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite(typename Mat<T>::V8 v) {
+  const I4 w = __builtin_bit_cast(I4, v);
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= ((uint32_t)w[i] & Mat<T>::kExp) + Mat<T>::kCarry;
+  return bad & 0x80008000u;
+}
+
+// A V operand with infinite or NaN values, of keys that some queries see and
+// others do not: *clean has zeros for them, *pos and *neg ones where a query that sees
+// the key has to get +inf or -inf (both: NaN).
+template <typename T>
+__device__ __forceinline__ void split_nonfinite(S8 v, S8* clean, S8* pos, S8* neg) {
+  constexpr uint32_t e = Mat<T>::kExp & 0xffff;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t x = (uint16_t)v[j];
+    const bool bad = (x & e) == e, nan = bad && (x & 0x7fff) != e;
+    (*clean)[j] = bad ? 0 : v[j];
+    (*pos)[j] = bad && (nan || !(x & 0x8000)) ? Mat<T>::kOne : 0;
+    (*neg)[j] = bad && (nan || (x & 0x8000)) ? Mat<T>::kOne : 0;
+  }
+}
+
+// ---- rows: 128 packed rows a workgroup ------------------------------------------------
+
+template <int NT>
+struct Geo {  // LDS rows of a step: 256 bytes (128 channels) or 128 (64)
+  static constexpr int kPitch = NT > 2 ? 256 : 128;
+  static constexpr int kChunks = kPitch / 16;
+  static __device__ int k_swizzle(int row) { return NT > 2 ? row & 15 : (row >> 1) & 7; }
+  static __device__ int v_swizzle(int row) { return NT > 2 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
+};
+
+// One workgroup: 4 waves of 32 packed rows over the keys of its piece in steps
+// of 64.  NT: head dim in units of 32 channels, rounded up.  MASKED: key mask.
+template <typename T, int NT, bool MASKED>
+__global__ __launch_bounds__(256, 2) void sfe_attn_rows_kernel(AttnArgs a) {
+  typedef Geo<NT> G;
+  typedef typename Mat<T>::V8 V8;
+  typedef typename Mat<T>::V2 V2;
+  constexpr int kStep = kAttnStepRows;
+  constexpr int kBuf = kStep * G::kPitch;  // bytes of a step of K (or V)
+  constexpr int kLoads = kBuf / 4096;      // load instructions of a wave for it
+  constexpr int kRowsPerLoad = 4096 / G::kPitch;
+  __shared__ __align__(1024) char lds[4 * kBuf];  // K, V of two steps
+  const int units = a.n_items * a.kv_heads;
+  const int u = unit_of_block(units);
+  if (u < 0) return;
+  const int kvh = u / a.n_items;
+  const AttnItem& it = a.items[u - kvh * a.n_items];
+  const int lq = it.lq, lk = it.lk, kv0 = it.kv0, kv1 = it.kv1, row0 = it.row0, part = it.part;
+  const int64_t q_row = it.q_row, k_row = it.k_row;
+  const int total = lq * a.group;
+  const int t = (int)threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5;
+  const int dim_bytes = 2 * a.dim;
+  const uint32_t base = lds_address(lds);
+
+  // ---- queries: lane's row, operand B of the first product
+  const int r = row0 + 32 * wave + (lane & 31);
+  const int rc = r < total ? r : total - 1;
+  const int pos = (int)((unsigned)rc / (unsigned)a.group);
+  int lo, hi;
+  visible(a, pos, lq, lk, &lo, &hi);
+  V8 q[2 * NT];
+  {
+    const char* p = a.q.data + (q_row + pos) * a.q.row + (int64_t)(kvh * a.group + rc - pos * a.group) * a.q.head;
+#pragma unroll
+    for (int s = 0; s < 2 * NT; ++s) {
+      const int c = 2 * s + half;
+      S8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * c < dim_bytes) v = *reinterpret_cast<const S8*>(p + 16 * c);
+      q[s] = __builtin_bit_cast(V8, v);
+    }
+  }
+  // the wave's common and joint ranges: rows ascend in query, so do their ranges
+  const int lo_all = __builtin_amdgcn_readlane(lo, 31), hi_all = __builtin_amdgcn_readlane(hi, 0);
+  const int lo_any = __builtin_amdgcn_readlane(lo, 0), hi_any = __builtin_amdgcn_readlane(hi, 31);
+
+  // ---- addresses
+  const int lrow = t / G::kChunks, lchunk = t % G::kChunks;
+  const int kc = lchunk ^ G::k_swizzle(lrow), vc = lchunk ^ G::v_swizzle(lrow);
+  const uint32_t k_off = 16 * kc < dim_bytes ? (uint32_t)(lrow * a.k.row) + 16 * kc : kOutside;
+  const uint32_t v_off = 16 * vc < dim_bytes ? (uint32_t)(lrow * a.v.row) + 16 * vc : kOutside;
+  const uint32_t k_next = (uint32_t)(kRowsPerLoad * a.k.row), v_next = (uint32_t)(kRowsPerLoad * a.v.row);
+  const uint32_t wave_base = __builtin_amdgcn_readfirstlane(base + 1024 * wave);
+  uint32_t k_addr[2 * NT];
+#pragma unroll
+  for (int s = 0; s < 2 * NT; ++s)
+    k_addr[s] = base + (lane & 31) * G::kPitch + 16 * ((2 * s + half) ^ G::k_swizzle(lane & 31));
+  uint32_t v_addr[NT];
+  {
+    const int row = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      v_addr[n] = base + 2 * kBuf + row * G::kPitch +
+                  16 * ((4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ G::v_swizzle(row)) + 8 * (lane & 1);
+  }
+
+  const uint8_t* mask = MASKED ? a.mask + k_row : nullptr;
+  auto mask_byte = [&](int kv) -> int { return kv + lane < lk ? mask[kv + lane] : 0; };
+  auto load_step = [&](int kv, int buf, uint64_t bits) {
+    const I4 kb = row_buffer(a.k, k_row + kv, lk - kv, kvh, dim_bytes);
+    const I4 vb = row_buffer(a.v, k_row + kv, lk - kv, kvh, dim_bytes);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      uint32_t ko = k_off == kOutside ? kOutside : k_off + i * k_next;
+      uint32_t vo = v_off == kOutside ? kOutside : v_off + i * v_next;
+      if (MASKED && !((bits >> (i * kRowsPerLoad + lrow)) & 1)) ko = vo = kOutside;
+      load_lds(kb, ko, wave_base + buf * kBuf + i * 4096);
+      load_lds(vb, vo, wave_base + (2 + buf) * kBuf + i * 4096);
+    }
+  };
+
+  F16 o[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[n][i] = 0.0f;
+  float m = kNever, l = 0.0f;
+  uint64_t bits = ~0ull, bits_next = ~0ull;
+  int byte_next = 0;
+  if (MASKED) {
+    bits = __ballot(mask_byte(kv0) != 0);
+    byte_next = mask_byte(kv0 + kStep);
+  }
+  if (kv0 < kv1) load_step(kv0, 0, bits);
+  int buf = 0;
+  for (int kv = kv0; kv < kv1; kv += kStep, buf ^= 1) {
+    // this step's keys have landed, and every wave is done with the step before
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (MASKED) {
+      bits_next = __ballot(byte_next != 0);
+      byte_next = mask_byte(kv + 2 * kStep);
+    }
+    if (kv + kStep < kv1) load_step(kv + kStep, buf ^ 1, bits_next);
+    const int end = kv1 < kv + kStep ? kv1 : kv + kStep;  // keys of the step: [kv, end)
+    if (lo_any < end && hi_any >= kv) {
+      const uint32_t kb = buf * kBuf;
+      F16 s[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[h][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2 * NT; ++c)
+          s[h] = Mat<T>::m32(read_k<T>(k_addr[c] + kb + h * 32 * G::kPitch), q[c], s[h]);
+      }
+      // `uneven`: keys (of the sequence) that some of the wave's rows do not see
+      const bool uneven = lo_all > kv || hi_all < (lk < kv + kStep ? lk : kv + kStep) - 1;
+      const bool edge = uneven || end < kv + kStep;
+      uint64_t see = ~0ull;
+      if (edge || (MASKED && bits != ~0ull)) {
+        // lane's keys are 32 h + 8 (i / 4) + 4 half + i % 4
+        see = span_bits(lo - kv, (hi < end - 1 ? hi : end - 1) - kv);
+        if (MASKED) see &= bits;
+        see >>= 4 * half;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[h][i] = (see >> (32 * h + 8 * (i / 4) + i % 4)) & 1 ? s[h][i] : -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
+      if (__any(top * a.scale_log2 > m + kRise)) {
+        const float nm = fmaxf(m, max_halves(top) * a.scale_log2 - kBelow);
+        const float f = exp2_fast(m - nm);
+        m = nm;
+        l *= f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[n][i] *= f;
+      }
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      V8 p[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const F2 w = {exp2_fast(__builtin_fmaf(s[h][i], a.scale_log2, -m)),
+                        exp2_fast(__builtin_fmaf(s[h][i + 1], a.scale_log2, -m))};
+          sum[i % 4] += w.x;
+          sum[i % 4 + 1] += w.y;
+          const V2 c = __builtin_convertvector(w, V2);
+          p[2 * h + i / 8][i % 8] = c.x;
+          p[2 * h + i / 8][i % 8 + 1] = c.y;
+        }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (!uneven) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            o[n] = Mat<T>::m32(
+                read_v<T>(v_addr[n] + kb + (16 * c) * G::kPitch, v_addr[n] + kb + (16 * c + 8) * G::kPitch), p[c], o[n]);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          const V8 pc = c < 2 ? (c == 0 ? p[0] : p[1]) : (c == 2 ? p[2] : p[3]);
+          S8 seen;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) seen[j] = (see >> (16 * c + 8 * (j / 4) + j % 4)) & 1 ? Mat<T>::kOne : 0;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            V8 v = read_v<T>(v_addr[n] + kb + 16 * c * G::kPitch, v_addr[n] + kb + (16 * c + 8) * G::kPitch);
+            // an infinite or NaN value would reach the rows that do not see it, as 0 * inf
+            if (__any(nonfinite<T>(v) != 0)) {
+              S8 clean, up, down;
+              split_nonfinite<T>(__builtin_bit_cast(S8, v), &clean, &up, &down);
+              F16 none;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) none[i] = 0.0f;
+              const F16 ups = Mat<T>::m32(__builtin_bit_cast(V8, up), __builtin_bit_cast(V8, seen), none);
+              const F16 downs = Mat<T>::m32(__builtin_bit_cast(V8, down), __builtin_bit_cast(V8, seen), none);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                if (ups[i] > 0.0f) o[n][i] += INFINITY;
+                if (downs[i] > 0.0f) o[n][i] -= INFINITY;
+              }
+              v = __builtin_bit_cast(V8, clean);
+            }
+            o[n] = Mat<T>::m32(v, pc, o[n]);
+          }
+        }
+      }
+    }
+    bits = bits_next;
+  }
+
+  l = sum_halves(l);
+  if (part >= 0) {
+    const int64_t at = ((int64_t)part * a.kv_heads + kvh) * kAttnTileRows + 32 * wave + (lane & 31);
+    float* po = a.part_o + at * (32 * NT);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<F4*>(po + 32 * n + 2 * i + 4 * half) = F4{o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]};
+    if (half == 0) a.part_ml[at] = make_float2(m, l);
+    return;
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing is zero)
+  // through LDS, so that a store instruction writes whole rows
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  char* mine = lds + wave * 32 * G::kPitch;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const F2 x = {o[n][i] * inv, o[n][i + 1] * inv}, y = {o[n][i + 2] * inv, o[n][i + 3] * inv};
+      const V2 c = __builtin_convertvector(x, V2), d = __builtin_convertvector(y, V2);
+      const int chunk = 4 * n + i / 4;
+      *reinterpret_cast<uint2*>(mine + (lane & 31) * G::kPitch + 16 * (chunk ^ G::k_swizzle(lane & 31)) + 8 * half) =
+          make_uint2(__builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d));
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32 * G::kChunks / 64; ++i) {
+    const int row = i * (64 / G::kChunks) + lane / G::kChunks, chunk = lane % G::kChunks;
+    const int rr = row0 + 32 * wave + row;
+    if (rr < total && 16 * chunk < dim_bytes) {
+      const int at = (int)((unsigned)rr / (unsigned)a.group);
+      char* p = const_cast<char*>(a.o.data) + (q_row + at) * a.o.row + (int64_t)(kvh * a.group + rr - at * a.group) * a.o.head;
+      *reinterpret_cast<uint4*>(p + 16 * chunk) =
+          *reinterpret_cast<const uint4*>(mine + row * G::kPitch + 16 * (chunk ^ G::k_swizzle(row)));
+    }
+  }
+}
+
+// ---- few: 16 packed rows a workgroup, its waves share the keys ---------------------------
+
+template <typename T, int NT, bool MASKED>
+__global__ __launch_bounds__(256, 1) void sfe_attn_few_kernel(AttnArgs a) {
+  typedef Geo<NT> G;
+  typedef typename Mat<T>::V8 V8;
+  typedef typename Mat<T>::V2 V2;
+  constexpr int kStep = kAttnStepFew, kWaves = kAttnWavesFew;
+  constexpr int kBuf = kStep * G::kPitch;  // bytes of a wave's step of K (or V)
+  constexpr int kLoads = kBuf / 1024;
+  constexpr int kRowsPerLoad = 1024 / G::kPitch;
+  constexpr int ND = 2 * NT;  // tiles of 16 channels
+  __shared__ __align__(1024) char lds[kWaves * 4 * kBuf];
+  const int units = a.n_items * a.kv_heads;
+  const int u = unit_of_block(units);
+  if (u < 0) return;
+  const int kvh = u / a.n_items;
+  const AttnItem& it = a.items[u - kvh * a.n_items];
+  const int lq = it.lq, lk = it.lk, kv0 = it.kv0, kv1 = it.kv1, row0 = it.row0, part = it.part;
+  const int64_t q_row = it.q_row, k_row = it.k_row;
+  const int total = lq * a.group;
+  const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), quarter = lane >> 4;
+  const int dim_bytes = 2 * a.dim;
+  const uint32_t base = lds_address(lds) + wave * 4 * kBuf;
+
+  const int r = row0 + (lane & 15);
+  const int rc = r < total ? r : total - 1;
+  const int pos = (int)((unsigned)rc / (unsigned)a.group);
+  int lo, hi;
+  visible(a, pos, lq, lk, &lo, &hi);
+  V8 q[NT];
+  {
+    const char* p = a.q.data + (q_row + pos) * a.q.row + (int64_t)(kvh * a.group + rc - pos * a.group) * a.q.head;
+#pragma unroll
+    for (int s = 0; s < NT; ++s) {
+      const int c = 4 * s + quarter;
+      S8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * c < dim_bytes) v = *reinterpret_cast<const S8*>(p + 16 * c);
+      q[s] = __builtin_bit_cast(V8, v);
+    }
+  }
+  const int lo_all = __builtin_amdgcn_readlane(lo, 15), hi_all = __builtin_amdgcn_readlane(hi, 0);
+
+  const int lrow = lane / G::kChunks, lchunk = lane % G::kChunks;
+  uint32_t k_addr[NT], v_addr[ND];
+#pragma unroll
+  for (int s = 0; s < NT; ++s)
+    k_addr[s] = base + (lane & 15) * G::kPitch + 16 * ((4 * s + quarter) ^ G::k_swizzle(lane & 15));
+  {
+    const int row = 4 * quarter + ((lane & 15) >> 2);
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+      v_addr[n] = base + 2 * kBuf + row * G::kPitch + 16 * ((2 * n + ((lane & 3) >> 1)) ^ G::v_swizzle(row)) + 8 * (lane & 1);
+  }
+  const uint8_t* mask = MASKED ? a.mask + k_row : nullptr;
+  auto mask_byte = [&](int kv) -> int { return kv + (lane & 31) < lk ? mask[kv + (lane & 31)] : 0; };
+  auto load_step = [&](int kv, int buf, uint32_t bits) {
+    const I4 kb = row_buffer(a.k, k_row + kv, lk - kv, kvh, dim_bytes);
+    const I4 vb = row_buffer(a.v, k_row + kv, lk - kv, kvh, dim_bytes);
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(base + buf * kBuf);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = i * kRowsPerLoad + lrow;
+      const int kc = 16 * (lchunk ^ G::k_swizzle(row)), vc = 16 * (lchunk ^ G::v_swizzle(row));
+      uint32_t ko = kc < dim_bytes ? (uint32_t)(row * a.k.row) + kc : kOutside;
+      uint32_t vo = vc < dim_bytes ? (uint32_t)(row * a.v.row) + vc : kOutside;
+      if (MASKED && !((bits >> row) & 1)) ko = vo = kOutside;
+      load_lds(kb, ko, dst + i * 1024);
+      load_lds(vb, vo, dst + 2 * kBuf + i * 1024);
+    }
+  };
+
+  F4 o[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n) o[n] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kNever, l = 0.0f;
+  constexpr int kTurn = kWaves * kStep;  // keys of all waves' steps
+  uint32_t bits = ~0u, bits_next = ~0u;
+  const int first = kv0 + wave * kStep;
+  if (MASKED && first < kv1) bits = (uint32_t)__ballot(mask_byte(first) != 0);
+  if (first < kv1) load_step(first, 0, bits);
+  int buf = 0;
+  for (int kv = first; kv < kv1; kv += kTurn, buf ^= 1) {
+    const bool more = kv + kTurn < kv1;
+    // (a wave's LDS buffers are its own: its reads of the buffer to be filled are
+    // done, and its loads are waited for by count)
+    if (MASKED && more) bits_next = (uint32_t)__ballot(mask_byte(kv + kTurn) != 0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) {
+      load_step(kv + kTurn, buf ^ 1, bits_next);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const int end = kv1 < kv + kStep ? kv1 : kv + kStep;
+    const uint32_t kb = buf * kBuf;
+    F4 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+        s[h] = Mat<T>::m16(read_k<T>(k_addr[c] + kb + h * 16 * G::kPitch), q[c], s[h]);
+    }
+    const bool uneven = lo_all > kv || hi_all < (lk < kv + kStep ? lk : kv + kStep) - 1;
+    const bool edge = uneven || end < kv + kStep;
+    uint32_t see = ~0u;
+    if (edge || (MASKED && bits != ~0u)) {
+      // lane's keys are 16 h + 4 quarter + i
+      see = (uint32_t)span_bits(lo - kv, (hi < end - 1 ? hi : end - 1) - kv);
+      if (MASKED) see &= bits;
+      see >>= 4 * quarter;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[h][i] = (see >> (16 * h + i)) & 1 ? s[h][i] : -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
+    if (__any(top * a.scale_log2 > m + kRise)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      const float nm = fmaxf(m, max_halves(top) * a.scale_log2 - kBelow);
+      const float f = exp2_fast(m - nm);
+      m = nm;
+      l *= f;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[n] *= f;
+    }
+    V8 p;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const F2 w = {exp2_fast(__builtin_fmaf(s[h][i], a.scale_log2, -m)),
+                      exp2_fast(__builtin_fmaf(s[h][i + 1], a.scale_log2, -m))};
+        l += w.x + w.y;
+        const V2 c = __builtin_convertvector(w, V2);
+        p[4 * h + i] = c.x;
+        p[4 * h + i + 1] = c.y;
+      }
+#pragma unroll
+    for (int n = 0; n < ND; ++n) {
+      V8 v = read_v<T>(v_addr[n] + kb, v_addr[n] + kb + 16 * G::kPitch);
+      if (uneven && __any(nonfinite<T>(v) != 0)) {  // (see the rows kernel)
+        S8 clean, up, down, seen;
+        split_nonfinite<T>(__builtin_bit_cast(S8, v), &clean, &up, &down);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) seen[j] = (see >> (16 * (j / 4) + j % 4)) & 1 ? Mat<T>::kOne : 0;
+        const F4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        const F4 ups = Mat<T>::m16(__builtin_bit_cast(V8, up), __builtin_bit_cast(V8, seen), zero);
+        const F4 downs = Mat<T>::m16(__builtin_bit_cast(V8, down), __builtin_bit_cast(V8, seen), zero);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (ups[i] > 0.0f) o[n][i] += INFINITY;
+          if (downs[i] > 0.0f) o[n][i] -= INFINITY;
+        }
+        v = __builtin_bit_cast(V8, clean);
+      }
+      o[n] = Mat<T>::m16(v, p, o[n]);
+    }
+    bits = bits_next;
+  }
+  l += __shfl_xor(l, 16);
+  l = sum_halves(l);
+
+  // ---- the waves' results, added up through LDS
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  constexpr int kDim = 32 * NT, kRowF = kDim + 4;  // floats of a row (4 of padding)
+  float* ow = reinterpret_cast<float*>(lds);                          // [wave][16][kRowF]
+  float2* ml = reinterpret_cast<float2*>(ow + kWaves * 16 * kRowF);   // [wave][16]
+  static_assert((kWaves * 16 * kRowF + 2 * kWaves * 16) * 4 <= (int)sizeof(lds), "results fit");
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+    *reinterpret_cast<F4*>(ow + (wave * 16 + (lane & 15)) * kRowF + 16 * n + 4 * quarter) = o[n];
+  if (quarter == 0) ml[wave * 16 + lane] = make_float2(m, l);
+  __syncthreads();
+  for (int e = t; e < 16 * (kDim / 4); e += 256) {
+    const int row = e / (kDim / 4), d = 4 * (e % (kDim / 4));
+    float mm = kNever;
+    for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, ml[w * 16 + row].x);
+    F4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
+    for (int w = 0; w < kWaves; ++w) {
+      const float2 x = ml[w * 16 + row];
+      if (x.x == kNever && x.y == 0.0f) continue;  // (saw nothing)
+      const float f = exp2_fast(x.x - mm);
+      sum += x.y * f;
+      acc += *reinterpret_cast<const F4*>(ow + (w * 16 + row) * kRowF + d) * f;
+    }
+    const int rr = row0 + row;
+    if (part >= 0) {
+      const int64_t at = ((int64_t)part * a.kv_heads + kvh) * kAttnTileFew + row;
+      *reinterpret_cast<F4*>(a.part_o + at * kDim + d) = acc;
+      if (d == 0) a.part_ml[at] = make_float2(mm, sum);
+    } else if (rr < total && d < a.dim) {
+      const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+      const int at = (int)((unsigned)rr / (unsigned)a.group);
+      char* p = const_cast<char*>(a.o.data) + (q_row + at) * a.o.row + (int64_t)(kvh * a.group + rr - at * a.group) * a.o.head;
+      const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};
+      const V2 c = __builtin_convertvector(x, V2), g = __builtin_convertvector(y, V2);
+      *reinterpret_cast<uint2*>(p + 2 * d) = make_uint2(__builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, g));
+    }
+  }
+}
+
+// ---- pieces added up ---------------------------------------------------------------------
+
+// A wave per packed row: sum over the row's pieces, 2 channels a lane.
+template <typename T, int NT, int TILE>
+__global__ __launch_bounds__(256) void sfe_attn_join_kernel(AttnArgs a) {
+  typedef typename Mat<T>::V2 V2;
+  constexpr int kDim = 32 * NT;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = (int)(threadIdx.x & 63);
+  const int row = (int)(w % TILE);
+  const int64_t jk = w / TILE;
+  const int kvh = (int)(jk % a.kv_heads);
+  if (jk / a.kv_heads >= a.n_joins) return;
+  const AttnJoin j = a.joins[jk / a.kv_heads];
+  const int rr = j.row0 + row;
+  if (rr >= j.lq * a.group) return;
+  float m = kNever;
+  for (int p = 0; p < j.parts; ++p)
+    m = fmaxf(m, a.part_ml[((int64_t)(j.part0 + p) * a.kv_heads + kvh) * TILE + row].x);
+  float x = 0.0f, y = 0.0f, sum = 0.0f;
+  for (int p = 0; p < j.parts; ++p) {
+    const int64_t at = ((int64_t)(j.part0 + p) * a.kv_heads + kvh) * TILE + row;
+    const float2 ml = a.part_ml[at];
+    if (ml.x == kNever && ml.y == 0.0f) continue;  // (saw nothing)
+    const float f = exp2_fast(ml.x - m);
+    sum += ml.y * f;
+    if (2 * lane < kDim) {
+      const float2 v = *reinterpret_cast<const float2*>(a.part_o + at * kDim + 2 * lane);
+      x += v.x * f;
+      y += v.y * f;
+    }
+  }
+  if (2 * lane >= a.dim) return;
+  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  const int at = (int)((unsigned)rr / (unsigned)a.group);
+  char* p = const_cast<char*>(a.o.data) + (j.q_row + at) * a.o.row + (int64_t)(kvh * a.group + rr - at * a.group) * a.o.head;
+  const F2 v = {x * inv, y * inv};
+  *reinterpret_cast<V2*>(p + 4 * lane) = __builtin_convertvector(v, V2);
+}
+
+template <typename T, int NT>
+hipError_t run_rows(const AttnArgs& a, hipStream_t stream) {
+  const unsigned blocks = (unsigned)(((int64_t)a.n_items * a.kv_heads + 7) / 8 * 8);
+  if (a.mask)
+    sfe_attn_rows_kernel<T, NT, true><<<dim3(blocks), dim3(256), 0, stream>>>(a);
+  else
+    sfe_attn_rows_kernel<T, NT, false><<<dim3(blocks), dim3(256), 0, stream>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.n_joins) return e;
+  sfe_attn_join_kernel<T, NT, kAttnTileRows>
+      <<<dim3((unsigned)((int64_t)a.n_joins * a.kv_heads * kAttnTileRows / 4)), dim3(256), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, int NT>
+hipError_t run_few(const AttnArgs& a, hipStream_t stream) {
+  const unsigned blocks = (unsigned)(((int64_t)a.n_items * a.kv_heads + 7) / 8 * 8);
+  if (a.mask)
+    sfe_attn_few_kernel<T, NT, true><<<dim3(blocks), dim3(256), 0, stream>>>(a);
+  else
+    sfe_attn_few_kernel<T, NT, false><<<dim3(blocks), dim3(256), 0, stream>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.n_joins) return e;
+  sfe_attn_join_kernel<T, NT, kAttnTileFew>
+      <<<dim3((unsigned)((int64_t)a.n_joins * a.kv_heads * kAttnTileFew / 4)), dim3(256), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_form(const AttnArgs& a, bool rows, hipStream_t stream) {
+  switch (attn_padded_dim(a.dim)) {
+    case 64: return rows ? run_rows<T, 2>(a, stream) : run_few<T, 2>(a, stream);
+    case 96: return rows ? run_rows<T, 3>(a, stream) : run_few<T, 3>(a, stream);
+    default: return rows ? run_rows<T, 4>(a, stream) : run_few<T, 4>(a, stream);
+  }
+}
+
+}  // namespace
+
+hipError_t launch_attn_rows(const AttnArgs& a, int type, hipStream_t stream) {
+  return type == kOpBf16 ? run_form<Bf>(a, true, stream) : run_form<Hf>(a, true, stream);
+}
+hipError_t launch_attn_few(const AttnArgs& a, int type, hipStream_t stream) {
+  return type == kOpBf16 ? run_form<Bf>(a, false, stream) : run_form<Hf>(a, false, stream);
+}
+
+}  // namespace sfe

@@ -21,6 +21,7 @@
 
 #include "../../include/scriptrs_fe.h"
 #include "sfe_internal.hpp"
+#include "sfe_ops.hpp"
 
 using sfe::Item;
 
@@ -312,6 +313,10 @@ struct sfe_ctx {
   // kNoAllocMaxItems items: the chunks' own items and the planner's lists.
   std::vector<Item> na_in;
   sfe::PlanWorkspace na_ws;
+  // The model operators (sfe_ops.cpp): buffers of freed plans, for the next
+  // plans; the calls' scratch, outgrown ones in front of the current one.
+  std::vector<std::pair<void*, size_t>> op_free;
+  std::vector<std::pair<void*, size_t>> op_scratch;
 };
 
 namespace {
@@ -605,6 +610,103 @@ int check_dtype(int32_t d) {
 
 }  // namespace
 
+namespace sfe {
+
+int op_fail(int code, const std::string& msg) { return fail(code, msg); }
+int op_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+int op_cus(sfe_ctx* ctx) { return ctx->cus; }
+
+int op_call(sfe_ctx* ctx, hipStream_t stream, const char* what, hipError_t (*body)(void* arg, int cus), void* arg) {
+  int rc = check_ctx(ctx);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  SFE_HIP(hipStreamIsCapturing(stream, &cap));
+  const bool captured = cap != hipStreamCaptureStatusNone;
+  if (!captured) {
+    SFE_HIP(order_after_last(ctx, stream));
+    ctx->unsettled = true;
+  }
+  const hipError_t e = body(arg, ctx->cus);
+  if (e != hipSuccess) return hip_fail(e, what);
+  if (!captured) SFE_HIP(mark_last(ctx, stream));
+  return SFE_OK;
+}
+
+int op_upload(sfe_ctx* ctx, const void* table, size_t bytes, size_t room, hipStream_t stream, void** buf, size_t* cap) {
+  int rc = check_ctx(ctx);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  SFE_HIP(hipStreamIsCapturing(stream, &status));
+  if (status != hipStreamCaptureStatusNone)
+    return fail(SFE_INVALID_ARG, "a plan cannot be made while its stream is being captured");
+  SFE_HIP(order_after_last(ctx, stream));
+  // the smallest freed buffer that is large enough and not far too large
+  size_t best = ctx->op_free.size();
+  for (size_t i = 0; i < ctx->op_free.size(); ++i) {
+    const size_t c = ctx->op_free[i].second;
+    if (c >= room && c / 8 <= room + 65536 && (best == ctx->op_free.size() || c < ctx->op_free[best].second)) best = i;
+  }
+  void* p = nullptr;
+  size_t got = 0;
+  ctx->op_free.reserve(ctx->op_free.size() + 1);
+  if (best < ctx->op_free.size()) {
+    p = ctx->op_free[best].first;
+    got = ctx->op_free[best].second;
+    ctx->op_free.erase(ctx->op_free.begin() + (std::ptrdiff_t)best);
+  } else {
+    got = (room + room / 4 + 65535) / 65536 * 65536;
+    const hipError_t e = hipMalloc(&p, got);
+    g_allocations.fetch_add(1);
+    if (e != hipSuccess) return hip_fail(e, "hipMalloc");
+  }
+  auto queue = [&]() -> int {
+    char* stage = nullptr;
+    SFE_HIP(ctx->h_meta.take(bytes, stream, &stage));
+    memcpy(stage, table, bytes);
+    ctx->unsettled = true;
+    SFE_HIP(sfe::launch_upload(stage, p, bytes, stream));
+    SFE_HIP(mark_last(ctx, stream));
+    return SFE_OK;
+  };
+  if ((rc = queue())) {
+    ctx->op_free.emplace_back(p, got);  // (reserved above: cannot throw)
+    return rc;
+  }
+  *buf = p;
+  *cap = got;
+  return SFE_OK;
+}
+
+void op_release(sfe_ctx* ctx, void* buf, size_t cap) {
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  ctx->op_free.emplace_back(buf, cap);
+}
+
+int op_scratch(sfe_ctx* ctx, size_t bytes, hipStream_t stream, void** out) {
+  int rc = check_ctx(ctx);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  if (ctx->op_scratch.empty() || ctx->op_scratch.back().second < bytes) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    SFE_HIP(hipStreamIsCapturing(stream, &status));
+    if (status != hipStreamCaptureStatusNone)
+      return fail(SFE_INVALID_ARG, "the scratch of a captured call has to be there: make one such call before the capture");
+    const size_t want = bytes + bytes / 2;
+    ctx->op_scratch.reserve(ctx->op_scratch.size() + 1);
+    void* p = nullptr;
+    const hipError_t e = hipMalloc(&p, want);
+    g_allocations.fetch_add(1);
+    if (e != hipSuccess) return hip_fail(e, "hipMalloc");
+    ctx->op_scratch.emplace_back(p, want);
+  }
+  *out = ctx->op_scratch.back().first;
+  return SFE_OK;
+}
+
+}  // namespace sfe
+
 extern "C" {
 
 void sfe_config_default(sfe_config* c) {
@@ -743,6 +845,8 @@ void sfe_destroy(sfe_ctx* ctx) {
   ctx->h_io_in.release();
   ctx->h_io_out.release();
   ctx->win.release();
+  for (auto& b : ctx->op_free) (void)hipFree(b.first);
+  for (auto& b : ctx->op_scratch) (void)hipFree(b.first);
   for (int i = 0; i < 2; ++i) {
     ctx->h_win[i].release();
     if (ctx->ev_copied[i]) (void)hipEventDestroy(ctx->ev_copied[i]);

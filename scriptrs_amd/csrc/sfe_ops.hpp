@@ -1,0 +1,171 @@
+// The model operators behind the features (attention over packed sequences,
+// rotary positions, norms around a block, beam search): what their entry
+// points (sfe_ops.cpp) share with the context (sfe_capi.cpp), and their
+// kernels' launchers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <string>
+#include <vector>
+
+struct sfe_ctx;
+
+namespace sfe {
+
+// ---- the context's part (sfe_capi.cpp) ----------------------------------------
+
+// Sets the calling thread's message and returns code.
+int op_fail(int code, const std::string& msg);
+int op_hip_fail(hipError_t e, const char* what);
+
+// Queues an operator on `stream` in the context's order: the device is made
+// current, the context locked, the stream ordered after the context's earlier
+// calls, body(arg, compute units) run, and the call's end marked.  On a stream
+// that is being captured the order is the caller's graph's: nothing is waited
+// for or marked.
+int op_call(sfe_ctx* ctx, hipStream_t stream, const char* what, hipError_t (*body)(void* arg, int cus), void* arg);
+
+// Memory of a plan: the first `bytes` of a device buffer of at least `room`
+// bytes are filled from `table` on `stream` (through the context's pinned
+// staging).  The buffer comes from the context's freed ones where one fits: the
+// upload is ordered after every earlier call that read it.  *buf and *cap
+// receive it.  Refused while `stream` is being captured.
+int op_upload(sfe_ctx* ctx, const void* table, size_t bytes, size_t room, hipStream_t stream, void** buf, size_t* cap);
+void op_release(sfe_ctx* ctx, void* buf, size_t cap);
+int op_cus(sfe_ctx* ctx);  // compute units of the context's device
+
+// Scratch of at least `bytes` for the calls of a context, which are ordered after
+// each other.  Outgrown buffers live as long as the context (a captured graph
+// may hold their addresses).  Growing while `stream` is captured fails.
+int op_scratch(sfe_ctx* ctx, size_t bytes, hipStream_t stream, void** out);
+
+// ---- element types ---------------------------------------------------------------
+enum OpType { kOpF32 = 0, kOpBf16 = 1, kOpF16 = 2 };  // sfe_dtype
+inline int op_size(int type) { return type == kOpF32 ? 4 : 2; }
+
+// ---- attention over packed sequences (sfe_attn.hip, sfe_attn_plan.cpp) -------------
+
+// A tile's piece: `rows` packed rows of one sequence (row = query * group +
+// head within the group: the queries of the heads that share a kv head) against
+// the keys [kv0, kv1).
+struct AttnItem {
+  int64_t q_row, k_row;  // first query and key row of the sequence
+  int32_t lq, lk;        // its queries and keys
+  int32_t row0;          // first packed row of the tile
+  int32_t kv0, kv1;
+  int32_t part;          // piece number among the partial results, or -1: the whole result
+  int32_t pad[2];
+};
+static_assert(sizeof(AttnItem) == 48, "layout shared with the kernels");
+// Pieces of one tile to be added up.
+struct AttnJoin {
+  int64_t q_row;
+  int32_t lq, row0, part0, parts;
+};
+static_assert(sizeof(AttnJoin) == 24, "layout shared with the kernels");
+
+// Packed rows of a tile and keys of a step, per kernel form: `rows` (4 waves of
+// 32 rows share a step's keys) and `few` (16 rows, each wave takes every
+// fourth step).
+constexpr int kAttnTileRows = 128, kAttnStepRows = 64;
+constexpr int kAttnTileFew = 16, kAttnStepFew = 32, kAttnWavesFew = 4;
+constexpr int kAttnMaxDim = 128;
+constexpr int32_t kAttnNoBound = 0x7fffffff;
+
+struct AttnForm {
+  std::vector<AttnItem> items;
+  std::vector<AttnJoin> joins;
+  int32_t parts = 0;  // pieces with a partial result
+};
+struct AttnPlanHost {
+  AttnForm rows, few;
+};
+// Lays the tiles of n sequences out (host only).  left, right: the window, or
+// kAttnNoBound.
+void attn_plan(const int64_t* q_offsets, const int64_t* k_offsets, int n, int group, int kv_heads, int head_dim,
+               int32_t left, int32_t right, int cus, AttnPlanHost* out);
+
+struct AttnTensor {
+  const char* data;
+  int64_t row, head;  // strides in bytes
+};
+struct AttnArgs {
+  AttnTensor q, k, v, o;
+  const uint8_t* mask;
+  const AttnItem* items;
+  const AttnJoin* joins;
+  float* part_o;    // [piece][kv head][tile row][padded head dim]
+  float2* part_ml;  // [piece][kv head][tile row]: (reference exponent, sum)
+  int32_t n_items, n_joins, kv_heads, group, dim;
+  int32_t left, right;
+  float scale_log2;  // scale * log2(e)
+};
+inline int attn_padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : 128); }
+hipError_t launch_attn_rows(const AttnArgs& a, int type, hipStream_t stream);
+hipError_t launch_attn_few(const AttnArgs& a, int type, hipStream_t stream);
+
+// ---- rotary positions (sfe_rotary.hip) ----------------------------------------------
+constexpr int kRotaryMaxPairs = 128;
+struct RotaryTensor {
+  const char* x;
+  char* y;
+  int64_t x_row, x_head, y_row, y_head;  // strides in elements
+  int32_t heads;
+};
+struct RotaryArgs {
+  uint64_t step[kRotaryMaxPairs];  // turns a position, as a fraction of 2^64
+  RotaryTensor t[2];
+  const int32_t* positions;
+  int64_t rows;
+  int32_t dim, rotary, inverse;
+  float magnitude;
+};
+hipError_t launch_rotary(const RotaryArgs& a, int type, bool interleaved, int cus, hipStream_t stream);
+
+// ---- norms around a block (sfe_residual.hip) ------------------------------------------
+enum NormKind { kNormNone = 0, kNormLayer = 1, kNormRms = 2 };
+struct ResidualArgs {
+  const char *x, *y, *gate;  // residual stream, block output, gate (or null)
+  char *xo, *z;              // new residual stream, its norm (or null)
+  const float *post_w, *post_b, *pre_w, *pre_b;
+  int64_t x_row, y_row, gate_row, xo_row, z_row;  // strides in elements
+  int64_t rows;
+  int32_t width, post, pre, sigmoid;
+  float scale, eps;
+};
+constexpr int kResidualMaxWidth = 16384;
+hipError_t launch_residual(const ResidualArgs& a, int stream_type, int block_type, hipStream_t stream);
+
+// ---- beam search (sfe_beam.hip) ----------------------------------------------------------
+constexpr int kMaxBeams = 32;
+struct BeamArgs {
+  const char* logits;
+  int64_t row;  // stride in elements
+  int32_t streams, beams, vocab, end;
+  const float* scores;
+  const uint8_t* finished;  // or null
+  float* out_scores;
+  int32_t *parents, *tokens;
+  uint8_t* out_finished;  // or null
+  char* scratch;
+};
+size_t beam_scratch_bytes(int streams, int beams, int vocab);
+hipError_t launch_beam_select(const BeamArgs& a, int type, hipStream_t stream);
+
+struct BeamState {
+  const char* in;
+  char* out;
+  int64_t outer, inner;  // [outer][streams * beams][inner bytes]
+};
+constexpr int kReorderStates = 8;  // of one launch
+struct ReorderArgs {
+  BeamState s[kReorderStates];
+  int32_t n, streams, beams;
+  const int32_t* parents;
+};
+hipError_t launch_beam_reorder(const ReorderArgs& a, hipStream_t stream);
+
+}  // namespace sfe

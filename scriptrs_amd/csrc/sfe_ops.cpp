@@ -495,8 +495,9 @@ int sfe_beam_select(sfe_ctx* ctx, int32_t dtype, const void* logits, int64_t row
     if (row_stride < 0 || row_stride >= kMaxStride) return op_fail(SFE_INVALID_ARG, "row_stride must be in [0, 2^40)");
     if (out_scores == scores || (out_finished && out_finished == finished))
       return op_fail(SFE_INVALID_ARG, "out_scores and out_finished must not be the inputs");
-    const int64_t groups = (int64_t)streams * beams * ((vocab + 8191) / 8192 + 1);
-    if (groups > (int64_t)(UINT32_MAX / 256)) return op_fail(SFE_INVALID_ARG, "batch too large for one launch");
+    // a launch holds fewer than 2^32 threads, of up to 64 a beam and up to 2 workgroups of
+    // 256 a row (more only where the rows alone do not fill the device)
+    if ((int64_t)streams * beams > (1 << 22)) return op_fail(SFE_INVALID_ARG, "batch too large for one launch");
     struct Call {
       sfe::BeamArgs a;
       int dtype;
@@ -505,13 +506,14 @@ int sfe_beam_select(sfe_ctx* ctx, int32_t dtype, const void* logits, int64_t row
     call.stream = static_cast<hipStream_t>(stream);
     call.dtype = dtype;
     void* scratch = nullptr;
-    const int rc = sfe::op_scratch(ctx, sfe::beam_scratch_bytes(streams, beams, vocab), call.stream, &scratch);
+    const size_t room = sfe::beam_scratch_bytes(streams, beams, vocab, sfe::op_cus(ctx));
+    const int rc = room ? sfe::op_scratch(ctx, room, call.stream, &scratch) : SFE_OK;
     if (rc) return rc;
     call.a = sfe::BeamArgs{static_cast<const char*>(logits), row_stride, streams, beams, vocab, end_token, scores, finished,
                            out_scores, parents, tokens, out_finished, static_cast<char*>(scratch)};
-    return sfe::op_call(ctx, call.stream, "beam select", [](void* arg, int) -> hipError_t {
+    return sfe::op_call(ctx, call.stream, "beam select", [](void* arg, int cus) -> hipError_t {
       Call& c = *static_cast<Call*>(arg);
-      return sfe::launch_beam_select(c.a, c.dtype, c.stream);
+      return sfe::launch_beam_select(c.a, c.dtype, cus, c.stream);
     }, &call);
   });
 }
@@ -533,8 +535,8 @@ int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int3
       const sfe_beam_state& s = states[i];
       const std::string name = "state " + std::to_string(i);
       if (s.outer < 0 || s.inner_bytes < 0) return op_fail(SFE_INVALID_ARG, name + ": negative size");
-      if (s.outer > (int64_t)1 << 40 || s.inner_bytes > (int64_t)1 << 40 ||
-          (double)s.outer * (double)s.inner_bytes * streams * beams > 1e15)
+      if (s.outer > (int64_t)1 << 40 || s.inner_bytes >= (int64_t)1 << 31 ||
+          (double)s.outer * (double)s.inner_bytes * streams * beams > 1e12)
         return op_fail(SFE_INVALID_ARG, name + " is too large");
       const int64_t bytes = s.outer * streams * beams * s.inner_bytes;
       if (bytes == 0) continue;

@@ -152,8 +152,8 @@ struct BeamArgs {
   uint8_t* out_finished;  // or null
   char* scratch;
 };
-size_t beam_scratch_bytes(int streams, int beams, int vocab);
-hipError_t launch_beam_select(const BeamArgs& a, int type, hipStream_t stream);
+size_t beam_scratch_bytes(int streams, int beams, int vocab, int cus);
+hipError_t launch_beam_select(const BeamArgs& a, int type, int cus, hipStream_t stream);
 
 struct BeamState {
   const char* in;

@@ -13,14 +13,13 @@
 // rad at 45,000).  Sine and cosine are their power series over an eighth of a
 // turn to either side, in f32 (error below 1e-7).
 //
-// Bound by memory: each element is read and written once.  A thread takes 16
-// bytes of each channel of a pair and walks a share of the row's heads with
-// the same 4 or 8 sines and cosines.
+// Bound by memory: each element is read and written once, and a row's sines and
+// cosines are computed once for all of its heads.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
-#include "sfe_internal.hpp"
 #include "sfe_ops.hpp"
 
 namespace sfe {
@@ -51,138 +50,112 @@ __device__ __forceinline__ void turn_cos_sin(uint32_t t, float* c, float* s) {
 }
 
 constexpr int kRotaryThreads = 256;
+constexpr int kRotaryTable = 4096;  // (cosine, sine) of a workgroup's rows and pairs
 
-// N: elements of a vector.  A unit is (row, slot, share of heads); slots
-// 0..turning - 1 hold N pairs each (half: two vectors R/2 apart; interleaved:
-// two consecutive vectors), the rest one vector of copied channels.
-template <typename T, int N, bool INTERLEAVED>
-__global__ __launch_bounds__(kRotaryThreads) void sfe_rotary_kernel(RotaryArgs a, int64_t unit0, int64_t units,
-                                                                    int slots, int shares) {
-  const int64_t u = unit0 + (int64_t)blockIdx.x * kRotaryThreads + threadIdx.x;
-  if (u >= units) return;
-  const int slot = (int)(u % slots);
-  const int64_t rest = u / slots;
-  const int share = (int)(rest % shares);
-  const int64_t row = rest / shares;
-  const int turning = a.rotary / 2 / N;
+// A workgroup takes RB times `per` rows: their sines and cosines go into LDS, then
+// a thread keeps its place in a row (head and channels) and turns it in RB rows,
+// all RB loads issued before the first store (outputs may be the inputs, so the
+// compiler cannot move loads past stores).  Places of a row, `places`: for each
+// head turning units, then copied ones.  N > 1: a unit is 16 bytes of N channels:
+// half, two vectors R/2 apart; interleaved, one vector of N / 2 pairs.  N = 1: a
+// pair, or a copied channel (tensors whose vectors are not aligned).
+template <typename T, int N, bool INTERLEAVED, int RB>
+__global__ __launch_bounds__(kRotaryThreads) void sfe_rotary_kernel(RotaryArgs a, int64_t first, uint32_t places,
+                                                                    uint32_t slots, uint32_t chunks, uint32_t per) {
+  constexpr bool kOne = INTERLEAVED && N > 1;  // both channels of a pair in one vector
+  constexpr int kPairs = kOne ? N / 2 : N;     // of a unit
+  typedef Vec<T, N> V;
+  __shared__ float2 table[kRotaryTable];
+  const uint32_t group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks;
+  const int64_t row0 = first + (int64_t)group * RB * per;
+  const int pairs = a.rotary / 2, t = (int)threadIdx.x;
+  const int rows = (int)(a.rows - row0 < (int64_t)(RB * per) ? a.rows - row0 : (int64_t)(RB * per));
+  const float m = a.magnitude, ms = a.inverse ? -a.magnitude : a.magnitude;
+  for (int e = t; e < rows * pairs; e += kRotaryThreads) {
+    const int r = (int)((unsigned)e / (unsigned)pairs), p = e - r * pairs;
+    float c, s;
+    turn_cos_sin((uint32_t)(((uint64_t)(int64_t)a.positions[row0 + r] * a.step[p]) >> 32), &c, &s);
+    table[e] = make_float2(m * c, ms * s);
+  }
+  __syncthreads();
+  const uint32_t in = per > 1 ? (uint32_t)t / places : 0;  // row within a pass
+  const uint32_t place = per > 1 ? (uint32_t)t - in * places : chunk * kRotaryThreads + (uint32_t)t;
+  if (place >= places || in >= per) return;
+  const int head = (int)(place / slots), slot = (int)(place - (uint32_t)head * slots);
+  const int turning = pairs / kPairs;
   const bool turn = slot < turning;
-  int d0, d1 = 0;
-  if (turn) {
-    d0 = INTERLEAVED ? 2 * N * slot : N * slot;
-    d1 = INTERLEAVED ? d0 + N : d0 + a.rotary / 2;
-  } else {
-    d0 = a.rotary + N * (slot - turning);
-  }
-  float cs[N], sn[N];
-  if (turn) {
-    const uint64_t at = (uint64_t)(int64_t)a.positions[row];
+  const int d0 = turn ? slot * (INTERLEAVED ? 2 * kPairs : kPairs) : a.rotary + N * (slot - turning);
+  const int d1 = INTERLEAVED ? d0 + 1 : d0 + pairs;  // (not of one vector)
+  const bool second = head >= a.t[0].heads;
+  const RotaryTensor& tn = a.t[second];
+  const int h = second ? head - a.t[0].heads : head;
+  const T* x = reinterpret_cast<const T*>(tn.x) + (row0 + in) * tn.x_row + h * tn.x_head;
+  T* y = reinterpret_cast<T*>(tn.y) + (row0 + in) * tn.y_row + h * tn.y_head;
+  V p[RB], q[RB];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      turn_cos_sin((uint32_t)((at * a.step[N * slot + i]) >> 32), &cs[i], &sn[i]);
-      cs[i] *= a.magnitude;
-      sn[i] *= a.inverse ? -a.magnitude : a.magnitude;
+  for (int k = 0; k < RB; ++k)
+    if ((int)(in + k * per) < rows) {
+      p[k] = *reinterpret_cast<const V*>(x + k * (int64_t)per * tn.x_row + d0);
+      if (!kOne && turn) q[k] = *reinterpret_cast<const V*>(x + k * (int64_t)per * tn.x_row + d1);
     }
-  }
-  const int heads = a.t[0].heads + a.t[1].heads;
-  for (int h = share; h < heads; h += shares) {
-    const bool second = h >= a.t[0].heads;
-    const RotaryTensor& t = a.t[second];
-    const int hh = second ? h - a.t[0].heads : h;
-    const T* x = reinterpret_cast<const T*>(t.x) + row * t.x_row + hh * t.x_head;
-    T* y = reinterpret_cast<T*>(t.y) + row * t.y_row + hh * t.y_head;
-    typedef Vec<T, N> V;
-    if (!turn) {
-      if (x != y) *reinterpret_cast<V*>(y + d0) = *reinterpret_cast<const V*>(x + d0);
-      continue;
-    }
-    const V p = *reinterpret_cast<const V*>(x + d0), q = *reinterpret_cast<const V*>(x + d1);
-    V r, w;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (INTERLEAVED) {
-        // values 2i and 2i + 1 of the two vectors
-        const float e = (float)(2 * i < N ? p.v[(2 * i) % N] : q.v[(2 * i) % N]);
-        const float f = (float)(2 * i < N ? p.v[(2 * i + 1) % N] : q.v[(2 * i + 1) % N]);
-        const T ye = (T)__builtin_fmaf(e, cs[i], -f * sn[i]), yf = (T)__builtin_fmaf(f, cs[i], e * sn[i]);
-        if (2 * i < N) {
-          r.v[(2 * i) % N] = ye;
-          r.v[(2 * i + 1) % N] = yf;
-        } else {
-          w.v[(2 * i) % N] = ye;
-          w.v[(2 * i + 1) % N] = yf;
-        }
-      } else {
-        const float e = (float)p.v[i], f = (float)q.v[i];
-        r.v[i] = (T)__builtin_fmaf(e, cs[i], -f * sn[i]);
-        w.v[i] = (T)__builtin_fmaf(f, cs[i], e * sn[i]);
+  for (int k = 0; k < RB; ++k)
+    if ((int)(in + k * per) < rows) {
+      T* yk = y + k * (int64_t)per * tn.y_row;
+      if (!turn) {
+        *reinterpret_cast<V*>(yk + d0) = p[k];
+        continue;
       }
+      const float2* cs = table + (in + k * per) * pairs + slot * kPairs;
+      V r, w;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const float e = (float)(kOne ? p[k].v[(2 * i) % N] : p[k].v[i]), f = (float)(kOne ? p[k].v[(2 * i + 1) % N] : q[k].v[i]);
+        const T ye = (T)__builtin_fmaf(e, cs[i].x, -f * cs[i].y), yf = (T)__builtin_fmaf(f, cs[i].x, e * cs[i].y);
+        r.v[kOne ? (2 * i) % N : i] = ye;
+        if (kOne) r.v[(2 * i + 1) % N] = yf;
+        else w.v[i] = yf;
+      }
+      *reinterpret_cast<V*>(yk + d0) = r;
+      if (!kOne) *reinterpret_cast<V*>(yk + d1) = w;
     }
-    *reinterpret_cast<V*>(y + d0) = r;
-    *reinterpret_cast<V*>(y + d1) = w;
-  }
 }
 
-// The same a pair at a time, for tensors whose vectors are not aligned or whose
-// R is no multiple of them.
-template <typename T, bool INTERLEAVED>
-__global__ __launch_bounds__(kRotaryThreads) void sfe_rotary_pairs_kernel(RotaryArgs a, int64_t unit0, int64_t units,
-                                                                          int slots, int shares) {
-  const int64_t u = unit0 + (int64_t)blockIdx.x * kRotaryThreads + threadIdx.x;
-  if (u >= units) return;
-  const int slot = (int)(u % slots);
-  const int64_t rest = u / slots;
-  const int share = (int)(rest % shares);
-  const int64_t row = rest / shares;
-  const int half = a.rotary / 2;
-  const bool turn = slot < half;
-  const int d0 = turn ? (INTERLEAVED ? 2 * slot : slot) : a.rotary + (slot - half);
-  const int d1 = INTERLEAVED ? d0 + 1 : d0 + half;
-  float c = 0.0f, s = 0.0f;
-  if (turn) {
-    turn_cos_sin((uint32_t)(((uint64_t)(int64_t)a.positions[row] * a.step[slot]) >> 32), &c, &s);
-    c *= a.magnitude;
-    s *= a.inverse ? -a.magnitude : a.magnitude;
+template <typename T, int N, bool INTERLEAVED, int RB>
+hipError_t run_rows(const RotaryArgs& a, uint32_t places, uint32_t slots, hipStream_t stream) {
+  const uint32_t chunks = (places + kRotaryThreads - 1) / kRotaryThreads;
+  const uint32_t per = chunks > 1 ? 1 : std::max(1u, std::min(kRotaryThreads / places, (uint32_t)(kRotaryTable / (RB * (a.rotary / 2)))));
+  // (launches of at most 2^22 workgroups)
+  const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 22) / chunks) * RB * per;
+  for (int64_t first = 0; first < a.rows; first += step) {
+    const int64_t rows = std::min(step, a.rows - first);
+    const unsigned blocks = (unsigned)((rows + RB * per - 1) / (RB * per) * chunks);
+    sfe_rotary_kernel<T, N, INTERLEAVED, RB><<<dim3(blocks), dim3(kRotaryThreads), 0, stream>>>(a, first, places, slots, chunks, per);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  const int heads = a.t[0].heads + a.t[1].heads;
-  for (int h = share; h < heads; h += shares) {
-    const bool second = h >= a.t[0].heads;
-    const RotaryTensor& t = a.t[second];
-    const int hh = second ? h - a.t[0].heads : h;
-    const T* x = reinterpret_cast<const T*>(t.x) + row * t.x_row + hh * t.x_head;
-    T* y = reinterpret_cast<T*>(t.y) + row * t.y_row + hh * t.y_head;
-    if (!turn) {
-      y[d0] = x[d0];
-      continue;
-    }
-    const float e = (float)x[d0], f = (float)x[d1];
-    y[d0] = (T)__builtin_fmaf(e, c, -f * s);
-    y[d1] = (T)__builtin_fmaf(f, c, e * s);
-  }
+  return hipSuccess;
+}
+
+template <typename T, int N, bool INTERLEAVED>
+hipError_t run_units(const RotaryArgs& a, int cus, hipStream_t stream) {
+  const int pairs = INTERLEAVED && N > 1 ? N / 2 : N;
+  const uint32_t slots = (uint32_t)(a.rotary / 2 / pairs + (a.dim - a.rotary) / N);
+  const uint32_t places = slots * (uint32_t)(a.t[0].heads + a.t[1].heads);
+  // One row a thread while the machine is not full at 4 rows a thread.
+  const bool many = a.rows * places >= (int64_t)cus * 8 * kRotaryThreads * 4;
+  return many ? run_rows<T, N, INTERLEAVED, 4>(a, places, slots, stream) : run_rows<T, N, INTERLEAVED, 1>(a, places, slots, stream);
 }
 
 template <typename T, bool INTERLEAVED>
 hipError_t run(const RotaryArgs& a, int cus, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
-  bool vec = a.rotary % (2 * N) == 0 && a.dim % N == 0;
+  bool vec = a.rotary % (INTERLEAVED ? N : 2 * N) == 0 && a.dim % N == 0;
   for (const RotaryTensor& t : a.t)
     if (t.heads)
       vec = vec && (reinterpret_cast<uintptr_t>(t.x) | reinterpret_cast<uintptr_t>(t.y)) % 16 == 0 &&
             (t.x_row | t.x_head | t.y_row | t.y_head) % N == 0;
-  const int step = vec ? N : 1;
-  const int slots = a.rotary / 2 / step + (a.dim - a.rotary) / step;
-  const int heads = a.t[0].heads + a.t[1].heads;
-  // Heads of a row are shared out among threads until about 8 waves a CU are there.
-  const int64_t want = (int64_t)cus * 8 * 64, have = a.rows * slots;
-  const int shares = (int)(have >= want ? 1 : (heads < (want + have - 1) / have ? heads : (want + have - 1) / have));
-  const int64_t units = have * shares;
-  return for_launches((units + kRotaryThreads - 1) / kRotaryThreads, kRotaryThreads, [&](int64_t first, unsigned blocks) {
-    const int64_t unit0 = first * kRotaryThreads;
-    if (vec)
-      sfe_rotary_kernel<T, N, INTERLEAVED><<<dim3(blocks), dim3(kRotaryThreads), 0, stream>>>(a, unit0, units, slots, shares);
-    else
-      sfe_rotary_pairs_kernel<T, INTERLEAVED><<<dim3(blocks), dim3(kRotaryThreads), 0, stream>>>(a, unit0, units, slots, shares);
-    return hipGetLastError();
-  });
+  return vec ? run_units<T, N, INTERLEAVED>(a, cus, stream) : run_units<T, 1, INTERLEAVED>(a, cus, stream);
 }
 
 template <typename T>

@@ -269,7 +269,7 @@ def selected(logits, scores, finished, end):
     parents = torch.where(found, at // V, place[:, :at.shape[1]])
     tokens = torch.where(found, at % V, -1)
     ended = torch.gather(finished.cpu(), 1, parents) if finished is not None else torch.zeros_like(found)
-    return value, parents.int(), tokens.int(), ended | (tokens == end)
+    return value, parents.int(), tokens.int(), ended | (found & (tokens == end))
 
 
 def beam_check(ops, logits, scores, finished=None, end=-1):

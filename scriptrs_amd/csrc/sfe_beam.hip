@@ -29,7 +29,6 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kEach = 32;                // logits of a thread and step
 constexpr int kStep = kThreads * kEach;  // logits of a workgroup and step
 constexpr int kSmall = 64 * kEach;       // logits of a wave
-constexpr int kList = 512;               // candidates held at once
 constexpr float kLog2e = 1.44269504f;
 
 // Scratch: [row][span] of (maximum, sum), then of beams (logit, token).
@@ -85,151 +84,191 @@ __device__ __forceinline__ float wave_nth(float x, int n) {
   return top;
 }
 
-// The best `n` candidates (value, index) that a workgroup has seen, in LDS, best
-// first.  A candidate is entered if it is not below `bound`, which is never above the
-// n-th best: after the first values few are.
+// The best candidates (value, index) that a wave has seen: up to 64 in its part of
+// LDS, in no order.  A candidate is entered if it comes before (bx, bi), which is
+// never before the n-th best of all that the wave has seen; when the list is full it is cut to
+// its n best, and the n-th of them is the new bound.  So ties, however many, cost
+// cuts and lose nothing, and no wave waits for another.
+constexpr int kListed = 64;
+struct Lists {
+  float x[16][kListed];
+  int i[16][kListed];
+  int n[16];
+};
 struct Best {
-  float bound;
-  int count, kept, cur;
-  float wx[16];
-  int wi[16];
-  float cx[kList], kx[2][kMaxBeams];
-  int ci[kList], ki[2][kMaxBeams];
+  float bx;
+  int bi, n;  // n: entries (the same in every lane)
 };
 
-__device__ __forceinline__ void best_clear(Best& b) {
-  if (threadIdx.x == 0) {
-    b.bound = -INFINITY;
-    b.count = b.kept = b.cur = 0;
+__device__ __forceinline__ Best best_none() { return Best{-INFINITY, INT32_MAX, 0}; }
+
+__device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ void best_cut(Best& b, int keep, float* lx, int* li) {
+  const int lane = (int)(threadIdx.x & 63);
+  lds_done();
+  float x = -INFINITY;
+  int i = INT32_MAX;
+  if (lane < b.n) {
+    x = lx[lane];
+    i = li[lane];
   }
-  __syncthreads();
+  int rank = 0;
+  for (int d = 0; d < b.n; ++d) {
+    const float y = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), d));
+    rank += before(y, __builtin_amdgcn_readlane(i, d), x, i);
+  }
+  if (lane < b.n && rank < keep) {
+    lx[rank] = x;
+    li[rank] = i;
+  }
+  lds_done();
+  if (b.n >= keep) {
+    b.n = keep;
+    b.bx = lx[keep - 1];
+    b.bi = li[keep - 1];
+  }
 }
 
-// Enters a thread's values x[0..E) of indexes index(k); top: their maximum.  Called by
-// the whole workgroup; first: a first bound is taken from the thread maxima.
+// Enters a lane's values x[0..E) of indexes index(k); top: their maximum.
 template <int E, class F>
-__device__ __forceinline__ void best_add(Best& b, int n, const float (&x)[E], float top, bool first, F&& index) {
-  const int t = (int)threadIdx.x, waves = (int)blockDim.x / 64;
-  if (first) {
-    const float w = wave_nth(top, n);
-    if ((t & 63) == 0) b.wx[t >> 6] = w;
-    __syncthreads();
-    float m = b.bound;
-    for (int i = 0; i < waves; ++i) m = fmaxf(m, b.wx[i]);
-    __syncthreads();
-    if (t == 0) b.bound = m;
-    __syncthreads();
+__device__ __forceinline__ void best_add(Best& b, int keep, float* lx, int* li, const float (&x)[E], float top, F&& index) {
+  if (b.n == 0 && E > 1) {  // a first bound: the keep-th largest of the lanes' maxima
+    const float first = wave_nth(top, keep);
+    if (first > b.bx) b.bx = first;  // (b.bi stays: values equal to it are entered)
   }
-  const float bound = b.bound;
-  if (top >= bound && top > -INFINITY) {
+  if (__ballot(top >= b.bx) == 0) return;
+  // each lane's values that may come in, one a turn (a copy of the code below for each of
+  // the E values would not fit the instruction cache)
+  uint32_t may = 0;
 #pragma unroll
-    for (int k = 0; k < E; ++k)
-      if (x[k] >= bound && x[k] > -INFINITY) {
-        const int c = atomicAdd(&b.count, 1);
-        if (c < kList) {
-          b.cx[c] = x[k];
-          b.ci[c] = index(k);
-        }
-      }
-  }
-  __syncthreads();
-  const int add = b.count, have = b.kept, cur = b.cur;
-  __syncthreads();
-  if (add == 0) return;
-  const float* ox = b.kx[cur];
-  const int* oi = b.ki[cur];
-  float* nx = b.kx[cur ^ 1];
-  int* ni = b.ki[cur ^ 1];
-  int found = 0;
-  if (add <= kList) {
-    // by rank: the list's order does not matter
-    for (int c = t; c < add + have; c += (int)blockDim.x) {
-      const float y = c < add ? b.cx[c] : ox[c - add];
-      const int i = c < add ? b.ci[c] : oi[c - add];
-      int rank = 0;
-      for (int d = 0; d < add; ++d) rank += before(b.cx[d], b.ci[d], y, i);
-      for (int d = 0; d < have; ++d) rank += before(ox[d], oi[d], y, i);
-      if (rank < n) {
-        nx[rank] = y;
-        ni[rank] = i;
-      }
-    }
-    found = min(n, add + have);
-  } else {
-    // many equal values: the best after the last one taken, n times
-    float lastx = INFINITY;
-    int lasti = -1;
-    for (; found < n; ++found) {
-      float y = -INFINITY;
-      int i = INT32_MAX;
-      if (t < have && before(lastx, lasti, ox[t], oi[t])) {
-        y = ox[t];
-        i = oi[t];
-      }
+  for (int k = 0; k < E; ++k) may |= x[k] >= b.bx && x[k] > -INFINITY ? 1u << k : 0u;
+  while (__ballot(may != 0)) {
+    const int k = may ? __builtin_ctz(may) : 0;
+    float v = x[0];
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        const int j = index(k);
-        if (x[k] > -INFINITY && before(lastx, lasti, x[k], j) && before(x[k], j, y, i)) {
-          y = x[k];
-          i = j;
-        }
+    for (int j = 1; j < E; ++j) v = k == j ? x[j] : v;
+    const int i = index(k);
+    bool c = may && before(v, i, b.bx, b.bi);
+    may &= may - 1;
+    for (uint64_t mask = __ballot(c); mask; mask = __ballot(c)) {
+      const int room = kListed - b.n;
+      const int place = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+      if (c && place < room) {
+        lx[b.n + place] = v;
+        li[b.n + place] = i;
       }
-      const float wy = wave_max(y);
-      int wi = y == wy ? i : INT32_MAX;
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1) wi = min(wi, __shfl_xor(wi, d));
-      if ((t & 63) == 0) {
-        b.wx[t >> 6] = wy;
-        b.wi[t >> 6] = wi;
-      }
-      __syncthreads();
-      lastx = b.wx[0];
-      lasti = b.wi[0];
-      for (int w = 1; w < waves; ++w)
-        if (before(b.wx[w], b.wi[w], lastx, lasti)) {
-          lastx = b.wx[w];
-          lasti = b.wi[w];
-        }
-      __syncthreads();
-      if (lasti == INT32_MAX) break;
-      if (t == 0) {
-        nx[found] = lastx;
-        ni[found] = lasti;
+      c = c && place >= room;
+      b.n += min(__builtin_popcountll(mask), room);
+      if (b.n == kListed) {
+        best_cut(b, keep, lx, li);
+        c = c && before(v, i, b.bx, b.bi);
       }
     }
   }
-  __syncthreads();
-  if (t == 0) {
-    b.count = 0;
-    b.kept = found;
-    b.cur = cur ^ 1;
-    if (found == n) b.bound = fmaxf(b.bound, nx[n - 1]);
-  }
-  __syncthreads();
 }
 
-// 16 bytes at an element's own alignment: which thread adds which logit does not
-// depend on where a row starts (a vocabulary of odd size puts rows on every alignment).
+// The workgroup's best of its waves' lists: entry `rank` of the result is given to
+// give(rank, value, index); returns how many there are (at most keep).  Barriers on
+// both sides of the lists.
+template <class F>
+__device__ __forceinline__ int best_join(Best& b, Lists& l, int keep, F&& give) {
+  const int waves = (int)blockDim.x / 64;
+  if (b.n > keep) best_cut(b, keep, l.x[threadIdx.x >> 6], l.i[threadIdx.x >> 6]);
+  if ((threadIdx.x & 63) == 0) l.n[threadIdx.x >> 6] = b.n;
+  __syncthreads();
+  int total = 0;
+  for (int w = 0; w < waves; ++w) total += l.n[w];
+  // a thread takes entry t % 64 of wave t / 64
+  const int w = (int)(threadIdx.x >> 6), e = (int)(threadIdx.x & 63);
+  if (e < l.n[w]) {
+    const float x = l.x[w][e];
+    const int i = l.i[w][e];
+    int rank = 0;
+    for (int v = 0; v < waves; ++v)
+      for (int d = 0; d < l.n[v]; ++d) rank += before(l.x[v][d], l.i[v][d], x, i);
+    if (rank < keep) give(rank, x, i);
+  }
+  return min(keep, total);
+}
+
+// 16 bytes of a row, read at an element's own alignment: which thread adds which logit
+// does not depend on where a row starts (a vocabulary of odd size puts rows on every
+// alignment).
+struct __attribute__((packed, aligned(2))) Raw {
+  U4 v;
+};
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Vec {
-  T v[16 / sizeof(T)];
+struct Bits;
+template <>
+struct Bits<float> {
+  static __device__ float at(const U4& v, int i) { return __uint_as_float(v[i]); }
+};
+template <>
+struct Bits<__bf16> {
+  static __device__ float at(const U4& v, int i) {
+    return __uint_as_float(i % 2 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16);
+  }
+};
+template <>
+struct Bits<_Float16> {
+  static __device__ float at(const U4& v, int i) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(v[i / 2] >> (i % 2 * 16)));
+  }
 };
 
-// Vector j of thread t: the elements first + (j * THREADS + t) * N.. of a row, -inf past
-// its end.
+// Vector j of thread t of a row holds the elements from first + (j * THREADS + t) * N on;
+// one that would pass the row's end is moved back to end with it, and its elements that
+// belong to the vector before do not count.  (Rows shorter than a vector are read by the
+// element.)
+template <int N, int THREADS>
+__device__ __forceinline__ int vector_at(int first, int j, int t) { return first + (j * THREADS + t) * N; }
+template <int N>
+__device__ __forceinline__ int moved_back(int e, int vocab) { return vocab >= N ? min(e, vocab - N) : e; }
+
 template <typename T, int NV, int THREADS>
-__device__ __forceinline__ void load_row(const T* p, int first, int t, int vocab, Vec<T> (&v)[NV]) {
+__device__ __forceinline__ void load_row(const T* p, int first, int t, int vocab, U4 (&v)[NV]) {
   constexpr int N = 16 / (int)sizeof(T);
+  if (vocab >= N) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      v[j] = reinterpret_cast<const Raw*>(p + moved_back<N>(vector_at<N, THREADS>(first, j, t), vocab))->v;
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int e = first + (j * THREADS + t) * N;
-    if (e + N <= vocab) {
-      v[j] = *reinterpret_cast<const Vec<T>*>(p + e);
-    } else {
+    const int e = vector_at<N, THREADS>(first, j, t);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[j].v[i] = e + i < vocab ? p[e + i] : (T)-INFINITY;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[j][i] = e + i < vocab ? __float_as_uint((float)p[e + i]) : 0;
+      } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+        const unsigned lo = e + 2 * i < vocab ? h[e + 2 * i] : 0, hi = e + 2 * i + 1 < vocab ? h[e + 2 * i + 1] : 0;
+        v[j][i] = lo | hi << 16;
+      }
     }
   }
+}
+// The vectors as floats, -inf where they do not count.
+template <typename T, int NV, int THREADS>
+__device__ __forceinline__ void row_values(const U4 (&v)[NV], int first, int t, int vocab, float (&x)[NV * 16 / sizeof(T)]) {
+  constexpr int N = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int k = 0; k < NV * N; ++k) x[k] = Bits<T>::at(v[k / N], k % N);
+  if (first + NV * THREADS * N <= vocab) return;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int e = vector_at<N, THREADS>(first, j, t), at = moved_back<N>(e, vocab);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[j * N + i] = at + i >= e && at + i < vocab ? x[j * N + i] : -INFINITY;
+  }
+}
+// The token of value k.
+template <typename T, int THREADS>
+__device__ __forceinline__ int token_of(int k, int first, int t, int vocab) {
+  constexpr int N = 16 / (int)sizeof(T);
+  return moved_back<N>(vector_at<N, THREADS>(first, k / N, t), vocab) + k % N;
 }
 
 // Sum of exponentials of x relative to m (0 where all is -inf; NaN stays).
@@ -249,71 +288,66 @@ __device__ __forceinline__ float max_of(const float (&x)[E]) {
   return m;
 }
 
-__device__ __forceinline__ void write_beams(const BeamArgs& a, const Best& b, int stream) {
-  const int r = (int)threadIdx.x;
-  if (r >= a.beams) return;
-  const bool found = r < b.kept;
-  const int i = b.ki[b.cur][r];
+__device__ __forceinline__ void write_beam(const BeamArgs& a, int stream, int r, bool found, float x, int i) {
   const int parent = found ? i / a.vocab : r, token = found ? i - parent * a.vocab : -1;
   const int64_t o = (int64_t)stream * a.beams + r;
-  a.out_scores[o] = found ? b.kx[b.cur][r] : -INFINITY;
+  a.out_scores[o] = x;
   a.parents[o] = parent;
   a.tokens[o] = token;
   if (a.out_finished)
     a.out_finished[o] = (a.finished && a.finished[(int64_t)stream * a.beams + parent]) || (found && token == a.end);
 }
+__device__ __forceinline__ void write_beams(const BeamArgs& a, int stream, Best& b, Lists& l) {
+  const int found = best_join(b, l, a.beams, [&](int r, float x, int i) { write_beam(a, stream, r, true, x, i); });
+  const int t = (int)threadIdx.x;
+  if (t >= found && t < a.beams) write_beam(a, stream, t, false, -INFINITY, 0);
+}
 
 // ---- small vocabularies -----------------------------------------------------------------
 
-template <typename T>
+// E: logits of a lane.
+template <typename T, int E>
 __global__ __launch_bounds__(1024) void sfe_beam_small_kernel(BeamArgs a) {
-  constexpr int N = 16 / (int)sizeof(T), NV = kEach / N;
-  __shared__ Best best;
+  constexpr int NV = E * (int)sizeof(T) / 16;
+  __shared__ Lists lists;
   const int stream = (int)blockIdx.x, lane = (int)(threadIdx.x & 63), waves = (int)blockDim.x / 64;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  best_clear(best);
-  for (int w0 = 0; w0 < a.beams; w0 += waves) {
-    const int w = w0 + wave;
-    float x[kEach];
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) x[k] = -INFINITY;
-    bool over = false;
-    if (w < a.beams) {
-      const int64_t row = (int64_t)stream * a.beams + w;
-      over = a.finished && a.finished[row];
-      const float score = a.scores[row];
-      if (over) {
-        if (lane == 0) x[0] = score;
-      } else {
-        const T* p = reinterpret_cast<const T*>(a.logits) + row * a.row;
-        Vec<T> v[NV];
-        load_row<T, NV, 64>(p, 0, lane, a.vocab, v);
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) x[k] = (float)v[k / N].v[k % N];
-        const float m = wave_max(max_of(x));
-        const float logz = m + logf(wave_sum(exp_sum(x, m)));
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) x[k] = score + (x[k] - logz);
-      }
+  Best best = best_none();
+  for (int w = wave; w < a.beams; w += waves) {
+    const int64_t row = (int64_t)stream * a.beams + w;
+    const float score = a.scores[row];
+    if (a.finished && a.finished[row]) {
+      const float x[1] = {lane == 0 ? score : -INFINITY};
+      best_add(best, a.beams, lists.x[wave], lists.i[wave], x, x[0], [&](int) { return w * a.vocab + a.end; });
+      continue;
     }
-    best_add(best, a.beams, x, max_of(x), w0 == 0, [&](int k) {
-      return w * a.vocab + (over ? a.end : (k / N * 64 + lane) * N + k % N);
-    });
+    U4 v[NV];
+    load_row<T, NV, 64>(reinterpret_cast<const T*>(a.logits) + row * a.row, 0, lane, a.vocab, v);
+    float x[E];
+    row_values<T, NV, 64>(v, 0, lane, a.vocab, x);
+    const float m = wave_max(max_of(x));
+    const float logz = m + logf(wave_sum(exp_sum(x, m)));
+#pragma unroll
+    for (int k = 0; k < E; ++k) x[k] = score + (x[k] - logz);
+    best_add(best, a.beams, lists.x[wave], lists.i[wave], x, max_of(x),
+             [&](int k) { return w * a.vocab + token_of<T, 64>(k, 0, lane, a.vocab); });
   }
-  write_beams(a, best, stream);
+  write_beams(a, stream, best, lists);
 }
 
 // ---- others: spans of rows, then streams -----------------------------------------------------
 
 // One workgroup: the steps of a span, the next step's loads in flight while one is
 // worked on.  Each thread keeps the sum of exponentials relative to its own running
-// maximum.
+// maximum.  (4 workgroups a CU: with 3, which 155 registers allow, 1,024 of them
+// went in two turns, 90 us against 55 for 512 rows of 128,000 in bf16.)
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sfe_beam_rows_kernel(BeamArgs a, int spans) {
+__global__ __launch_bounds__(kThreads, 4) void sfe_beam_rows_kernel(BeamArgs a, int spans) {
   constexpr int N = 16 / (int)sizeof(T), NV = kEach / N;
-  __shared__ Best best;
+  __shared__ Lists lists;
+  __shared__ Part parts[kWaves];
   const int row = (int)(blockIdx.x / (unsigned)spans), span = (int)(blockIdx.x % (unsigned)spans);
-  const int t = (int)threadIdx.x;
+  const int t = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   Part* part = reinterpret_cast<Part*>(a.scratch);
   Cand* cand = reinterpret_cast<Cand*>(part + (int64_t)a.streams * a.beams * spans);
   const int64_t at = (int64_t)row * spans + span;
@@ -321,47 +355,45 @@ __global__ __launch_bounds__(kThreads) void sfe_beam_rows_kernel(BeamArgs a, int
   const T* p = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row;
   const int steps = (a.vocab + kStep - 1) / kStep;
   const int step0 = (int)((int64_t)steps * span / spans), step1 = (int)((int64_t)steps * (span + 1) / spans);
-  best_clear(best);
+  Best best = best_none();
   float tm = -INFINITY, sum = 0.0f;
-  Vec<T> next[NV];
+  U4 next[NV];
   if (step0 < step1) load_row<T, NV, kThreads>(p, step0 * kStep, t, a.vocab, next);
   for (int step = step0; step < step1; ++step) {
     float x[kEach];
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) x[k] = (float)next[k / N].v[k % N];
+    row_values<T, NV, kThreads>(next, step * kStep, t, a.vocab, x);
     if (step + 1 < step1) load_row<T, NV, kThreads>(p, (step + 1) * kStep, t, a.vocab, next);
     const float sm = max_of(x), m = fmaxf(tm, sm);
     sum = sum * (tm == m ? 1.0f : __builtin_amdgcn_exp2f((tm - m) * kLog2e)) + exp_sum(x, m);
     tm = m;
-    best_add(best, a.beams, x, sm, step == step0,
-             [&](int k) { return step * kStep + (k / N * kThreads + t) * N + k % N; });
+    best_add(best, a.beams, lists.x[wave], lists.i[wave], x, sm,
+             [&](int k) { return token_of<T, kThreads>(k, step * kStep, t, a.vocab); });
   }
   const float wm = wave_max(tm);
   const float ws = wave_sum(sum * (tm == wm ? 1.0f : __builtin_amdgcn_exp2f((tm - wm) * kLog2e)));
-  __shared__ Part waves[kWaves];
-  if ((t & 63) == 0) waves[t >> 6] = Part{wm, ws};
-  __syncthreads();
+  if ((t & 63) == 0) parts[wave] = Part{wm, ws};
+  const int found = best_join(best, lists, a.beams, [&](int r, float x, int i) { cand[at * a.beams + r] = Cand{x, i}; });
+  if (t >= found && t < a.beams) cand[at * a.beams + t] = Cand{-INFINITY, -1};
   if (t == 0) {
     Part r{-INFINITY, 0.0f};
-    for (int w = 0; w < kWaves; ++w) r.top = fmaxf(r.top, waves[w].top);
+    for (int w = 0; w < kWaves; ++w) r.top = fmaxf(r.top, parts[w].top);
     for (int w = 0; w < kWaves; ++w)
-      r.sum += waves[w].sum * (waves[w].top == r.top ? 1.0f : __builtin_amdgcn_exp2f((waves[w].top - r.top) * kLog2e));
+      r.sum += parts[w].sum * (parts[w].top == r.top ? 1.0f : __builtin_amdgcn_exp2f((parts[w].top - r.top) * kLog2e));
     part[at] = r;
   }
-  if (t < a.beams)
-    cand[at * a.beams + t] = t < best.kept ? Cand{best.kx[best.cur][t], best.ki[best.cur][t]} : Cand{-INFINITY, -1};
 }
 
 __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, int spans) {
-  __shared__ Best best;
+  __shared__ Lists lists;
   __shared__ float logz[kMaxBeams];
   const int b = (int)blockIdx.x, t = (int)threadIdx.x, W = a.beams;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Part* part = reinterpret_cast<const Part*>(a.scratch) + (int64_t)b * W * spans;
   const Cand* cand = reinterpret_cast<const Cand*>(reinterpret_cast<const Part*>(a.scratch) +
                                                    (int64_t)a.streams * W * spans) + (int64_t)b * W * spans * W;
   const float* scores = a.scores + (int64_t)b * W;
   const uint8_t* finished = a.finished ? a.finished + (int64_t)b * W : nullptr;
-  for (int w = t >> 6; w < W; w += kWaves) {
+  for (int w = wave; w < W; w += kWaves) {
     if (finished && finished[w]) continue;
     float top = -INFINITY, sum = 0.0f;
     for (int c = t & 63; c < spans; c += 64) top = fmaxf(top, part[w * spans + c].top);
@@ -373,10 +405,11 @@ __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, 
     sum = wave_sum(sum);
     if ((t & 63) == 0) logz[w] = top + logf(sum);
   }
-  best_clear(best);
+  __syncthreads();
+  Best best = best_none();
   const int each = spans * W;  // candidates of a row
-  for (int e0 = 0; e0 < W * each; e0 += kThreads) {
-    const int e = e0 + t;
+  for (int e0 = 64 * wave; e0 < W * each; e0 += kThreads) {
+    const int e = e0 + (t & 63);
     float x[1] = {-INFINITY};
     int i = 0;
     if (e < W * each) {
@@ -390,9 +423,9 @@ __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, 
         if (c.t >= 0) x[0] = scores[w] + (c.x - logz[w]);
       }
     }
-    best_add(best, W, x, x[0], e0 == 0, [&](int) { return i; });
+    best_add(best, W, lists.x[wave], lists.i[wave], x, x[0], [&](int) { return i; });
   }
-  write_beams(a, best, b);
+  write_beams(a, b, best, lists);
 }
 
 // ---- states ------------------------------------------------------------------------------
@@ -484,7 +517,13 @@ bool small(int vocab) { return vocab <= kSmall; }
 template <typename T>
 hipError_t select(const BeamArgs& a, int cus, hipStream_t stream) {
   if (small(a.vocab)) {
-    sfe_beam_small_kernel<T><<<dim3((unsigned)a.streams), dim3(64 * std::min(a.beams, 16)), 0, stream>>>(a);
+    const dim3 grid((unsigned)a.streams), block(64 * std::min(a.beams, 16));
+    if (a.vocab <= 64 * 16)
+      sfe_beam_small_kernel<T, 16><<<grid, block, 0, stream>>>(a);
+    else if (a.vocab <= 64 * 24)
+      sfe_beam_small_kernel<T, 24><<<grid, block, 0, stream>>>(a);
+    else
+      sfe_beam_small_kernel<T, kEach><<<grid, block, 0, stream>>>(a);
     return hipGetLastError();
   }
   const int rows = a.streams * a.beams, spans = spans_of(rows, a.vocab, cus);

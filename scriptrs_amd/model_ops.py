@@ -24,31 +24,40 @@ MAX_BEAMS = 32
 
 
 def _dtype_of(t, what: str) -> int:
-    import torch
-    code = {torch.float32: _lib.SFE_F32, torch.bfloat16: _lib.SFE_BF16, torch.float16: _lib.SFE_F16}.get(t.dtype)
+    code = _DTYPES.get(t.dtype)
     if code is None:
         raise InvalidModelOutput(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
     return code
 
 
-def _on_device(device: int, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not getattr(t, "is_cuda", False):
-            raise InvalidModelOutput(f"{name} must be a device tensor")
-        if t.device.index != device:
-            raise InvalidModelOutput(f"{name} is on {t.device}, the operators are on cuda:{device}")
+class _Dtypes(dict):
+    """torch dtype -> sfe_dtype, filled on first use (torch is imported lazily)."""
+
+    def get(self, dtype):
+        if not self:
+            import torch
+            self.update({torch.float32: _lib.SFE_F32, torch.bfloat16: _lib.SFE_BF16, torch.float16: _lib.SFE_F16})
+        return super().get(dtype)
 
 
-def _heads(t, name: str) -> SfeHeads:
-    """A [rows, heads, channels] tensor, channels contiguous."""
-    if t.dim() != 3:
-        raise InvalidModelOutput(f"{name} must be [rows, heads, channels], got {list(t.shape)}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+_DTYPES = _Dtypes()
+
+
+def _wrong_device(name: str, t, device: int):
+    if not getattr(t, "is_cuda", False):
+        raise InvalidModelOutput(f"{name} must be a device tensor")
+    raise InvalidModelOutput(f"{name} is on {t.device}, the operators are on cuda:{device}")
+
+
+def _heads(t, name: str, shape, out):
+    """Writes a [rows, heads, channels] tensor, channels contiguous, into an sfe_heads."""
+    rows, heads, dim = shape
+    row, head, channel = t.stride()
+    if channel != 1 and dim > 1:
         raise InvalidModelOutput(f"{name}: channels must be contiguous")
-    return SfeHeads(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2],
-                    t.stride(1) if t.shape[1] > 1 else t.shape[2])
+    out.data = t.data_ptr()
+    out.row_stride = row if rows > 1 else heads * dim
+    out.head_stride = head if heads > 1 else dim
 
 
 def _same(t, like, name: str) -> None:
@@ -57,14 +66,10 @@ def _same(t, like, name: str) -> None:
 
 
 def _contiguous(t, name: str, dtype, shape) -> int:
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise InvalidModelOutput(f"{name} must be a contiguous {dtype} tensor of {list(shape)}, got {t.dtype} of "
                                  f"{list(t.shape)}")
     return t.data_ptr()
-
-
-def _ref(x):
-    return ctypes.byref(x) if x is not None else None
 
 
 class RotaryTable:
@@ -91,6 +96,7 @@ class RotaryTable:
                                           self.SCALINGS[scaling], float(factor), float(original_length), float(low),
                                           float(high), float(magnitude)))
         self.rotary_dim, self.layout = int(rotary_dim), layout
+        self.p = ctypes.byref(self.c)
 
 
 class AttentionPlan:
@@ -101,6 +107,7 @@ class AttentionPlan:
         self._ops, self._handle = ops, handle
         self.total_q, self.total_k = total_q, total_k
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.scale = 1.0 / math.sqrt(head_dim)
 
     def close(self) -> None:
         if self._handle and self._ops._fe._ctx:  # (a closed context has freed it)
@@ -121,9 +128,22 @@ class ModelOps:
     ``sfe_ctx`` or shares ``extractor``'s; calls on it are ordered after each other)."""
 
     def __init__(self, device: int = 0, extractor: ParakeetFeatureExtractor | None = None):
+        import torch
         self._own = extractor is None
         self._fe = extractor or ParakeetFeatureExtractor(device=device)
         self.device = self._fe.device
+        self._lib = _lib.lib()
+        self._stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        # argument structs, filled for each call (calls come from one host thread)
+        self._h = [SfeHeads() for _ in range(4)]
+        self._hp = [ctypes.byref(h) for h in self._h]
+        self._residual = SfeResidual()
+        self._residual_p = ctypes.byref(self._residual)
+
+    def _stream(self, stream) -> int | None:
+        if stream is None and self._stream_of is not None:
+            return self._stream_of(self.device)
+        return _stream_handle(stream)
 
     def close(self) -> None:
         if self._own:
@@ -150,36 +170,49 @@ class ModelOps:
         ``q`` [queries, heads, head_dim], ``k`` and ``v`` [keys, kv_heads, head_dim] in
         bfloat16 or float16 (views of a joint projection will do), ``key_mask``
         [keys] bool, False hides a key.  Queries that see no key give zeros."""
-        import torch
-        _on_device(self.device, q=q, k=k, v=v, key_mask=key_mask, out=out)
-        if plan._handle is None:
+        handle = plan._handle
+        if handle is None:
             raise InvalidModelOutput("the plan is closed")
         if plan._ops is not self:
             raise InvalidModelOutput("the plan belongs to another ModelOps")
-        if q.dtype not in (torch.bfloat16, torch.float16):
-            raise InvalidModelOutput(f"q must be bfloat16 or float16, got {q.dtype}")
-        for name, t, n, h in (("q", q, plan.total_q, plan.heads), ("k", k, plan.total_k, plan.kv_heads),
-                              ("v", v, plan.total_k, plan.kv_heads)):
-            if t.dtype != q.dtype or t.dim() != 3 or t.shape[0] < n or t.shape[1:] != (h, plan.head_dim):
-                raise InvalidModelOutput(f"{name} must be {q.dtype} of [{n}, {h}, {plan.head_dim}], got {t.dtype} of "
-                                         f"{list(t.shape)}")
+        dtype, device = q.dtype, self.device
+        code = _dtype_of(q, "q")
+        if code == _lib.SFE_F32:
+            raise InvalidModelOutput(f"q must be bfloat16 or float16, got {dtype}")
+        hq, hk, hv, ho = self._h
+        tail_q, tail_k = (plan.heads, plan.head_dim), (plan.kv_heads, plan.head_dim)
+        for name, t, n, tail, h in (("q", q, plan.total_q, tail_q, hq), ("k", k, plan.total_k, tail_k, hk),
+                                    ("v", v, plan.total_k, tail_k, hv)):
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
+            shape = t.shape
+            if t.dtype != dtype or len(shape) != 3 or shape[0] < n or shape[1:] != tail:
+                raise InvalidModelOutput(f"{name} must be {dtype} of [{n}, {tail[0]}, {tail[1]}], got {t.dtype} of "
+                                         f"{list(shape)}")
+            _heads(t, name, shape, h)
         mask = None
         if key_mask is not None:
+            import torch
+            if key_mask.get_device() != device:
+                _wrong_device("key_mask", key_mask, device)
             if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 1 or \
                     key_mask.shape[0] < plan.total_k or not key_mask.is_contiguous():
                 raise InvalidModelOutput(f"key_mask must be a contiguous bool tensor of [{plan.total_k}]")
             mask = key_mask.data_ptr()
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
         else:
             _same(out, q, "out")
+            if out.get_device() != device:
+                _wrong_device("out", out, device)
         if q.shape[0] > plan.total_q:
             out[plan.total_q:].zero_()
-        qh, kh, vh, oh = (_heads(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
-        _check(_lib.lib().sfe_attention(plan._handle, _dtype_of(q, "q"), ctypes.byref(qh), ctypes.byref(kh),
-                                        ctypes.byref(vh), mask,
-                                        1.0 / math.sqrt(plan.head_dim) if scale is None else float(scale),
-                                        ctypes.byref(oh), _stream_handle(stream)))
+        _heads(out, "out", q.shape, ho)
+        pq, pk, pv, po = self._hp
+        rc = self._lib.sfe_attention(handle, code, pq, pk, pv, mask, plan.scale if scale is None else scale, po,
+                                     self._stream(stream))
+        if rc:
+            _check(rc)
         return out
 
     # -- rotary positions ----------------------------------------------------------
@@ -188,20 +221,35 @@ class ModelOps:
         """``q`` (and ``k``) [rows, heads, head_dim] turned by ``positions``
         [rows] int32; returns ``(q, k)`` (k None without one).  ``inverse`` turns back."""
         import torch
-        _on_device(self.device, positions=positions, q=q, k=k)
-        rows, dim = q.shape[0], q.shape[-1]
+        device, code, shape = self.device, _dtype_of(q, "q"), q.shape
+        if len(shape) != 3:
+            raise InvalidModelOutput(f"q must be [rows, heads, channels], got {list(shape)}")
+        rows, heads, dim = shape
+        for name, t in (("positions", positions), ("q", q)):
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
         pos = _contiguous(positions, "positions", torch.int32, (rows,))
-        code = _dtype_of(q, "q")
-        if k is not None and (k.dtype != q.dtype or k.dim() != 3 or k.shape[0] != rows or k.shape[2] != dim):
-            raise InvalidModelOutput(f"k must be {q.dtype} of [{rows}, heads, {dim}], got {k.dtype} of {list(k.shape)}")
-        qo = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else k if inplace else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        qh, qoh = _heads(q, "q"), _heads(qo, "q")
-        kh, koh = (None, None) if k is None else (_heads(k, "k"), _heads(ko, "k"))
-        _check(_lib.lib().sfe_rotary(self._fe._handle(), ctypes.byref(table.c), 1 if inverse else 0, code, pos, rows,
-                                     dim, q.shape[1], ctypes.byref(qh), ctypes.byref(qoh),
-                                     0 if k is None else k.shape[1], _ref(kh), _ref(koh), _stream_handle(stream)))
-        return qo, ko
+        hq, hqo, hk, hko = self._h
+        _heads(q, "q", shape, hq)
+        q_out = q if inplace else q.new_empty(shape)
+        _heads(q_out, "q", shape, hqo)
+        k_out, kv_heads = None, 0
+        if k is not None:
+            if k.get_device() != device:
+                _wrong_device("k", k, device)
+            shape = k.shape
+            if k.dtype != q.dtype or len(shape) != 3 or shape[0] != rows or shape[2] != dim:
+                raise InvalidModelOutput(f"k must be {q.dtype} of [{rows}, heads, {dim}], got {k.dtype} of {list(shape)}")
+            kv_heads = shape[1]
+            _heads(k, "k", shape, hk)
+            k_out = k if inplace else k.new_empty(shape)
+            _heads(k_out, "k", shape, hko)
+        pq, pqo, pk, pko = self._hp
+        rc = self._lib.sfe_rotary(self._fe._handle(), table.p, 1 if inverse else 0, code, pos, rows, dim, heads, pq, pqo,
+                                  kv_heads, pk, pko, self._stream(stream))
+        if rc:
+            _check(rc)
+        return q_out, k_out
 
     # -- norms around a block ---------------------------------------------------------
     _NORMS = {None: 0, "layer": 1, "rms": 2}
@@ -216,48 +264,64 @@ class ModelOps:
         "layer" or "rms" with float32 weights (and biases) [width].  Returns
         ``(x, norm)``; norm is None without ``pre``.  ``out`` may be ``residual``
         and ``norm_out`` may be ``block``."""
-        import torch
-        _on_device(self.device, residual=residual, block=block, gate=gate, post_weight=post_weight, post_bias=post_bias,
-                   pre_weight=pre_weight, pre_bias=pre_bias, out=out, norm_out=norm_out)
         if post not in self._NORMS or pre not in self._NORMS:
             raise InvalidModelOutput("norms are None, 'layer' or 'rms'")
-        if gate_activation not in (None, "sigmoid"):
+        if gate_activation is not None and gate_activation != "sigmoid":
             raise InvalidModelOutput(f"unknown gate activation {gate_activation!r}")
-        if residual.dim() != 2 or block.shape != residual.shape:
-            raise InvalidModelOutput(f"residual and block must be [rows, width], got {list(residual.shape)} and "
+        device, shape = self.device, residual.shape
+        if len(shape) != 2 or block.shape != shape:
+            raise InvalidModelOutput(f"residual and block must be [rows, width], got {list(shape)} and "
                                      f"{list(block.shape)}")
-        rows, width = residual.shape
-        a = SfeResidual()
+        rows, width = shape
+        a = self._residual
         a.stream_dtype, a.block_dtype = _dtype_of(residual, "residual"), _dtype_of(block, "block")
         a.rows, a.width, a.post, a.pre = rows, width, self._NORMS[post], self._NORMS[pre]
-        a.gate_sigmoid, a.scale, a.eps = int(gate_activation == "sigmoid"), float(scale), float(eps)
+        a.gate_sigmoid, a.scale, a.eps = 0 if gate_activation is None else 1, scale, eps
 
-        def put(name, t):
-            if t.shape[1] > 1 and t.stride(1) != 1:
+        def rows_of(name, t):
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
+            row, channel = t.stride()
+            if channel != 1 and width > 1:
                 raise InvalidModelOutput(f"{name}: channels must be contiguous")
-            setattr(a, name, t.data_ptr())
-            setattr(a, name + "_row", t.stride(0) if rows > 1 else width)
-        put("residual", residual)
-        put("block", block)
+            return t.data_ptr(), row if rows > 1 else width
+        a.residual, a.residual_row = rows_of("residual", residual)
+        a.block, a.block_row = rows_of("block", block)
+        a.gate = None
         if gate is not None:
-            if gate.dtype != block.dtype or gate.shape not in ((width,), residual.shape):
+            if gate.dtype != block.dtype or gate.shape != (width,) and gate.shape != shape:
                 raise InvalidModelOutput(f"gate must be {block.dtype} of [{width}] or [{rows}, {width}], got {gate.dtype} "
                                          f"of {list(gate.shape)}")
-            put("gate", gate.expand(rows, width) if gate.dim() == 1 else gate)
-        for name, w in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
-                        ("pre_bias", pre_bias)):
-            if w is not None:
-                setattr(a, name, _contiguous(w, name, torch.float32, (width,)))
-        x = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device) if out is None else out
-        _same(x, residual, "out")
-        put("residual_out", x)
-        z = None
-        if pre is not None:
-            z = torch.empty(block.shape, dtype=block.dtype, device=block.device) if norm_out is None else norm_out
-            _same(z, block, "norm_out")
-            put("norm_out", z)
-        _check(_lib.lib().sfe_residual_norm(self._fe._handle(), ctypes.byref(a), _stream_handle(stream)))
-        return x, z
+            a.gate, a.gate_row = rows_of("gate", gate if gate.dim() == 2 else gate.expand(rows, width))
+        a.post_weight = None if post_weight is None else self._weight("post_weight", post_weight, width)
+        a.post_bias = None if post_bias is None else self._weight("post_bias", post_bias, width)
+        a.pre_weight = None if pre_weight is None else self._weight("pre_weight", pre_weight, width)
+        a.pre_bias = None if pre_bias is None else self._weight("pre_bias", pre_bias, width)
+        if out is None:
+            out = residual.new_empty(shape)
+        else:
+            _same(out, residual, "out")
+        a.residual_out, a.residual_out_row = rows_of("out", out)
+        if pre is None:
+            norm_out = a.norm_out = None
+        else:
+            if norm_out is None:
+                norm_out = block.new_empty(shape)
+            else:
+                _same(norm_out, block, "norm_out")
+            a.norm_out, a.norm_out_row = rows_of("norm_out", norm_out)
+        rc = self._lib.sfe_residual_norm(self._fe._handle(), self._residual_p, self._stream(stream))
+        if rc:
+            _check(rc)
+        return out, norm_out
+
+    def _weight(self, name: str, w, width: int) -> int:
+        if w.get_device() != self.device:
+            _wrong_device(name, w, self.device)
+        if _dtype_of(w, name) != _lib.SFE_F32 or w.shape != (width,) or not w.is_contiguous():
+            raise InvalidModelOutput(f"{name} must be a contiguous float32 tensor of [{width}], got {w.dtype} of "
+                                     f"{list(w.shape)}")
+        return w.data_ptr()
 
     # -- beam search --------------------------------------------------------------------
     def beam_select(self, logits, scores, finished=None, end_token: int = -1, stream=None):
@@ -267,26 +331,31 @@ class ModelOps:
         finished)`` of [streams, beams] (float32, int32, int32, bool); ties go to
         the lowest (beam, token), a place without a candidate has score -inf and token -1."""
         import torch
-        _on_device(self.device, logits=logits, scores=scores, finished=finished)
-        if scores.dim() != 2:
-            raise InvalidModelOutput(f"scores must be [streams, beams], got {list(scores.shape)}")
-        streams, beams = scores.shape
-        if logits.dim() != 2 or logits.shape[0] != streams * beams or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        device, shape = self.device, scores.shape
+        if len(shape) != 2:
+            raise InvalidModelOutput(f"scores must be [streams, beams], got {list(shape)}")
+        streams, beams = shape
+        if logits.dim() != 2 or logits.shape[0] != streams * beams or (logits.stride(1) != 1 and logits.shape[1] > 1):
             raise InvalidModelOutput(f"logits must be [{streams * beams}, vocab] with contiguous rows, got "
                                      f"{list(logits.shape)}")
+        for name, t in (("logits", logits), ("scores", scores)):
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
         code, vocab = _dtype_of(logits, "logits"), logits.shape[1]
-        sp = _contiguous(scores, "scores", torch.float32, (streams, beams))
-        fp = None
+        sp, fp = _contiguous(scores, "scores", torch.float32, shape), None
         if finished is not None:
-            fp = _contiguous(finished, "finished", torch.bool, (streams, beams))
-        new = torch.empty_like(scores)
-        picked = torch.empty((2, streams, beams), dtype=torch.int32, device=scores.device)
-        ended = torch.empty((streams, beams), dtype=torch.bool, device=scores.device)
-        _check(_lib.lib().sfe_beam_select(self._fe._handle(), code, logits.data_ptr(),
-                                          logits.stride(0) if logits.shape[0] > 1 else vocab, streams, beams, vocab, sp,
-                                          fp, int(end_token), new.data_ptr(), picked[0].data_ptr(),
-                                          picked[1].data_ptr(), ended.data_ptr(), _stream_handle(stream)))
-        return new, picked[0], picked[1], ended
+            if finished.get_device() != device:
+                _wrong_device("finished", finished, device)
+            fp = _contiguous(finished, "finished", torch.bool, shape)
+        new = scores.new_empty(shape)
+        parents, tokens = torch.empty((2, streams, beams), dtype=torch.int32, device=scores.device).unbind(0)
+        ended = torch.empty(shape, dtype=torch.bool, device=scores.device)
+        rc = self._lib.sfe_beam_select(self._fe._handle(), code, logits.data_ptr(), logits.stride(0), streams, beams,
+                                       vocab, sp, fp, end_token, new.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                                       ended.data_ptr(), self._stream(stream))
+        if rc:
+            _check(rc)
+        return new, parents, tokens, ended
 
     def beam_reorder(self, parents, states, dim: int = 0, out=None, stream=None):
         """``states`` (contiguous device tensors whose dimension ``dim`` is streams *
@@ -298,22 +367,29 @@ class ModelOps:
         out = [torch.empty_like(s) for s in states] if out is None else list(out)
         if len(out) != len(states):
             raise InvalidModelOutput("out must have a tensor for each state")
-        _on_device(self.device, parents=parents, **{f"state {i}": s for i, s in enumerate(states)},
-                   **{f"out {i}": s for i, s in enumerate(out)})
-        if parents.dim() != 2:
-            raise InvalidModelOutput(f"parents must be [streams, beams], got {list(parents.shape)}")
-        streams, beams = parents.shape
-        pp = _contiguous(parents, "parents", torch.int32, (streams, beams))
+        if parents.get_device() != self.device:
+            _wrong_device("parents", parents, self.device)
+        shape = parents.shape
+        if len(shape) != 2:
+            raise InvalidModelOutput(f"parents must be [streams, beams], got {list(shape)}")
+        streams, beams = shape
+        pp = _contiguous(parents, "parents", torch.int32, shape)
         table = (SfeBeamState * max(1, len(states)))()
         for i, (s, o) in enumerate(zip(states, out)):
-            if not s.is_contiguous() or s.dim() <= dim or s.shape[dim] != streams * beams:
+            for t in (s, o):
+                if t.get_device() != self.device:
+                    _wrong_device(f"state {i}", t, self.device)
+            full = s.shape
+            if not s.is_contiguous() or len(full) <= dim or full[dim] != streams * beams:
                 raise InvalidModelOutput(f"state {i} must be contiguous with {streams * beams} beams in dimension {dim}, "
-                                         f"got {list(s.shape)}")
+                                         f"got {list(full)}")
             _same(o, s, f"out {i}")
             if not o.is_contiguous():
                 raise InvalidModelOutput(f"out {i} must be contiguous")
-            table[i] = SfeBeamState(s.data_ptr(), o.data_ptr(), math.prod(s.shape[:dim]),
-                                    math.prod(s.shape[dim + 1:]) * s.element_size())
-        _check(_lib.lib().sfe_beam_reorder(self._fe._handle(), pp, streams, beams, table, len(states),
-                                           _stream_handle(stream)))
+            row = table[i]
+            row.in_, row.out = s.data_ptr(), o.data_ptr()
+            row.outer, row.inner_bytes = math.prod(full[:dim]), math.prod(full[dim + 1:]) * s.element_size()
+        rc = self._lib.sfe_beam_reorder(self._fe._handle(), pp, streams, beams, table, len(states), self._stream(stream))
+        if rc:
+            _check(rc)
         return out

@@ -28,6 +28,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "sfe_ops.hpp"
 
@@ -177,6 +178,39 @@ struct Geo {  // LDS rows of a step: 256 bytes (128 channels) or 128 (64)
   static __device__ int k_swizzle(int row) { return NT > 2 ? row & 15 : (row >> 1) & 7; }
   static __device__ int v_swizzle(int row) { return NT > 2 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
 };
+
+// Writes a wave's 32 rows, through its own 32 rows of LDS, so that a store instruction writes
+// whole rows.
+template <typename T, int NT>
+__device__ __forceinline__ void store_rows(const AttnArgs& a, const F16 (&o)[NT], float l, char* mine, int64_t q_row, int kvh,
+                                           int row0, int total, int lane) {
+  typedef Geo<NT> G;
+  typedef typename Mat<T>::V2 V2;
+  const int half = lane >> 5;
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing is zero)
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const F2 x = {o[n][i] * inv, o[n][i + 1] * inv}, y = {o[n][i + 2] * inv, o[n][i + 3] * inv};
+      const V2 c = __builtin_convertvector(x, V2), d = __builtin_convertvector(y, V2);
+      const int chunk = 4 * n + i / 4;
+      *reinterpret_cast<uint2*>(mine + (lane & 31) * G::kPitch + 16 * (chunk ^ G::k_swizzle(lane & 31)) + 8 * half) =
+          make_uint2(__builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d));
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32 * G::kChunks / 64; ++i) {
+    const int row = i * (64 / G::kChunks) + lane / G::kChunks, chunk = lane % G::kChunks;
+    const int rr = row0 + row;
+    if (rr < total && 16 * chunk < 2 * a.dim) {
+      const int at = (int)((unsigned)rr / (unsigned)a.group);
+      char* p = const_cast<char*>(a.o.data) + (q_row + at) * a.o.row + (int64_t)(kvh * a.group + rr - at * a.group) * a.o.head;
+      *reinterpret_cast<uint4*>(p + 16 * chunk) =
+          *reinterpret_cast<const uint4*>(mine + row * G::kPitch + 16 * (chunk ^ G::k_swizzle(row)));
+    }
+  }
+}
 
 // One workgroup: 4 waves of 32 packed rows over the keys of its piece in steps
 // of 64.  NT: head dim in units of 32 channels, rounded up.  MASKED: key mask.
@@ -390,32 +424,340 @@ __global__ __launch_bounds__(256, 2) void sfe_attn_rows_kernel(AttnArgs a) {
     if (half == 0) a.part_ml[at] = make_float2(m, l);
     return;
   }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing is zero)
-  // through LDS, so that a store instruction writes whole rows
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  char* mine = lds + wave * 32 * G::kPitch;
+  store_rows<T, NT>(a, o, l, lds + wave * 32 * G::kPitch, q_row, kvh, row0 + 32 * wave, total, lane);
+}
+
+// ---- tall: 256 packed rows a workgroup ----------------------------------------------------
+
+// One workgroup: 8 waves of 32 packed rows, two on each SIMD: waves 0-3 and 4-7 take turns at
+// the matrix cores.  An interval is the time between two barriers; in it one half runs
+// the products of a step (S of step j, then O of step j - 1) and the other the softmax of
+// its step, so that on every SIMD matrix and vector instructions issue side by side.  (Left to
+// themselves two waves of a SIMD overlapped little: causal prompts of up to 8192 took 2,660
+// cycles a step and wave, its products 1,024 and its vector instructions 1,150.)
+// K and V lie in 3 buffers each; the loads of K of step j + 2 and V of step j + 1 are issued
+// in interval 2j, after the last read of the buffers' former steps, and waited for two
+// intervals later by count, so every wave issues the same number in every step (steps past
+// the end load nothing: all their offsets are outside).
+template <typename T, int NT, bool MASKED>
+__global__ __launch_bounds__(512, 2) void sfe_attn_tall_kernel(AttnArgs a) {
+  typedef Geo<NT> G;
+  typedef typename Mat<T>::V8 V8;
+  typedef typename Mat<T>::V2 V2;
+  constexpr int kStep = kAttnStepRows;
+  constexpr int kBuf = kStep * G::kPitch;  // bytes of a step of K (or V)
+  constexpr int kLoads = kBuf / 8192;      // load instructions of a wave for it
+  constexpr int kRowsPerLoad = 8192 / G::kPitch;
+  __shared__ __align__(1024) char lds[6 * kBuf];  // 3 steps of K, 3 of V
+  const int units = a.n_items * a.kv_heads;
+  const int u = unit_of_block(units);
+  if (u < 0) return;
+  const int kvh = u / a.n_items;
+  const AttnItem& it = a.items[u - kvh * a.n_items];
+  const int lq = it.lq, lk = it.lk, kv0 = it.kv0, kv1 = it.kv1, row0 = it.row0, part = it.part;
+  const int64_t q_row = it.q_row, k_row = it.k_row;
+  const int total = lq * a.group;
+  const int t = (int)threadIdx.x, lane = t & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int dim_bytes = 2 * a.dim;
+  const uint32_t base = lds_address(lds);
+
+  // ---- queries: lane's row, operand B of the first product
+  const int r = row0 + 32 * wave + (lane & 31);
+  const int rc = r < total ? r : total - 1;
+  const int pos = (int)((unsigned)rc / (unsigned)a.group);
+  int lo, hi;
+  visible(a, pos, lq, lk, &lo, &hi);
+  V8 q[2 * NT];
+  {
+    const char* p = a.q.data + (q_row + pos) * a.q.row + (int64_t)(kvh * a.group + rc - pos * a.group) * a.q.head;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const F2 x = {o[n][i] * inv, o[n][i + 1] * inv}, y = {o[n][i + 2] * inv, o[n][i + 3] * inv};
-      const V2 c = __builtin_convertvector(x, V2), d = __builtin_convertvector(y, V2);
-      const int chunk = 4 * n + i / 4;
-      *reinterpret_cast<uint2*>(mine + (lane & 31) * G::kPitch + 16 * (chunk ^ G::k_swizzle(lane & 31)) + 8 * half) =
-          make_uint2(__builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d));
+    for (int s = 0; s < 2 * NT; ++s) {
+      const int c = 2 * s + half;
+      S8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * c < dim_bytes) v = *reinterpret_cast<const S8*>(p + 16 * c);
+      q[s] = __builtin_bit_cast(V8, v);
     }
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // (waited for here: a wait within the loop would be one for the loads into LDS too)
 #pragma unroll
-  for (int i = 0; i < 32 * G::kChunks / 64; ++i) {
-    const int row = i * (64 / G::kChunks) + lane / G::kChunks, chunk = lane % G::kChunks;
-    const int rr = row0 + 32 * wave + row;
-    if (rr < total && 16 * chunk < dim_bytes) {
-      const int at = (int)((unsigned)rr / (unsigned)a.group);
-      char* p = const_cast<char*>(a.o.data) + (q_row + at) * a.o.row + (int64_t)(kvh * a.group + rr - at * a.group) * a.o.head;
-      *reinterpret_cast<uint4*>(p + 16 * chunk) =
-          *reinterpret_cast<const uint4*>(mine + row * G::kPitch + 16 * (chunk ^ G::k_swizzle(row)));
-    }
+    for (int s = 0; s < 2 * NT; ++s) asm volatile("" : "+v"(q[s]));
   }
+  const bool idle = row0 + 32 * wave >= total;  // none of the wave's rows exists
+  const int lo_all = __builtin_amdgcn_readlane(lo, 31), hi_all = __builtin_amdgcn_readlane(hi, 0);
+  const int lo_any = __builtin_amdgcn_readlane(lo, 0), hi_any = idle ? -1 : __builtin_amdgcn_readlane(hi, 31);
+
+  // ---- addresses
+  const int lrow = t / G::kChunks, lchunk = t % G::kChunks;
+  const int kc = lchunk ^ G::k_swizzle(lrow), vc = lchunk ^ G::v_swizzle(lrow);
+  const uint32_t k_off = 16 * kc < dim_bytes ? (uint32_t)(lrow * a.k.row) + 16 * kc : kOutside;
+  const uint32_t v_off = 16 * vc < dim_bytes ? (uint32_t)(lrow * a.v.row) + 16 * vc : kOutside;
+  const uint32_t k_next = (uint32_t)(kRowsPerLoad * a.k.row), v_next = (uint32_t)(kRowsPerLoad * a.v.row);
+  const uint32_t wave_base = __builtin_amdgcn_readfirstlane(base + 1024 * wave);
+  uint32_t k_addr[2 * NT];
+#pragma unroll
+  for (int s = 0; s < 2 * NT; ++s)
+    k_addr[s] = base + (lane & 31) * G::kPitch + 16 * ((2 * s + half) ^ G::k_swizzle(lane & 31));
+  uint32_t v_addr[NT];
+  {
+    const int row = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      v_addr[n] = base + 3 * kBuf + row * G::kPitch +
+                  16 * ((4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ G::v_swizzle(row)) + 8 * (lane & 1);
+  }
+
+  const uint8_t* mask = MASKED ? a.mask + k_row : nullptr;
+  auto mask_bits = [&](int kv) -> uint64_t {
+    if (!MASKED) return ~0ull;
+    return __ballot(kv + lane < lk && mask[kv + lane] != 0);
+  };
+  // rows of K (or V) of the step at kv into buffer `slot`
+  auto load_rows = [&](const AttnTensor& x, uint32_t off, uint32_t next, int kv, uint32_t dst, uint64_t bits) {
+    const I4 b = row_buffer(x, k_row + kv, kv < kv1 ? lk - kv : 0, kvh, dim_bytes);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      uint32_t o = off == kOutside ? kOutside : off + i * next;
+      if (MASKED && !((bits >> (i * kRowsPerLoad + lrow)) & 1)) o = kOutside;
+      load_lds(b, o, wave_base + dst + i * 8192);
+    }
+  };
+  auto after = [](uint32_t slot) -> uint32_t { return slot == 2 * kBuf ? 0 : slot + kBuf; };
+
+  F16 o[NT];
+  float m, l;
+
+  // Runs over the keys.  CAREFUL: values of V that are not finite are kept from the rows that
+  // do not see their key (they would reach them as 0 * inf).
+  auto run = [&](auto careful) {
+    constexpr bool kCareful = decltype(careful)::value;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[n][i] = 0.0f;
+    m = kNever;
+    l = 0.0f;
+    uint64_t bits0 = mask_bits(kv0), bits1 = mask_bits(kv0 + kStep), bits2 = mask_bits(kv0 + 2 * kStep);
+    load_rows(a.v, v_off, v_next, kv1, 5 * kBuf, ~0ull);  // (zeros: the first step's weights of the step before are too)
+    load_rows(a.k, k_off, k_next, kv0, 0, bits0);
+    load_rows(a.k, k_off, k_next, kv0 + kStep, kBuf, bits1);
+    load_rows(a.v, v_off, v_next, kv0, 3 * kBuf, bits0);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory");
+    uint32_t k2 = 2 * kBuf, v1 = kBuf;  // buffers of K of step j + 2 and V of step j + 1
+    uint32_t kj = 0, vp = 2 * kBuf;     // ... of K of step j and V of step j - 1
+    F16 s[2];
+    V8 p[4];
+    // weights of step j - 1, zero where the wave's rows saw none of it
+#pragma unroll
+    for (int c = 0; c < 4; ++c) p[c] = V8{0, 0, 0, 0, 0, 0, 0, 0};
+    bool did = false;
+    uint64_t see_before = 0;
+    auto careful_products = [&]() {
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        const V8 pc = c < 2 ? (c == 0 ? p[0] : p[1]) : (c == 2 ? p[2] : p[3]);
+        S8 seen;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) seen[j] = (see_before >> (16 * c + 8 * (j / 4) + j % 4)) & 1 ? Mat<T>::kOne : 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          V8 v = read_v<T>(v_addr[n] + vp + 16 * c * G::kPitch, v_addr[n] + vp + (16 * c + 8) * G::kPitch);
+          if (__any(nonfinite<T>(v) != 0)) {
+            S8 clean, up, down;
+            split_nonfinite<T>(__builtin_bit_cast(S8, v), &clean, &up, &down);
+            F16 none;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) none[i] = 0.0f;
+            const F16 ups = Mat<T>::m32(__builtin_bit_cast(V8, up), __builtin_bit_cast(V8, seen), none);
+            const F16 downs = Mat<T>::m32(__builtin_bit_cast(V8, down), __builtin_bit_cast(V8, seen), none);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (ups[i] > 0.0f) o[n][i] += INFINITY;
+              if (downs[i] > 0.0f) o[n][i] -= INFINITY;
+            }
+            v = __builtin_bit_cast(V8, clean);
+          }
+          o[n] = Mat<T>::m32(v, pc, o[n]);
+        }
+      }
+    };
+    // the loads of interval 2j, for the step after next
+    auto loads = [&](int kv) {
+      load_rows(a.k, k_off, k_next, kv + 2 * kStep, k2, bits2);
+      load_rows(a.v, v_off, v_next, kv + kStep, 3 * kBuf + v1, bits1);
+      k2 = after(k2);
+      v1 = after(v1);
+    };
+    auto products = [&](int kv) {
+      const int end = kv1 < kv + kStep ? kv1 : kv + kStep;  // keys of the step: [kv, end)
+      const bool now = kv < kv1 && lo_any < end && hi_any >= kv;
+      if (now || did) {
+        // Both products as one stream of matrix instructions, operands read kAhead pairs (K)
+        // or fragments (V) ahead of their use; the fences keep the compiler from reading
+        // each just before it (every product then waited for its read) or all at once.
+        __builtin_amdgcn_s_setprio(1);  // (1,194 us without, on the same prompts)
+        constexpr int kK = 2 * NT, kV = kCareful ? 0 : 4 * NT, kAhead = 3;
+        V8 kf[kK][2], vf[4 * NT];
+        auto read_pair = [&](int c) {
+          kf[c][0] = read_k<T>(k_addr[c] + kj);
+          kf[c][1] = read_k<T>(k_addr[c] + kj + 32 * G::kPitch);
+        };
+        auto read_value = [&](int i) {
+          const uint32_t at = v_addr[i % NT] + vp + 16 * (i / NT) * G::kPitch;
+          vf[i] = read_v<T>(at, at + 8 * G::kPitch);
+        };
+#pragma unroll
+        for (int c = 0; c < kAhead; ++c) read_pair(c);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[h][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kK; ++c) {
+          if (c + kAhead < kK) {
+            read_pair(c + kAhead);
+          } else if (!kCareful) {
+            read_value(2 * (c + kAhead - kK));
+            read_value(2 * (c + kAhead - kK) + 1);
+          }
+          s[0] = Mat<T>::m32(kf[c][0], q[c], s[0]);
+          s[1] = Mat<T>::m32(kf[c][1], q[c], s[1]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          if (i + 2 * kAhead < kV) read_value(i + 2 * kAhead);
+          o[i % NT] = Mat<T>::m32(vf[i], p[i / NT], o[i % NT]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (kCareful) careful_products();
+      }
+      did = now;
+      kj = after(kj);
+      vp = after(vp);
+    };
+    auto softmax = [&](int kv, uint64_t bits) {
+      if (!did) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) p[c] = V8{0, 0, 0, 0, 0, 0, 0, 0};
+        see_before = 0;
+        return;
+      }
+      const int end = kv1 < kv + kStep ? kv1 : kv + kStep;
+      // keys that some of the wave's rows do not see
+      const bool edge = lo_all > kv || hi_all < kv + kStep - 1 || end < kv + kStep;
+      if (kCareful) see_before = ~0ull;
+      if (edge || (MASKED && bits != ~0ull)) {
+        // lane's keys are 32 h + 8 (i / 4) + 4 half + i % 4
+        uint64_t see = span_bits(lo - kv, (hi < end - 1 ? hi : end - 1) - kv);
+        if (MASKED) see &= bits;
+        see >>= 4 * half;
+        if (kCareful) see_before = see;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[h][i] = (see >> (32 * h + 8 * (i / 4) + i % 4)) & 1 ? s[h][i] : -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
+      if (__any(top * a.scale_log2 > m + kRise)) {
+        const float nm = fmaxf(m, max_halves(top) * a.scale_log2 - kBelow);
+        const float f = exp2_fast(m - nm);
+        m = nm;
+        l *= f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[n][i] *= f;
+      }
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const F2 w = {exp2_fast(__builtin_fmaf(s[h][i], a.scale_log2, -m)),
+                        exp2_fast(__builtin_fmaf(s[h][i + 1], a.scale_log2, -m))};
+          sum[i % 4] += w.x;
+          sum[i % 4 + 1] += w.y;
+          const V2 c = __builtin_convertvector(w, V2);
+          p[2 * h + i / 8][i % 8] = c.x;
+          p[2 * h + i / 8][i % 8 + 1] = c.y;
+        }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    auto barrier = []() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // (after the loads of one more step have been issued, those of the step before are done)
+    auto landed = []() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory"); };
+    if (wave < 4) {
+      for (int kv = kv0; kv < kv1; kv += kStep) {
+        loads(kv);
+        products(kv);
+        barrier();
+        softmax(kv, bits0);
+        bits0 = bits1, bits1 = bits2, bits2 = mask_bits(kv + 3 * kStep);
+        landed();
+      }
+      products(kv1);
+      barrier();
+    } else {
+      loads(kv0);
+      barrier();
+      for (int kv = kv0; kv < kv1; kv += kStep) {
+        products(kv);
+        const uint64_t bits = bits0;
+        bits0 = bits1, bits1 = bits2, bits2 = mask_bits(kv + 3 * kStep);
+        landed();
+        loads(kv + kStep);
+        softmax(kv, bits);
+        barrier();
+      }
+      products(kv1);
+    }
+    l = sum_halves(l);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  if (kv0 < kv1) {
+    run(std::false_type());
+    // A result that is not finite may be a hidden value's: then once more, with care
+    bool bad = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bad |= !(__builtin_fabsf(o[n][i]) < INFINITY);
+    int* again = reinterpret_cast<int*>(lds);
+    if (lane == 0) again[wave] = 0;
+    if (__any(bad) && lane == 0) again[wave] = 1;
+    __syncthreads();
+    int any = 0;
+    for (int w = 0; w < 8; ++w) any |= again[w];
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(any)) run(std::true_type());
+  } else {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[n][i] = 0.0f;
+    m = kNever;
+    l = 0.0f;
+  }
+
+  if (part >= 0) {
+    const int64_t at = ((int64_t)part * a.kv_heads + kvh) * kAttnTileTall + 32 * wave + (lane & 31);
+    float* po = a.part_o + at * (32 * NT);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<F4*>(po + 32 * n + 2 * i + 4 * half) = F4{o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]};
+    if (half == 0) a.part_ml[at] = make_float2(m, l);
+    return;
+  }
+  store_rows<T, NT>(a, o, l, lds + wave * 32 * G::kPitch, q_row, kvh, row0 + 32 * wave, total, lane);
 }
 
 // ---- few: 16 packed rows a workgroup, its waves share the keys ---------------------------
@@ -666,50 +1008,52 @@ __global__ __launch_bounds__(256) void sfe_attn_join_kernel(AttnArgs a) {
   *reinterpret_cast<V2*>(p + 4 * lane) = __builtin_convertvector(v, V2);
 }
 
-template <typename T, int NT>
-hipError_t run_rows(const AttnArgs& a, hipStream_t stream) {
-  const unsigned blocks = (unsigned)(((int64_t)a.n_items * a.kv_heads + 7) / 8 * 8);
-  if (a.mask)
-    sfe_attn_rows_kernel<T, NT, true><<<dim3(blocks), dim3(256), 0, stream>>>(a);
-  else
-    sfe_attn_rows_kernel<T, NT, false><<<dim3(blocks), dim3(256), 0, stream>>>(a);
-  hipError_t e = hipGetLastError();
+template <typename T, int NT, int FORM>
+hipError_t run_form(const AttnArgs& a, hipStream_t stream) {
+  const dim3 blocks((unsigned)(((int64_t)a.n_items * a.kv_heads + 7) / 8 * 8));
+  constexpr int kTile = FORM == kAttnTall ? kAttnTileTall : (FORM == kAttnRows ? kAttnTileRows : kAttnTileFew);
+  if constexpr (FORM == kAttnTall) {
+    if (a.mask)
+      sfe_attn_tall_kernel<T, NT, true><<<blocks, dim3(512), 0, stream>>>(a);
+    else
+      sfe_attn_tall_kernel<T, NT, false><<<blocks, dim3(512), 0, stream>>>(a);
+  } else if constexpr (FORM == kAttnRows) {
+    if (a.mask)
+      sfe_attn_rows_kernel<T, NT, true><<<blocks, dim3(256), 0, stream>>>(a);
+    else
+      sfe_attn_rows_kernel<T, NT, false><<<blocks, dim3(256), 0, stream>>>(a);
+  } else {
+    if (a.mask)
+      sfe_attn_few_kernel<T, NT, true><<<blocks, dim3(256), 0, stream>>>(a);
+    else
+      sfe_attn_few_kernel<T, NT, false><<<blocks, dim3(256), 0, stream>>>(a);
+  }
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.n_joins) return e;
-  sfe_attn_join_kernel<T, NT, kAttnTileRows>
-      <<<dim3((unsigned)((int64_t)a.n_joins * a.kv_heads * kAttnTileRows / 4)), dim3(256), 0, stream>>>(a);
+  sfe_attn_join_kernel<T, NT, kTile>
+      <<<dim3((unsigned)((int64_t)a.n_joins * a.kv_heads * kTile / 4)), dim3(256), 0, stream>>>(a);
   return hipGetLastError();
 }
 
-template <typename T, int NT>
-hipError_t run_few(const AttnArgs& a, hipStream_t stream) {
-  const unsigned blocks = (unsigned)(((int64_t)a.n_items * a.kv_heads + 7) / 8 * 8);
-  if (a.mask)
-    sfe_attn_few_kernel<T, NT, true><<<dim3(blocks), dim3(256), 0, stream>>>(a);
-  else
-    sfe_attn_few_kernel<T, NT, false><<<dim3(blocks), dim3(256), 0, stream>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !a.n_joins) return e;
-  sfe_attn_join_kernel<T, NT, kAttnTileFew>
-      <<<dim3((unsigned)((int64_t)a.n_joins * a.kv_heads * kAttnTileFew / 4)), dim3(256), 0, stream>>>(a);
-  return hipGetLastError();
+template <typename T, int FORM>
+hipError_t run_dim(const AttnArgs& a, hipStream_t stream) {
+  switch (attn_padded_dim(a.dim)) {
+    case 64: return run_form<T, 2, FORM>(a, stream);
+    case 96: return run_form<T, 3, FORM>(a, stream);
+    default: return run_form<T, 4, FORM>(a, stream);
+  }
 }
 
 template <typename T>
-hipError_t run_form(const AttnArgs& a, bool rows, hipStream_t stream) {
-  switch (attn_padded_dim(a.dim)) {
-    case 64: return rows ? run_rows<T, 2>(a, stream) : run_few<T, 2>(a, stream);
-    case 96: return rows ? run_rows<T, 3>(a, stream) : run_few<T, 3>(a, stream);
-    default: return rows ? run_rows<T, 4>(a, stream) : run_few<T, 4>(a, stream);
-  }
+hipError_t run(const AttnArgs& a, int form, hipStream_t stream) {
+  if (form == kAttnTall) return run_dim<T, kAttnTall>(a, stream);
+  return form == kAttnRows ? run_dim<T, kAttnRows>(a, stream) : run_dim<T, kAttnFew>(a, stream);
 }
 
 }  // namespace
 
-hipError_t launch_attn_rows(const AttnArgs& a, int type, hipStream_t stream) {
-  return type == kOpBf16 ? run_form<Bf>(a, true, stream) : run_form<Hf>(a, true, stream);
-}
-hipError_t launch_attn_few(const AttnArgs& a, int type, hipStream_t stream) {
-  return type == kOpBf16 ? run_form<Bf>(a, false, stream) : run_form<Hf>(a, false, stream);
+hipError_t launch_attn(const AttnArgs& a, int form, int type, hipStream_t stream) {
+  return type == kOpBf16 ? run<Bf>(a, form, stream) : run<Hf>(a, form, stream);
 }
 
 }  // namespace sfe

@@ -59,24 +59,25 @@ int64_t piece_keys(const std::vector<Tile>& tiles, int kv_heads, int64_t slots, 
 void attn_plan(const int64_t* q_offsets, const int64_t* k_offsets, int n, int group, int kv_heads, int head_dim,
                int32_t left, int32_t right, int cus, AttnPlanHost* out) {
   (void)head_dim;
-  std::vector<Tile> rows, few;
+  std::vector<Tile> tiles[kAttnForms];
   for (int s = 0; s < n; ++s) {
     const int64_t lq = q_offsets[s + 1] - q_offsets[s], lk = k_offsets[s + 1] - k_offsets[s];
     const int64_t total = lq * group;
-    const bool small = total <= 4 * kAttnTileFew;
-    const int tile = small ? kAttnTileFew : kAttnTileRows;
+    const int form = total <= kAttnTileFew ? kAttnFew : (total <= kAttnTileRows ? kAttnRows : kAttnTall);
+    const int tile = attn_tile(form);
     // (the last tiles of a causal sequence see the most keys: they go first)
     for (int64_t t = (total + tile - 1) / tile - 1; t >= 0; --t) {
       int64_t lo, hi;
       key_range(lq, lk, t * tile / group, (std::min(total, (t + 1) * tile) - 1) / group, left, right, &lo, &hi);
-      (small ? few : rows)
-          .push_back(Tile{q_offsets[s], k_offsets[s], (int32_t)lq, (int32_t)lk, (int32_t)(t * tile), (int32_t)lo,
-                          (int32_t)hi});
+      tiles[form].push_back(
+          Tile{q_offsets[s], k_offsets[s], (int32_t)lq, (int32_t)lk, (int32_t)(t * tile), (int32_t)lo, (int32_t)hi});
     }
   }
-  cut(rows, piece_keys(rows, kv_heads, 2 * cus, 4 * kAttnStepRows), kAttnStepRows, &out->rows);
-  const int unit = kAttnWavesFew * kAttnStepFew;
-  cut(few, piece_keys(few, kv_heads, 2 * cus, 2 * unit), unit, &out->few);
+  for (int form = 0; form < kAttnForms; ++form) {
+    const int unit = form == kAttnFew ? kAttnWavesFew * kAttnStepFew : kAttnStepRows;
+    const int64_t slots = form == kAttnRows ? 2 * cus : cus;
+    cut(tiles[form], piece_keys(tiles[form], kv_heads, slots, form == kAttnFew ? 2 * unit : 4 * unit), unit, &out->form[form]);
+  }
 }
 
 }  // namespace sfe

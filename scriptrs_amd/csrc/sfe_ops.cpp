@@ -19,12 +19,14 @@ using sfe::op_fail;
 struct sfe_attn_plan {
   sfe_ctx* ctx = nullptr;
   int32_t heads = 0, kv_heads = 0, dim = 0, left = 0, right = 0;
-  int32_t n_rows = 0, n_few = 0, rows_joins = 0, few_joins = 0;
+  struct Form {
+    int32_t n_items = 0, n_joins = 0;
+    size_t items = 0, joins = 0, part_o = 0, part_ml = 0;  // offsets into buf
+  } form[sfe::kAttnForms];
+  bool empty = true;  // no queries
   int64_t total_q = 0, total_k = 0;
   void* buf = nullptr;
   size_t cap = 0;
-  // offsets into buf
-  size_t rows_items = 0, few_items = 0, rows_join = 0, few_join = 0, rows_o = 0, rows_ml = 0, few_o = 0, few_ml = 0;
 };
 
 namespace {
@@ -142,14 +144,12 @@ int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_
     sfe::AttnPlanHost h;
     sfe::attn_plan(q_offsets, k_offsets, n, group, kv_heads, head_dim, plan->left, plan->right, sfe::op_cus(ctx), &h);
     // a launch holds fewer than 2^32 threads
-    const int64_t most = (int64_t)(UINT32_MAX / 256 - 8) / kv_heads;
-    if ((int64_t)h.rows.items.size() > most || (int64_t)h.few.items.size() > most)
-      return op_fail(SFE_INVALID_ARG, "batch too large for one launch");
-    plan->n_rows = (int32_t)h.rows.items.size();
-    plan->n_few = (int32_t)h.few.items.size();
-    plan->rows_joins = (int32_t)h.rows.joins.size();
-    plan->few_joins = (int32_t)h.few.joins.size();
-    if (plan->n_rows + plan->n_few == 0) {
+    const int64_t most = (int64_t)(UINT32_MAX / 512 - 8) / kv_heads;
+    for (const auto& f : h.form) {
+      if ((int64_t)f.items.size() > most) return op_fail(SFE_INVALID_ARG, "batch too large for one launch");
+      if (!f.items.empty()) plan->empty = false;
+    }
+    if (plan->empty) {
       *out = plan.release();
       return SFE_OK;
     }
@@ -159,26 +159,24 @@ int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_
       at += up(bytes);
       return o;
     };
-    plan->rows_items = place(h.rows.items.size() * sizeof(sfe::AttnItem));
-    plan->few_items = place(h.few.items.size() * sizeof(sfe::AttnItem));
-    plan->rows_join = place(h.rows.joins.size() * sizeof(sfe::AttnJoin));
-    plan->few_join = place(h.few.joins.size() * sizeof(sfe::AttnJoin));
+    for (int i = 0; i < sfe::kAttnForms; ++i) {
+      plan->form[i].n_items = (int32_t)h.form[i].items.size();
+      plan->form[i].n_joins = (int32_t)h.form[i].joins.size();
+      plan->form[i].items = place(h.form[i].items.size() * sizeof(sfe::AttnItem));
+      plan->form[i].joins = place(h.form[i].joins.size() * sizeof(sfe::AttnJoin));
+    }
     const size_t bytes = at;
-    const size_t dim = (size_t)sfe::attn_padded_dim(head_dim);
-    const size_t rows = (size_t)h.rows.parts * kv_heads * sfe::kAttnTileRows;
-    const size_t few = (size_t)h.few.parts * kv_heads * sfe::kAttnTileFew;
-    plan->rows_o = place(rows * dim * 4);
-    plan->rows_ml = place(rows * 8);
-    plan->few_o = place(few * dim * 4);
-    plan->few_ml = place(few * 8);
     std::vector<char> table(bytes);
     auto put = [&](size_t o, const void* p, size_t size) {
       if (size) memcpy(table.data() + o, p, size);
     };
-    put(plan->rows_items, h.rows.items.data(), h.rows.items.size() * sizeof(sfe::AttnItem));
-    put(plan->few_items, h.few.items.data(), h.few.items.size() * sizeof(sfe::AttnItem));
-    put(plan->rows_join, h.rows.joins.data(), h.rows.joins.size() * sizeof(sfe::AttnJoin));
-    put(plan->few_join, h.few.joins.data(), h.few.joins.size() * sizeof(sfe::AttnJoin));
+    for (int i = 0; i < sfe::kAttnForms; ++i) {
+      put(plan->form[i].items, h.form[i].items.data(), h.form[i].items.size() * sizeof(sfe::AttnItem));
+      put(plan->form[i].joins, h.form[i].joins.data(), h.form[i].joins.size() * sizeof(sfe::AttnJoin));
+      const size_t rows = (size_t)h.form[i].parts * kv_heads * sfe::attn_tile(i);
+      plan->form[i].part_o = place(rows * sfe::attn_padded_dim(head_dim) * sizeof(float));
+      plan->form[i].part_ml = place(rows * sizeof(float2));
+    }
     if ((rc = sfe::op_upload(ctx, table.data(), bytes, at, static_cast<hipStream_t>(stream), &plan->buf, &plan->cap)))
       return rc;
     *out = plan.release();
@@ -201,7 +199,7 @@ int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const 
     if (!plan || !q || !k || !v || !out) return op_fail(SFE_INVALID_ARG, "null argument");
     if (dtype != SFE_BF16 && dtype != SFE_F16) return op_fail(SFE_INVALID_ARG, "dtype must be SFE_BF16 or SFE_F16");
     if (!(scale > 0.0f) || scale > 1e30f) return op_fail(SFE_INVALID_ARG, "scale must be positive and finite");
-    if (plan->n_rows + plan->n_few == 0) return SFE_OK;  // no queries
+    if (plan->empty) return SFE_OK;  // no queries
     int rc;
     const struct {
       const char* name;
@@ -221,7 +219,6 @@ int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const 
                           rows_of("v", *v, plan->total_k, plan->kv_heads, plan->dim, 2)})
       if (share(mine, o)) return op_fail(SFE_INVALID_ARG, std::string("out overlaps ") + o.name);
     if (plan->total_k > 0 && (!k->data || !v->data)) return op_fail(SFE_INVALID_ARG, "null k or v");
-    const char* base = static_cast<const char*>(plan->buf);
     auto tensor = [](const sfe_heads* t) {
       return sfe::AttnTensor{static_cast<const char*>(t->data), t->row_stride * 2, t->head_stride * 2};
     };
@@ -238,26 +235,27 @@ int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const 
     a.right = plan->right;
     a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     struct Call {
-      sfe::AttnArgs rows, few;
+      sfe::AttnArgs a;
+      const sfe_attn_plan* plan;
       int dtype;
       hipStream_t stream;
-    } call{a, a, dtype, static_cast<hipStream_t>(stream)};
-    auto form = [&](sfe::AttnArgs* f, int n, size_t items, int joins, size_t join, size_t po, size_t ml) {
-      f->n_items = n;
-      f->items = reinterpret_cast<const sfe::AttnItem*>(base + items);
-      f->n_joins = joins;
-      f->joins = reinterpret_cast<const sfe::AttnJoin*>(base + join);
-      f->part_o = reinterpret_cast<float*>(const_cast<char*>(base) + po);
-      f->part_ml = reinterpret_cast<float2*>(const_cast<char*>(base) + ml);
-    };
-    form(&call.rows, plan->n_rows, plan->rows_items, plan->rows_joins, plan->rows_join, plan->rows_o, plan->rows_ml);
-    form(&call.few, plan->n_few, plan->few_items, plan->few_joins, plan->few_join, plan->few_o, plan->few_ml);
+    } call{a, plan, dtype, static_cast<hipStream_t>(stream)};
     return sfe::op_call(plan->ctx, call.stream, "attention", [](void* arg, int) -> hipError_t {
       Call& c = *static_cast<Call*>(arg);
-      hipError_t e = hipSuccess;
-      if (c.rows.n_items) e = sfe::launch_attn_rows(c.rows, c.dtype, c.stream);
-      if (e == hipSuccess && c.few.n_items) e = sfe::launch_attn_few(c.few, c.dtype, c.stream);
-      return e;
+      char* base = static_cast<char*>(c.plan->buf);
+      for (int i = 0; i < sfe::kAttnForms; ++i) {
+        const auto& f = c.plan->form[i];
+        if (!f.n_items) continue;
+        c.a.n_items = f.n_items;
+        c.a.items = reinterpret_cast<const sfe::AttnItem*>(base + f.items);
+        c.a.n_joins = f.n_joins;
+        c.a.joins = reinterpret_cast<const sfe::AttnJoin*>(base + f.joins);
+        c.a.part_o = reinterpret_cast<float*>(base + f.part_o);
+        c.a.part_ml = reinterpret_cast<float2*>(base + f.part_ml);
+        const hipError_t e = sfe::launch_attn(c.a, i, c.dtype, c.stream);
+        if (e != hipSuccess) return e;
+      }
+      return hipSuccess;
     }, &call);
   });
 }

@@ -67,13 +67,15 @@ struct AttnJoin {
 };
 static_assert(sizeof(AttnJoin) == 24, "layout shared with the kernels");
 
-// Packed rows of a tile and keys of a step, per kernel form: `rows` (4 waves of
-// 32 rows share a step's keys) and `few` (16 rows, each wave takes every
-// fourth step).
-constexpr int kAttnTileRows = 128, kAttnStepRows = 64;
+// Kernel forms, packed rows of their tiles and keys of their steps: `tall` (8 waves of 32 rows
+// share a step's keys, in two halves that take turns at the matrix cores), `rows` (4 waves of
+// 32 rows) and `few` (16 rows, each of 4 waves takes every fourth step).
+enum AttnKernel { kAttnTall = 0, kAttnRows = 1, kAttnFew = 2, kAttnForms = 3 };
+constexpr int kAttnTileTall = 256, kAttnTileRows = 128, kAttnStepRows = 64;
 constexpr int kAttnTileFew = 16, kAttnStepFew = 32, kAttnWavesFew = 4;
 constexpr int kAttnMaxDim = 128;
 constexpr int32_t kAttnNoBound = 0x7fffffff;
+inline int attn_tile(int form) { return form == kAttnTall ? kAttnTileTall : (form == kAttnRows ? kAttnTileRows : kAttnTileFew); }
 
 struct AttnForm {
   std::vector<AttnItem> items;
@@ -81,7 +83,7 @@ struct AttnForm {
   int32_t parts = 0;  // pieces with a partial result
 };
 struct AttnPlanHost {
-  AttnForm rows, few;
+  AttnForm form[kAttnForms];
 };
 // Lays the tiles of n sequences out (host only).  left, right: the window, or
 // kAttnNoBound.
@@ -104,8 +106,7 @@ struct AttnArgs {
   float scale_log2;  // scale * log2(e)
 };
 inline int attn_padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : 128); }
-hipError_t launch_attn_rows(const AttnArgs& a, int type, hipStream_t stream);
-hipError_t launch_attn_few(const AttnArgs& a, int type, hipStream_t stream);
+hipError_t launch_attn(const AttnArgs& a, int form, int type, hipStream_t stream);
 
 // ---- rotary positions (sfe_rotary.hip) ----------------------------------------------
 constexpr int kRotaryMaxPairs = 128;

@@ -54,16 +54,69 @@ int64_t piece_keys(const std::vector<Tile>& tiles, int kv_heads, int64_t slots, 
   return std::max(least, std::min(longest, (total + slots - 1) / slots));
 }
 
+// Time of a sequence's tiles in a form, in microseconds of a CU: steps and a fixed part a tile,
+// fitted to 40,000 rows of 8 heads of 128 (steps of 2.03 us for 256 rows, 1.31 for 128).  It
+// chooses as measured: full attention of 188, 260, 384, 512, 1024, 4096 keys takes 118 (rows) / 131
+// (tall), 136 / 180, 126 / 139, 153 / 127, 244 / 190, 756 / 585 us; causal 384, 512, 768, 4096: 100 / 117,
+// 131 / 118, 146 / 125, 396 / 353; windows of 64, 256, 512, 1024 to either side: 93 / 107, 150 / 156,
+// 235 / 222, 406 / 364.  Heads of 64 channels and less leave room for 3 workgroups of the rows
+// form on a CU, which is then faster everywhere (4096 keys 695 / 727 us, 512 119 / 145).
+double tile_costs(int form, int64_t lq, int64_t lk, int group, int32_t left, int32_t right) {
+  const bool causal = left == kAttnNoBound && right == 0;
+  const double step = form == kAttnTall ? 2.03 : 1.31, fixed = form == kAttnTall ? (causal ? 10.0 : 13.0) : 5.2;
+  const int64_t tile = attn_tile(form), total = lq * group;
+  double cost = 0.0;
+  for (int64_t t = 0; t * tile < total; ++t) {
+    int64_t lo, hi;
+    key_range(lq, lk, t * tile / group, (std::min(total, (t + 1) * tile) - 1) / group, left, right, &lo, &hi);
+    cost += fixed + step * (double)((hi - lo + kAttnStepRows - 1) / kAttnStepRows);
+    if (t == 4096) return cost * ((double)total / (double)((t + 1) * tile));  // (long enough to tell)
+  }
+  return cost;
+}
+
+// The form of a sequence.  few: up to 16 packed rows, as single tokens have, where the call has
+// only such sequences or the keys are many; a launch of its own for a few short ones would cost
+// more than their place among the rows (256 clips of 13-251 frames: 51 us with it, 46 without).
+int form_of(int64_t lq, int64_t lk, int group, int head_dim, int32_t left, int32_t right, bool all_few) {
+  const int64_t total = lq * group;
+  if (total <= kAttnTileFew && (all_few || lk >= 1024)) return kAttnFew;
+  if (total <= kAttnTileRows || attn_padded_dim(head_dim) <= 64) return kAttnRows;
+  return tile_costs(kAttnTall, lq, lk, group, left, right) < tile_costs(kAttnRows, lq, lk, group, left, right) ? kAttnTall
+                                                                                                              : kAttnRows;
+}
+
+// Cuts the units (kv head by kv head, in a head the items in order) into 8 shares of about equal
+// work, one an XCD.
+void share_out(int kv_heads, AttnForm* f) {
+  const int64_t n = (int64_t)f->items.size();
+  std::vector<double> sum((size_t)n + 1, 0.0);
+  for (int64_t i = 0; i < n; ++i) {
+    const AttnItem& it = f->items[(size_t)i];
+    sum[(size_t)i + 1] = sum[(size_t)i] + 4.0 + (double)((it.kv1 - it.kv0 + kAttnStepRows - 1) / kAttnStepRows);
+  }
+  f->share[0] = 0;
+  for (int x = 1; x < 8; ++x) {
+    const double at = sum[(size_t)n] * kv_heads * x / 8.0;
+    const int64_t head = std::min<int64_t>(kv_heads - 1, (int64_t)(at / sum[(size_t)n]));
+    const double rest = at - (double)head * sum[(size_t)n];
+    const int64_t i = std::lower_bound(sum.begin(), sum.end(), rest - 1e-6 * sum[(size_t)n]) - sum.begin();
+    f->share[x] = std::max<int32_t>(f->share[x - 1], (int32_t)std::min<int64_t>(head * n + i, n * kv_heads));
+  }
+  f->share[8] = (int32_t)(n * kv_heads);
+}
+
 }  // namespace
 
 void attn_plan(const int64_t* q_offsets, const int64_t* k_offsets, int n, int group, int kv_heads, int head_dim,
                int32_t left, int32_t right, int cus, AttnPlanHost* out) {
-  (void)head_dim;
+  bool all_few = true;
+  for (int s = 0; s < n; ++s) all_few = all_few && (q_offsets[s + 1] - q_offsets[s]) * group <= kAttnTileFew;
   std::vector<Tile> tiles[kAttnForms];
   for (int s = 0; s < n; ++s) {
     const int64_t lq = q_offsets[s + 1] - q_offsets[s], lk = k_offsets[s + 1] - k_offsets[s];
     const int64_t total = lq * group;
-    const int form = total <= kAttnTileFew ? kAttnFew : (total <= kAttnTileRows ? kAttnRows : kAttnTall);
+    const int form = form_of(lq, lk, group, head_dim, left, right, all_few);
     const int tile = attn_tile(form);
     // (the last tiles of a causal sequence see the most keys: they go first)
     for (int64_t t = (total + tile - 1) / tile - 1; t >= 0; --t) {
@@ -77,6 +130,7 @@ void attn_plan(const int64_t* q_offsets, const int64_t* k_offsets, int n, int gr
     const int unit = form == kAttnFew ? kAttnWavesFew * kAttnStepFew : kAttnStepRows;
     const int64_t slots = form == kAttnRows ? 2 * cus : cus;
     cut(tiles[form], piece_keys(tiles[form], kv_heads, slots, form == kAttnFew ? 2 * unit : 4 * unit), unit, &out->form[form]);
+    share_out(kv_heads, &out->form[form]);
   }
 }
 

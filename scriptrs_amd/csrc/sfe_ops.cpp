@@ -21,9 +21,11 @@ struct sfe_attn_plan {
   int32_t heads = 0, kv_heads = 0, dim = 0, left = 0, right = 0;
   struct Form {
     int32_t n_items = 0, n_joins = 0;
+    int32_t share[9] = {0};
     size_t items = 0, joins = 0, part_o = 0, part_ml = 0;  // offsets into buf
   } form[sfe::kAttnForms];
   bool empty = true;  // no queries
+  size_t mask = 0;    // packed key mask
   int64_t total_q = 0, total_k = 0;
   void* buf = nullptr;
   size_t cap = 0;
@@ -162,10 +164,12 @@ int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_
     for (int i = 0; i < sfe::kAttnForms; ++i) {
       plan->form[i].n_items = (int32_t)h.form[i].items.size();
       plan->form[i].n_joins = (int32_t)h.form[i].joins.size();
+      memcpy(plan->form[i].share, h.form[i].share, sizeof(h.form[i].share));
       plan->form[i].items = place(h.form[i].items.size() * sizeof(sfe::AttnItem));
       plan->form[i].joins = place(h.form[i].joins.size() * sizeof(sfe::AttnJoin));
     }
     const size_t bytes = at;
+    plan->mask = place((size_t)sfe::attn_mask_words(plan->total_k) * sizeof(uint64_t));
     std::vector<char> table(bytes);
     auto put = [&](size_t o, const void* p, size_t size) {
       if (size) memcpy(table.data() + o, p, size);
@@ -227,7 +231,6 @@ int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const 
     a.k = tensor(k);
     a.v = tensor(v);
     a.o = tensor(out);
-    a.mask = key_mask;
     a.kv_heads = plan->kv_heads;
     a.group = plan->heads / plan->kv_heads;
     a.dim = plan->dim;
@@ -237,22 +240,30 @@ int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const 
     struct Call {
       sfe::AttnArgs a;
       const sfe_attn_plan* plan;
+      const uint8_t* key_mask;
       int dtype;
       hipStream_t stream;
-    } call{a, plan, dtype, static_cast<hipStream_t>(stream)};
-    return sfe::op_call(plan->ctx, call.stream, "attention", [](void* arg, int) -> hipError_t {
+    } call{a, plan, key_mask, dtype, static_cast<hipStream_t>(stream)};
+    return sfe::op_call(plan->ctx, call.stream, "attention", [](void* arg, int cus) -> hipError_t {
       Call& c = *static_cast<Call*>(arg);
       char* base = static_cast<char*>(c.plan->buf);
+      if (c.key_mask) {
+        uint64_t* words = reinterpret_cast<uint64_t*>(base + c.plan->mask);
+        const hipError_t e = sfe::launch_attn_mask(c.key_mask, c.plan->total_k, words, c.stream);
+        if (e != hipSuccess) return e;
+        c.a.mask = words;
+      }
       for (int i = 0; i < sfe::kAttnForms; ++i) {
         const auto& f = c.plan->form[i];
         if (!f.n_items) continue;
         c.a.n_items = f.n_items;
+        memcpy(c.a.share, f.share, sizeof(f.share));
         c.a.items = reinterpret_cast<const sfe::AttnItem*>(base + f.items);
         c.a.n_joins = f.n_joins;
         c.a.joins = reinterpret_cast<const sfe::AttnJoin*>(base + f.joins);
         c.a.part_o = reinterpret_cast<float*>(base + f.part_o);
         c.a.part_ml = reinterpret_cast<float2*>(base + f.part_ml);
-        const hipError_t e = sfe::launch_attn(c.a, i, c.dtype, c.stream);
+        const hipError_t e = sfe::launch_attn(c.a, i, c.dtype, cus, c.stream);
         if (e != hipSuccess) return e;
       }
       return hipSuccess;

@@ -81,6 +81,7 @@ struct AttnForm {
   std::vector<AttnItem> items;
   std::vector<AttnJoin> joins;
   int32_t parts = 0;  // pieces with a partial result
+  int32_t share[9];   // units of XCD x: [share[x], share[x + 1])
 };
 struct AttnPlanHost {
   AttnForm form[kAttnForms];
@@ -96,17 +97,21 @@ struct AttnTensor {
 };
 struct AttnArgs {
   AttnTensor q, k, v, o;
-  const uint8_t* mask;
+  const uint64_t* mask;  // packed, or null
   const AttnItem* items;
   const AttnJoin* joins;
   float* part_o;    // [piece][kv head][tile row][padded head dim]
   float2* part_ml;  // [piece][kv head][tile row]: (reference exponent, sum)
   int32_t n_items, n_joins, kv_heads, group, dim;
+  int32_t share[9];  // units of XCD x: [share[x], share[x + 1])
   int32_t left, right;
   float scale_log2;  // scale * log2(e)
 };
 inline int attn_padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : 128); }
-hipError_t launch_attn(const AttnArgs& a, int form, int type, hipStream_t stream);
+// Words of a packed key mask: a step's 64 keys may start within the last.
+inline int64_t attn_mask_words(int64_t keys) { return (keys + 63) / 64 + 1; }
+hipError_t launch_attn_mask(const uint8_t* mask, int64_t keys, uint64_t* words, hipStream_t stream);
+hipError_t launch_attn(const AttnArgs& a, int form, int type, int cus, hipStream_t stream);
 
 // ---- rotary positions (sfe_rotary.hip) ----------------------------------------------
 constexpr int kRotaryMaxPairs = 128;

@@ -891,7 +891,7 @@ __global__ __launch_bounds__(512, 2) void sfe_attn_tall_kernel(AttnArgs a) {
 // ---- few: 16 packed rows a workgroup, its waves share the keys ---------------------------
 
 template <typename T, int NT, bool MASKED>
-__global__ __launch_bounds__(256, 1) void sfe_attn_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWavesFew, 1) void sfe_attn_few_kernel(AttnArgs a) {
   typedef Geo<NT> G;
   typedef typename Mat<T>::V8 V8;
   typedef typename Mat<T>::V2 V2;
@@ -910,24 +910,6 @@ __global__ __launch_bounds__(256, 1) void sfe_attn_few_kernel(AttnArgs a) {
   const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), quarter = lane >> 4;
   const int dim_bytes = 2 * a.dim;
   const uint32_t base = lds_address(lds) + wave * 4 * kBuf;
-
-  const int r = row0 + (lane & 15);
-  const int rc = r < total ? r : total - 1;
-  const int pos = (int)((unsigned)rc / (unsigned)a.group);
-  int lo, hi;
-  visible(a, pos, lq, lk, &lo, &hi);
-  V8 q[NT];
-  {
-    const char* p = a.q.data + (q_row + pos) * a.q.row + (int64_t)(kvh * a.group + rc - pos * a.group) * a.q.head;
-#pragma unroll
-    for (int s = 0; s < NT; ++s) {
-      const int c = 4 * s + quarter;
-      S8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (16 * c < dim_bytes) v = *reinterpret_cast<const S8*>(p + 16 * c);
-      q[s] = __builtin_bit_cast(V8, v);
-    }
-  }
-  const int lo_all = __builtin_amdgcn_readlane(lo, 15), hi_all = __builtin_amdgcn_readlane(hi, 0);
 
   const int lrow = lane / G::kChunks, lchunk = lane % G::kChunks;
   uint32_t k_addr[NT], v_addr[ND];
@@ -961,27 +943,45 @@ __global__ __launch_bounds__(256, 1) void sfe_attn_few_kernel(AttnArgs a) {
     }
   };
 
-  F4 o[ND];
-#pragma unroll
-  for (int n = 0; n < ND; ++n) o[n] = F4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kNever, l = 0.0f;
+  // the first two steps' loads, those of the queries behind them
   constexpr int kTurn = kWaves * kStep;  // keys of all waves' steps
   uint32_t bits = ~0u, bits_next = ~0u;
   if (MASKED && first < kv1) bits = (uint32_t)key_bits(a, k_row + first);
   if (first < kv1) load_step(0, bits);
+  if (MASKED && first + kTurn < kv1) bits_next = (uint32_t)key_bits(a, k_row + first + kTurn);
+  if (first + kTurn < kv1) load_step(1, bits_next);
+  const int r = row0 + (lane & 15);
+  const int rc = r < total ? r : total - 1;
+  const int pos = (int)((unsigned)rc / (unsigned)a.group);
+  int lo, hi;
+  visible(a, pos, lq, lk, &lo, &hi);
+  V8 q[NT];
+  {
+    const char* p = a.q.data + (q_row + pos) * a.q.row + (int64_t)(kvh * a.group + rc - pos * a.group) * a.q.head;
+#pragma unroll
+    for (int s = 0; s < NT; ++s) {
+      const int c = 4 * s + quarter;
+      S8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * c < dim_bytes) v = *reinterpret_cast<const S8*>(p + 16 * c);
+      q[s] = __builtin_bit_cast(V8, v);
+    }
+    // (waited for here: a wait within the loop would be one for the loads into LDS too)
+#pragma unroll
+    for (int s = 0; s < NT; ++s) asm volatile("" : "+v"(q[s]));
+  }
+  const int lo_all = __builtin_amdgcn_readlane(lo, 15), hi_all = __builtin_amdgcn_readlane(hi, 0);
+
+  F4 o[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n) o[n] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kNever, l = 0.0f;
   int buf = 0;
   for (int kv = first; kv < kv1; kv += kTurn, buf ^= 1) {
-    const bool more = kv + kTurn < kv1;
-    // (a wave's LDS buffers are its own: its reads of the buffer to be filled are
-    // done, and its loads are waited for by count)
-    if (MASKED && more) bits_next = (uint32_t)key_bits(a, k_row + kv + kTurn);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) {
-      load_step(buf ^ 1, bits_next);
+    // (a wave's LDS buffers are its own: its loads are waited for by count)
+    if (kv + kTurn < kv1)
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
-    } else {
+    else
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
     const int end = kv1 < kv + kStep ? kv1 : kv + kStep;
     const uint32_t kb = buf * kBuf;
     F4 s[2];
@@ -1052,6 +1052,11 @@ __global__ __launch_bounds__(256, 1) void sfe_attn_few_kernel(AttnArgs a) {
       o[n] = Mat<T>::m16(v, p, o[n]);
     }
     bits = bits_next;
+    if (kv + 2 * kTurn < kv1) {  // into the buffer just read
+      if (MASKED) bits_next = (uint32_t)key_bits(a, k_row + kv + 2 * kTurn);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      load_step(buf, bits_next);
+    }
   }
   l += __shfl_xor(l, 16);
   l = sum_halves(l);
@@ -1067,7 +1072,7 @@ __global__ __launch_bounds__(256, 1) void sfe_attn_few_kernel(AttnArgs a) {
     *reinterpret_cast<F4*>(ow + (wave * 16 + (lane & 15)) * kRowF + 16 * n + 4 * quarter) = o[n];
   if (quarter == 0) ml[wave * 16 + lane] = make_float2(m, l);
   __syncthreads();
-  for (int e = t; e < 16 * (kDim / 4); e += 256) {
+  for (int e = t; e < 16 * (kDim / 4); e += 64 * kWaves) {
     const int row = e / (kDim / 4), d = 4 * (e % (kDim / 4));
     float mm = kNever;
     for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, ml[w * 16 + row].x);
@@ -1098,37 +1103,47 @@ __global__ __launch_bounds__(256, 1) void sfe_attn_few_kernel(AttnArgs a) {
 
 // ---- pieces added up ---------------------------------------------------------------------
 
-// A wave per packed row: sum over the row's pieces, 2 channels a lane.
+// A workgroup per packed row, 2 channels a lane: each wave adds every fourth piece up, relative
+// to the row's largest reference exponent, and the first wave the four sums.
 template <typename T, int NT, int TILE>
 __global__ __launch_bounds__(256) void sfe_attn_join_kernel(AttnArgs a) {
   typedef typename Mat<T>::V2 V2;
   constexpr int kDim = 32 * NT;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = (int)(threadIdx.x & 63);
-  const int row = (int)(w % TILE);
-  const int64_t jk = w / TILE;
-  const int kvh = (int)(jk % a.kv_heads);
-  if (jk / a.kv_heads >= a.n_joins) return;
+  __shared__ float2 part[4][64];
+  __shared__ float sums[4];
+  const int64_t jk = blockIdx.x / TILE;
+  const int row = (int)(blockIdx.x % TILE), kvh = (int)(jk % a.kv_heads);
+  const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
   const AttnJoin j = a.joins[jk / a.kv_heads];
   const int rr = j.row0 + row;
   if (rr >= j.lq * a.group) return;
+  // piece p of the row is at at0 + p * step
+  const int64_t at0 = ((int64_t)j.part0 * a.kv_heads + kvh) * TILE + row, step = (int64_t)a.kv_heads * TILE;
   float m = kNever;
-  for (int p = 0; p < j.parts; ++p)
-    m = fmaxf(m, a.part_ml[((int64_t)(j.part0 + p) * a.kv_heads + kvh) * TILE + row].x);
+  for (int p = lane; p < j.parts; p += 64) m = fmaxf(m, a.part_ml[at0 + p * step].x);
+  m = max_halves(m);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
   float x = 0.0f, y = 0.0f, sum = 0.0f;
-  for (int p = 0; p < j.parts; ++p) {
-    const int64_t at = ((int64_t)(j.part0 + p) * a.kv_heads + kvh) * TILE + row;
+#pragma unroll 8
+  for (int p = wave; p < j.parts; p += 4) {
+    const int64_t at = at0 + p * step;
     const float2 ml = a.part_ml[at];
-    if (ml.x == kNever && ml.y == 0.0f) continue;  // (saw nothing)
-    const float f = exp2_fast(ml.x - m);
+    // (a piece that saw nothing: all zeros)
+    const float f = ml.x == kNever && ml.y == 0.0f ? 0.0f : exp2_fast(ml.x - m);
     sum += ml.y * f;
-    if (2 * lane < kDim) {
-      const float2 v = *reinterpret_cast<const float2*>(a.part_o + at * kDim + 2 * lane);
-      x += v.x * f;
-      y += v.y * f;
-    }
+    float2 v = make_float2(0.0f, 0.0f);
+    if (2 * lane < kDim) v = *reinterpret_cast<const float2*>(a.part_o + at * kDim + 2 * lane);
+    x += v.x * f;
+    y += v.y * f;
   }
-  if (2 * lane >= a.dim) return;
+  part[wave][lane] = make_float2(x, y);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  if (wave > 0 || 2 * lane >= a.dim) return;
+  x = (part[0][lane].x + part[1][lane].x) + (part[2][lane].x + part[3][lane].x);
+  y = (part[0][lane].y + part[1][lane].y) + (part[2][lane].y + part[3][lane].y);
+  sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
   const int at = (int)((unsigned)rr / (unsigned)a.group);
   char* p = const_cast<char*>(a.o.data) + (j.q_row + at) * a.o.row + (int64_t)(kvh * a.group + rr - at * a.group) * a.o.head;
@@ -1156,14 +1171,14 @@ hipError_t run_form(const AttnArgs& a, int cus, hipStream_t stream) {
       sfe_attn_rows_kernel<T, NT, false><<<few, dim3(256), 0, stream>>>(a);
   } else {
     if (a.mask)
-      sfe_attn_few_kernel<T, NT, true><<<blocks, dim3(256), 0, stream>>>(a);
+      sfe_attn_few_kernel<T, NT, true><<<blocks, dim3(64 * kAttnWavesFew), 0, stream>>>(a);
     else
-      sfe_attn_few_kernel<T, NT, false><<<blocks, dim3(256), 0, stream>>>(a);
+      sfe_attn_few_kernel<T, NT, false><<<blocks, dim3(64 * kAttnWavesFew), 0, stream>>>(a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.n_joins) return e;
   sfe_attn_join_kernel<T, NT, kTile>
-      <<<dim3((unsigned)((int64_t)a.n_joins * a.kv_heads * kTile / 4)), dim3(256), 0, stream>>>(a);
+      <<<dim3((unsigned)((int64_t)a.n_joins * a.kv_heads * kTile)), dim3(256), 0, stream>>>(a);
   return hipGetLastError();
 }
 

@@ -42,14 +42,15 @@ void cut(const std::vector<Tile>& tiles, int64_t most, int unit, AttnForm* f) {
   }
 }
 
-// The longest piece for which the tiles' pieces fill `slots` workgroups about
-// once (no cut where the tiles alone do), at least `least` keys.
-int64_t piece_keys(const std::vector<Tile>& tiles, int kv_heads, int64_t slots, int64_t least) {
+// The longest piece for which the tiles' pieces fill `slots` workgroups about once, at least
+// `least` keys; tiles of up to `whole` keys are not cut (adding the pieces up is one more launch).
+int64_t piece_keys(const std::vector<Tile>& tiles, int kv_heads, int64_t slots, int64_t least, int64_t whole) {
   int64_t total = 0, longest = 0;
   for (const Tile& t : tiles) {
     total += t.kv1 - t.kv0;
     longest = std::max<int64_t>(longest, t.kv1 - t.kv0);
   }
+  if (longest <= whole) return std::max(least, longest);
   total *= kv_heads;
   return std::max(least, std::min(longest, (total + slots - 1) / slots));
 }
@@ -75,12 +76,27 @@ double tile_costs(int form, int64_t lq, int64_t lk, int group, int32_t left, int
   return cost;
 }
 
-// The form of a sequence.  few: up to 16 packed rows, as single tokens have, where the call has
-// only such sequences or the keys are many; a launch of its own for a few short ones would cost
-// more than their place among the rows (256 clips of 13-251 frames: 51 us with it, 46 without).
+// Whether the few form takes the whole call: only sequences of up to 16 packed rows, or so few
+// tiles of 16 that they get a CU each and not many keys, so that the whole call is one trip
+// through memory (one sequence of 126, 8 heads of 128: 7.3 us against 9.9 in the rows form; 500: 11.3 / 24.4; 1125,
+// 568 tiles: 43.7 / 38.9).
+bool whole_call_few(const int64_t* q_offsets, const int64_t* k_offsets, int n, int group, int kv_heads, int cus) {
+  int64_t units = 0, rows = 0, keys = 0;
+  for (int s = 0; s < n; ++s) {
+    const int64_t total = (q_offsets[s + 1] - q_offsets[s]) * group;
+    units += (total + kAttnTileFew - 1) / kAttnTileFew * kv_heads;
+    rows = std::max(rows, total);
+    keys = std::max(keys, k_offsets[s + 1] - k_offsets[s]);
+  }
+  return rows <= kAttnTileFew || (units <= cus * 5 / 4 && keys <= 2048);
+}
+
+// The form of a sequence of a call that does not take the few form as a whole: few for up to 16 packed rows
+// over many keys (a launch of its own for a few short ones would cost more than their place
+// among the rows: 256 clips of 13-251 frames 51 us with it, 46 without).
 int form_of(int64_t lq, int64_t lk, int group, int head_dim, int32_t left, int32_t right, bool all_few) {
   const int64_t total = lq * group;
-  if (total <= kAttnTileFew && (all_few || lk >= 1024)) return kAttnFew;
+  if (all_few || (total <= kAttnTileFew && lk >= 1024)) return kAttnFew;
   if (total <= kAttnTileRows || attn_padded_dim(head_dim) <= 64) return kAttnRows;
   return tile_costs(kAttnTall, lq, lk, group, left, right) < tile_costs(kAttnRows, lq, lk, group, left, right) ? kAttnTall
                                                                                                               : kAttnRows;
@@ -110,8 +126,7 @@ void share_out(int kv_heads, AttnForm* f) {
 
 void attn_plan(const int64_t* q_offsets, const int64_t* k_offsets, int n, int group, int kv_heads, int head_dim,
                int32_t left, int32_t right, int cus, AttnPlanHost* out) {
-  bool all_few = true;
-  for (int s = 0; s < n; ++s) all_few = all_few && (q_offsets[s + 1] - q_offsets[s]) * group <= kAttnTileFew;
+  const bool all_few = whole_call_few(q_offsets, k_offsets, n, group, kv_heads, cus);
   std::vector<Tile> tiles[kAttnForms];
   for (int s = 0; s < n; ++s) {
     const int64_t lq = q_offsets[s + 1] - q_offsets[s], lk = k_offsets[s + 1] - k_offsets[s];
@@ -126,12 +141,16 @@ void attn_plan(const int64_t* q_offsets, const int64_t* k_offsets, int n, int gr
           Tile{q_offsets[s], k_offsets[s], (int32_t)lq, (int32_t)lk, (int32_t)(t * tile), (int32_t)lo, (int32_t)hi});
     }
   }
-  for (int form = 0; form < kAttnForms; ++form) {
-    const int unit = form == kAttnFew ? kAttnWavesFew * kAttnStepFew : kAttnStepRows;
-    const int64_t slots = form == kAttnRows ? 2 * cus : cus;
-    cut(tiles[form], piece_keys(tiles[form], kv_heads, slots, form == kAttnFew ? 2 * unit : 4 * unit), unit, &out->form[form]);
+  // (64 single-token steps of 4 beams over 126-1500 keys, 4 kv heads: 27 us cut to 256 workgroups' worth,
+  // 21 whole; 4 over 2000 keys 22.6 whole)
+  const int unit_few = kAttnWavesFew * kAttnStepFew;
+  auto lay = [&](int form, int unit, int64_t slots, int64_t least, int64_t whole) {
+    cut(tiles[form], piece_keys(tiles[form], kv_heads, slots, least, whole), unit, &out->form[form]);
     share_out(kv_heads, &out->form[form]);
-  }
+  };
+  lay(kAttnTall, kAttnStepRows, cus, 4 * kAttnStepRows, 0);
+  lay(kAttnRows, kAttnStepRows, 2 * cus, 4 * kAttnStepRows, 0);
+  lay(kAttnFew, unit_few, cus, 4 * unit_few, 2 * (int64_t)tiles[kAttnFew].size() * kv_heads >= cus ? 2048 : 768);
 }
 
 }  // namespace sfe

@@ -145,10 +145,9 @@ int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_
     plan->total_k = n ? k_offsets[n] : 0;
     sfe::AttnPlanHost h;
     sfe::attn_plan(q_offsets, k_offsets, n, group, kv_heads, head_dim, plan->left, plan->right, sfe::op_cus(ctx), &h);
-    // a launch holds fewer than 2^32 threads
-    const int64_t most = (int64_t)(UINT32_MAX / 512 - 8) / kv_heads;
+    // (a launch holds fewer than 2^32 threads: 512 for each of 8 shares of at most all units)
     for (const auto& f : h.form) {
-      if ((int64_t)f.items.size() > most) return op_fail(SFE_INVALID_ARG, "batch too large for one launch");
+      if ((int64_t)f.items.size() * kv_heads > 1000000) return op_fail(SFE_INVALID_ARG, "batch too large for one launch");
       if (!f.items.empty()) plan->empty = false;
     }
     if (plan->empty) {

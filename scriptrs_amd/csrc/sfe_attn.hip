@@ -65,9 +65,12 @@ struct Mat<Hf> {
   static constexpr uint32_t kExp = 0x7c007c00, kCarry = 0x04000400, kOne = 0x3c00;
 };
 
-constexpr float kNever = -1e30f;  // reference exponent before the first visible key
+constexpr float kNever = -3e38f;  // reference exponent before the first visible key: below every score
 constexpr float kRise = 15.0f;    // the reference moves when a score passes it by this much
 constexpr float kBelow = 7.0f;    // ... to this much below the maximum
+// Scores past this are scaled and rounded before the reference is taken off: the f32 reference of such
+// a row is a rounded score itself, and exact products less it would be off by its rounding.
+constexpr float kLarge = 1048576.0f;
 constexpr uint32_t kOutside = 0x80000000u;  // an offset past every buffer's range
 constexpr int kBufWord3 = 0x00020000;
 
@@ -118,6 +121,13 @@ __device__ __forceinline__ typename Mat<T>::V8 read_v(uint32_t lo, uint32_t hi) 
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// s * c rounded, less m (never one fused operation).
+__device__ __forceinline__ float scaled_less(float s, float c, float m) {
+#pragma clang fp contract(off)
+  const float x = s * c;
+  return x - m;
+}
 
 // The larger (sum) of this lane's value and that of the lane 32 away.
 __device__ __forceinline__ float max_halves(float x) {
@@ -280,6 +290,9 @@ __device__ __forceinline__ bool not_finite(const F16 (&o)[NT]) {
   return (z[0] + z[1]) + (z[2] + z[3]) != 0.0f;
 }
 
+// Whether a row's scores were too large for the loops without care.
+__device__ __forceinline__ bool large(float m) { return fabsf(m) > kLarge && m != kNever; }
+
 // Writes a wave's 32 rows.  The two lanes of a row hold 4 channels of every 8 each; an exchange
 // gives either all 8 of every other chunk, 16 bytes a store.  (Through LDS, so that a store
 // instruction wrote whole rows, the end of a workgroup took 1.5 us against 0.8.)
@@ -317,7 +330,8 @@ __device__ __forceinline__ void store_rows(const AttnArgs& a, const F16 (&o)[NT]
 // in flight and, once the scores are there, its queries.  (280 sequences of 188, 8 heads of 128:
 // 128 us with a workgroup per unit.)  Units whose result is not finite are noted and done
 // again at the end, CAREFUL: values of V that are not finite are kept from the rows that do not
-// see their key (they would reach them as 0 * inf).  280 sequences of 188, 8 heads of 128: 119 us, 3.6 TB/s; 45,000
+// see their key (they would reach them as 0 * inf), and scores past 2^20 are rounded before their reference is
+// taken off.  280 sequences of 188, 8 heads of 128: 119 us, 3.6 TB/s; 45,000
 // rows that see 128 to either side 130 us, 2.8 TB/s; 256 of 13-251, 8 heads of 64, masked, 38 us, 2.2 TB/s.  Bound by the
 // latency of a unit's few steps (its vector instructions take 36-44% of the time).
 // Units of a workgroup at most.  (One after the other in 2 or 3 workgroups a CU for the whole
@@ -490,7 +504,7 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void sfe_attn_rows_kernel(Att
 #pragma unroll
           for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
         if (__any(top * a.scale_log2 > m + kRise)) {
-          const float nm = fmaxf(m, max_halves(top) * a.scale_log2 - kBelow);
+          const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, kBelow));
           const float f = exp2_fast(m - nm);
           m = nm;
           l *= f;
@@ -499,14 +513,16 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void sfe_attn_rows_kernel(Att
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[n][i] *= f;
         }
+        auto less = [&](float x) {
+          return kCareful ? scaled_less(x, a.scale_log2, m) : __builtin_fmaf(x, a.scale_log2, -m);
+        };
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         V8 p[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const F2 w = {exp2_fast(__builtin_fmaf(s[h][i], a.scale_log2, -m)),
-                          exp2_fast(__builtin_fmaf(s[h][i + 1], a.scale_log2, -m))};
+            const F2 w = {exp2_fast(less(s[h][i])), exp2_fast(less(s[h][i + 1]))};
             sum[i % 4] += w.x;
             sum[i % 4 + 1] += w.y;
             const V2 c = __builtin_convertvector(w, V2);
@@ -574,7 +590,7 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void sfe_attn_rows_kernel(Att
     const bool more = u + stride < last;
     const Unit next = unit_at(a, more ? u + stride : u);
     run(std::false_type(), un, next, more, bits, bits_next);
-    if (__any(not_finite(o)) && lane == 0) again[k] = 1;
+    if (__any(not_finite(o) || large(m)) && lane == 0) again[k] = 1;
     un = next;
   }
   __syncthreads();
@@ -814,7 +830,7 @@ __global__ __launch_bounds__(512, 2) void sfe_attn_tall_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
       if (__any(top * a.scale_log2 > m + kRise)) {
-        const float nm = fmaxf(m, max_halves(top) * a.scale_log2 - kBelow);
+        const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, kBelow));
         const float f = exp2_fast(m - nm);
         m = nm;
         l *= f;
@@ -823,13 +839,15 @@ __global__ __launch_bounds__(512, 2) void sfe_attn_tall_kernel(AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[n][i] *= f;
       }
+      auto less = [&](float x) {
+        return kCareful ? scaled_less(x, a.scale_log2, m) : __builtin_fmaf(x, a.scale_log2, -m);
+      };
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const F2 w = {exp2_fast(__builtin_fmaf(s[h][i], a.scale_log2, -m)),
-                        exp2_fast(__builtin_fmaf(s[h][i + 1], a.scale_log2, -m))};
+          const F2 w = {exp2_fast(less(s[h][i])), exp2_fast(less(s[h][i + 1]))};
           sum[i % 4] += w.x;
           sum[i % 4 + 1] += w.y;
           const V2 c = __builtin_convertvector(w, V2);
@@ -869,8 +887,8 @@ __global__ __launch_bounds__(512, 2) void sfe_attn_tall_kernel(AttnArgs a) {
     l = sum_halves(l);
   };
   run(std::false_type());
-  // A result that is not finite may be a hidden value's: then once more, with care
-  const int flag = __any(not_finite(o));
+  // A result that is not finite may be a hidden value's, one of large scores off: then once more, with care
+  const int flag = __any(not_finite(o) || large(m));
   if (lane == 0) again[wave] = flag;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   if (__any(again[lane & 7])) {
@@ -1022,7 +1040,7 @@ __global__ __launch_bounds__(64 * kAttnWavesFew, 1) void sfe_attn_few_kernel(Att
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
     if (__any(top * a.scale_log2 > m + kRise)) {
       top = fmaxf(top, __shfl_xor(top, 16));
-      const float nm = fmaxf(m, max_halves(top) * a.scale_log2 - kBelow);
+      const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, kBelow));
       const float f = exp2_fast(m - nm);
       m = nm;
       l *= f;
@@ -1034,8 +1052,8 @@ __global__ __launch_bounds__(64 * kAttnWavesFew, 1) void sfe_attn_few_kernel(Att
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const F2 w = {exp2_fast(__builtin_fmaf(s[h][i], a.scale_log2, -m)),
-                      exp2_fast(__builtin_fmaf(s[h][i + 1], a.scale_log2, -m))};
+        const F2 w = {exp2_fast(scaled_less(s[h][i], a.scale_log2, m)),
+                      exp2_fast(scaled_less(s[h][i + 1], a.scale_log2, m))};
         l += w.x + w.y;
         const V2 c = __builtin_convertvector(w, V2);
         p[4 * h + i] = c.x;

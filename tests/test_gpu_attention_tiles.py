@@ -271,3 +271,19 @@ def test_captured(ops):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dim,lengths", [(64, [33]), (128, [33]), (64, FILL), (128, FILL + [600])], ids=["few64", "few128", "rows", "tall"])
+def test_scores_near_the_lowest(ops, dim, lengths):
+    """All of a row's scores far below zero (down to -1e38): the highest still takes the whole weight."""
+    import torch
+    o = offsets(lengths)
+    g = torch.Generator(device="cuda").manual_seed(14)
+    q = torch.full((o[-1], 2, dim), 1e17, device="cuda").bfloat16()
+    # key j of a sequence scores about -(j + 1) 1e34 x dim, up to the 40th
+    place = torch.cat([torch.arange(n, device="cuda") for n in lengths]).clamp(max=40)
+    k = (-(place + 1.0) * 1e17)[:, None, None].expand(-1, 2, dim).bfloat16()
+    v = torch.randn(o[-1], 2, dim, device="cuda", generator=g).bfloat16()
+    out = ops.attention(ops.attention_plan(o, o, 2, 2, dim), q, k, v, scale=1.0)
+    first = torch.tensor(o[:-1], device="cuda").repeat_interleave(torch.tensor(lengths, device="cuda"))
+    assert torch.equal(out, v[first])

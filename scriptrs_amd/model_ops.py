@@ -93,9 +93,10 @@ class AttentionPlan:
     """Division of a batch's sequences into tiles; made by
     ``ModelOps.attention_plan`` and good for every layer over the same lengths."""
 
-    def __init__(self, ops: "ModelOps", handle, total_q: int, total_k: int, heads: int, kv_heads: int, head_dim: int):
+    def __init__(self, ops: "ModelOps", handle, first_q: int, total_q: int, total_k: int, heads: int, kv_heads: int,
+                 head_dim: int):
         self._ops, self._handle = ops, handle
-        self.total_q, self.total_k = total_q, total_k
+        self.first_q, self.total_q, self.total_k = first_q, total_q, total_k
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
         self.scale = 1.0 / math.sqrt(head_dim)
 
@@ -158,13 +159,15 @@ class ModelOps:
         _check(_lib.lib().sfe_attention_plan(self._fe._handle(), _ip(qo), _ip(ko), qo.size - 1, int(heads), int(kv_heads),
                                              int(head_dim), int(left), int(right), _stream_handle(stream),
                                              ctypes.byref(handle)))
-        return AttentionPlan(self, handle, int(qo[-1]), int(ko[-1]), int(heads), int(kv_heads), int(head_dim))
+        return AttentionPlan(self, handle, int(qo[0]), int(qo[-1]), int(ko[-1]), int(heads), int(kv_heads),
+                             int(head_dim))
 
     def attention(self, plan: AttentionPlan, q, k, v, key_mask=None, scale: float | None = None, stream=None, out=None):
         """``softmax(scale q k^T) v`` of each of the plan's sequences:
         ``q`` [queries, heads, head_dim], ``k`` and ``v`` [keys, kv_heads, head_dim] in
         bfloat16 or float16 (views of a joint projection will do), ``key_mask``
-        [keys] bool, False hides a key.  Queries that see no key give zeros."""
+        [keys] bool, False hides a key.  Queries that see no key give zeros, and so do rows
+        before the first sequence and past the last."""
         handle = plan._handle
         if handle is None:
             raise InvalidModelOutput("the plan is closed")
@@ -202,14 +205,25 @@ class ModelOps:
             if out.get_device() != device:
                 _wrong_device("out", out, device)
             _heads(out, "out", q.shape, ho)
-        if q.shape[0] > plan.total_q:
-            out[plan.total_q:].zero_()
         pq, pk, pv, po = self._hp
         rc = self._lib.sfe_attention(handle, code, pq, pk, pv, mask, plan.scale if scale is None else scale, po,
                                      self._stream(stream))
         if rc:
             _check(rc)
+        if plan.first_q or q.shape[0] > plan.total_q:
+            self._zero_outside(plan, out, stream)
         return out
+
+    def _zero_outside(self, plan: AttentionPlan, out, stream) -> None:
+        """Zeros the rows of no sequence, on the call's stream."""
+        torch = self._torch
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        elif not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(_stream_handle(stream).value or 0, device=self.device)
+        with torch.cuda.stream(stream):
+            out[:plan.first_q].zero_()
+            out[plan.total_q:].zero_()
 
     # -- rotary positions ----------------------------------------------------------
     def rotary(self, table: RotaryTable, positions, q, k=None, inverse: bool = False, inplace: bool = False,

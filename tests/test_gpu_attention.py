@@ -316,3 +316,27 @@ def test_refusals(ops):
         ops.attention(plan, x, x, x)
     empty = ops.attention_plan([0], [0], 2, 2, 64)
     assert ops.attention(empty, x[:0], x[:0], x[:0]).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_rows_of_no_sequence_are_zero(ops, own_stream):
+    """Rows before the first sequence and past the last, on the call's stream; a refused call writes nothing."""
+    import torch
+    from scriptrs_amd.frontend import InvalidModelOutput
+    g = torch.Generator(device="cuda").manual_seed(15)
+    q, k, v = (torch.randn(40, 2, 64, device="cuda", generator=g).bfloat16() for _ in range(3))
+    out = torch.full_like(q, 7.0)
+    stream = torch.cuda.Stream() if own_stream else None
+    torch.cuda.synchronize()
+    plan = ops.attention_plan([3, 20, 33], [5, 20, 40], 2, 2, 64, stream=stream)
+    with pytest.raises(InvalidModelOutput):
+        ops.attention(plan, q, k, v, scale=-1.0, stream=stream, out=out)
+    torch.cuda.synchronize()
+    assert torch.all(out == 7.0)
+    assert ops.attention(plan, q, k, v, stream=stream, out=out) is out
+    torch.cuda.synchronize()
+    assert not out[:3].any() and not out[33:].any()
+    cut = ops.attention_plan([0, 17, 30], [0, 15, 35], 2, 2, 64)
+    assert torch.equal(out[3:33], ops.attention(cut, q[3:33], k[5:], v[5:]))
+    none = ops.attention_plan([5], [5], 2, 2, 64)
+    assert not ops.attention(none, q, k, v).any()

@@ -371,7 +371,8 @@ int sfe_residual_norm(sfe_ctx* ctx, const sfe_residual* args, void* stream);
 /* A step of beam search over logits [streams * beams][vocab] (rows row_stride
  * elements apart): for each stream the `beams` best of its beams * vocab candidates
  *   scores[w] + logit[w][t] - log sum_t exp(logit[w][t]),
- * best first, ties to the lowest (w, t).  A beam with finished[w] != 0 (NULL: none)
+ * best first, ties to the lowest (w, t).  Totals are f32: where a beam's unequal logits give equal
+ * totals at the last place, vocabularies above 2,048 may keep the larger logit.  A beam with finished[w] != 0 (NULL: none)
  * has the one candidate (scores[w], end_token) and its logits are not read.
  * Totals of -inf or NaN are no candidates (a stream's first step gives all beams but
  * one the score -inf); a place without a candidate gets score -inf, token -1 and

@@ -79,13 +79,14 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 }
 
 // The rows of a tensor's head as a raw buffer that moves along them: from row `row`, `rows`
-// of them in reach (as far as 32-bit offsets go; the others read as zeros).
+// of them in reach (as far as 32-bit offsets go; the others read as zeros; without rows, none, whatever the
+// stride: rows of one address, stride 0, too).
 struct RowBuffer {
   uint64_t at;
   int64_t bytes;
   __device__ __forceinline__ RowBuffer(const AttnTensor& t, int64_t row, int64_t rows, int head, int dim_bytes)
       : at((uint64_t)(uintptr_t)t.data + (uint64_t)(row * t.row + (int64_t)head * t.head)),
-        bytes((rows - 1) * t.row + dim_bytes) {}
+        bytes(rows > 0 ? (rows - 1) * t.row + dim_bytes : 0) {}
   __device__ __forceinline__ void advance(int64_t by) {
     at += (uint64_t)by;
     bytes -= by;

@@ -6,7 +6,8 @@
 // -inf or NaN are no candidates, and places without one hold score -inf, token
 // -1 and their own beam as parent.
 //
-// Within a row, candidates order as its logits do.  Small vocabularies: one launch, a
+// Within a row, candidates order as its logits do, but that unequal logits may have totals that round to
+// the same f32: the row's cut to `beams` is then by the logits, which say more.  Small vocabularies: one launch, a
 // workgroup per stream and a wave per row, the row in registers.  Others: two; the
 // first reads each logit once, a workgroup leaving its span's maximum, sum of
 // exponentials and `beams` best logits, and the second chooses among beams * spans *

@@ -340,3 +340,23 @@ def test_rows_of_no_sequence_are_zero(ops, own_stream):
     assert torch.equal(out[3:33], ops.attention(cut, q[3:33], k[5:], v[5:]))
     none = ops.attention_plan([5], [5], 2, 2, 64)
     assert not ops.attention(none, q, k, v).any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_no_keys_at_all(ops, dim):
+    """Without a key nothing of k and v is read, whatever their stride (C callers: null, stride 0)."""
+    import ctypes
+
+    import torch
+    from scriptrs_amd import _lib
+    o = offsets([200] * 50)
+    plan = ops.attention_plan(o, [0] * 51, 8, 8, dim)
+    q = torch.randn(o[-1], 8, dim, device="cuda").bfloat16()
+    out = torch.full_like(q, 7.0)
+    rows, none = 8 * dim, _lib.SfeHeads(None, 0, 0)
+    args = [ctypes.byref(h) for h in (_lib.SfeHeads(q.data_ptr(), rows, dim), none, none)]
+    to = _lib.SfeHeads(out.data_ptr(), rows, dim)
+    rc = _lib.lib().sfe_attention(plan._handle, _lib.SFE_BF16, *args, None, 0.125, ctypes.byref(to),
+                                  ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == _lib.SFE_OK, _lib.last_error()
+    assert not out.any()

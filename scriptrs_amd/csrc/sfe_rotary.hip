@@ -58,8 +58,10 @@ constexpr int kRotaryTable = 4096;  // (cosine, sine) of a workgroup's rows and 
 // all RB loads issued before the first store (outputs may be the inputs, so the
 // compiler cannot move loads past stores).  Places of a row, `places`: for each
 // head turning units, then copied ones.  N > 1: a unit is 16 bytes of N channels:
-// half, two vectors R/2 apart; interleaved, one vector of N / 2 pairs.  N = 1: a
-// pair, or a copied channel (tensors whose vectors are not aligned).
+// half, two vectors R/2 apart; interleaved, one vector of N / 2 pairs; 8 bytes where 16 do not divide
+// the parts or are not aligned (52,640 rows of 2 x 8 heads of 80 in bf16, 40 turned in halves: 78 us, 198 by
+// the pair; 80 turned, of 16 bytes, 54).  N = 1: a pair, or a copied channel (tensors whose
+// vectors are not aligned).
 template <typename T, int N, bool INTERLEAVED, int RB>
 __global__ __launch_bounds__(kRotaryThreads) void sfe_rotary_kernel(RotaryArgs a, int64_t first, uint32_t places,
                                                                     uint32_t slots, uint32_t chunks, uint32_t per) {
@@ -148,15 +150,23 @@ hipError_t run_units(const RotaryArgs& a, int cus, hipStream_t stream) {
   return many ? run_rows<T, N, INTERLEAVED, 4>(a, places, slots, stream) : run_rows<T, N, INTERLEAVED, 1>(a, places, slots, stream);
 }
 
+// Whether all vectors of N channels lie whole in a tensor's parts, aligned to their size.
+template <typename T, int N, bool INTERLEAVED>
+bool vectors(const RotaryArgs& a) {
+  bool ok = a.rotary % (INTERLEAVED ? N : 2 * N) == 0 && a.dim % N == 0;
+  for (const RotaryTensor& t : a.t)
+    if (t.heads)
+      ok = ok && (reinterpret_cast<uintptr_t>(t.x) | reinterpret_cast<uintptr_t>(t.y)) % (N * sizeof(T)) == 0 &&
+           (t.x_row | t.x_head | t.y_row | t.y_head) % N == 0;
+  return ok;
+}
+
 template <typename T, bool INTERLEAVED>
 hipError_t run(const RotaryArgs& a, int cus, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
-  bool vec = a.rotary % (INTERLEAVED ? N : 2 * N) == 0 && a.dim % N == 0;
-  for (const RotaryTensor& t : a.t)
-    if (t.heads)
-      vec = vec && (reinterpret_cast<uintptr_t>(t.x) | reinterpret_cast<uintptr_t>(t.y)) % 16 == 0 &&
-            (t.x_row | t.x_head | t.y_row | t.y_head) % N == 0;
-  return vec ? run_units<T, N, INTERLEAVED>(a, cus, stream) : run_units<T, 1, INTERLEAVED>(a, cus, stream);
+  if (vectors<T, N, INTERLEAVED>(a)) return run_units<T, N, INTERLEAVED>(a, cus, stream);
+  if (vectors<T, N / 2, INTERLEAVED>(a)) return run_units<T, N / 2, INTERLEAVED>(a, cus, stream);
+  return run_units<T, 1, INTERLEAVED>(a, cus, stream);
 }
 
 template <typename T>

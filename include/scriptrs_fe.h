@@ -304,7 +304,7 @@ void sfe_attention_plan_free(sfe_attn_plan* plan);
  * [head_dim], of dtype SFE_BF16 or SFE_F16, 16-byte aligned (data and
  * strides), rows less than 2^23 elements apart.  key_mask: a byte for each
  * key row, 0 hides it from every query (NULL: none hidden).  scale > 0.  out must
- * not overlap the inputs. */
+ * not overlap the inputs; its rows of no sequence are not written. */
 int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
                   const uint8_t* key_mask, float scale, const sfe_heads* out, void* stream);
 

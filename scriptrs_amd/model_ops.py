@@ -375,8 +375,8 @@ class ModelOps:
         return new, parents, tokens, ended
 
     def beam_reorder(self, parents, states, dim: int = 0, out=None, stream=None):
-        """``states`` (contiguous device tensors whose dimension ``dim`` is streams *
-        beams) with every beam's state taken from its parent, in one launch.
+        """``states`` (contiguous device tensors whose dimension ``dim``, from the end if negative, is
+        streams * beams) with every beam's state taken from its parent, in one launch.
         ``out``: tensors to write, ``states`` themselves for in place; returns the list
         written."""
         torch = self._torch
@@ -397,7 +397,8 @@ class ModelOps:
             if s.get_device() != self.device:
                 _wrong_device(f"state {i}", s, self.device)
             full = s.shape
-            if not s.is_contiguous() or len(full) <= dim or full[dim] != streams * beams:
+            at = dim + len(full) if dim < 0 else dim
+            if not s.is_contiguous() or not 0 <= at < len(full) or full[at] != streams * beams:
                 raise InvalidModelOutput(f"state {i} must be contiguous with {streams * beams} beams in dimension {dim}, "
                                          f"got {list(full)}")
             if given is None:
@@ -412,7 +413,7 @@ class ModelOps:
             out.append(o)
             row = table[i]
             row.in_, row.out = s.data_ptr(), o.data_ptr()
-            row.outer, row.inner_bytes = math.prod(full[:dim]), math.prod(full[dim + 1:]) * s.element_size()
+            row.outer, row.inner_bytes = math.prod(full[:at]), math.prod(full[at + 1:]) * s.element_size()
         rc = self._lib.sfe_beam_reorder(self._fe._handle(), pp, streams, beams, table, n, self._stream(stream))
         if rc:
             _check(rc)

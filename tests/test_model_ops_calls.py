@@ -1,0 +1,77 @@
+"""What ModelOps hands to the library, without a GPU: the library's calls are replaced by ones that record their
+arguments, and the tensors are the host's (device -1)."""
+import ctypes
+
+import pytest
+import torch
+
+from scriptrs_amd import InvalidModelOutput, ModelOps, _lib
+
+
+class Extractor:
+    """Stands in for the feature extractor: a context that is never looked into."""
+    device = -1
+
+    def __init__(self):
+        self._ctx = ctypes.c_void_p(1)
+
+    def _handle(self):
+        return self._ctx
+
+    def close(self):
+        self._ctx = ctypes.c_void_p()
+
+
+class Library:
+    """Records the operators' calls; the rest is the library's own."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name in ("sfe_rotary_init", "sfe_last_error"):
+            return getattr(REAL, name)
+
+        def call(*args):
+            self.calls.append((name, args))
+            return _lib.SFE_OK
+        return call
+
+
+REAL = _lib.lib()
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    library = Library()
+    monkeypatch.setattr(_lib, "lib", lambda: library)
+    m = ModelOps(extractor=Extractor())
+    m._stream_of = lambda device: 0
+    m.recorded = library.calls
+    return m
+
+
+def states_of(ops):
+    name, (_, _, streams, beams, table, n, _) = ops.recorded[-1]
+    assert name == "sfe_beam_reorder"
+    return [(s.outer, streams * beams, s.inner_bytes) for s in table[:n]]
+
+
+@pytest.mark.parametrize("shape,dim", [((3, 8), 1), ((3, 8), -1), ((8, 5), 0), ((8, 5), -2), ((2, 8, 7), 1),
+                                       ((2, 8, 7), -2), ((8,), -1), ((8,), 0), ((8, 8, 8), -1)])
+def test_reordered_states_are_the_tensors(ops, shape, dim):
+    """outer x beams x inner is the tensor, with dimensions counted from either end."""
+    state = torch.zeros(shape)
+    parents = torch.zeros(2, 4, dtype=torch.int32)
+    ops.beam_reorder(parents, [state], dim=dim)
+    (outer, rows, inner), = states_of(ops)
+    at = dim % len(shape)
+    assert (outer, rows, inner) == (torch.Size(shape[:at]).numel(), 8, 4 * torch.Size(shape[at + 1:]).numel())
+    assert outer * rows * inner == state.numel() * state.element_size()
+
+
+@pytest.mark.parametrize("dim", [2, -3, 99, -99])
+def test_dimensions_that_a_state_does_not_have_are_refused(ops, dim):
+    with pytest.raises(InvalidModelOutput, match="dimension"):
+        ops.beam_reorder(torch.zeros(2, 4, dtype=torch.int32), [torch.zeros(8, 8)], dim=dim)
+    assert not ops.recorded

@@ -384,8 +384,8 @@ int sfe_beam_select(sfe_ctx* ctx, int32_t dtype, const void* logits, int64_t row
 
 /* Reorders beam states to their parents: out[o][b * beams + w] = in[o][b * beams +
  * parents[b * beams + w]] for states [outer][streams * beams][inner_bytes].  out may be in
- * (in place).  A parent outside [0, beams) leaves the place its own state.
- * inner_bytes is less than 2^31. */
+ * (in place); an output that overlaps any other tensor of the call is refused.  A
+ * parent outside [0, beams) leaves the place its own state.  inner_bytes is less than 2^31. */
 typedef struct sfe_beam_state {
   const void* in;
   void* out;

@@ -539,6 +539,16 @@ int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int3
       hipStream_t stream;
     } call;
     call.stream = static_cast<hipStream_t>(stream);
+    // What the launch reads and writes (all states at once): an output may share memory with nothing but its own
+    // input, in place.
+    struct Used {
+      uintptr_t begin, end;
+      bool out;
+      int32_t state;
+    };
+    std::vector<Used> used;
+    used.reserve(2 * (size_t)n + 1);
+    used.push_back(Used{(uintptr_t)parents, (uintptr_t)(parents + (int64_t)streams * beams), false, -1});
     for (int32_t i = 0; i < n; ++i) {
       const sfe_beam_state& s = states[i];
       const std::string name = "state " + std::to_string(i);
@@ -549,8 +559,8 @@ int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int3
       const int64_t bytes = s.outer * streams * beams * s.inner_bytes;
       if (bytes == 0) continue;
       if (!s.in || !s.out) return op_fail(SFE_INVALID_ARG, name + " is null");
-      if (s.in != s.out && share(Rows{"", s.in, 1, bytes, bytes}, Rows{"", s.out, 1, bytes, bytes}))
-        return op_fail(SFE_INVALID_ARG, name + ": out overlaps in without being it");
+      used.push_back(Used{(uintptr_t)s.out, (uintptr_t)s.out + (uintptr_t)bytes, true, i});
+      if (s.in != s.out) used.push_back(Used{(uintptr_t)s.in, (uintptr_t)s.in + (uintptr_t)bytes, false, i});
       if (call.launches.empty() || call.launches.back().n == sfe::kReorderStates) {
         call.launches.emplace_back();
         memset(&call.launches.back(), 0, sizeof(sfe::ReorderArgs));
@@ -562,6 +572,15 @@ int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int3
       l.s[l.n++] = sfe::BeamState{static_cast<const char*>(s.in), static_cast<char*>(s.out), s.outer, s.inner_bytes};
     }
     if (call.launches.empty()) return SFE_OK;
+    std::sort(used.begin(), used.end(), [](const Used& a, const Used& b) { return a.begin < b.begin; });
+    uintptr_t any = 0, out = 0;  // ends of what begins at or before the range looked at, and of the outputs among it
+    for (const Used& u : used) {
+      if (u.begin < (u.out ? any : out))
+        return op_fail(SFE_INVALID_ARG, u.state < 0 ? std::string("parents: an output overlaps them")
+                                                    : "state " + std::to_string(u.state) + " overlaps another tensor of the call");
+      any = std::max(any, u.end);
+      if (u.out) out = std::max(out, u.end);
+    }
     return sfe::op_call(ctx, call.stream, "beam reorder", [](void* arg, int) -> hipError_t {
       Call& c = *static_cast<Call*>(arg);
       for (const sfe::ReorderArgs& l : c.launches) {

@@ -377,8 +377,8 @@ class ModelOps:
     def beam_reorder(self, parents, states, dim: int = 0, out=None, stream=None):
         """``states`` (contiguous device tensors whose dimension ``dim``, from the end if negative, is
         streams * beams) with every beam's state taken from its parent, in one launch.
-        ``out``: tensors to write, ``states`` themselves for in place; returns the list
-        written."""
+        ``out``: tensors to write, ``states`` themselves for in place (an output may share memory with
+        no other tensor); returns the list written."""
         torch = self._torch
         states = list(states)
         given = None if out is None else list(out)

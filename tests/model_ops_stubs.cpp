@@ -1,0 +1,46 @@
+// What the model operators' entry points (scriptrs_amd/csrc/sfe_ops.cpp) need of a context, without one and
+// without a GPU: nothing is launched, calls that pass their checks are counted.
+#include <string>
+
+#include "sfe_ops.hpp"
+
+namespace {
+int calls = 0;
+std::string message;
+}  // namespace
+
+extern "C" int stub_calls() { return calls; }
+extern "C" const char* stub_message() { return message.c_str(); }
+
+namespace sfe {
+
+int op_fail(int code, const std::string& msg) {
+  message = msg;
+  return code;
+}
+int op_hip_fail(hipError_t, const char* what) { return op_fail(3, what); }
+int op_cus(sfe_ctx*) { return 256; }
+int op_call(sfe_ctx*, hipStream_t, const char*, hipError_t (*)(void*, int), void*) {
+  ++calls;
+  return 0;
+}
+int op_upload(sfe_ctx*, const void*, size_t, size_t room, hipStream_t, void** buf, size_t* cap) {
+  *buf = nullptr;
+  *cap = room;
+  return 0;
+}
+void op_release(sfe_ctx*, void*, size_t) {}
+int op_scratch(sfe_ctx*, size_t, hipStream_t, void** out) {
+  *out = nullptr;
+  return 0;
+}
+
+hipError_t launch_attn_mask(const uint8_t*, int64_t, uint64_t*, hipStream_t) { return hipSuccess; }
+hipError_t launch_attn(const AttnArgs&, int, int, int, hipStream_t) { return hipSuccess; }
+hipError_t launch_rotary(const RotaryArgs&, int, bool, int, hipStream_t) { return hipSuccess; }
+hipError_t launch_residual(const ResidualArgs&, int, int, hipStream_t) { return hipSuccess; }
+size_t beam_scratch_bytes(int, int, int, int) { return 0; }
+hipError_t launch_beam_select(const BeamArgs&, int, int, hipStream_t) { return hipSuccess; }
+hipError_t launch_beam_reorder(const ReorderArgs&, hipStream_t) { return hipSuccess; }
+
+}  // namespace sfe

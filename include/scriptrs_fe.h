@@ -292,8 +292,8 @@ typedef struct sfe_heads {
  * A plan holds the sequences' division into tiles, and the partial results of
  * tiles that are cut along their keys; one plan serves every layer over the same
  * lengths, on any stream, and can be captured (its making cannot).  Free it
- * before its context, and after the graphs that hold it.  head_dim is a multiple of 8,
- * at most 128. */
+ * after the graphs that hold it.  A plan that outlives its context is refused by
+ * sfe_attention and has still to be freed.  head_dim is a multiple of 8, at most 128. */
 typedef struct sfe_attn_plan sfe_attn_plan;
 int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_offsets, int32_t n, int32_t heads,
                        int32_t kv_heads, int32_t head_dim, int64_t left, int64_t right, void* stream,

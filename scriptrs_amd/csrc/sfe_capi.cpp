@@ -313,9 +313,9 @@ struct sfe_ctx {
   // kNoAllocMaxItems items: the chunks' own items and the planner's lists.
   std::vector<Item> na_in;
   sfe::PlanWorkspace na_ws;
-  // The model operators (sfe_ops.cpp): buffers of freed plans, for the next
-  // plans; the calls' scratch, outgrown ones in front of the current one.
-  std::vector<std::pair<void*, size_t>> op_free;
+  // The model operators (sfe_ops.cpp): their plans; the calls' scratch, outgrown
+  // ones in front of the current one.
+  sfe::OpPlans op_plans;
   std::vector<std::pair<void*, size_t>> op_scratch;
 };
 
@@ -633,7 +633,22 @@ int op_call(sfe_ctx* ctx, hipStream_t stream, const char* what, hipError_t (*bod
   return SFE_OK;
 }
 
-int op_upload(sfe_ctx* ctx, const void* table, size_t bytes, size_t room, hipStream_t stream, void** buf, size_t* cap) {
+int op_adopt(sfe_ctx* ctx, OpPlan* plan) {
+  int rc = check_ctx(ctx);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  ctx->op_plans.adopt(plan, ctx);
+  return SFE_OK;
+}
+
+void op_drop(OpPlan* plan) noexcept {
+  if (!plan->ctx) return;
+  std::lock_guard<std::mutex> lock(plan->ctx->mu);
+  plan->ctx->op_plans.drop(plan);
+}
+
+int op_upload(OpPlan* plan, const void* table, size_t bytes, size_t room, hipStream_t stream) {
+  sfe_ctx* ctx = plan->ctx;
   int rc = check_ctx(ctx);
   if (rc) return rc;
   std::lock_guard<std::mutex> lock(ctx->mu);
@@ -642,20 +657,9 @@ int op_upload(sfe_ctx* ctx, const void* table, size_t bytes, size_t room, hipStr
   if (status != hipStreamCaptureStatusNone)
     return fail(SFE_INVALID_ARG, "a plan cannot be made while its stream is being captured");
   SFE_HIP(order_after_last(ctx, stream));
-  // the smallest freed buffer that is large enough and not far too large
-  size_t best = ctx->op_free.size();
-  for (size_t i = 0; i < ctx->op_free.size(); ++i) {
-    const size_t c = ctx->op_free[i].second;
-    if (c >= room && c / 8 <= room + 65536 && (best == ctx->op_free.size() || c < ctx->op_free[best].second)) best = i;
-  }
   void* p = nullptr;
   size_t got = 0;
-  ctx->op_free.reserve(ctx->op_free.size() + 1);
-  if (best < ctx->op_free.size()) {
-    p = ctx->op_free[best].first;
-    got = ctx->op_free[best].second;
-    ctx->op_free.erase(ctx->op_free.begin() + (std::ptrdiff_t)best);
-  } else {
+  if (!ctx->op_plans.take(room, &p, &got)) {
     got = (room + room / 4 + 65535) / 65536 * 65536;
     const hipError_t e = hipMalloc(&p, got);
     g_allocations.fetch_add(1);
@@ -671,17 +675,12 @@ int op_upload(sfe_ctx* ctx, const void* table, size_t bytes, size_t room, hipStr
     return SFE_OK;
   };
   if ((rc = queue())) {
-    ctx->op_free.emplace_back(p, got);  // (reserved above: cannot throw)
+    ctx->op_plans.give(p, got);
     return rc;
   }
-  *buf = p;
-  *cap = got;
+  plan->buf = p;
+  plan->cap = got;
   return SFE_OK;
-}
-
-void op_release(sfe_ctx* ctx, void* buf, size_t cap) {
-  std::lock_guard<std::mutex> lock(ctx->mu);
-  ctx->op_free.emplace_back(buf, cap);
 }
 
 int op_scratch(sfe_ctx* ctx, size_t bytes, hipStream_t stream, void** out) {
@@ -845,7 +844,7 @@ void sfe_destroy(sfe_ctx* ctx) {
   ctx->h_io_in.release();
   ctx->h_io_out.release();
   ctx->win.release();
-  for (auto& b : ctx->op_free) (void)hipFree(b.first);
+  ctx->op_plans.close([](void* p) { (void)hipFree(p); });
   for (auto& b : ctx->op_scratch) (void)hipFree(b.first);
   for (int i = 0; i < 2; ++i) {
     ctx->h_win[i].release();

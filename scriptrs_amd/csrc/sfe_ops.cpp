@@ -16,8 +16,8 @@
 
 using sfe::op_fail;
 
-struct sfe_attn_plan {
-  sfe_ctx* ctx = nullptr;
+struct sfe_attn_plan : sfe::OpPlan {
+  ~sfe_attn_plan() { sfe::op_drop(this); }
   int32_t heads = 0, kv_heads = 0, dim = 0, left = 0, right = 0;
   struct Form {
     int32_t n_items = 0, n_joins = 0;
@@ -27,8 +27,6 @@ struct sfe_attn_plan {
   bool empty = true;  // no queries
   size_t mask = 0;    // packed key mask
   int64_t total_q = 0, total_k = 0;
-  void* buf = nullptr;
-  size_t cap = 0;
 };
 
 namespace {
@@ -135,7 +133,7 @@ int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_
         return op_fail(SFE_INVALID_ARG, "a sequence has more than 2^30 queries of grouped heads");
     if (!ctx) return op_fail(SFE_INVALID_ARG, "null context");
     auto plan = std::make_unique<sfe_attn_plan>();
-    plan->ctx = ctx;
+    if ((rc = sfe::op_adopt(ctx, plan.get()))) return rc;
     plan->heads = heads;
     plan->kv_heads = kv_heads;
     plan->dim = head_dim;
@@ -180,27 +178,20 @@ int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_
       plan->form[i].part_o = place(rows * sfe::attn_padded_dim(head_dim) * sizeof(float));
       plan->form[i].part_ml = place(rows * sizeof(float2));
     }
-    if ((rc = sfe::op_upload(ctx, table.data(), bytes, at, static_cast<hipStream_t>(stream), &plan->buf, &plan->cap)))
-      return rc;
+    if ((rc = sfe::op_upload(plan.get(), table.data(), bytes, at, static_cast<hipStream_t>(stream)))) return rc;
     *out = plan.release();
     return SFE_OK;
   });
 }
 
-void sfe_attention_plan_free(sfe_attn_plan* plan) {
-  if (!plan) return;
-  (void)guarded([&]() -> int {
-    if (plan->buf) sfe::op_release(plan->ctx, plan->buf, plan->cap);
-    return SFE_OK;
-  });
-  delete plan;
-}
+void sfe_attention_plan_free(sfe_attn_plan* plan) { delete plan; }
 
 int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
                   const uint8_t* key_mask, float scale, const sfe_heads* out, void* stream) {
   return guarded([&]() -> int {
     if (!plan || !q || !k || !v || !out) return op_fail(SFE_INVALID_ARG, "null argument");
     if (dtype != SFE_BF16 && dtype != SFE_F16) return op_fail(SFE_INVALID_ARG, "dtype must be SFE_BF16 or SFE_F16");
+    if (!plan->ctx) return op_fail(SFE_INVALID_ARG, "the plan's context has been destroyed");
     if (!(scale > 0.0f) || scale > 1e30f) return op_fail(SFE_INVALID_ARG, "scale must be positive and finite");
     if (plan->empty) return SFE_OK;  // no queries
     int rc;

@@ -8,7 +8,9 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <string>
+#include <utility>
 #include <vector>
 
 struct sfe_ctx;
@@ -28,13 +30,67 @@ int op_hip_fail(hipError_t e, const char* what);
 // for or marked.
 int op_call(sfe_ctx* ctx, hipStream_t stream, const char* what, hipError_t (*body)(void* arg, int cus), void* arg);
 
-// Memory of a plan: the first `bytes` of a device buffer of at least `room`
+// A plan's part that its context knows: which context it is of, until that is destroyed, and its
+// device buffer.
+struct OpPlan {
+  sfe_ctx* ctx = nullptr;
+  void* buf = nullptr;
+  size_t cap = 0;
+};
+// The plans of a context and the buffers of freed ones, which the next plans take.  A context that is destroyed takes
+// its plans' buffers along; what is left of such a plan is only good for freeing.
+class OpPlans {
+ public:
+  void adopt(OpPlan* p, sfe_ctx* ctx) {
+    live_.reserve(live_.size() + 1);
+    free_.reserve(free_.size() + live_.size() + 1);  // (so that drop and give cannot throw)
+    live_.push_back(p);
+    p->ctx = ctx;
+  }
+  void drop(OpPlan* p) noexcept {
+    live_.erase(std::find(live_.begin(), live_.end(), p));
+    if (p->buf) give(p->buf, p->cap);
+    *p = OpPlan{};
+  }
+  // The smallest freed buffer that is large enough and not far too large.
+  bool take(size_t room, void** buf, size_t* cap) noexcept {
+    size_t best = free_.size();
+    for (size_t i = 0; i < free_.size(); ++i) {
+      const size_t c = free_[i].second;
+      if (c >= room && c / 8 <= room + 65536 && (best == free_.size() || c < free_[best].second)) best = i;
+    }
+    if (best == free_.size()) return false;
+    *buf = free_[best].first;
+    *cap = free_[best].second;
+    free_.erase(free_.begin() + (std::ptrdiff_t)best);
+    return true;
+  }
+  // A buffer of an adopted plan that has none, back.
+  void give(void* buf, size_t cap) noexcept { free_.emplace_back(buf, cap); }
+  template <class F>
+  void close(F&& free_buffer) noexcept {
+    for (OpPlan* p : live_) {
+      if (p->buf) free_buffer(p->buf);
+      *p = OpPlan{};
+    }
+    for (auto& b : free_) free_buffer(b.first);
+    live_.clear();
+    free_.clear();
+  }
+
+ private:
+  std::vector<OpPlan*> live_;
+  std::vector<std::pair<void*, size_t>> free_;
+};
+
+// Enters a plan into its context; it stays there until op_drop (which does nothing for a plan of no context).
+int op_adopt(sfe_ctx* ctx, OpPlan* plan);
+void op_drop(OpPlan* plan) noexcept;
+// Memory of an adopted plan: the first `bytes` of a device buffer of at least `room`
 // bytes are filled from `table` on `stream` (through the context's pinned
 // staging).  The buffer comes from the context's freed ones where one fits: the
-// upload is ordered after every earlier call that read it.  *buf and *cap
-// receive it.  Refused while `stream` is being captured.
-int op_upload(sfe_ctx* ctx, const void* table, size_t bytes, size_t room, hipStream_t stream, void** buf, size_t* cap);
-void op_release(sfe_ctx* ctx, void* buf, size_t cap);
+// upload is ordered after every earlier call that read it.  Refused while `stream` is being captured.
+int op_upload(OpPlan* plan, const void* table, size_t bytes, size_t room, hipStream_t stream);
 int op_cus(sfe_ctx* ctx);  // compute units of the context's device
 
 // Scratch of at least `bytes` for the calls of a context, which are ordered after

@@ -91,7 +91,8 @@ class RotaryTable:
 
 class AttentionPlan:
     """Division of a batch's sequences into tiles; made by
-    ``ModelOps.attention_plan`` and good for every layer over the same lengths."""
+    ``ModelOps.attention_plan`` and good for every layer over the same lengths, until its context (the
+    ``ModelOps`` or the extractor that it shares) is closed."""
 
     def __init__(self, ops: "ModelOps", handle, first_q: int, total_q: int, total_k: int, heads: int, kv_heads: int,
                  head_dim: int):
@@ -101,7 +102,7 @@ class AttentionPlan:
         self.scale = 1.0 / math.sqrt(head_dim)
 
     def close(self) -> None:
-        if self._handle and self._ops._fe._ctx:  # (a closed context has freed it)
+        if self._handle:
             _lib.lib().sfe_attention_plan_free(self._handle)
         self._handle = None
 

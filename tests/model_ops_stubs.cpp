@@ -1,5 +1,6 @@
 // What the model operators' entry points (scriptrs_amd/csrc/sfe_ops.cpp) need of a context, without one and
 // without a GPU: nothing is launched, calls that pass their checks are counted.
+#include <cstdlib>
 #include <string>
 
 #include "sfe_ops.hpp"
@@ -9,6 +10,21 @@ int calls = 0;
 std::string message;
 }  // namespace
 
+struct sfe_ctx {
+  sfe::OpPlans plans;
+};
+
+extern "C" sfe_ctx* stub_context() { return new sfe_ctx; }
+// Destroys a context; returns how many device buffers it freed.
+extern "C" int stub_destroy(sfe_ctx* ctx) {
+  int n = 0;
+  ctx->plans.close([&](void* p) {
+    free(p);
+    ++n;
+  });
+  delete ctx;
+  return n;
+}
 extern "C" int stub_calls() { return calls; }
 extern "C" const char* stub_message() { return message.c_str(); }
 
@@ -24,12 +40,20 @@ int op_call(sfe_ctx*, hipStream_t, const char*, hipError_t (*)(void*, int), void
   ++calls;
   return 0;
 }
-int op_upload(sfe_ctx*, const void*, size_t, size_t room, hipStream_t, void** buf, size_t* cap) {
-  *buf = nullptr;
-  *cap = room;
+int op_adopt(sfe_ctx* ctx, OpPlan* plan) {
+  ctx->plans.adopt(plan, ctx);
   return 0;
 }
-void op_release(sfe_ctx*, void*, size_t) {}
+void op_drop(OpPlan* plan) noexcept {
+  if (plan->ctx) plan->ctx->plans.drop(plan);
+}
+int op_upload(OpPlan* plan, const void*, size_t, size_t room, hipStream_t) {
+  if (!plan->ctx->plans.take(room, &plan->buf, &plan->cap)) {
+    plan->buf = malloc(room);
+    plan->cap = room;
+  }
+  return 0;
+}
 int op_scratch(sfe_ctx*, size_t, hipStream_t, void** out) {
   *out = nullptr;
   return 0;

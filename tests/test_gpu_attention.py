@@ -360,3 +360,24 @@ def test_no_keys_at_all(ops, dim):
                                   ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
     assert rc == _lib.SFE_OK, _lib.last_error()
     assert not out.any()
+
+
+def test_plans_end_with_their_context():
+    """After close() a plan's calls are refused, on the same operators opened again too; other plans are not touched."""
+    import torch
+    from scriptrs_amd import InvalidModelOutput, ModelOps
+    own = ModelOps()
+    x = torch.randn(200, 2, 64, device="cuda").bfloat16()
+    plan, kept = (own.attention_plan([0, 80, 200], [0, 80, 200], 2, 2, 64) for _ in range(2))
+    want = own.attention(plan, x, x, x)
+    own.close()
+    with pytest.raises(InvalidModelOutput, match="destroyed"):
+        own.attention(plan, x, x, x)
+    again = own.attention_plan([0, 80, 200], [0, 80, 200], 2, 2, 64)
+    with pytest.raises(InvalidModelOutput, match="destroyed"):
+        own.attention(plan, x, x, x)
+    plan.close()
+    assert torch.equal(own.attention(again, x, x, x), want)
+    again.close()
+    own.close()
+    del kept

@@ -75,3 +75,17 @@ def test_dimensions_that_a_state_does_not_have_are_refused(ops, dim):
     with pytest.raises(InvalidModelOutput, match="dimension"):
         ops.beam_reorder(torch.zeros(2, 4, dtype=torch.int32), [torch.zeros(8, 8)], dim=dim)
     assert not ops.recorded
+
+
+@pytest.mark.parametrize("order", ["plan first", "context first", "context reopened"])
+def test_a_plan_is_freed_once_whatever_its_context(ops, order):
+    plan = ops.attention_plan([0, 4], [0, 4], 2, 2, 64, stream=0)
+    plan._handle = ctypes.c_void_p(2)
+    if order != "plan first":
+        ops._fe.close()
+    if order == "context reopened":
+        ops._fe._ctx = ctypes.c_void_p(3)
+    plan.close()
+    plan.close()
+    freed = [args for name, args in ops.recorded if name == "sfe_attention_plan_free"]
+    assert len(freed) == 1 and freed[0][0].value == 2

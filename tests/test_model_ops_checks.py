@@ -70,3 +70,53 @@ def test_reordered_states_share_no_memory(checks):
 def test_reordered_states_leave_the_parents(checks):
     passes(checks, reorder(checks, (AT, AT, 1, 100), parents=AT + 600))
     refused(checks, reorder(checks, (AT, AT, 1, 100), parents=AT + 596), "overlaps")
+
+
+def offsets(*o):
+    return (ctypes.c_int64 * len(o))(*o)
+
+
+def make_plan(L, ctx, q=(0, 40, 300), k=(0, 40, 300)):
+    plan = ctypes.c_void_p()
+    passes(L, L.sfe_attention_plan(ctx, offsets(*q), offsets(*k), len(q) - 1, 2, 2, 64, -1, -1, None, ctypes.byref(plan)))
+    return plan
+
+
+def attend(L, plan):
+    x, out = _lib.SfeHeads(AT, 128, 64), _lib.SfeHeads(1 << 30, 128, 64)
+    return L.sfe_attention(plan, _lib.SFE_BF16, x, x, x, None, 0.125, out, None)
+
+
+@pytest.fixture
+def contexts(checks):
+    checks.stub_context.restype = ctypes.c_void_p
+    checks.stub_destroy.argtypes = [ctypes.c_void_p]
+    return checks
+
+
+@pytest.mark.parametrize("q", [(0, 40, 300), (0, 0, 0)], ids=["rows", "none"])
+def test_plans_that_outlive_their_context(contexts, q):
+    """Refused, and freeing them touches neither the context that is gone nor one made since."""
+    L = contexts
+    ctx = L.stub_context()
+    plan = make_plan(L, ctx, q=q)
+    passes(L, attend(L, plan))
+    assert L.stub_destroy(ctx) == (1 if q[-1] else 0)
+    refused(L, attend(L, plan), "destroyed")
+    other = L.stub_context()
+    refused(L, attend(L, plan), "destroyed")
+    L.sfe_attention_plan_free(plan)
+    assert L.stub_destroy(other) == 0
+
+
+def test_buffers_of_freed_plans_are_reused(contexts):
+    L = contexts
+    ctx = L.stub_context()
+    a, b = make_plan(L, ctx), make_plan(L, ctx)
+    L.sfe_attention_plan_free(a)
+    c = make_plan(L, ctx)  # (takes a's buffer)
+    L.sfe_attention_plan_free(b)
+    L.sfe_attention_plan_free(c)
+    d = make_plan(L, ctx)
+    assert L.stub_destroy(ctx) == 2
+    L.sfe_attention_plan_free(d)

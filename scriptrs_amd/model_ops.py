@@ -138,8 +138,10 @@ class ModelOps:
         self._states = (SfeBeamState * 8)()
 
     def _stream(self, stream) -> int | None:
-        if stream is None and self._stream_of is not None:
-            return self._stream_of(self.device)
+        if stream is None:
+            if self._stream_of is not None:
+                return self._stream_of(self.device)
+            stream = self._torch.cuda.current_stream(self.device)
         return _stream_handle(stream)
 
     def close(self) -> None:
@@ -158,7 +160,7 @@ class ModelOps:
             raise InvalidModelOutput("q_offsets and k_offsets must have one entry more than there are sequences")
         handle = ctypes.c_void_p()
         _check(_lib.lib().sfe_attention_plan(self._fe._handle(), _ip(qo), _ip(ko), qo.size - 1, int(heads), int(kv_heads),
-                                             int(head_dim), int(left), int(right), _stream_handle(stream),
+                                             int(head_dim), int(left), int(right), self._stream(stream),
                                              ctypes.byref(handle)))
         return AttentionPlan(self, handle, int(qo[0]), int(qo[-1]), int(ko[-1]), int(heads), int(kv_heads),
                              int(head_dim))

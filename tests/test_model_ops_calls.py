@@ -89,3 +89,15 @@ def test_a_plan_is_freed_once_whatever_its_context(ops, order):
     plan.close()
     freed = [args for name, args in ops.recorded if name == "sfe_attention_plan_free"]
     assert len(freed) == 1 and freed[0][0].value == 2
+
+
+def test_calls_without_a_stream_take_their_devices(ops):
+    """The current stream of the operators' device, which need not be torch's current device."""
+    ops._stream_of = lambda device: 1000 + device
+    plan = ops.attention_plan([0, 4], [0, 4], 2, 2, 64)
+    plan._handle = ctypes.c_void_p(2)
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    ops.attention(plan, x, x, x)
+    assert {name: args[9 if name == "sfe_attention_plan" else 8] for name, args in ops.recorded} == {
+        "sfe_attention_plan": 999, "sfe_attention": 999}
+    plan._handle = None

@@ -308,6 +308,11 @@ void sfe_attention_plan_free(sfe_attn_plan* plan);
 int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
                   const uint8_t* key_mask, float scale, const sfe_heads* out, void* stream);
 
+/* The same for an out of `rows` rows, at least q_offsets[n]: those of no sequence, before
+ * q_offsets[0] and from q_offsets[n] on, are zeroed (none of out's rows may overlap the inputs). */
+int sfe_attention_rows(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
+                       const uint8_t* key_mask, float scale, const sfe_heads* out, int64_t rows, void* stream);
+
 /* Rotary positions.  A pair of channels (a, b) of the first rotary_dim of each
  * head turns by angle = position * f_p, f_p = base^(-2p / rotary_dim) as scaled:
  *   a' = magnitude (a cos - b sin),  b' = magnitude (b cos + a sin);

@@ -25,7 +25,7 @@ EXPORTS = (
     "sfe_extract_chunks_padded", "sfe_extract_chunks_streamed", "sfe_extract_chunks_streamed_pcm",
     "sfe_set_frame_sharing", "sfe_set_timing", "sfe_get_timing", "sfe_vad_num_windows", "sfe_vad_frames", "sfe_extract_chunks_noalloc",
     "sfe_debug_allocation_count", "sfe_debug_mel_schedule", "sfe_debug_stamps",
-    "sfe_attention_plan", "sfe_attention_plan_free", "sfe_attention", "sfe_rotary_init", "sfe_rotary",
+    "sfe_attention_plan", "sfe_attention_plan_free", "sfe_attention", "sfe_attention_rows", "sfe_rotary_init", "sfe_rotary",
     "sfe_residual_norm", "sfe_beam_select", "sfe_beam_reorder",
 )
 
@@ -129,6 +129,8 @@ def lib() -> ctypes.CDLL:
         "sfe_attention_plan_free": (None, [vp]),
         "sfe_attention": (ctypes.c_int, [vp, i32, P(SfeHeads), P(SfeHeads), P(SfeHeads), vp, ctypes.c_float,
                                          P(SfeHeads), vp]),
+        "sfe_attention_rows": (ctypes.c_int, [vp, i32, P(SfeHeads), P(SfeHeads), P(SfeHeads), vp, ctypes.c_float,
+                                              P(SfeHeads), i64, vp]),
         "sfe_rotary_init": (ctypes.c_int, [P(SfeRotaryTable), i32, i32, ctypes.c_double, i32] + [ctypes.c_double] * 5),
         "sfe_rotary": (ctypes.c_int, [vp, P(SfeRotaryTable), i32, i32, vp, i64, i32, i32, P(SfeHeads), P(SfeHeads),
                                       i32, P(SfeHeads), P(SfeHeads), vp]),

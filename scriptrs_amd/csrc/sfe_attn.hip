@@ -209,6 +209,17 @@ __global__ __launch_bounds__(256) void sfe_attn_mask_kernel(const uint8_t* __res
   if ((threadIdx.x & 63) == 0) words[w] = bits;
 }
 
+// Zeros chunk n of 16 bytes of the output's rows of no sequence: [0, first), then from `last` on.
+__global__ __launch_bounds__(256) void sfe_attn_zero_kernel(AttnTensor out, int heads, int chunks, int64_t first, int64_t last,
+                                                            int64_t n, int64_t total) {
+  n += (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= total) return;
+  const int64_t r = n / (heads * chunks);
+  const int c = (int)(n - r * (heads * chunks)), h = c / chunks;
+  char* p = const_cast<char*>(out.data) + (r < first ? r : r - first + last) * out.row + h * out.head;
+  *reinterpret_cast<uint4*>(p + 16 * (c - h * chunks)) = make_uint4(0, 0, 0, 0);
+}
+
 // Whether any of a V operand's 8 values is infinite or NaN.
 template <typename T>
 __device__ __forceinline__ uint32_t nonfinite(typename Mat<T>::V8 v) {
@@ -1235,6 +1246,16 @@ hipError_t launch_attn_mask(const uint8_t* mask, int64_t keys, uint64_t* words, 
   const int64_t n = attn_mask_words(keys);
   return for_launches((n + 3) / 4, 256, [&](int64_t first, unsigned blocks) {
     sfe_attn_mask_kernel<<<dim3(blocks), dim3(256), 0, stream>>>(mask + 256 * first, keys - 256 * first, words + 4 * first, n - 4 * first);
+    return hipGetLastError();
+  });
+}
+
+hipError_t launch_attn_zero(const AttnTensor& out, int heads, int dim, int64_t first, int64_t last, int64_t rows,
+                            hipStream_t stream) {
+  const int chunks = dim / 8;
+  const int64_t total = (first + rows - last) * heads * chunks;
+  return for_launches((total + 255) / 256, 256, [&](int64_t block, unsigned blocks) {
+    sfe_attn_zero_kernel<<<dim3(blocks), dim3(256), 0, stream>>>(out, heads, chunks, first, last, 256 * block, total);
     return hipGetLastError();
   });
 }

@@ -26,7 +26,7 @@ struct sfe_attn_plan : sfe::OpPlan {
   } form[sfe::kAttnForms];
   bool empty = true;  // no queries
   size_t mask = 0;    // packed key mask
-  int64_t total_q = 0, total_k = 0;
+  int64_t first_q = 0, total_q = 0, total_k = 0;
 };
 
 namespace {
@@ -105,6 +105,92 @@ int check_offsets(const char* name, const int64_t* off, int32_t n) {
 
 size_t up(size_t x) { return (x + 255) / 256 * 256; }
 
+// sfe_attention, and sfe_attention_rows where all_rows is given.
+int attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
+              const uint8_t* key_mask, float scale, const sfe_heads* out, const int64_t* all_rows, void* stream) {
+  if (!plan || !q || !k || !v || !out) return op_fail(SFE_INVALID_ARG, "null argument");
+  if (dtype != SFE_BF16 && dtype != SFE_F16) return op_fail(SFE_INVALID_ARG, "dtype must be SFE_BF16 or SFE_F16");
+  if (!plan->ctx) return op_fail(SFE_INVALID_ARG, "the plan's context has been destroyed");
+  if (!(scale > 0.0f) || scale > 1e30f) return op_fail(SFE_INVALID_ARG, "scale must be positive and finite");
+  if (all_rows && (*all_rows < plan->total_q || *all_rows > (int64_t)1 << 40))
+    return op_fail(SFE_INVALID_ARG, "rows must be in [q_offsets[n], 2^40]");
+  const int64_t rows = all_rows ? *all_rows : plan->total_q;
+  const bool outside = all_rows && (plan->first_q > 0 || rows > plan->total_q);
+  if (plan->empty && !outside) return SFE_OK;  // no queries
+  int rc;
+  const struct {
+    const char* name;
+    const sfe_heads* t;
+  } all[] = {{"q", q}, {"k", k}, {"v", v}, {"out", out}};
+  for (const auto& x : all) {
+    if (plan->empty && x.t != out) continue;  // (not read)
+    // (k and v of sequences without keys are not read)
+    if ((rc = check_heads(x.name, x.t, x.t == q || x.t == out ? 1 : 0, 2, 16))) return rc;
+    if (x.t->row_stride >= (1 << 23))
+      return op_fail(SFE_INVALID_ARG, std::string(x.name) + ": rows more than 2^23 elements apart");
+  }
+  if (!apart(*out, rows, plan->heads, plan->dim))
+    return op_fail(SFE_INVALID_ARG, "out: rows or heads overlap");
+  const Rows mine = rows_of("out", *out, rows, plan->heads, plan->dim, 2);
+  for (const Rows& o : {rows_of("q", *q, plan->total_q, plan->heads, plan->dim, 2),
+                        rows_of("k", *k, plan->total_k, plan->kv_heads, plan->dim, 2),
+                        rows_of("v", *v, plan->total_k, plan->kv_heads, plan->dim, 2)})
+    if (!plan->empty && share(mine, o)) return op_fail(SFE_INVALID_ARG, std::string("out overlaps ") + o.name);
+  if (!plan->empty && plan->total_k > 0 && (!k->data || !v->data)) return op_fail(SFE_INVALID_ARG, "null k or v");
+  auto tensor = [](const sfe_heads* t) {
+    return sfe::AttnTensor{static_cast<const char*>(t->data), t->row_stride * 2, t->head_stride * 2};
+  };
+  sfe::AttnArgs a{};
+  a.q = tensor(q);
+  a.k = tensor(k);
+  a.v = tensor(v);
+  a.o = tensor(out);
+  a.kv_heads = plan->kv_heads;
+  a.group = plan->heads / plan->kv_heads;
+  a.dim = plan->dim;
+  a.left = plan->left;
+  a.right = plan->right;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  struct Call {
+    sfe::AttnArgs a;
+    const sfe_attn_plan* plan;
+    const uint8_t* key_mask;
+    int dtype;
+    int64_t rows;  // with those of no sequence to be zeroed, or 0
+    hipStream_t stream;
+  } call{a, plan, key_mask, dtype, outside ? rows : 0, static_cast<hipStream_t>(stream)};
+  return sfe::op_call(plan->ctx, call.stream, "attention", [](void* arg, int cus) -> hipError_t {
+    Call& c = *static_cast<Call*>(arg);
+    char* base = static_cast<char*>(c.plan->buf);
+    if (c.rows) {
+      const hipError_t e = sfe::launch_attn_zero(c.a.o, c.plan->heads, c.plan->dim, c.plan->first_q, c.plan->total_q, c.rows,
+                                                 c.stream);
+      if (e != hipSuccess) return e;
+    }
+    if (c.plan->empty) return hipSuccess;
+    if (c.key_mask) {
+      uint64_t* words = reinterpret_cast<uint64_t*>(base + c.plan->mask);
+      const hipError_t e = sfe::launch_attn_mask(c.key_mask, c.plan->total_k, words, c.stream);
+      if (e != hipSuccess) return e;
+      c.a.mask = words;
+    }
+    for (int i = 0; i < sfe::kAttnForms; ++i) {
+      const auto& f = c.plan->form[i];
+      if (!f.n_items) continue;
+      c.a.n_items = f.n_items;
+      memcpy(c.a.share, f.share, sizeof(f.share));
+      c.a.items = reinterpret_cast<const sfe::AttnItem*>(base + f.items);
+      c.a.n_joins = f.n_joins;
+      c.a.joins = reinterpret_cast<const sfe::AttnJoin*>(base + f.joins);
+      c.a.part_o = reinterpret_cast<float*>(base + f.part_o);
+      c.a.part_ml = reinterpret_cast<float2*>(base + f.part_ml);
+      const hipError_t e = sfe::launch_attn(c.a, i, c.dtype, cus, c.stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }, &call);
+}
+
 }  // namespace
 
 extern "C" {
@@ -139,7 +225,8 @@ int sfe_attention_plan(sfe_ctx* ctx, const int64_t* q_offsets, const int64_t* k_
     plan->dim = head_dim;
     plan->left = left < 0 || left >= sfe::kAttnNoBound ? sfe::kAttnNoBound : (int32_t)left;
     plan->right = right < 0 || right >= sfe::kAttnNoBound ? sfe::kAttnNoBound : (int32_t)right;
-    plan->total_q = n ? q_offsets[n] : 0;
+    plan->first_q = q_offsets[0];
+    plan->total_q = q_offsets[n];
     plan->total_k = n ? k_offsets[n] : 0;
     sfe::AttnPlanHost h;
     sfe::attn_plan(q_offsets, k_offsets, n, group, kv_heads, head_dim, plan->left, plan->right, sfe::op_cus(ctx), &h);
@@ -188,77 +275,12 @@ void sfe_attention_plan_free(sfe_attn_plan* plan) { delete plan; }
 
 int sfe_attention(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
                   const uint8_t* key_mask, float scale, const sfe_heads* out, void* stream) {
-  return guarded([&]() -> int {
-    if (!plan || !q || !k || !v || !out) return op_fail(SFE_INVALID_ARG, "null argument");
-    if (dtype != SFE_BF16 && dtype != SFE_F16) return op_fail(SFE_INVALID_ARG, "dtype must be SFE_BF16 or SFE_F16");
-    if (!plan->ctx) return op_fail(SFE_INVALID_ARG, "the plan's context has been destroyed");
-    if (!(scale > 0.0f) || scale > 1e30f) return op_fail(SFE_INVALID_ARG, "scale must be positive and finite");
-    if (plan->empty) return SFE_OK;  // no queries
-    int rc;
-    const struct {
-      const char* name;
-      const sfe_heads* t;
-    } all[] = {{"q", q}, {"k", k}, {"v", v}, {"out", out}};
-    for (const auto& x : all) {
-      // (k and v of sequences without keys are not read)
-      if ((rc = check_heads(x.name, x.t, x.t == q || x.t == out ? 1 : 0, 2, 16))) return rc;
-      if (x.t->row_stride >= (1 << 23))
-        return op_fail(SFE_INVALID_ARG, std::string(x.name) + ": rows more than 2^23 elements apart");
-    }
-    if (!apart(*out, plan->total_q, plan->heads, plan->dim))
-      return op_fail(SFE_INVALID_ARG, "out: rows or heads overlap");
-    const Rows mine = rows_of("out", *out, plan->total_q, plan->heads, plan->dim, 2);
-    for (const Rows& o : {rows_of("q", *q, plan->total_q, plan->heads, plan->dim, 2),
-                          rows_of("k", *k, plan->total_k, plan->kv_heads, plan->dim, 2),
-                          rows_of("v", *v, plan->total_k, plan->kv_heads, plan->dim, 2)})
-      if (share(mine, o)) return op_fail(SFE_INVALID_ARG, std::string("out overlaps ") + o.name);
-    if (plan->total_k > 0 && (!k->data || !v->data)) return op_fail(SFE_INVALID_ARG, "null k or v");
-    auto tensor = [](const sfe_heads* t) {
-      return sfe::AttnTensor{static_cast<const char*>(t->data), t->row_stride * 2, t->head_stride * 2};
-    };
-    sfe::AttnArgs a{};
-    a.q = tensor(q);
-    a.k = tensor(k);
-    a.v = tensor(v);
-    a.o = tensor(out);
-    a.kv_heads = plan->kv_heads;
-    a.group = plan->heads / plan->kv_heads;
-    a.dim = plan->dim;
-    a.left = plan->left;
-    a.right = plan->right;
-    a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-    struct Call {
-      sfe::AttnArgs a;
-      const sfe_attn_plan* plan;
-      const uint8_t* key_mask;
-      int dtype;
-      hipStream_t stream;
-    } call{a, plan, key_mask, dtype, static_cast<hipStream_t>(stream)};
-    return sfe::op_call(plan->ctx, call.stream, "attention", [](void* arg, int cus) -> hipError_t {
-      Call& c = *static_cast<Call*>(arg);
-      char* base = static_cast<char*>(c.plan->buf);
-      if (c.key_mask) {
-        uint64_t* words = reinterpret_cast<uint64_t*>(base + c.plan->mask);
-        const hipError_t e = sfe::launch_attn_mask(c.key_mask, c.plan->total_k, words, c.stream);
-        if (e != hipSuccess) return e;
-        c.a.mask = words;
-      }
-      for (int i = 0; i < sfe::kAttnForms; ++i) {
-        const auto& f = c.plan->form[i];
-        if (!f.n_items) continue;
-        c.a.n_items = f.n_items;
-        memcpy(c.a.share, f.share, sizeof(f.share));
-        c.a.items = reinterpret_cast<const sfe::AttnItem*>(base + f.items);
-        c.a.n_joins = f.n_joins;
-        c.a.joins = reinterpret_cast<const sfe::AttnJoin*>(base + f.joins);
-        c.a.part_o = reinterpret_cast<float*>(base + f.part_o);
-        c.a.part_ml = reinterpret_cast<float2*>(base + f.part_ml);
-        const hipError_t e = sfe::launch_attn(c.a, i, c.dtype, cus, c.stream);
-        if (e != hipSuccess) return e;
-      }
-      return hipSuccess;
-    }, &call);
-  });
+  return guarded([&]() -> int { return attention(plan, dtype, q, k, v, key_mask, scale, out, nullptr, stream); });
+}
+
+int sfe_attention_rows(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, const sfe_heads* k, const sfe_heads* v,
+                       const uint8_t* key_mask, float scale, const sfe_heads* out, int64_t rows, void* stream) {
+  return guarded([&]() -> int { return attention(plan, dtype, q, k, v, key_mask, scale, out, &rows, stream); });
 }
 
 // ---- rotary ---------------------------------------------------------------------------

@@ -168,6 +168,9 @@ inline int attn_padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 96 ? 96 : 
 // of them across two words.
 inline int64_t attn_mask_words(int64_t keys) { return (keys + 63) / 64 + 3 * kAttnStepRows / 64 + 2; }
 hipError_t launch_attn_mask(const uint8_t* mask, int64_t keys, uint64_t* words, hipStream_t stream);
+// Zeros the rows [0, first) and [last, rows) of `out` of heads x dim.
+hipError_t launch_attn_zero(const AttnTensor& out, int heads, int dim, int64_t first, int64_t last, int64_t rows,
+                            hipStream_t stream);
 hipError_t launch_attn(const AttnArgs& a, int form, int type, int cus, hipStream_t stream);
 
 // ---- rotary positions (sfe_rotary.hip) ----------------------------------------------

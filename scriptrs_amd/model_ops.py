@@ -209,24 +209,15 @@ class ModelOps:
                 _wrong_device("out", out, device)
             _heads(out, "out", q.shape, ho)
         pq, pk, pv, po = self._hp
-        rc = self._lib.sfe_attention(handle, code, pq, pk, pv, mask, plan.scale if scale is None else scale, po,
-                                     self._stream(stream))
+        if scale is None:
+            scale = plan.scale
+        if plan.first_q or q.shape[0] > plan.total_q:  # rows of no sequence
+            rc = self._lib.sfe_attention_rows(handle, code, pq, pk, pv, mask, scale, po, q.shape[0], self._stream(stream))
+        else:
+            rc = self._lib.sfe_attention(handle, code, pq, pk, pv, mask, scale, po, self._stream(stream))
         if rc:
             _check(rc)
-        if plan.first_q or q.shape[0] > plan.total_q:
-            self._zero_outside(plan, out, stream)
         return out
-
-    def _zero_outside(self, plan: AttentionPlan, out, stream) -> None:
-        """Zeros the rows of no sequence, on the call's stream."""
-        torch = self._torch
-        if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        elif not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(_stream_handle(stream).value or 0, device=self.device)
-        with torch.cuda.stream(stream):
-            out[:plan.first_q].zero_()
-            out[plan.total_q:].zero_()
 
     # -- rotary positions ----------------------------------------------------------
     def rotary(self, table: RotaryTable, positions, q, k=None, inverse: bool = False, inplace: bool = False,

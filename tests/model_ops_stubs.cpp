@@ -60,6 +60,7 @@ int op_scratch(sfe_ctx*, size_t, hipStream_t, void** out) {
 }
 
 hipError_t launch_attn_mask(const uint8_t*, int64_t, uint64_t*, hipStream_t) { return hipSuccess; }
+hipError_t launch_attn_zero(const AttnTensor&, int, int, int64_t, int64_t, int64_t, hipStream_t) { return hipSuccess; }
 hipError_t launch_attn(const AttnArgs&, int, int, int, hipStream_t) { return hipSuccess; }
 hipError_t launch_rotary(const RotaryArgs&, int, bool, int, hipStream_t) { return hipSuccess; }
 hipError_t launch_residual(const ResidualArgs&, int, int, hipStream_t) { return hipSuccess; }

@@ -381,3 +381,33 @@ def test_plans_end_with_their_context():
     again.close()
     own.close()
     del kept
+
+
+@pytest.mark.parametrize("heads,dim,dtype", [(1, 8, "f16"), (2, 64, "bf16"), (5, 104, "bf16")])
+def test_rows_of_no_sequence_in_the_contexts_order(heads, dim, dtype):
+    """Zeroed within the call: an operator queued after it on another stream reads zeros."""
+    import torch
+    from scriptrs_amd import ModelOps
+    own = ModelOps()
+    t = {"bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    first, last, rows = 700, 900, 30_000
+    plan = own.attention_plan([first, last], [0, 50], heads, heads, dim)
+    q = torch.randn(rows, heads, dim, device="cuda").to(t)
+    k = torch.randn(50, heads, dim, device="cuda").to(t)
+    out = torch.empty(rows, heads, dim + 8, dtype=t, device="cuda")
+    block = torch.zeros(rows, heads * (dim + 8), dtype=t, device="cuda")
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    want = own.attention(plan, q, k, k)
+    for stream in (a, b):  # (the context's first calls on other streams wait on the host)
+        own.residual_norm(block, block, stream=stream)
+    for _ in range(3):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        own.attention(plan, q, k, k, stream=a, out=out[..., :dim])
+        read, _ = own.residual_norm(block, out.view(rows, -1), stream=b)
+        torch.cuda.synchronize()
+        read = read.view(out.shape)
+        assert (read[..., dim:] == 7).all() and torch.equal(read[..., :dim], want)
+        assert not read[:first, :, :dim].any() and not read[last:, :, :dim].any() and read[first:last, :, :dim].all(-1).all()
+    plan.close()
+    own.close()

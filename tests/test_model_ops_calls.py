@@ -101,3 +101,17 @@ def test_calls_without_a_stream_take_their_devices(ops):
     assert {name: args[9 if name == "sfe_attention_plan" else 8] for name, args in ops.recorded} == {
         "sfe_attention_plan": 999, "sfe_attention": 999}
     plan._handle = None
+
+
+@pytest.mark.parametrize("offsets,rows,name", [([0, 4], 4, "sfe_attention"), ([0, 4], 6, "sfe_attention_rows"),
+                                               ([1, 4], 4, "sfe_attention_rows"), ([3], 5, "sfe_attention_rows")])
+def test_rows_of_no_sequence_are_part_of_the_call(ops, offsets, rows, name):
+    """They are zeroed by the call itself, in the context's order; nothing is queued behind it."""
+    plan = ops.attention_plan(offsets, offsets, 2, 2, 64, stream=0)
+    plan._handle = ctypes.c_void_p(2)
+    q, out = torch.zeros(rows, 2, 64, dtype=torch.bfloat16), torch.ones(rows, 2, 64, dtype=torch.bfloat16)
+    ops.attention(plan, q, q, q, out=out, stream=0)
+    assert [n for n, _ in ops.recorded] == ["sfe_attention_plan", name] and bool((out == 1).all())
+    if name == "sfe_attention_rows":
+        assert ops.recorded[-1][1][8] == rows
+    plan._handle = None

@@ -120,3 +120,29 @@ def test_buffers_of_freed_plans_are_reused(contexts):
     d = make_plan(L, ctx)
     assert L.stub_destroy(ctx) == 2
     L.sfe_attention_plan_free(d)
+
+
+def test_rows_of_no_sequence_overlap_nothing(contexts):
+    """sfe_attention_rows writes all of out's rows, also past the last sequence."""
+    L = contexts
+    ctx = L.stub_context()
+    plan = make_plan(L, ctx, q=(2, 10), k=(2, 10))
+    x, row = _lib.SfeHeads(AT, 128, 64), 256
+
+    def call(out, rows, p=plan):
+        return L.sfe_attention_rows(p, _lib.SFE_BF16, x, x, x, None, 0.125, _lib.SfeHeads(out, 128, 64), rows, None)
+    passes(L, call(AT + 10 * row, 10))
+    passes(L, call(AT + 10 * row, 20))
+    passes(L, call(AT - 20 * row, 20))
+    refused(L, call(AT - 20 * row, 21), "overlaps")
+    refused(L, call(AT + 9 * row, 10), "overlaps")
+    refused(L, call(AT + 10 * row, 9), "rows")
+    refused(L, call(AT + 10 * row, (1 << 40) + 1), "rows")
+    refused(L, call(None, 20), "null out")
+    empty, before = make_plan(L, ctx, q=(3, 3), k=(3, 3)), L.stub_calls()
+    passes(L, call(AT, 3, empty))
+    refused(L, call(None, 4, empty), "null out")
+    assert L.stub_calls() == before + 1  # (rows of no sequence are work)
+    for p in (plan, empty):
+        L.sfe_attention_plan_free(p)
+    assert L.stub_destroy(ctx) == 1

@@ -117,7 +117,8 @@ class ModelOps:
     """The operators on one device.
 
     One instance per host thread, like the feature extractor (it owns an
-    ``sfe_ctx`` or shares ``extractor``'s; calls on it are ordered after each other)."""
+    ``sfe_ctx`` or shares ``extractor``'s; calls on it are ordered after each other).
+    ``stream``: a call's stream (torch's, or its handle), the current one without; its inputs have to be ready there."""
 
     def __init__(self, device: int = 0, extractor: ParakeetFeatureExtractor | None = None):
         import torch
@@ -143,6 +144,34 @@ class ModelOps:
                 return self._stream_of(self.device)
             stream = self._torch.cuda.current_stream(self.device)
         return _stream_handle(stream)
+
+    def _other(self, stream):
+        """The call's stream as torch's, where it is not the current one."""
+        if stream is None:
+            return None
+        torch, handle = self._torch, _stream_handle(stream).value or 0
+        if handle == (self._stream(None) or 0):
+            return None
+        if isinstance(stream, torch.cuda.Stream):
+            return stream
+        return torch.cuda.ExternalStream(handle, device=self.device) if handle else torch.cuda.default_stream(self.device)
+
+    def _new(self, other, like, dtype=None):
+        """An output, of the memory of the stream that writes it (the current stream's may have just been freed and
+        still be in use there), held for the current stream too, on which the caller may read it later."""
+        if other is None:
+            return self._empty_like(like) if dtype is None else self._empty_like(like, dtype=dtype)
+        with self._torch.cuda.stream(other):
+            t = self._empty_like(like, dtype=dtype or like.dtype)
+        t.record_stream(self._torch.cuda.current_stream(self.device))
+        return t
+
+    @staticmethod
+    def _held(other, *tensors) -> None:
+        """Given tensors keep their memory until the call's stream is done with them, freed meanwhile or not."""
+        for t in tensors:
+            if t is not None:
+                t.record_stream(other)
 
     def close(self) -> None:
         if self._own:
@@ -200,8 +229,11 @@ class ModelOps:
                     key_mask.shape[0] < plan.total_k or not key_mask.is_contiguous():
                 raise InvalidModelOutput(f"key_mask must be a contiguous bool tensor of [{plan.total_k}]")
             mask = key_mask.data_ptr()
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, q, k, v, key_mask, out)
         if out is None:
-            out = self._empty_like(q)
+            out = self._empty_like(q) if other is None else self._new(other, q)
             ho.data, ho.row_stride, ho.head_stride = out.data_ptr(), plan.heads * plan.head_dim, plan.head_dim
         else:
             _same(out, q, "out")
@@ -235,9 +267,12 @@ class ModelOps:
         pos = _contiguous(positions, "positions", torch.int32, (rows,))
         hq, hqo, hk, hko = self._h
         _heads(q, "q", shape, hq)
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, positions, q, k)
         q_out = q
         if not inplace:
-            q_out = self._empty_like(q)
+            q_out = self._empty_like(q) if other is None else self._new(other, q)
             hqo.data, hqo.row_stride, hqo.head_stride = q_out.data_ptr(), heads * dim, dim
         k_out, kv_heads = None, 0
         if k is not None:
@@ -250,7 +285,7 @@ class ModelOps:
             _heads(k, "k", shape, hk)
             k_out = k
             if not inplace:
-                k_out = self._empty_like(k)
+                k_out = self._empty_like(k) if other is None else self._new(other, k)
                 hko.data, hko.row_stride, hko.head_stride = k_out.data_ptr(), kv_heads * dim, dim
         pq, pqo, pk, pko = self._hp
         if inplace:
@@ -307,8 +342,11 @@ class ModelOps:
         a.post_bias = None if post_bias is None else self._weight("post_bias", post_bias, width)
         a.pre_weight = None if pre_weight is None else self._weight("pre_weight", pre_weight, width)
         a.pre_bias = None if pre_bias is None else self._weight("pre_bias", pre_bias, width)
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, residual, block, gate, post_weight, post_bias, pre_weight, pre_bias, out, norm_out)
         if out is None:
-            out = self._empty_like(residual)
+            out = self._empty_like(residual) if other is None else self._new(other, residual)
             a.residual_out, a.residual_out_row = out.data_ptr(), width
         else:
             _same(out, residual, "out")
@@ -316,7 +354,7 @@ class ModelOps:
         if pre is None:
             norm_out = a.norm_out = None
         elif norm_out is None:
-            norm_out = self._empty_like(block)
+            norm_out = self._empty_like(block) if other is None else self._new(other, block)
             a.norm_out, a.norm_out_row = norm_out.data_ptr(), width
         else:
             _same(norm_out, block, "norm_out")
@@ -358,9 +396,12 @@ class ModelOps:
             if finished.get_device() != device:
                 _wrong_device("finished", finished, device)
             fp = _contiguous(finished, "finished", torch.bool, shape)
-        new = torch.empty_like(scores)
-        parents, tokens = torch.empty_like(scores, dtype=torch.int32), torch.empty_like(scores, dtype=torch.int32)
-        ended = torch.empty_like(scores, dtype=torch.bool)
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, logits, scores, finished)
+        new = self._new(other, scores)
+        parents, tokens = self._new(other, scores, torch.int32), self._new(other, scores, torch.int32)
+        ended = self._new(other, scores, torch.bool)
         rc = self._lib.sfe_beam_select(self._fe._handle(), code, logits.data_ptr(), logits.stride(0), streams, beams,
                                        vocab, sp, fp, end_token, new.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
                                        ended.data_ptr(), self._stream(stream))
@@ -386,6 +427,9 @@ class ModelOps:
         streams, beams = shape
         pp = _contiguous(parents, "parents", torch.int32, shape)
         n, out = len(states), []
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, parents)
         table = self._states if n <= len(self._states) else (SfeBeamState * n)()
         for i, s in enumerate(states):
             if s.get_device() != self.device:
@@ -396,7 +440,7 @@ class ModelOps:
                 raise InvalidModelOutput(f"state {i} must be contiguous with {streams * beams} beams in dimension {dim}, "
                                          f"got {list(full)}")
             if given is None:
-                o = torch.empty_like(s)
+                o = self._new(other, s)
             else:
                 o = given[i]
                 if o.get_device() != self.device:
@@ -405,6 +449,8 @@ class ModelOps:
                 if not o.is_contiguous():
                     raise InvalidModelOutput(f"out {i} must be contiguous")
             out.append(o)
+            if other is not None:
+                self._held(other, s, o)
             row = table[i]
             row.in_, row.out = s.data_ptr(), o.data_ptr()
             row.outer, row.inner_bytes = math.prod(full[:at]), math.prod(full[at + 1:]) * s.element_size()

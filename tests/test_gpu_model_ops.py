@@ -433,3 +433,60 @@ def test_captured(ops):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def busy():
+    """Holds the current stream for milliseconds, long after the host's next calls."""
+    import torch
+    torch.cuda._sleep(5_000_000)
+
+
+def test_outputs_of_calls_on_another_stream(ops):
+    """Memory that the current stream has freed and still reads is not the output of a call on another stream."""
+    import torch
+    side, n = torch.cuda.Stream(), 1 << 20
+    x = torch.ones(1024, 1024, device="cuda")
+    for _ in range(3):
+        ops.residual_norm(x, x, stream=side)
+        torch.cuda.synchronize()
+        a, kept = torch.full((n,), 3.0, device="cuda").view(1024, 1024), torch.empty(n, device="cuda").view(1024, 1024)
+        torch.cuda.synchronize()
+        busy()
+        kept.copy_(a)
+        del a
+        y, _ = ops.residual_norm(x, x, stream=side)
+        torch.cuda.synchronize()
+        assert (kept == 3).all() and (y == 2).all()
+
+
+def test_inputs_of_calls_on_another_stream(ops):
+    """An input that is freed after a call on another stream keeps its memory until the call has read it."""
+    import torch
+    side, x = torch.cuda.Stream(), torch.ones(1024, 1024, device="cuda")
+    for _ in range(3):
+        ops.residual_norm(x, x, stream=side)
+        a = torch.full_like(x, 3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            busy()
+        y, _ = ops.residual_norm(x, a, stream=side)
+        del a
+        junk = [torch.full_like(x, 9.0) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert (y == 4).all()
+        del junk
+
+
+def test_outputs_of_another_stream_read_on_the_current_one(ops):
+    """An output that is freed while the current stream reads it is not written by the other stream's next call."""
+    import torch
+    side, x = torch.cuda.Stream(), torch.ones(1024, 1024, device="cuda")
+    for _ in range(3):
+        y, _ = ops.residual_norm(x, x, stream=side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+        busy()
+        kept = y * 1
+        del y
+        z, _ = ops.residual_norm(x, x, scale=6.0, stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        assert (kept == 2).all() and (z == 7).all()

@@ -1,5 +1,6 @@
 """What ModelOps hands to the library, without a GPU: the library's calls are replaced by ones that record their
 arguments, and the tensors are the host's (device -1)."""
+import contextlib
 import ctypes
 
 import pytest
@@ -115,3 +116,74 @@ def test_rows_of_no_sequence_are_part_of_the_call(ops, offsets, rows, name):
     if name == "sfe_attention_rows":
         assert ops.recorded[-1][1][8] == rows
     plan._handle = None
+
+
+class Streams:
+    """torch's streams replaced: which is current, and which tensors were allocated on or held for which."""
+
+    def __init__(self, monkeypatch, ops):
+        self.current, self.allocated, self.held = "main", [], []
+        empty_like = ops._empty_like
+
+        def allocate(like, **kw):
+            t = empty_like(like, **kw)
+            self.allocated.append((self.current, t.data_ptr()))
+            return t
+
+        def hold(t, stream):
+            self.held.append((stream, t.data_ptr()))
+        monkeypatch.setattr(ops, "_empty_like", allocate)
+        monkeypatch.setattr(torch, "empty_like", allocate)
+        monkeypatch.setattr(torch.Tensor, "record_stream", hold)
+        monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: f"stream {handle}")
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: self.current)
+        monkeypatch.setattr(torch.cuda, "stream", self.use)
+
+    @contextlib.contextmanager
+    def use(self, stream):
+        before, self.current = self.current, stream
+        yield
+        self.current = before
+
+
+def operator_calls(ops):
+    """Each operator's (inputs, call); the call returns its outputs."""
+    from scriptrs_amd import RotaryTable
+    plan = ops.attention_plan([0, 4], [0, 4], 2, 2, 64, stream=0)
+    plan._handle = ctypes.c_void_p(2)
+    h, mask = [torch.zeros(4, 2, 64, dtype=torch.bfloat16) for _ in range(3)], torch.ones(4, dtype=torch.bool)
+    pos, w = torch.zeros(4, dtype=torch.int32), [torch.ones(16) for _ in range(4)]
+    x = [torch.zeros(4, 16) for _ in range(3)]
+    logits, scores, ended = torch.zeros(4, 9), torch.zeros(2, 2), torch.zeros(2, 2, dtype=torch.bool)
+    parents = torch.zeros(2, 2, dtype=torch.int32)
+    norms = dict(post="layer", post_weight=w[0], post_bias=w[1], pre="layer", pre_weight=w[2], pre_bias=w[3])
+    yield [*h, mask], lambda s: [ops.attention(plan, *h, key_mask=mask, stream=s)]
+    yield [pos, *h[:2]], lambda s: ops.rotary(RotaryTable(64), pos, *h[:2], stream=s)
+    yield [*x, *w], lambda s: ops.residual_norm(x[0], x[1], gate=x[2], **norms, stream=s)
+    yield [logits, scores, ended], lambda s: ops.beam_select(logits, scores, ended, 3, stream=s)
+    yield [parents, *x], lambda s: ops.beam_reorder(parents, x, stream=s)
+    plan._handle = None
+
+
+def test_tensors_of_calls_on_another_stream(ops, monkeypatch):
+    """Outputs are of the call's stream's memory, inputs are held for it; on the current stream neither is needed."""
+    streams = Streams(monkeypatch, ops)
+    for given, call in operator_calls(ops):
+        for stream in (None, 0):
+            streams.allocated.clear()
+            outputs = call(stream)
+            assert streams.allocated == [("main", t.data_ptr()) for t in outputs] and not streams.held
+        streams.allocated.clear()
+        outputs = call(77)
+        assert streams.allocated == [("stream 77", t.data_ptr()) for t in outputs]
+        assert {("stream 77", t.data_ptr()) for t in given} | {("main", t.data_ptr()) for t in outputs} <= set(streams.held)
+        streams.held.clear()
+
+
+def test_given_outputs_are_held_for_another_stream(ops, monkeypatch):
+    streams = Streams(monkeypatch, ops)
+    x, y = torch.zeros(4, 16), torch.zeros(4, 16)
+    parents, out = torch.zeros(2, 2, dtype=torch.int32), [torch.zeros(4, 16) for _ in range(3)]
+    ops.residual_norm(x, y, pre="rms", pre_weight=torch.ones(16), out=out[0], norm_out=out[1], stream=77)
+    ops.beam_reorder(parents, [x], out=[out[2]], stream=77)
+    assert {("stream 77", t.data_ptr()) for t in out} <= set(streams.held) and not streams.allocated

@@ -1,7 +1,9 @@
 // A step of beam search.
 //
-// total(w, t) = score_w + (logit_wt - log sum_t exp(logit_wt)); a finished beam
-// has the one candidate (score_w, end token).  A stream's next beams are the best
+// total(w, t) = score_w + ((logit_wt - m_w) - log sum_t exp(logit_wt - m_w)), m_w the row's
+// maximum: the sum and its logarithm do not see where a row lies, so that neither do its totals
+// (formed as logit - (m + log sum), rows at 10^6 were off by 0.02 against each other, and a row wholly at
+// the lowest f32 had none).  A finished beam has the one candidate (score_w, end token).  A stream's next beams are the best
 // of its beams * vocabulary candidates, ties to the lowest (beam, token); totals of
 // -inf or NaN are no candidates, and places without one hold score -inf, token
 // -1 and their own beam as parent.
@@ -343,15 +345,13 @@ __device__ __forceinline__ int token_of(int k, int first, int t, int vocab) {
   return moved_back<N>(vector_at<N, THREADS>(first, k / N, t), vocab) + k % N;
 }
 
-// Sum of exponentials of x relative to m (0 where all is -inf; NaN stays).  The product's one
-// rounding of m log2(e) is a common factor: at most 2^-24 |m| of the logarithm, which rounds by as
-// much when m is added.
+// Sum of exponentials of x - m (0 where all is -inf; NaN stays).
 template <int E>
 __device__ __forceinline__ float exp_sum(const float (&x)[E], float m) {
-  const float c = m == -INFINITY ? 0.0f : -kLog2e * m;
+  const float r = m == -INFINITY ? 0.0f : m;
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int k = 0; k < E; ++k) s[k % 4] += __builtin_amdgcn_exp2f(fmaf(x[k], kLog2e, c));
+  for (int k = 0; k < E; ++k) s[k % 4] += __builtin_amdgcn_exp2f((x[k] - r) * kLog2e);
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 __device__ __forceinline__ void write_beam(const BeamArgs& a, int stream, int r, bool found, float x, int i) {
@@ -392,9 +392,9 @@ __global__ __launch_bounds__(1024) void sfe_beam_small_kernel(BeamArgs a) {
     float x[E], groups[E / kGroup];
     row_values<T, NV, 64>(v, 0, lane, a.vocab, x);
     const float m = wave_max(max_of(x, groups));
-    const float logz = m + logf(wave_sum(exp_sum(x, m)));
+    const float log_sum = logf(wave_sum(exp_sum(x, m)));
 #pragma unroll
-    for (int k = 0; k < E; ++k) x[k] = score + (x[k] - logz);
+    for (int k = 0; k < E; ++k) x[k] = score + ((x[k] - m) - log_sum);
     const float top = max_of(x, groups);
     best_add(best, a.beams, lists.x[wave], lists.i[wave], x, top, groups,
              [&](int k) { return w * a.vocab + token_of<T, 64>(k, 0, lane, a.vocab); });
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(kThreads, 4) void sfe_beam_rows_kernel(BeamArgs a, 
 // latency (one row's sums, one round of candidates, the join).
 __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, int spans) {
   __shared__ Lists lists;
-  __shared__ float logz[kMaxBeams];
+  __shared__ float tops[kMaxBeams], log_sums[kMaxBeams];
   const int b = (int)blockIdx.x, t = (int)threadIdx.x, W = a.beams;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Part* part = reinterpret_cast<const Part*>(a.scratch) + (int64_t)b * W * spans;
@@ -478,7 +478,10 @@ __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, 
       sum += p.sum * (p.top == top ? 1.0f : __builtin_amdgcn_exp2f((p.top - top) * kLog2e));
     }
     sum = wave_sum(sum);
-    if ((t & 63) == 0) logz[w] = top + logf(sum);
+    if ((t & 63) == 0) {
+      tops[w] = top;
+      log_sums[w] = logf(sum);
+    }
   }
   __syncthreads();
   Best best = best_none();
@@ -495,7 +498,7 @@ __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, 
       } else {
         const Cand c = cand[e];
         i = w * a.vocab + c.t;
-        if (c.t >= 0) x = scores[w] + (c.x - logz[w]);
+        if (c.t >= 0) x = scores[w] + ((c.x - tops[w]) - log_sums[w]);
       }
     }
     best_enter(best, W, lists.x[wave], lists.i[wave], x, i);

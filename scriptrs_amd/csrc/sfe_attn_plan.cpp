@@ -106,12 +106,13 @@ int form_of(int64_t lq, int64_t lk, int group, int head_dim, int32_t left, int32
 // work, one an XCD.
 void share_out(int kv_heads, AttnForm* f) {
   const int64_t n = (int64_t)f->items.size();
+  std::fill(f->share, f->share + 9, 0);
+  if (n == 0) return;  // (no work to have a part of)
   std::vector<double> sum((size_t)n + 1, 0.0);
   for (int64_t i = 0; i < n; ++i) {
     const AttnItem& it = f->items[(size_t)i];
     sum[(size_t)i + 1] = sum[(size_t)i] + 4.0 + (double)((it.kv1 - it.kv0 + kAttnStepRows - 1) / kAttnStepRows);
   }
-  f->share[0] = 0;
   for (int x = 1; x < 8; ++x) {
     const double at = sum[(size_t)n] * kv_heads * x / 8.0;
     const int64_t head = std::min<int64_t>(kv_heads - 1, (int64_t)(at / sum[(size_t)n]));

@@ -135,3 +135,18 @@ def test_beam_refusals():
     refused(L.sfe_beam_reorder(None, 64, 2, 4, s, 1, None), "null context")
     refused(L.sfe_beam_reorder(None, 64, 2, 40, s, 1, None), "beams")
     refused(L.sfe_beam_reorder(None, 64, 2, 4, s, -1, None), "negative")
+
+
+@pytest.mark.parametrize("seed", [1, 2])
+def test_planner_without_undefined_behaviour(tmp_path, seed):
+    """The planner's host run with every undefined operation a trap, conversions and divisions of doubles included."""
+    if not os.path.exists(HIPCC):
+        pytest.skip("hipcc not available")
+    exe = str(tmp_path / "attn_plan")
+    subprocess.run([HIPCC, "-O1", "-g", "-std=c++17", "-x", "hip", "--cuda-host-only", "-Wno-unused-command-line-argument",
+                    "-Xarch_host", "-fsanitize=undefined,float-cast-overflow,float-divide-by-zero",
+                    "-Xarch_host", "-fsanitize-trap=all",
+                    "-I", os.path.join(ROOT, "include"), "-I", CSRC, os.path.join(ROOT, "tests", "attn_plan_driver.cpp"),
+                    os.path.join(CSRC, "sfe_attn_plan.cpp"), "-o", exe], check=True, stderr=subprocess.DEVNULL)
+    r = subprocess.run([exe, str(seed)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "bad 0", (r.returncode, r.stdout + r.stderr)

@@ -308,18 +308,20 @@ int sfe_rotary_init(sfe_rotary_table* table, int32_t rotary_dim, int32_t layout,
     table->rotary_dim = rotary_dim;
     table->layout = layout;
     table->magnitude = (float)magnitude;
-    const double R = rotary_dim, two_pi = 6.283185307179586476925;
-    const double b = scaling == SFE_ROTARY_BASE ? base * pow(factor, R / (R - 2)) : base;
+    // (64 bits of mantissa: a double's 53 are off by 2^-25 of a turn and more at the farthest positions)
+    typedef long double Real;
+    const Real R = rotary_dim, two_pi = 6.28318530717958647692528676655900577L;
+    const Real b = scaling == SFE_ROTARY_BASE ? base * powl(factor, R / (R - 2)) : (Real)base;
     for (int p = 0; p < rotary_dim / 2; ++p) {
-      double f = pow(b, -2.0 * p / R);
+      Real f = powl(b, -2 * p / R);
       if (scaling == SFE_ROTARY_LINEAR) f /= factor;
       if (scaling == SFE_ROTARY_PARTS) {
-        const double turns = original_length * f / two_pi;
-        const double keep = std::min(1.0, std::max(0.0, (turns - low) / (high - low)));
+        const Real turns = original_length * f / two_pi;
+        const Real keep = std::min<Real>(1, std::max<Real>(0, (turns - low) / ((Real)high - low)));
         f *= (1 - keep) / factor + keep;
       }
       // at most 1 radian a position: below a turn
-      table->step[p] = (uint64_t)rint(f / two_pi * 18446744073709551616.0);
+      table->step[p] = (uint64_t)rintl(f / two_pi * 18446744073709551616.0L);
     }
     return SFE_OK;
   });

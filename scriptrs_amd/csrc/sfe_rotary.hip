@@ -9,8 +9,9 @@
 // The angle of a far position has to be exact modulo a turn: f_p is held as a
 // fraction of a turn in 64 bits and multiplied by the position modulo 2^64, so
 // whole turns drop out and the top 32 bits are the turn's fraction, correct to
-// 2^-32 at any 32-bit position (in f32, position * f_p would be off by 3e-3
-// rad at 45,000).  Sine and cosine are their power series over an eighth of a
+// 2^-31 at any 32-bit position: 2^-32 for the bits that are cut off and less than
+// that for the step, which is off by half a unit and 2^-61 of it (in f32, position *
+// f_p would be off by 3e-3 rad at 45,000).  Sine and cosine are their power series over an eighth of a
 // turn to either side, in f32 (error below 1e-7).
 //
 // Bound by memory: each element is read and written once, and a row's sines and

@@ -150,3 +150,34 @@ def test_planner_without_undefined_behaviour(tmp_path, seed):
                     os.path.join(CSRC, "sfe_attn_plan.cpp"), "-o", exe], check=True, stderr=subprocess.DEVNULL)
     r = subprocess.run([exe, str(seed)], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip() == "bad 0", (r.returncode, r.stdout + r.stderr)
+
+
+ROTARY_SCALINGS = {"none": (0, 1.0, 1.0, 0.0, 1.0), "linear": (1, 4.0, 1.0, 0.0, 1.0), "base": (2, 8.0, 1.0, 0.0, 1.0),
+                   "parts": (3, 8.0, 4096.0, 1.0, 32.0)}
+
+
+@pytest.mark.parametrize("scaling", ROTARY_SCALINGS)
+@pytest.mark.parametrize("R", [2, 30, 64, 96, 128, 256])
+def test_rotary_steps_at_the_farthest_position(R, scaling):
+    """A step is off by half a unit of 2^-64 turns for its rounding and by a few roundings of 2^-64 of it: at
+    position 2^31 - 1 the angle is off by less than 2^-32 of a turn.  In 60 digits; the inputs are doubles."""
+    from decimal import Decimal, getcontext
+    getcontext().prec = 60
+    kind, factor, length, low, high = ROTARY_SCALINGS[scaling]
+    if scaling == "base" and R < 4:
+        pytest.skip("scaling the base needs at least 2 pairs")
+    two_pi = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+    base = 500_000.0
+    log_base = Decimal(base).ln() + (Decimal(factor).ln() * R / (R - 2) if scaling == "base" else 0)
+    t = _lib.SfeRotaryTable()
+    assert _lib.lib().sfe_rotary_init(ctypes.byref(t), R, 0, base, kind, factor, length, low, high, 1.0) == _lib.SFE_OK
+    for p in range(R // 2):
+        f = (log_base * -2 * p / R).exp()
+        if scaling == "linear":
+            f /= Decimal(factor)
+        if scaling == "parts":
+            keep = min(Decimal(1), max(Decimal(0), (Decimal(length) * f / two_pi - Decimal(low)) / Decimal(high - low)))
+            f *= (1 - keep) / Decimal(factor) + keep
+        want = f / two_pi * 2 ** 64
+        assert abs(t.step[p] - want) <= Decimal("0.5") + want / 2 ** 61, p
+        assert abs(t.step[p] - want) * (2 ** 31 - 1) < 2 ** 32, p

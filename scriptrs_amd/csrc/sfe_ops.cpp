@@ -10,6 +10,7 @@
 #include <exception>
 #include <memory>
 #include <new>
+#include <numeric>
 
 #include "../../include/scriptrs_fe.h"
 #include "sfe_ops.hpp"
@@ -49,21 +50,34 @@ int guarded(F&& body) {
 
 bool known_dtype(int32_t d) { return d == SFE_F32 || d == SFE_BF16 || d == SFE_F16; }
 
-// A tensor's rows: n of len bytes, row bytes apart.
+// A tensor's rows: n of len bytes, row bytes apart; each of `heads` pieces of `piece` bytes, head bytes apart.
 struct Rows {
   const char* name;
   const void* p;
   int64_t n, row, len;
+  int64_t heads, head, piece;
+  Rows(const char* name_, const void* p_, int64_t n_, int64_t row_, int64_t len_)
+      : Rows(name_, p_, n_, row_, 1, 0, len_) {}
+  Rows(const char* name_, const void* p_, int64_t n_, int64_t row_, int64_t heads_, int64_t head_, int64_t piece_)
+      : name(name_), p(p_), n(n_), row(row_), len((heads_ - 1) * head_ + piece_), heads(heads_), head(head_), piece(piece_) {}
   int64_t extent() const { return n <= 0 ? 0 : (n - 1) * row + len; }
+  int64_t row_pitch() const { return n > 1 ? row : 0; }
+  int64_t head_pitch() const { return heads > 1 ? head : 0; }
 };
-// Whether two tensors may share memory.  Rows of one pitch may lie between each
-// other (views of one projection); otherwise whole extents are compared.
+// Whether two tensors may share memory.  Views of one buffer lie between each other: where all parts of
+// both (whole rows, single pieces, or a head's pieces of all rows) begin at multiples of one pitch from their
+// first, their places within the pitch tell; otherwise whole extents do.
 bool share(const Rows& a, const Rows& b) {
   const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
   if (a.extent() == 0 || b.extent() == 0 || x >= y + (uintptr_t)b.extent() || y >= x + (uintptr_t)a.extent()) return false;
-  if (a.row != b.row || a.len > a.row || b.len > b.row) return true;
-  const int64_t d = ((int64_t)(y - x) % a.row + a.row) % a.row;
-  return d < a.len || d + b.len > a.row;
+  auto between = [&](int64_t pitch, int64_t mine, int64_t other) {
+    if (pitch == 0) return false;
+    const int64_t d = ((int64_t)(y - x) % pitch + pitch) % pitch;
+    return d >= mine && d + other <= pitch;
+  };
+  const int64_t rows = std::gcd(a.row_pitch(), b.row_pitch()), heads = std::gcd(a.head_pitch(), b.head_pitch());
+  return !between(rows, a.len, b.len) && !between(std::gcd(rows, heads), a.piece, b.piece) &&
+         !between(heads, (a.n - 1) * a.row + a.piece, (b.n - 1) * b.row + b.piece);
 }
 // An output that is an input's own view.
 bool same_view(const Rows& a, const Rows& b) {
@@ -90,7 +104,7 @@ bool apart(const sfe_heads& t, int64_t rows, int heads, int dim) {
   return rows <= 1 || heads <= 1 || r >= (heads - 1) * h + dim || h >= (rows - 1) * r + dim;
 }
 Rows rows_of(const char* name, const sfe_heads& t, int64_t rows, int heads, int dim, int esize) {
-  return Rows{name, t.data, rows, t.row_stride * esize, ((heads - 1) * t.head_stride + dim) * esize};
+  return Rows(name, t.data, rows, t.row_stride * esize, heads, t.head_stride * esize, (int64_t)dim * esize);
 }
 
 int check_offsets(const char* name, const int64_t* off, int32_t n) {
@@ -442,9 +456,7 @@ int sfe_residual_norm(sfe_ctx* ctx, const sfe_residual* r, void* stream) {
                {{"residual_out", r->residual_out, r->rows, r->residual_out_row, r->width}, xs, true},
                {{"norm_out", r->pre != SFE_NORM_NONE ? r->norm_out : nullptr, r->rows, r->norm_out_row, r->width}, ys, true}};
     auto in_bytes = [](Rows x, int size) {
-      x.row *= size;
-      x.len *= size;
-      return x;
+      return Rows(x.name, x.p, x.n, x.row * size, x.len * size);
     };
     for (const auto& t : all) {
       if (!t.r.p) continue;

@@ -490,3 +490,26 @@ def test_outputs_of_another_stream_read_on_the_current_one(ops):
         z, _ = ops.residual_norm(x, x, scale=6.0, stream=side.cuda_stream)
         torch.cuda.synchronize()
         assert (kept == 2).all() and (z == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape,order", [((500, 3, 4, 64), (0, 2, 3)), ((500, 4, 3, 64), (0, 1, 3)), ((4, 500, 3, 64), (1, 0, 3)),
+                                         ((4, 3, 500, 64), (2, 0, 3)), ((3, 4, 500, 64), (2, 1, 3))], ids=str)
+def test_rotary_in_place_on_views_of_one_projection(ops, shape, order, dtype):
+    """q and k interleaved by rows, by heads or head by head: turned where they lie, the third part untouched."""
+    import torch
+    from scriptrs_amd import RotaryTable
+    x = torch.randn(shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).to(torch_dtype(dtype))
+    part = next(i for i in range(4) if i not in order)
+
+    def views(t):
+        kept = [d for d in range(4) if d != part]
+        return [t.select(part, i).permute([kept.index(d) for d in order]) for i in range(3)]
+    q, k, v = views(x)
+    assert q.shape == (500, 4, 64)
+    pos = torch.arange(500, device="cuda", dtype=torch.int32)
+    table, before = RotaryTable(64), v.clone()
+    qo, ko = ops.rotary(table, pos, q, k)
+    assert not torch.equal(qo, q)
+    ops.rotary(table, pos, q, k, inplace=True)
+    assert torch.equal(q, qo) and torch.equal(k, ko) and torch.equal(v, before)

@@ -146,3 +146,66 @@ def test_rows_of_no_sequence_overlap_nothing(contexts):
     for p in (plan, empty):
         L.sfe_attention_plan_free(p)
     assert L.stub_destroy(ctx) == 1
+
+
+# views of one buffer: (row stride, head stride, starts of q and k) in elements of 4 rows, 2 heads, 64 channels
+ROWS, HEADS, DIM = 4, 2, 64
+LAYOUTS = {"parts of a row": (3 * HEADS * DIM, DIM, 0, HEADS * DIM),
+           "parts of a head": (3 * HEADS * DIM, 3 * DIM, 0, DIM),
+           "parts of a head, the last before the first": (3 * HEADS * DIM, 3 * DIM, 2 * DIM, 0),
+           "heads outermost, parts of a row": (3 * DIM, ROWS * 3 * DIM, 0, DIM),
+           "heads outermost, parts of a head": (DIM, 3 * ROWS * DIM, 0, ROWS * DIM),
+           "one after the other": (HEADS * DIM, DIM, 0, ROWS * HEADS * DIM)}
+
+
+def bytes_of(start, row, head, size):
+    at = {start + r * row + h * head + d for r in range(ROWS) for h in range(HEADS) for d in range(DIM)}
+    return {b for e in at for b in range(e * size, (e + 1) * size)}
+
+
+def turn_in_place(L, table, q, k):
+    return L.sfe_rotary(CTX, ctypes.byref(table), 0, _lib.SFE_BF16, AT - 4096, ROWS, DIM, HEADS, q, q, HEADS, k, k, None)
+
+
+@pytest.fixture
+def table(checks):
+    t = _lib.SfeRotaryTable()
+    passes(checks, checks.sfe_rotary_init(ctypes.byref(t), DIM, 0, 1e4, 0, 1.0, 1.0, 0.0, 1.0, 1.0))
+    return t
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_views_of_one_projection(contexts, table, layout):
+    """Views that lie between each other without sharing a byte are no overlap, in any order of rows, heads and parts."""
+    L = contexts
+    row, head, q0, k0 = LAYOUTS[layout]
+    q, k = (_lib.SfeHeads(AT + 2 * x, row, head) for x in (q0, k0))
+    assert not bytes_of(q0, row, head, 2) & bytes_of(k0, row, head, 2)
+    passes(L, turn_in_place(L, table, q, k))
+    ctx = L.stub_context()
+    plan = make_plan(L, ctx, q=(0, ROWS), k=(0, ROWS))
+    passes(L, L.sfe_attention(plan, _lib.SFE_BF16, q, q, q, None, 0.125, k, None))
+    L.sfe_attention_plan_free(plan)
+    L.stub_destroy(ctx)
+
+
+def test_views_are_refused_where_they_share_a_byte(contexts, table):
+    """For k moved over q by every 16 bytes, the views of each layout: refused whenever bytes are shared."""
+    L = contexts
+    for row, head, q0, _ in LAYOUTS.values():
+        mine = bytes_of(q0, row, head, 2)
+        q = _lib.SfeHeads(AT + 2 * q0, row, head)
+        for k0 in range(0, 3 * ROWS * HEADS * DIM, 8):
+            rc = turn_in_place(L, table, q, _lib.SfeHeads(AT + 2 * k0, row, head))
+            if mine & bytes_of(k0, row, head, 2):
+                refused(L, rc, "overlaps")
+
+
+def test_views_of_other_strides(contexts, table):
+    """Strides of q and k that differ: a pitch that divides all of them tells them apart or not."""
+    L = contexts
+    wide, narrow = 6 * DIM, 3 * DIM
+    q = _lib.SfeHeads(AT, 2 * wide, wide)
+    passes(L, turn_in_place(L, table, q, _lib.SfeHeads(AT + 2 * DIM, 2 * narrow, narrow)))
+    refused(L, turn_in_place(L, table, q, _lib.SfeHeads(AT + 2 * (DIM - 8), 2 * narrow, narrow)), "overlaps")
+    refused(L, turn_in_place(L, table, q, _lib.SfeHeads(AT + 2 * (wide - 8), 2 * narrow, narrow)), "overlaps")

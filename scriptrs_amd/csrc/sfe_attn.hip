@@ -1010,6 +1010,7 @@ __global__ __launch_bounds__(64 * kAttnWavesFew, 1) void sfe_attn_few_kernel(Att
     for (int s = 0; s < NT; ++s) asm volatile("" : "+v"(q[s]));
   }
   const int lo_all = __builtin_amdgcn_readlane(lo, 15), hi_all = __builtin_amdgcn_readlane(hi, 0);
+  const bool overlaid = a.v.row < dim_bytes;
 
   F4 o[ND];
 #pragma unroll
@@ -1032,7 +1033,9 @@ __global__ __launch_bounds__(64 * kAttnWavesFew, 1) void sfe_attn_few_kernel(Att
       for (int c = 0; c < NT; ++c)
         s[h] = Mat<T>::m16(read_k<T>(k_addr[c] + kb + h * 16 * G::kPitch), q[c], s[h]);
     }
-    const bool uneven = lo_all > kv || hi_all < (lk < kv + kStep ? lk : kv + kStep) - 1;
+    // keys that some rows do not see; rows past the last key read as values of it where v's rows lie over each other
+    // (stride 0 for one value of all keys), and as zeros elsewhere
+    const bool uneven = lo_all > kv || hi_all < (lk < kv + kStep ? lk : kv + kStep) - 1 || (overlaid && end < kv + kStep);
     const bool edge = uneven || end < kv + kStep;
     uint32_t see = ~0u;
     if (edge || (MASKED && bits != ~0u)) {

@@ -411,3 +411,23 @@ def test_rows_of_no_sequence_in_the_contexts_order(heads, dim, dtype):
         assert not read[:first, :, :dim].any() and not read[last:, :, :dim].any() and read[first:last, :, :dim].all(-1).all()
     plan.close()
     own.close()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("lq,lk,heads", [([1], [10], 2), ([3, 1], [33, 90], 2), ([1], [2100], 2), ([126], [126], 2),
+                                         ([40] * 40, [40] * 40, 8), ([700, 5], [700, 5], 8)], ids=str)
+def test_one_value_for_all_keys(ops, lq, lk, heads, bad):
+    """A value row broadcast over the keys (stride 0), and rows that overlap each other: what is not finite arrives as it
+    is, though the rows past a step's last key read as values too."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(16)
+    for dim in (64, 128):
+        q = torch.randn(sum(lq), heads, dim, device="cuda", generator=g).bfloat16()
+        k = torch.randn(sum(lk), heads, dim, device="cuda", generator=g).bfloat16()
+        row = torch.randn(1, heads, dim, device="cuda", generator=g).bfloat16()
+        row[0, 0, 5] = bad
+        check(ops, lq, lk, heads, heads, dim, q=q, k=k, v=row.expand(sum(lk), heads, dim))
+        # rows 8 channels apart of one line of numbers, the last 8 of them not finite: only the last key's row holds them
+        line = torch.randn(8 * (sum(lk) - 1) + dim, device="cuda", generator=g).bfloat16()
+        line[-8:] = bad
+        check(ops, lq, lk, heads, 1, dim, q=q, k=k[:, :1], v=line.as_strided((sum(lk), 1, dim), (8, dim, 1)))

@@ -22,6 +22,7 @@ from ._lib import SfeBeamState, SfeHeads, SfeResidual, SfeRotaryTable
 from .frontend import InvalidModelOutput, ParakeetFeatureExtractor, _check, _ip, _stream_handle
 
 MAX_BEAMS = 32
+MAX_INT32 = (1 << 31) - 1  # (sizes are passed in 32 bits)
 
 _DTYPES: dict = {}  # torch dtype -> sfe_dtype, filled by the first ModelOps (torch is imported lazily)
 
@@ -55,6 +56,14 @@ def _same(t, like, name: str) -> None:
         raise InvalidModelOutput(f"{name} must be {like.dtype} of {list(like.shape)}, got {t.dtype} of {list(t.shape)}")
 
 
+def _int32(value, name: str) -> int:
+    """An argument that is passed in 32 bits (ctypes would drop the bits above)."""
+    value = int(value)
+    if not -(1 << 31) <= value < 1 << 31:
+        raise InvalidModelOutput(f"{name} does not fit 32 bits: {value}")
+    return value
+
+
 def _contiguous(t, name: str, dtype, shape) -> int:
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise InvalidModelOutput(f"{name} must be a contiguous {dtype} tensor of {list(shape)}, got {t.dtype} of "
@@ -82,7 +91,7 @@ class RotaryTable:
         if scaling not in self.SCALINGS:
             raise InvalidModelOutput(f"unknown rotary scaling {scaling!r}")
         self.c = SfeRotaryTable()
-        _check(_lib.lib().sfe_rotary_init(ctypes.byref(self.c), int(rotary_dim), self.LAYOUTS[layout], float(base),
+        _check(_lib.lib().sfe_rotary_init(ctypes.byref(self.c), _int32(rotary_dim, "rotary_dim"), self.LAYOUTS[layout], float(base),
                                           self.SCALINGS[scaling], float(factor), float(original_length), float(low),
                                           float(high), float(magnitude)))
         self.rotary_dim, self.layout = int(rotary_dim), layout
@@ -188,11 +197,11 @@ class ModelOps:
         if qo.size == 0 or qo.size != ko.size:
             raise InvalidModelOutput("q_offsets and k_offsets must have one entry more than there are sequences")
         handle = ctypes.c_void_p()
-        _check(_lib.lib().sfe_attention_plan(self._fe._handle(), _ip(qo), _ip(ko), qo.size - 1, int(heads), int(kv_heads),
-                                             int(head_dim), int(left), int(right), self._stream(stream),
-                                             ctypes.byref(handle)))
-        return AttentionPlan(self, handle, int(qo[0]), int(qo[-1]), int(ko[-1]), int(heads), int(kv_heads),
-                             int(head_dim))
+        heads, kv_heads, head_dim = _int32(heads, "heads"), _int32(kv_heads, "kv_heads"), _int32(head_dim, "head_dim")
+        left, right = (min(max(int(bound), -1), 1 << 62) for bound in (left, right))
+        _check(_lib.lib().sfe_attention_plan(self._fe._handle(), _ip(qo), _ip(ko), _int32(qo.size - 1, "sequences"), heads,
+                                             kv_heads, head_dim, left, right, self._stream(stream), ctypes.byref(handle)))
+        return AttentionPlan(self, handle, int(qo[0]), int(qo[-1]), int(ko[-1]), heads, kv_heads, head_dim)
 
     def attention(self, plan: AttentionPlan, q, k, v, key_mask=None, scale: float | None = None, stream=None, out=None):
         """``softmax(scale q k^T) v`` of each of the plan's sequences:
@@ -261,6 +270,8 @@ class ModelOps:
         if len(shape) != 3:
             raise InvalidModelOutput(f"q must be [rows, heads, channels], got {list(shape)}")
         rows, heads, dim = shape
+        if heads > MAX_INT32 or dim > MAX_INT32:
+            raise InvalidModelOutput("heads and channels must be below 2^31")
         for name, t in (("positions", positions), ("q", q)):
             if t.get_device() != device:
                 _wrong_device(name, t, device)
@@ -279,7 +290,7 @@ class ModelOps:
             if k.get_device() != device:
                 _wrong_device("k", k, device)
             shape = k.shape
-            if k.dtype != q.dtype or len(shape) != 3 or shape[0] != rows or shape[2] != dim:
+            if k.dtype != q.dtype or len(shape) != 3 or shape[0] != rows or shape[2] != dim or shape[1] > MAX_INT32:
                 raise InvalidModelOutput(f"k must be {q.dtype} of [{rows}, heads, {dim}], got {k.dtype} of {list(shape)}")
             kv_heads = shape[1]
             _heads(k, "k", shape, hk)
@@ -318,6 +329,8 @@ class ModelOps:
             raise InvalidModelOutput(f"residual and block must be [rows, width], got {list(shape)} and "
                                      f"{list(block.shape)}")
         rows, width = shape
+        if width > MAX_INT32:
+            raise InvalidModelOutput(f"width {width} does not fit 32 bits")
         a = self._residual
         a.stream_dtype, a.block_dtype = _dtype_of(residual, "residual"), _dtype_of(block, "block")
         a.rows, a.width, a.post, a.pre = rows, width, self._NORMS[post], self._NORMS[pre]
@@ -391,6 +404,9 @@ class ModelOps:
             if t.get_device() != device:
                 _wrong_device(name, t, device)
         code, vocab = _dtype_of(logits, "logits"), logits.shape[1]
+        if not -1 <= end_token < vocab <= MAX_INT32 or streams > MAX_INT32 or beams > MAX_INT32:
+            raise InvalidModelOutput(f"end_token must be a token, or -1, and sizes below 2^31: got {end_token}, {streams} x "
+                                     f"{beams} beams of {vocab}")
         sp, fp = _contiguous(scores, "scores", torch.float32, shape), None
         if finished is not None:
             if finished.get_device() != device:
@@ -422,7 +438,7 @@ class ModelOps:
         if parents.get_device() != self.device:
             _wrong_device("parents", parents, self.device)
         shape = parents.shape
-        if len(shape) != 2:
+        if len(shape) != 2 or max(shape) > MAX_INT32:
             raise InvalidModelOutput(f"parents must be [streams, beams], got {list(shape)}")
         streams, beams = shape
         pp = _contiguous(parents, "parents", torch.int32, shape)

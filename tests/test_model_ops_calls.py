@@ -187,3 +187,30 @@ def test_given_outputs_are_held_for_another_stream(ops, monkeypatch):
     ops.residual_norm(x, y, pre="rms", pre_weight=torch.ones(16), out=out[0], norm_out=out[1], stream=77)
     ops.beam_reorder(parents, [x], out=[out[2]], stream=77)
     assert {("stream 77", t.data_ptr()) for t in out} <= set(streams.held) and not streams.allocated
+
+
+def test_numbers_past_32_bits_are_refused(ops):
+    """ctypes would pass their low 32 bits: another token, table or number of heads."""
+    from scriptrs_amd import RotaryTable
+    logits, scores = torch.zeros(4, 9), torch.zeros(2, 2)
+    far = 1 << 32
+    row = torch.empty(1, far + 16, dtype=torch.bfloat16)  # (never touched)
+    bad = [lambda: ops.beam_select(logits, scores, end_token=far + 3), lambda: ops.beam_select(logits, scores, end_token=-far),
+           lambda: ops.attention_plan([0, 4], [0, 4], far + 2, 2, 64, stream=0),
+           lambda: ops.attention_plan([0, 4], [0, 4], 2, far + 2, 64, stream=0),
+           lambda: ops.attention_plan([0, 4], [0, 4], 2, 2, far + 64, stream=0),
+           lambda: RotaryTable(far + 32), lambda: RotaryTable(64 - far),
+           lambda: ops.beam_select(row, scores[:1, :1]), lambda: ops.residual_norm(row, row, out=row),
+           lambda: ops.rotary(RotaryTable(16), torch.zeros(1, dtype=torch.int32), row.view(1, 1, -1), inplace=True)]
+    for i, f in enumerate(bad):
+        with pytest.raises(InvalidModelOutput):
+            f()
+            raise AssertionError(f"call {i} was not refused")
+    assert not ops.recorded
+
+
+@pytest.mark.parametrize("bound,passed", [(1 << 62, 1 << 62), ((1 << 64) + 5, 1 << 62), (-(1 << 64) + 5, -1), (7, 7), (-1, -1)])
+def test_windows_past_64_bits_set_no_bound(ops, bound, passed):
+    plan = ops.attention_plan([0, 4], [0, 4], 2, 2, 64, left=bound, right=bound, stream=0)
+    assert ops.recorded[-1][1][7:9] == (passed, passed)
+    plan._handle = None

@@ -382,7 +382,8 @@ int sfe_residual_norm(sfe_ctx* ctx, const sfe_residual* args, void* stream);
  * Totals of -inf or NaN are no candidates (a stream's first step gives all beams but
  * one the score -inf); a place without a candidate gets score -inf, token -1 and
  * parent its own place.  out_finished (may be NULL): the parent was finished or the
- * token is end_token (-1: no such token).  1 to 32 beams. */
+ * token is end_token (-1: no such token).  1 to 32 beams.  No output may overlap
+ * another tensor of the call. */
 int sfe_beam_select(sfe_ctx* ctx, int32_t dtype, const void* logits, int64_t row_stride, int32_t streams, int32_t beams,
                     int32_t vocab, const float* scores, const uint8_t* finished, int32_t end_token, float* out_scores,
                     int32_t* parents, int32_t* tokens, uint8_t* out_finished, void* stream);

@@ -84,6 +84,30 @@ bool same_view(const Rows& a, const Rows& b) {
   return a.p == b.p && a.n == b.n && a.len == b.len && (a.n <= 1 || a.row == b.row);
 }
 
+// Bytes that a call reads or writes as a whole.
+struct Span {
+  uintptr_t begin, end;
+  bool out;
+  const char* name;
+  int32_t number;  // of the tensors of the name, or -1
+  Span(const void* p, int64_t bytes, bool out_, const char* name_, int32_t number_ = -1)
+      : begin((uintptr_t)p), end((uintptr_t)p + (uintptr_t)bytes), out(out_), name(name_), number(number_) {}
+};
+// Refuses outputs that share memory with any other span.
+int check_apart(Span* spans, size_t n) {
+  std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uintptr_t any = 0, out = 0;  // ends of what begins at or before the span looked at, and of the outputs among it
+  for (size_t i = 0; i < n; ++i) {
+    const Span& s = spans[i];
+    if (s.begin < (s.out ? any : out))
+      return op_fail(SFE_INVALID_ARG, std::string(s.name) + (s.number < 0 ? "" : " " + std::to_string(s.number)) +
+                                          " overlaps another tensor of the call");
+    any = std::max(any, s.end);
+    if (s.out) out = std::max(out, s.end);
+  }
+  return SFE_OK;
+}
+
 constexpr int64_t kMaxStride = (int64_t)1 << 40;  // elements: keeps 64-bit offsets far from their end
 
 int check_heads(const char* name, const sfe_heads* t, int64_t rows, int esize, int align) {
@@ -528,11 +552,22 @@ int sfe_beam_select(sfe_ctx* ctx, int32_t dtype, const void* logits, int64_t row
     if (!logits || !scores || !out_scores || !parents || !tokens) return op_fail(SFE_INVALID_ARG, "null argument");
     if ((uintptr_t)logits % sfe::op_size(dtype)) return op_fail(SFE_INVALID_ARG, "logits are not aligned to their element size");
     if (row_stride < 0 || row_stride >= kMaxStride) return op_fail(SFE_INVALID_ARG, "row_stride must be in [0, 2^40)");
-    if (out_scores == scores || (out_finished && out_finished == finished))
-      return op_fail(SFE_INVALID_ARG, "out_scores and out_finished must not be the inputs");
     // a launch holds fewer than 2^32 threads, of up to 64 a beam and up to 2 workgroups of
     // 256 a row (more only where the rows alone do not fill the device)
     if ((int64_t)streams * beams > (1 << 22)) return op_fail(SFE_INVALID_ARG, "batch too large for one launch");
+    const int64_t rows = (int64_t)streams * beams;
+    Span spans[] = {{scores, 4 * rows, false, "scores"},
+                    {finished, finished ? rows : 0, false, "finished"},
+                    {out_scores, 4 * rows, true, "out_scores"},
+                    {parents, 4 * rows, true, "parents"},
+                    {tokens, 4 * rows, true, "tokens"},
+                    {out_finished, out_finished ? rows : 0, true, "out_finished"}};
+    if (const int rc = check_apart(spans, sizeof(spans) / sizeof(*spans))) return rc;
+    const int esize = sfe::op_size(dtype);
+    for (const Span& s : spans)
+      if (s.out && share(Rows("logits", logits, rows, row_stride * esize, (int64_t)vocab * esize),
+                         Rows(s.name, (const void*)s.begin, 1, 0, (int64_t)(s.end - s.begin))))
+        return op_fail(SFE_INVALID_ARG, std::string(s.name) + " overlaps logits");
     struct Call {
       sfe::BeamArgs a;
       int dtype;
@@ -568,14 +603,9 @@ int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int3
     call.stream = static_cast<hipStream_t>(stream);
     // What the launch reads and writes (all states at once): an output may share memory with nothing but its own
     // input, in place.
-    struct Used {
-      uintptr_t begin, end;
-      bool out;
-      int32_t state;
-    };
-    std::vector<Used> used;
+    std::vector<Span> used;
     used.reserve(2 * (size_t)n + 1);
-    used.push_back(Used{(uintptr_t)parents, (uintptr_t)(parents + (int64_t)streams * beams), false, -1});
+    used.emplace_back(parents, (int64_t)streams * beams * 4, false, "parents");
     for (int32_t i = 0; i < n; ++i) {
       const sfe_beam_state& s = states[i];
       const std::string name = "state " + std::to_string(i);
@@ -586,8 +616,8 @@ int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int3
       const int64_t bytes = s.outer * streams * beams * s.inner_bytes;
       if (bytes == 0) continue;
       if (!s.in || !s.out) return op_fail(SFE_INVALID_ARG, name + " is null");
-      used.push_back(Used{(uintptr_t)s.out, (uintptr_t)s.out + (uintptr_t)bytes, true, i});
-      if (s.in != s.out) used.push_back(Used{(uintptr_t)s.in, (uintptr_t)s.in + (uintptr_t)bytes, false, i});
+      used.emplace_back(s.out, bytes, true, "state", i);
+      if (s.in != s.out) used.emplace_back(s.in, bytes, false, "state", i);
       if (call.launches.empty() || call.launches.back().n == sfe::kReorderStates) {
         call.launches.emplace_back();
         memset(&call.launches.back(), 0, sizeof(sfe::ReorderArgs));
@@ -599,15 +629,7 @@ int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int3
       l.s[l.n++] = sfe::BeamState{static_cast<const char*>(s.in), static_cast<char*>(s.out), s.outer, s.inner_bytes};
     }
     if (call.launches.empty()) return SFE_OK;
-    std::sort(used.begin(), used.end(), [](const Used& a, const Used& b) { return a.begin < b.begin; });
-    uintptr_t any = 0, out = 0;  // ends of what begins at or before the range looked at, and of the outputs among it
-    for (const Used& u : used) {
-      if (u.begin < (u.out ? any : out))
-        return op_fail(SFE_INVALID_ARG, u.state < 0 ? std::string("parents: an output overlaps them")
-                                                    : "state " + std::to_string(u.state) + " overlaps another tensor of the call");
-      any = std::max(any, u.end);
-      if (u.out) out = std::max(out, u.end);
-    }
+    if (const int rc = check_apart(used.data(), used.size())) return rc;
     return sfe::op_call(ctx, call.stream, "beam reorder", [](void* arg, int) -> hipError_t {
       Call& c = *static_cast<Call*>(arg);
       for (const sfe::ReorderArgs& l : c.launches) {

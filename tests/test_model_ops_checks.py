@@ -209,3 +209,32 @@ def test_views_of_other_strides(contexts, table):
     passes(L, turn_in_place(L, table, q, _lib.SfeHeads(AT + 2 * DIM, 2 * narrow, narrow)))
     refused(L, turn_in_place(L, table, q, _lib.SfeHeads(AT + 2 * (DIM - 8), 2 * narrow, narrow)), "overlaps")
     refused(L, turn_in_place(L, table, q, _lib.SfeHeads(AT + 2 * (wide - 8), 2 * narrow, narrow)), "overlaps")
+
+
+def test_a_beam_steps_outputs_share_memory_with_nothing(checks):
+    """Streams are chosen side by side: an output over part of an input or of another output raced."""
+    L, streams, beams, vocab = checks, 2, 3, 10
+    place = {"logits": AT, "scores": AT + 1000, "finished": AT + 2000, "out_scores": AT + 3000, "parents": AT + 4000,
+             "tokens": AT + 5000, "out_finished": AT + 6000}
+
+    def select(**moved):
+        p = {**place, **moved}
+        return L.sfe_beam_select(CTX, 0, p["logits"], 12, streams, beams, vocab, p["scores"], p["finished"], 3,
+                                 p["out_scores"], p["parents"], p["tokens"], p["out_finished"], None)
+    passes(L, select())
+    passes(L, select(out_finished=None))
+    passes(L, select(out_scores=AT + 1024, parents=AT + 1048, tokens=AT + 1072, out_finished=AT + 2006))
+    passes(L, select(scores=AT + 5 * 48 + 40))  # (right behind the last row's 10 logits)
+    passes(L, select(out_finished=AT + 2 * 48 + 42))  # (between rows)
+    refused(L, select(out_finished=AT + 2 * 48 + 43), "overlaps")
+    for out, size in (("out_scores", 24), ("parents", 24), ("tokens", 24), ("out_finished", 6)):
+        for other, length in (("logits", 5 * 48 + 40), ("scores", 24), ("finished", 6), ("out_scores", 24), ("parents", 24),
+                              ("tokens", 24), ("out_finished", 6)):
+            if out == other:
+                continue
+            step = 1 if out == "out_finished" else 4
+            last = (length - 1) // step * step  # the last place that begins within the other
+            for at in (0, last, step - size if step < size else 0):
+                refused(L, select(**{out: place[other] + at}), "overlap")
+            passes(L, select(**{out: place[other] - size}))
+            passes(L, select(**{out: (place[other] + length + step - 1) // step * step}))

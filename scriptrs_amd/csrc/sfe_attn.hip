@@ -6,9 +6,10 @@
 // there is none.  One pass over the keys with a running reference exponent and
 // sum: with x_j = scale log2(e) q_i . k_j and any reference m, the weights are
 // 2^(x_j - m) / sum 2^(x_j - m).  m follows the running maximum only when that
-// rises 15 above it, to 7 below the new maximum, so most steps rescale nothing;
-// weights stay below 2^15 (f16 holds 65504) and weights down to 2^-17 of the
-// largest keep all their bits in f16 (bf16 has the range anyway).  Scores, m,
+// has risen by 8 since it last did, so most steps rescale nothing.  In f16 weights
+// go from 2^7 of a new maximum up to 2^15 (it holds 65504), so that those down to 2^-17 of the
+// largest keep all their bits; in bf16, which has the range anyway, from 2^-8 up to 1, so
+// that no value that a mean of values can have is passed on the way to it.  Scores, m,
 // sums and outputs are f32; a weight is rounded to the inputs' type for the
 // product with v, whose inputs are of that type too (an error of 2^-9 of
 // each term in bf16, as in v itself).
@@ -55,6 +56,8 @@ struct Mat<Bf> {
   static __device__ F16 m32(V8 a, V8 b, F16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ F4 m16(V8 a, V8 b, F4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static constexpr uint32_t kExp = 0x7f807f80, kCarry = 0x00800080, kOne = 0x3f80;
+  // the reference moves when a score passes it by kRise, to kBelow below the maximum
+  static constexpr float kRise = 0.0f, kBelow = -8.0f;
 };
 template <>
 struct Mat<Hf> {
@@ -63,11 +66,10 @@ struct Mat<Hf> {
   static __device__ F16 m32(V8 a, V8 b, F16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ F4 m16(V8 a, V8 b, F4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static constexpr uint32_t kExp = 0x7c007c00, kCarry = 0x04000400, kOne = 0x3c00;
+  static constexpr float kRise = 15.0f, kBelow = 7.0f;
 };
 
-constexpr float kNever = -3e38f;  // reference exponent before the first visible key: below every score
-constexpr float kRise = 15.0f;    // the reference moves when a score passes it by this much
-constexpr float kBelow = 7.0f;    // ... to this much below the maximum
+constexpr float kNever = -3e38f;  // reference exponent before the first visible key: below every score that counts
 // Scores past this are scaled and rounded before the reference is taken off: the f32 reference of such
 // a row is a rounded score itself, and exact products less it would be off by its rounding.
 constexpr float kLarge = 1048576.0f;
@@ -515,8 +517,8 @@ __global__ __launch_bounds__(256, NT == 2 ? 3 : 2) void sfe_attn_rows_kernel(Att
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
-        if (__any(top * a.scale_log2 > m + kRise)) {
-          const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, kBelow));
+        if (__any(top * a.scale_log2 > m + Mat<T>::kRise)) {
+          const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, Mat<T>::kBelow));
           const float f = exp2_fast(m - nm);
           m = nm;
           l *= f;
@@ -841,8 +843,8 @@ __global__ __launch_bounds__(512, 2) void sfe_attn_tall_kernel(AttnArgs a) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
-      if (__any(top * a.scale_log2 > m + kRise)) {
-        const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, kBelow));
+      if (__any(top * a.scale_log2 > m + Mat<T>::kRise)) {
+        const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, Mat<T>::kBelow));
         const float f = exp2_fast(m - nm);
         m = nm;
         l *= f;
@@ -1053,9 +1055,9 @@ __global__ __launch_bounds__(64 * kAttnWavesFew, 1) void sfe_attn_few_kernel(Att
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
-    if (__any(top * a.scale_log2 > m + kRise)) {
+    if (__any(top * a.scale_log2 > m + Mat<T>::kRise)) {
       top = fmaxf(top, __shfl_xor(top, 16));
-      const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, kBelow));
+      const float nm = fmaxf(m, scaled_less(max_halves(top), a.scale_log2, Mat<T>::kBelow));
       const float f = exp2_fast(m - nm);
       m = nm;
       l *= f;

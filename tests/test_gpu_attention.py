@@ -431,3 +431,19 @@ def test_one_value_for_all_keys(ops, lq, lk, heads, bad):
         line = torch.randn(8 * (sum(lk) - 1) + dim, device="cuda", generator=g).bfloat16()
         line[-8:] = bad
         check(ops, lq, lk, heads, 1, dim, q=q, k=k[:, :1], v=line.as_strided((sum(lk), 1, dim), (8, dim, 1)))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lq,lk,heads", [([1], [10], 2), ([3, 1], [33, 900], 2), ([1], [5000], 2), ([126], [126], 2),
+                                         ([40] * 40, [40] * 40, 8), ([700, 5], [700, 5], 8), ([2100], [2100], 8)], ids=str)
+def test_large_values(ops, lq, lk, heads, dim):
+    """Values of 1e36: a mean of them is no larger than they are, and so are the sums on the way to it (below 1e36 times
+    a few hundred keys of weight up to 1)."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(17)
+    q, k, v = (torch.randn(n, heads, dim, device="cuda", generator=g).bfloat16() for n in (sum(lq), sum(lk), sum(lk)))
+    small = check(ops, lq, lk, heads, heads, dim, q=q, k=k, v=v)
+    big = 2.0 ** 120  # 1.3e36; a power of 2: the same bits but for the exponent
+    plan = ops.attention_plan(offsets(lq), offsets(lk), heads, heads, dim)
+    out = ops.attention(plan, q, k, (v.float() * big).bfloat16())
+    assert torch.isfinite(out).all() and torch.equal(out.float() / big, small.float())

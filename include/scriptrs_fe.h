@@ -321,7 +321,8 @@ int sfe_attention_rows(sfe_attn_plan* plan, int32_t dtype, const sfe_heads* q, c
  *   LINEAR  f / factor
  *   BASE    base * factor^(rotary_dim / (rotary_dim - 2)) as the base
  *   PARTS   f ((1 - keep) / factor + keep), keep = (original_length f / 2 pi -
- *           low) / (high - low) limited to [0, 1].
+ *           low) / (high - low) limited to [0, 1] (the ramp is linear in the turns
+ *           that a pair makes in original_length positions, not in its number).
  * The table is plain host memory of the caller. */
 typedef enum sfe_rotary_layout { SFE_ROTARY_HALF = 0, SFE_ROTARY_INTERLEAVED = 1 } sfe_rotary_layout;
 typedef enum sfe_rotary_scaling {

@@ -56,12 +56,25 @@ int64_t piece_keys(const std::vector<Tile>& tiles, int kv_heads, int64_t slots, 
 }
 
 // Time of a sequence's tiles in a form, in microseconds of a CU: steps and a fixed part a tile,
-// fitted to 40,000 rows of 8 heads of 128 (steps of 2.03 us for 256 rows, 1.31 for 128).  It
-// chooses as measured: full attention of 188, 260, 384, 512, 1024, 4096 keys takes 118 (rows) / 131
-// (tall), 136 / 180, 126 / 139, 153 / 127, 244 / 190, 756 / 585 us; causal 384, 512, 768, 4096: 100 / 117,
-// 131 / 118, 146 / 125, 396 / 353; windows of 64, 256, 512, 1024 to either side: 93 / 107, 150 / 156,
-// 235 / 222, 406 / 364.  Heads of 64 channels and less leave room for 3 workgroups of the rows
+// fitted to 40,000 rows of 8 heads of 128 (steps of 2.03 us for 256 rows, 1.31 for 128).  Measured
+// on both sides (rows / tall, us; such a call fills the chip):
+//   full attention of 188, 260, 384, 512, 1024, 4096 keys
+//     heads of 128   96 / 107, 130 / 177, 122 / 140, 147 / 131, 238 / 197, 757 / 600
+//     heads of 96    72 / 87, 100 / 140, 85 / 109, 102 / 104, 175 / 158, 628 / 502
+//     heads of 80    75 / 85, 99 / 137, 84 / 106, 104 / 100, 174 / 153, 626 / 488
+//   causal 384, 512, 768, 4096
+//     heads of 128   101 / 120, 132 / 122, 146 / 128, 397 / 356
+//     heads of 96    74 / 96, 97 / 100, 113 / 102, 334 / 302
+//     heads of 80    73 / 93, 97 / 98, 112 / 99, 326 / 293
+//   windows of 64, 256, 512, 1024 to either side
+//     heads of 128   94 / 110, 150 / 158, 236 / 224, 406 / 377
+//     heads of 96    77 / 95, 129 / 133, 200 / 191, 345 / 311
+//     heads of 80    77 / 93, 126 / 131, 197 / 187, 337 / 301
+// It chooses the shorter one in all of them but causal 512 in heads of 80 and 96 and full 512 in
+// heads of 96 (1-3% longer).  Heads of 64 channels and less leave room for 3 workgroups of the rows
 // form on a CU, which is then faster everywhere (4096 keys 695 / 727 us, 512 119 / 145).
+// A call that leaves CUs empty is not what was fitted: one sequence of 700 rows in 8 heads of 128
+// takes 25 (rows) / 29 (tall, as chosen), of 2000 51 / 50, of 4000 107 / 102.
 double tile_costs(int form, int64_t lq, int64_t lk, int group, int32_t left, int32_t right) {
   const bool causal = left == kAttnNoBound && right == 0;
   const double step = form == kAttnTall ? 2.03 : 1.31, fixed = form == kAttnTall ? (causal ? 10.0 : 13.0) : 5.2;
@@ -78,8 +91,10 @@ double tile_costs(int form, int64_t lq, int64_t lk, int group, int32_t left, int
 
 // Whether the few form takes the whole call: only sequences of up to 16 packed rows, or so few
 // tiles of 16 that they get a CU each and not many keys, so that the whole call is one trip
-// through memory (one sequence of 126, 8 heads of 128: 7.3 us against 9.9 in the rows form; 500: 11.3 / 24.4; 1125,
-// 568 tiles: 43.7 / 38.9).
+// through memory.  One sequence of 250, 500, 700, 1125, 2000, 4000 rows in 8 heads, in this form / the
+// faster of the others: heads of 128 9.1 / 13.3 us, 11.9 / 21.4, 23.9 / 25.3, 42.6 / 37.6, 83.5 / 50.2, 283 / 102; of 64
+// 7.2 / 11.0, 8.7 / 17.8, 11.2 / 20.4, 20.7 / 30.0, 32.8 / 41.7, 104 / 82.  (The bound of 5 tiles to 4 CUs, up to 640
+// rows here, fits heads of 128; heads of 64 would go on to about 2000.)
 bool whole_call_few(const int64_t* q_offsets, const int64_t* k_offsets, int n, int group, int kv_heads, int cus) {
   int64_t units = 0, rows = 0, keys = 0;
   for (int s = 0; s < n; ++s) {

@@ -227,7 +227,8 @@ __device__ __forceinline__ void best_add(Best& b, int keep, float* lx, int* li, 
     }
   }
   // (a bound that stays behind costs more than cutting the list: 512 rows of 128,000, 8 beams, 39.4 us
-  // with a cut at every entry, 37.8 at 4 and at 8 past the beams, 43.9 when full)
+  // with a cut at every entry, 37.8 at 4 and at 8 past the beams, 43.9 when full, all of them before the maximum
+  // was taken off each logit)
   if (b.n >= keep + kSlack) {
     best_cut(b, keep, lx, li);
     if (told.all) tell(told, lx[told.share - 1]);
@@ -371,7 +372,7 @@ __device__ __forceinline__ void write_beams(const BeamArgs& a, int stream, Best&
 
 // ---- small vocabularies -----------------------------------------------------------------
 
-// E: logits of a lane.  16 streams of 4 beams over 1,025 tokens in f32: 6 us, bound by latency (a
+// E: logits of a lane.  16 streams of 4 beams over 1,025 tokens in f32: 7.6 us, bound by latency (a
 // row's loads, its sum, the choice, the join).
 template <typename T, int E>
 __global__ __launch_bounds__(1024) void sfe_beam_small_kernel(BeamArgs a) {
@@ -405,9 +406,9 @@ __global__ __launch_bounds__(1024) void sfe_beam_small_kernel(BeamArgs a) {
 // ---- others: spans of rows, then streams -----------------------------------------------------
 
 // One workgroup: the steps of a span, the next step's loads in flight while one is
-// worked on.  512 rows of 128,000 in bf16, 8 beams: 38 us, of which the pass over the logits
-// alone takes 25 (5.2 TB/s) and the best 8 of the first step and of the waves 4 each.  Each thread keeps the sum of exponentials relative to its own running
-// maximum.  (4 workgroups a CU: with 3, which 155 registers allow, 1,024 of them
+// worked on.  512 rows of 128,000 in bf16, 8 beams: 40 us, of which the pass over the logits
+// alone takes 25 (5.2 TB/s), the best 8 of the first step and of the waves 4 each, and the maximum taken off
+// each logit 2.  Each thread keeps the sum of exponentials relative to its own running maximum.  (4 workgroups a CU: with 3, which 155 registers allow, 1,024 of them
 // went in two turns, 90 us against 55.)
 template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void sfe_beam_rows_kernel(BeamArgs a, int spans) {
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(kThreads, 4) void sfe_beam_rows_kernel(BeamArgs a, 
   }
 }
 
-// A workgroup per stream, over the candidates its rows' spans left: 8 us for 64 streams of 8 beams, bound by
+// A workgroup per stream, over the candidates its rows' spans left: 9 us for 64 streams of 8 beams, bound by
 // latency (one row's sums, one round of candidates, the join).
 __global__ __launch_bounds__(kThreads) void sfe_beam_streams_kernel(BeamArgs a, int spans) {
   __shared__ Lists lists;

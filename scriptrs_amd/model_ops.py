@@ -78,7 +78,8 @@ class RotaryTable:
     2p with 2p + 1.  ``scaling`` for long contexts: None, "linear" (positions /
     factor), "base" (base * factor^(R / (R - 2))) or "parts" (pairs that turn at least
     ``high`` times in ``original_length`` positions are kept, those below
-    ``low`` divided by ``factor``, the ones between in proportion)."""
+    ``low`` divided by ``factor``, the ones between in proportion to their turns, not to
+    their number p: tables that ramp over p are others)."""
 
     LAYOUTS = {"half": 0, "interleaved": 1}
     SCALINGS = {None: 0, "none": 0, "linear": 1, "base": 2, "parts": 3}
@@ -127,7 +128,8 @@ class ModelOps:
 
     One instance per host thread, like the feature extractor (it owns an
     ``sfe_ctx`` or shares ``extractor``'s; calls on it are ordered after each other).
-    ``stream``: a call's stream (torch's, or its handle), the current one without; its inputs have to be ready there."""
+    ``stream``: a call's stream (torch's, or its handle), the current one without; its inputs have to be ready there, and
+    a stream given by its handle has to outlive the tensors of its calls (their memory is held for it)."""
 
     def __init__(self, device: int = 0, extractor: ParakeetFeatureExtractor | None = None):
         import torch

@@ -402,6 +402,118 @@ typedef struct sfe_beam_state {
 int sfe_beam_reorder(sfe_ctx* ctx, const int32_t* parents, int32_t streams, int32_t beams, const sfe_beam_state* states,
                      int32_t n, void* stream);
 
+/* ---- a decoder's step over a paged cache ----------------------------------------
+ *
+ * Operators of a decoder whose keys and values are kept in pages: norms of heads with
+ * rotary positions in the same pass, the cache's write and read, attention of new tokens
+ * over it, and the steering of logits before sfe_beam_select.  Called as the model operators above are. */
+
+/* Norms of each head and rotary positions: y = N(x) weight, of which the table's first rotary_dim channels
+ * turn as sfe_rotary's do; one rounding.  norm: SFE_NORM_RMS or SFE_NORM_LAYER
+ * (without a bias) over the head's channels; q_weight, k_weight: f32 [head_dim] or NULL (ones).
+ * head_dim is at most 256; the rest as for sfe_rotary. */
+int sfe_norm_rotary(sfe_ctx* ctx, const sfe_rotary_table* table, int32_t norm, float eps, int32_t dtype,
+                    const int32_t* positions, int64_t rows, int32_t head_dim, int32_t q_heads, const float* q_weight,
+                    const sfe_heads* q, const sfe_heads* q_out, int32_t k_heads, const float* k_weight,
+                    const sfe_heads* k, const sfe_heads* k_out, void* stream);
+
+/* A cache of keys and values: `data` is [pages][kv_heads][sfe_cache_record bytes], 16-byte aligned device
+ * memory of the caller.  A record holds page_size tokens of one kv head: K [page_size][head_dim],
+ * V [page_size][head_dim], and for the types of 8 bits f32 scales, K [page_size] and V [page_size].
+ * SFE_CACHE_E4M3 and SFE_CACHE_INT8 keep a token's channels of one kv head as codes and one scale:
+ * with a their largest magnitude (at least 2^-96) and M 448 or 127, code = x M / a rounded to the
+ * type (halves to even), scale = a / M, and a code stands for code * scale.  Channels that are not all finite
+ * read as NaN, all of them.  page_size is a power of two from 16 to 1024, head_dim a multiple of 16, at
+ * most 128. */
+typedef enum sfe_cache_type {
+  SFE_CACHE_BF16 = 1,
+  SFE_CACHE_F16 = 2,
+  SFE_CACHE_E4M3 = 3,
+  SFE_CACHE_INT8 = 4
+} sfe_cache_type;
+typedef struct sfe_cache {
+  void* data;
+  int64_t pages;
+  int32_t page_size, kv_heads, head_dim, type;
+} sfe_cache;
+/* Bytes of a record, 0 for sizes or types that are refused (sfe_last_error has the reason). */
+int64_t sfe_cache_record(int32_t page_size, int32_t head_dim, int32_t type);
+
+/* Where a batch's tokens are (device memory, read by the kernels when they run, so that a captured call
+ * follows a growing cache): token p of sequence s is in the page
+ * page_table[s * table_stride + p / page_size].  lengths[s] counts a sequence's tokens, the call's
+ * new ones included.  A token before the first (where lengths[s] is below the number of new ones), past
+ * table_pages pages, or of a page number outside [0, pages) is in no place: it is
+ * not written, reads as zeros and is seen by no query. */
+typedef struct sfe_cache_tokens {
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t table_pages;
+  const int32_t* lengths;
+} sfe_cache_tokens;
+
+/* The new tokens of n sequences, packed: those of sequence s are the rows [offsets[s], offsets[s + 1])
+ * (host array of n + 1 from 0 on; none is fine), its last tokens.  heads: of the queries (a multiple of kv_heads).
+ * Made, shared, captured and freed as an sfe_attn_plan is. */
+typedef struct sfe_cache_plan sfe_cache_plan;
+int sfe_cache_plan_make(sfe_ctx* ctx, const int64_t* offsets, int32_t n, int32_t heads, int32_t kv_heads,
+                        int32_t head_dim, void* stream, sfe_cache_plan** out);
+void sfe_cache_plan_free(sfe_cache_plan* plan);
+
+/* Writes k, v [offsets[n]][kv_heads][head_dim] of dtype (SFE_F32, SFE_BF16 or SFE_F16; 16-byte aligned data and
+ * strides) into the new tokens' places; nothing else of the cache changes.  Two new tokens must not have
+ * one place (sequences that share a page they write): it then holds parts of either. */
+int sfe_cache_write(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache_tokens* tokens, int32_t dtype,
+                    const sfe_heads* k, const sfe_heads* v, void* stream);
+
+/* Reads the plan's tokens back into k, v, rounded once to dtype.  Of a plan whose new tokens are
+ * all of each sequence's, the whole sequences, as sfe_attention takes them. */
+int sfe_cache_read(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache_tokens* tokens, int32_t dtype,
+                   const sfe_heads* k, const sfe_heads* v, void* stream);
+
+/* Attention of the new tokens' queries q [offsets[n]][heads][head_dim] over the cache, which holds their
+ * keys and values already:
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens before the new ones and the new
+ * tokens that i sees, zero where there is none.  tree NULL: itself and those before it.  tree [offsets[n]]: bit j
+ * of row i is set where i sees new token j of its sequence (of at most 64; bits past its last are ignored).
+ * What is not seen contributes nothing, whatever its values.  dtype: SFE_BF16 or SFE_F16, a cache of 16
+ * bits has the same.  q and out are 16-byte aligned (data and strides); out must not overlap q, the cache or the tree.
+ * rows: rows of out, at least offsets[n]; those past the last sequence are zeroed. */
+int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache_tokens* tokens, int32_t dtype,
+                        const sfe_heads* q, const uint64_t* tree, float scale, const sfe_heads* out, int64_t rows,
+                        void* stream);
+
+/* Steers logits [rows][vocab] before a choice.  With c the times that token t stands in its row's history:
+ *   z = logit; where c > 0, z = z > 0 ? z / repetition : z * repetition, then z -= presence + frequency * c;
+ *   z += bias[t]; a token without its bit in the row's mask: z = -inf
+ * in f32, rounded once.  out may be logits (in place). */
+typedef struct sfe_logits {
+  int32_t dtype; /* SFE_F32, SFE_BF16 or SFE_F16 */
+  int32_t rows, vocab; /* vocab at most 2^24 */
+  int32_t history_most;
+  const void* logits;
+  void* out;
+  int64_t logits_row, out_row; /* strides in elements */
+  /* Tokens said before, history_most of each row (or the first lengths[r] of them); those outside
+   * [0, vocab) count for nothing.  NULL: none. */
+  const int32_t* history;
+  int64_t history_row;
+  const int32_t* lengths;
+  /* Of all rows, or of each (f32 [rows]) where the pointer is not NULL.  repetition is positive. */
+  float repetition, presence, frequency;
+  const float *repetitions, *presences, *frequencies;
+  const float* bias; /* f32, rows bias_row apart (0: one for all rows); NULL: none */
+  int64_t bias_row;
+  /* Masks of a grammar's states: token t's bit is bit t % 32 of word t / 32, rows allowed_row words apart,
+   * n_allowed of them; row r takes mask states[r] (states NULL: mask r), and none where that is outside
+   * [0, n_allowed).  NULL: none. */
+  const uint32_t* allowed;
+  int64_t allowed_row;
+  int32_t n_allowed;
+  const int32_t* states;
+} sfe_logits;
+int sfe_adjust_logits(sfe_ctx* ctx, const sfe_logits* args, void* stream);
+
 /* ---- tuning and instrumentation (no reference counterpart) ----------- */
 
 /* Shared frames: on by default.  Overlapping chunk tasks of one call

@@ -27,6 +27,8 @@ EXPORTS = (
     "sfe_debug_allocation_count", "sfe_debug_mel_schedule", "sfe_debug_stamps",
     "sfe_attention_plan", "sfe_attention_plan_free", "sfe_attention", "sfe_attention_rows", "sfe_rotary_init", "sfe_rotary",
     "sfe_residual_norm", "sfe_beam_select", "sfe_beam_reorder",
+    "sfe_norm_rotary", "sfe_cache_record", "sfe_cache_plan_make", "sfe_cache_plan_free", "sfe_cache_write",
+    "sfe_cache_read", "sfe_cache_attention", "sfe_adjust_logits",
 )
 
 
@@ -72,6 +74,28 @@ class SfeResidual(ctypes.Structure):
 class SfeBeamState(ctypes.Structure):
     _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("outer", ctypes.c_int64),
                 ("inner_bytes", ctypes.c_int64)]
+
+
+class SfeCache(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("type", ctypes.c_int32)]
+
+
+class SfeCacheTokens(ctypes.Structure):
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_pages", ctypes.c_int32),
+                ("lengths", ctypes.c_void_p)]
+
+
+class SfeLogits(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("vocab", ctypes.c_int32),
+                ("history_most", ctypes.c_int32), ("logits", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("logits_row", ctypes.c_int64), ("out_row", ctypes.c_int64),
+                ("history", ctypes.c_void_p), ("history_row", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+                ("repetition", ctypes.c_float), ("presence", ctypes.c_float), ("frequency", ctypes.c_float),
+                ("repetitions", ctypes.c_void_p), ("presences", ctypes.c_void_p), ("frequencies", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("bias_row", ctypes.c_int64),
+                ("allowed", ctypes.c_void_p), ("allowed_row", ctypes.c_int64), ("n_allowed", ctypes.c_int32),
+                ("states", ctypes.c_void_p)]
 
 
 _lib = None
@@ -137,6 +161,16 @@ def lib() -> ctypes.CDLL:
         "sfe_residual_norm": (ctypes.c_int, [vp, P(SfeResidual), vp]),
         "sfe_beam_select": (ctypes.c_int, [vp, i32, vp, i64, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp]),
         "sfe_beam_reorder": (ctypes.c_int, [vp, vp, i32, i32, P(SfeBeamState), i32, vp]),
+        "sfe_norm_rotary": (ctypes.c_int, [vp, P(SfeRotaryTable), i32, ctypes.c_float, i32, vp, i64, i32, i32, vp,
+                                           P(SfeHeads), P(SfeHeads), i32, vp, P(SfeHeads), P(SfeHeads), vp]),
+        "sfe_cache_record": (i64, [i32, i32, i32]),
+        "sfe_cache_plan_make": (ctypes.c_int, [vp, i64p, i32, i32, i32, i32, vp, P(vp)]),
+        "sfe_cache_plan_free": (None, [vp]),
+        "sfe_cache_write": (ctypes.c_int, [vp, P(SfeCache), P(SfeCacheTokens), i32, P(SfeHeads), P(SfeHeads), vp]),
+        "sfe_cache_read": (ctypes.c_int, [vp, P(SfeCache), P(SfeCacheTokens), i32, P(SfeHeads), P(SfeHeads), vp]),
+        "sfe_cache_attention": (ctypes.c_int, [vp, P(SfeCache), P(SfeCacheTokens), i32, P(SfeHeads), vp, ctypes.c_float,
+                                               P(SfeHeads), i64, vp]),
+        "sfe_adjust_logits": (ctypes.c_int, [vp, P(SfeLogits), vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)

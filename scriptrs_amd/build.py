@@ -45,6 +45,11 @@ SOURCES = [
     ("sfe_beam.hip", ["-x", "hip"]),
     ("sfe_attn_plan.cpp", ["-x", "hip"]),
     ("sfe_ops.cpp", ["-x", "hip"]),
+    ("sfe_norm_rotary.hip", ["-x", "hip"]),
+    ("sfe_cache.hip", ["-x", "hip"]),
+    ("sfe_cache_attn.hip", ["-x", "hip"]),
+    ("sfe_logits.hip", ["-x", "hip"]),
+    ("sfe_decode.cpp", ["-x", "hip"]),
     # bit-exact table construction: every f32/f64 op rounded separately
     ("sfe_tables.cpp", ["-x", "hip", "-ffp-contract=off"]),
     ("sfe_share.cpp", ["-x", "hip"]),

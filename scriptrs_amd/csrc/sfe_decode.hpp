@@ -1,0 +1,87 @@
+// Operators of a decoder's step over a paged cache (head norms with rotary
+// positions, the cache's write and read, attention of new tokens over it, and the steering of
+// logits): what their entry points (sfe_decode.cpp) share with their kernels.
+#pragma once
+
+#include "sfe_ops.hpp"
+
+namespace sfe {
+
+// ---- norms of heads and rotary positions in one pass (sfe_norm_rotary.hip) -----------
+constexpr int kNormRotaryMaxDim = 256;
+struct NormRotaryArgs {
+  uint64_t step[kRotaryMaxPairs];  // turns a position, as a fraction of 2^64
+  RotaryTensor t[2];
+  const float* weight[2];  // [dim], or null
+  const int32_t* positions;
+  int64_t rows;
+  int32_t dim, rotary;
+  float magnitude, eps;
+};
+hipError_t launch_norm_rotary(const NormRotaryArgs& a, int type, bool interleaved, bool layer, int cus, hipStream_t stream);
+
+// ---- the paged cache (sfe_cache.hip) ----------------------------------------------------
+// Element types of a cache: sfe_dtype's 16-bit ones, then codes of 8 bits with an f32
+// scale for each token and kv head.
+enum CacheType { kCacheBf16 = 1, kCacheF16 = 2, kCacheE4m3 = 3, kCacheInt8 = 4 };
+constexpr bool cache_coded(int type) { return type == kCacheE4m3 || type == kCacheInt8; }
+constexpr int kCacheMaxDim = 128;
+// A record, one kv head's part of a page: K [page][dim], V [page][dim], then for codes their
+// scales, f32 K [page] and V [page].
+inline int64_t cache_record(int page, int dim, int type) {
+  return (int64_t)2 * page * dim * (cache_coded(type) ? 1 : 2) + (cache_coded(type) ? 8 * page : 0);
+}
+
+// Tokens of one sequence: its new tokens are the last n of `lengths[seq]`.
+struct CacheTile {
+  int64_t first;  // packed row of the sequence's first new token
+  int32_t seq, n;
+  int32_t at, count;  // write, read: tokens [at, at + count); attention: packed rows (token x head of a group) from `at` on
+};
+static_assert(sizeof(CacheTile) == 24, "layout shared with the kernels");
+constexpr int kCacheTileTokens = 16;
+
+struct CacheArgs {
+  char* data;  // [pages][kv_heads][record]
+  int64_t pages, record;
+  const int32_t* table;  // [sequences][table_pages], rows table_row apart
+  const int32_t* lengths;
+  const CacheTile* tiles;
+  int64_t table_row;
+  int32_t n_tiles, table_pages, shift, kv_heads, dim;  // shift: log2 of the page's size
+};
+hipError_t launch_cache_write(const CacheArgs& c, int type, const AttnTensor& k, const AttnTensor& v, int dtype, hipStream_t stream);
+hipError_t launch_cache_read(const CacheArgs& c, int type, const AttnTensor& k, const AttnTensor& v, int dtype, hipStream_t stream);
+
+// ---- attention of new tokens over the cache (sfe_cache_attn.hip) ---------------------------
+struct CacheAttnArgs {
+  CacheArgs c;
+  AttnTensor q, o;
+  const uint64_t* tree;  // bit j of a row: it sees new token j of its sequence; null: its own and those before
+  int32_t group;
+  float scale_log2;  // scale * log2(e)
+};
+hipError_t launch_cache_attn(const CacheAttnArgs& a, int type, int dtype, hipStream_t stream);
+
+// ---- steering of logits (sfe_logits.hip) -----------------------------------------------------
+struct LogitsArgs {
+  const char* in;
+  char* out;
+  int64_t in_row, out_row;  // strides in elements
+  int32_t rows, vocab;
+  const int32_t* history;  // or null
+  const int32_t* lengths;  // or null: all of a row
+  int64_t history_row;
+  int32_t history_most;
+  float repetition, presence, frequency;
+  const float *repetitions, *presences, *frequencies;  // of each row, or null
+  const float* bias;  // or null
+  int64_t bias_row;
+  const uint32_t* allowed;  // or null
+  int64_t allowed_row;
+  int32_t n_allowed;
+  const int32_t* states;  // or null: row r takes mask r
+};
+hipError_t launch_logits(const LogitsArgs& a, int type, hipStream_t stream);
+
+}  // namespace sfe

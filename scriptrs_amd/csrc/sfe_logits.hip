@@ -1,0 +1,150 @@
+// Steering of logits before a choice: penalties for tokens said before, a bias, and a grammar's masks.
+//
+// With c the times that token t stands in its row's history:
+//   z = logit; c > 0: z = z / repetition (z > 0) or z * repetition, then z -= presence + frequency c;
+//   z += bias[t]; a token that the row's mask lacks: z = -inf.
+// In f32, rounded once.
+//
+// One pass over the logits: a workgroup takes a span of one row's tokens, has all of its
+// logits in flight, counts the history's tokens of its span in LDS meanwhile (whole numbers:
+// their order does not matter), and writes.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sfe_decode.hpp"
+#include "sfe_internal.hpp"
+#include "sfe_turn.hpp"
+
+namespace sfe {
+namespace {
+
+constexpr int kThreads = 256;
+
+// The mask bits of n <= 32 tokens from t on.
+__device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int t, int n, int vocab) {
+  const int w = t >> 5, shift = t & 31;
+  uint32_t bits = words[w] >> shift;
+  if (shift && shift + n > 32 && 32 * (w + 1) < vocab) bits |= words[w + 1] << (32 - shift);
+  return bits;
+}
+
+// N: elements of a vector (16 bytes, or one); V: vectors of a thread.  Vectors begin at multiples of 16 bytes:
+// the first of a row may begin up to N - 1 elements before it.
+template <typename T, int N, int V, bool HISTORY, bool BIAS, bool MASK>
+__global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int64_t first, int spans) {
+  typedef Vec<T, N> Vector;
+  constexpr int kSpan = kThreads * N * V;
+  __shared__ uint32_t counts[HISTORY ? kSpan : 1];
+  const int64_t block = first + blockIdx.x, r = block / spans;
+  const int t = (int)threadIdx.x;
+  const T* in = reinterpret_cast<const T*>(a.in) + r * a.in_row;
+  T* out = reinterpret_cast<T*>(a.out) + r * a.out_row;
+  const int before = N > 1 ? (int)((uintptr_t)in / sizeof(T) % N) : 0;
+  const int span0 = (int)(block - r * spans) * kSpan - before;  // first token of the span
+
+  Vector x[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int at = span0 + (v * kThreads + t) * N;
+    if (N > 1 && at >= 0 && at + N <= a.vocab) {
+      x[v] = *reinterpret_cast<const Vector*>(in + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[v].v[i] = at + i >= 0 && at + i < a.vocab ? in[at + i] : (T)0.0f;
+    }
+  }
+  float rep = 1.0f, presence = 0.0f, frequency = 0.0f;
+  if (HISTORY) {
+    for (int e = t; e < kSpan; e += kThreads) counts[e] = 0;
+    __syncthreads();
+    const int32_t* said = a.history + r * a.history_row;
+    int n = a.history_most;
+    if (a.lengths) n = min(n, a.lengths[r]);
+    for (int e = t; e < n; e += kThreads) {
+      const int32_t token = said[e], at = token - span0;
+      if (token >= 0 && token < a.vocab && at >= 0 && at < kSpan) atomicAdd(counts + at, 1u);
+    }
+    rep = a.repetitions ? a.repetitions[r] : a.repetition;
+    presence = a.presences ? a.presences[r] : a.presence;
+    frequency = a.frequencies ? a.frequencies[r] : a.frequency;
+    __syncthreads();
+  }
+  const uint32_t* words = nullptr;
+  if (MASK) {
+    const int64_t state = a.states ? a.states[r] : r;
+    if (state >= 0 && state < a.n_allowed) words = a.allowed + state * a.allowed_row;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int place = (v * kThreads + t) * N, at = span0 + place;
+    if (at >= a.vocab || at + N <= 0) continue;
+    const bool whole = at >= 0 && at + N <= a.vocab;
+    const uint32_t bits = !MASK || !words ? ~0u : (at >= 0 ? mask_bits(words, at, N, a.vocab) : words[0] << -at);
+    Vector y;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float z = (float)x[v].v[i];
+      if (HISTORY) {
+        const uint32_t c = counts[place + i];
+        if (c) {
+          z = z > 0.0f ? z / rep : z * rep;
+          z -= presence + frequency * (float)c;
+        }
+      }
+      if (BIAS && (whole || (at + i >= 0 && at + i < a.vocab))) z += a.bias[r * a.bias_row + at + i];
+      if (MASK) z = bits >> i & 1 ? z : -INFINITY;
+      y.v[i] = (T)z;
+    }
+    if (N > 1 && whole) {
+      *reinterpret_cast<Vector*>(out + at) = y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (at + i >= 0 && at + i < a.vocab) out[at + i] = y.v[i];
+    }
+  }
+}
+
+template <typename T, int N, int V, bool HISTORY, bool BIAS, bool MASK>
+hipError_t run(const LogitsArgs& a, hipStream_t stream) {
+  constexpr int kSpan = kThreads * N * V;
+  const int spans = (int)(((int64_t)a.vocab + (N - 1) + kSpan - 1) / kSpan);
+  return for_launches((int64_t)a.rows * spans, kThreads, [&](int64_t first, unsigned blocks) {
+    sfe_logits_kernel<T, N, V, HISTORY, BIAS, MASK><<<dim3(blocks), dim3(kThreads), 0, stream>>>(a, first, spans);
+    return hipGetLastError();
+  });
+}
+
+template <typename T, int N, int V>
+hipError_t run_what(const LogitsArgs& a, hipStream_t stream) {
+  const int what = (a.history ? 4 : 0) | (a.bias ? 2 : 0) | (a.allowed ? 1 : 0);
+  switch (what) {
+    case 0: return run<T, N, V, false, false, false>(a, stream);
+    case 1: return run<T, N, V, false, false, true>(a, stream);
+    case 2: return run<T, N, V, false, true, false>(a, stream);
+    case 3: return run<T, N, V, false, true, true>(a, stream);
+    case 4: return run<T, N, V, true, false, false>(a, stream);
+    case 5: return run<T, N, V, true, false, true>(a, stream);
+    case 6: return run<T, N, V, true, true, false>(a, stream);
+    default: return run<T, N, V, true, true, true>(a, stream);
+  }
+}
+
+template <typename T>
+hipError_t run_type(const LogitsArgs& a, hipStream_t stream) {
+  constexpr int N = 16 / (int)sizeof(T);
+  // vectors where a row's input and output lie alike
+  const bool alike = (uintptr_t)a.in % 16 == (uintptr_t)a.out % 16 && (a.in_row - a.out_row) % N == 0;
+  return alike ? run_what<T, N, 4>(a, stream) : run_what<T, 1, 4>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_logits(const LogitsArgs& a, int type, hipStream_t stream) {
+  if (type == kOpF32) return run_type<float>(a, stream);
+  if (type == kOpBf16) return run_type<__bf16>(a, stream);
+  return run_type<_Float16>(a, stream);
+}
+
+}  // namespace sfe

@@ -5,7 +5,9 @@ searches for the transcript (closed bundles in the reference, src/model.rs).
 ``ModelOps`` has the operators that such a model is built from beside plain
 matrix products: attention over packed sequences with grouped heads, rotary
 positions, the norms around a block with its gate and residual scale, and a
-step of beam search with its states' reordering.  All of them run in
+step of beam search with its states' reordering; and for a decoder that keeps its keys and values
+in pages (``KvCache``): norms of heads with rotary positions in one pass, the cache's write and read, attention
+of new tokens or trees of drafted ones over it, and the steering of logits.  All of them run in
 ``libscriptrs_fe.so``; arguments are checked before any device work, and a
 refused call raises ``InvalidModelOutput``.
 """
@@ -18,7 +20,7 @@ import math
 import numpy as np
 
 from . import _lib
-from ._lib import SfeBeamState, SfeHeads, SfeResidual, SfeRotaryTable
+from ._lib import SfeBeamState, SfeCache, SfeCacheTokens, SfeHeads, SfeLogits, SfeResidual, SfeRotaryTable
 from .frontend import InvalidModelOutput, ParakeetFeatureExtractor, _check, _ip, _stream_handle
 
 MAX_BEAMS = 32
@@ -123,6 +125,62 @@ class AttentionPlan:
             pass
 
 
+class KvCache:
+    """Keys and values of a decoder's tokens, in pages (``sfe_cache``).
+
+    ``dtype``: "bf16" or "f16", or 8 bits with a scale for each token and kv head, "e4m3" or "int8".
+    ``data``, uint8 of [pages, kv_heads, record], holds all of it, zeros at first (or the caller's own
+    contiguous tensor): a page is ``data[p]``, so that pages can be copied, and beams reordered, as
+    any other state.  ``page_size`` is a power of two from 16 to 1024, ``head_dim`` a
+    multiple of 16, at most 128."""
+
+    TYPES = {"bf16": 1, "f16": 2, "e4m3": 3, "int8": 4}
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "bf16", device: int = 0,
+                 data=None):
+        import torch
+        if dtype not in self.TYPES:
+            raise InvalidModelOutput(f"unknown cache type {dtype!r}")
+        pages, kv_heads = _int32(pages, "pages"), _int32(kv_heads, "kv_heads")
+        page_size, head_dim = _int32(page_size, "page_size"), _int32(head_dim, "head_dim")
+        if pages < 0 or not 0 < kv_heads <= 1024:
+            raise InvalidModelOutput(f"pages must not be negative and kv_heads in [1, 1024]: got {pages} and {kv_heads}")
+        record = _lib.lib().sfe_cache_record(page_size, head_dim, self.TYPES[dtype])
+        if not record:
+            raise InvalidModelOutput(_lib.last_error())
+        shape = (pages, kv_heads, record)
+        if data is None:
+            data = torch.zeros(shape, dtype=torch.uint8, device=torch.device("cuda", device))
+        _contiguous(data, "data", torch.uint8, shape)
+        self.data, self.dtype = data, dtype
+        self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
+        self.c = SfeCache(data.data_ptr(), pages, page_size, kv_heads, head_dim, self.TYPES[dtype])
+        self.p = ctypes.byref(self.c)
+
+
+class CachePlan:
+    """The new tokens of a batch's sequences, packed; made by ``ModelOps.cache_plan`` and good for every
+    layer and step with as many new tokens, until its context (the ``ModelOps`` or the extractor that
+    it shares) is closed."""
+
+    def __init__(self, ops: "ModelOps", handle, sequences: int, rows: int, heads: int, kv_heads: int, head_dim: int):
+        self._ops, self._handle = ops, handle
+        self.sequences, self.rows = sequences, rows
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.scale = 1.0 / math.sqrt(head_dim)
+
+    def close(self) -> None:
+        if self._handle:
+            _lib.lib().sfe_cache_plan_free(self._handle)
+        self._handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class ModelOps:
     """The operators on one device.
 
@@ -148,6 +206,8 @@ class ModelOps:
         self._residual = SfeResidual()
         self._residual_p = ctypes.byref(self._residual)
         self._states = (SfeBeamState * 8)()
+        self._tokens, self._logits = SfeCacheTokens(), SfeLogits()
+        self._tokens_p, self._logits_p = ctypes.byref(self._tokens), ctypes.byref(self._logits)
 
     def _stream(self, stream) -> int | None:
         if stream is None:
@@ -473,6 +533,277 @@ class ModelOps:
             row.in_, row.out = s.data_ptr(), o.data_ptr()
             row.outer, row.inner_bytes = math.prod(full[:at]), math.prod(full[at + 1:]) * s.element_size()
         rc = self._lib.sfe_beam_reorder(self._fe._handle(), pp, streams, beams, table, n, self._stream(stream))
+        if rc:
+            _check(rc)
+        return out
+
+    # -- norms of heads and rotary positions ---------------------------------------------
+    def norm_rotary(self, table: RotaryTable, positions, q, k=None, norm: str = "rms", q_weight=None, k_weight=None,
+                    eps: float = 1e-5, inplace: bool = False, stream=None):
+        """``rotary`` of each head's norm: ``q`` (and ``k``) [rows, heads, head_dim] become ``N(q) * q_weight``, of
+        which the first ``table.rotary_dim`` channels are turned by ``positions`` [rows] int32.  ``norm``: "rms" or "layer",
+        over a head's channels; weights float32 [head_dim], None for ones.  Returns ``(q, k)`` (k None without
+        one)."""
+        torch = self._torch
+        if norm not in ("layer", "rms"):
+            raise InvalidModelOutput("the norm is 'layer' or 'rms'")
+        device, code, shape = self.device, _dtype_of(q, "q"), q.shape
+        if len(shape) != 3:
+            raise InvalidModelOutput(f"q must be [rows, heads, channels], got {list(shape)}")
+        rows, heads, dim = shape
+        if heads > MAX_INT32 or dim > MAX_INT32:
+            raise InvalidModelOutput("heads and channels must be below 2^31")
+        for name, t in (("positions", positions), ("q", q)):
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
+        pos = _contiguous(positions, "positions", torch.int32, (rows,))
+        qw = None if q_weight is None else self._weight("q_weight", q_weight, dim)
+        kw = None if k_weight is None else self._weight("k_weight", k_weight, dim)
+        hq, hqo, hk, hko = self._h
+        _heads(q, "q", shape, hq)
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, positions, q, k, q_weight, k_weight)
+        q_out = q
+        if not inplace:
+            q_out = self._empty_like(q) if other is None else self._new(other, q)
+            hqo.data, hqo.row_stride, hqo.head_stride = q_out.data_ptr(), heads * dim, dim
+        k_out, kv_heads = None, 0
+        if k is not None:
+            if k.get_device() != device:
+                _wrong_device("k", k, device)
+            shape = k.shape
+            if k.dtype != q.dtype or len(shape) != 3 or shape[0] != rows or shape[2] != dim or shape[1] > MAX_INT32:
+                raise InvalidModelOutput(f"k must be {q.dtype} of [{rows}, heads, {dim}], got {k.dtype} of {list(shape)}")
+            kv_heads = shape[1]
+            _heads(k, "k", shape, hk)
+            k_out = k
+            if not inplace:
+                k_out = self._empty_like(k) if other is None else self._new(other, k)
+                hko.data, hko.row_stride, hko.head_stride = k_out.data_ptr(), kv_heads * dim, dim
+        elif k_weight is not None:
+            raise InvalidModelOutput("k_weight without k")
+        pq, pqo, pk, pko = self._hp
+        if inplace:
+            pqo, pko = pq, pk
+        rc = self._lib.sfe_norm_rotary(self._fe._handle(), table.p, self._NORMS[norm], eps, code, pos, rows, dim, heads, qw,
+                                       pq, pqo, kv_heads, kw, pk, pko, self._stream(stream))
+        if rc:
+            _check(rc)
+        return q_out, k_out
+
+    # -- a paged cache -------------------------------------------------------------------
+    def cache_plan(self, offsets, heads: int, kv_heads: int, head_dim: int, stream=None) -> CachePlan:
+        """Plan for sequences whose new tokens are the packed rows ``offsets[s]:offsets[s + 1]`` (from 0 on): each
+        sequence's last tokens.  ``heads``: of the queries."""
+        off = np.ascontiguousarray(offsets, np.int64).reshape(-1)
+        if off.size == 0:
+            raise InvalidModelOutput("offsets must have one entry more than there are sequences")
+        handle = ctypes.c_void_p()
+        heads, kv_heads, head_dim = _int32(heads, "heads"), _int32(kv_heads, "kv_heads"), _int32(head_dim, "head_dim")
+        _check(_lib.lib().sfe_cache_plan_make(self._fe._handle(), _ip(off), _int32(off.size - 1, "sequences"), heads, kv_heads,
+                                              head_dim, self._stream(stream), ctypes.byref(handle)))
+        return CachePlan(self, handle, off.size - 1, int(off[-1]), heads, kv_heads, head_dim)
+
+    def _cached(self, plan: CachePlan, cache: KvCache, page_table, lengths):
+        """Checks what a call over a cache has in common and writes the tokens' places into their struct."""
+        handle, device, int32 = plan._handle, self.device, self._torch.int32
+        if handle is None:
+            raise InvalidModelOutput("the plan is closed")
+        if plan._ops is not self:
+            raise InvalidModelOutput("the plan belongs to another ModelOps")
+        for name, t in (("the cache", cache.data), ("page_table", page_table), ("lengths", lengths)):
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
+        n, shape = plan.sequences, page_table.shape
+        if page_table.dtype != int32 or len(shape) != 2 or shape[0] != n or shape[1] > MAX_INT32 or \
+                (page_table.stride(1) != 1 and shape[1] > 1):
+            raise InvalidModelOutput(f"page_table must be an int32 tensor of [{n}, pages] with contiguous rows, got "
+                                     f"{page_table.dtype} of {list(shape)}")
+        t = self._tokens
+        t.lengths = _contiguous(lengths, "lengths", int32, (n,))
+        t.page_table, t.table_pages = page_table.data_ptr(), shape[1]
+        t.table_stride = page_table.stride(0) if n > 1 else shape[1]
+        return handle
+
+    def _rows_of(self, name, t, dtype, rows, heads, dim, h) -> None:
+        if t.get_device() != self.device:
+            _wrong_device(name, t, self.device)
+        shape = t.shape
+        if t.dtype != dtype or len(shape) != 3 or shape[0] < rows or shape[1:] != (heads, dim):
+            raise InvalidModelOutput(f"{name} must be {dtype} of [{rows}, {heads}, {dim}], got {t.dtype} of {list(shape)}")
+        _heads(t, name, shape, h)
+
+    def cache_write(self, plan: CachePlan, cache: KvCache, page_table, lengths, k, v, stream=None) -> None:
+        """Writes the new tokens' ``k`` and ``v`` [rows, kv_heads, head_dim] into the cache (float32, bfloat16 or float16,
+        whatever its type).  ``lengths`` [sequences] int32 count each sequence's tokens, the new ones included: new token
+        i of n is token ``lengths[s] - n + i``, in page ``page_table[s, token // page_size]`` (int32; a page number outside
+        the cache, past the table or before the first token: in no place, not written).  No two
+        new tokens may have one place."""
+        handle = self._cached(plan, cache, page_table, lengths)
+        code = _dtype_of(k, "k")
+        hk, hv = self._h[1], self._h[2]
+        self._rows_of("k", k, k.dtype, plan.rows, plan.kv_heads, plan.head_dim, hk)
+        self._rows_of("v", v, k.dtype, plan.rows, plan.kv_heads, plan.head_dim, hv)
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, cache.data, page_table, lengths, k, v)
+        rc = self._lib.sfe_cache_write(handle, cache.p, self._tokens_p, code, self._hp[1], self._hp[2], self._stream(stream))
+        if rc:
+            _check(rc)
+
+    def cache_read(self, plan: CachePlan, cache: KvCache, page_table, lengths, dtype=None, stream=None, out=None):
+        """The plan's tokens out of the cache, ``(k, v)`` of [rows, kv_heads, head_dim] in ``dtype`` (bfloat16
+        without; float32 or float16), rounded once; ``out``: the two tensors to write.  With a plan of whole sequences (its new tokens
+        are all of each) these are the keys and values that ``attention`` takes.  Tokens in no place are zeros."""
+        torch = self._torch
+        handle = self._cached(plan, cache, page_table, lengths)
+        hk, hv = self._h[1], self._h[2]
+        other = None if stream is None else self._other(stream)
+        if out is None:
+            shape, dtype = (plan.rows, plan.kv_heads, plan.head_dim), dtype or torch.bfloat16
+            if other is None:
+                k, v = (torch.empty(shape, dtype=dtype, device=cache.data.device) for _ in range(2))
+            else:
+                with torch.cuda.stream(other):
+                    k, v = (torch.empty(shape, dtype=dtype, device=cache.data.device) for _ in range(2))
+                for t in (k, v):
+                    t.record_stream(torch.cuda.current_stream(self.device))
+        else:
+            k, v = out
+            if dtype is not None and k.dtype != dtype:
+                raise InvalidModelOutput(f"out must be of {dtype}, got {k.dtype}")
+        code = _dtype_of(k, "k")
+        self._rows_of("k", k, k.dtype, plan.rows, plan.kv_heads, plan.head_dim, hk)
+        self._rows_of("v", v, k.dtype, plan.rows, plan.kv_heads, plan.head_dim, hv)
+        if other is not None:
+            self._held(other, cache.data, page_table, lengths, k, v)
+        rc = self._lib.sfe_cache_read(handle, cache.p, self._tokens_p, code, self._hp[1], self._hp[2], self._stream(stream))
+        if rc:
+            _check(rc)
+        return k, v
+
+    def cache_attention(self, plan: CachePlan, cache: KvCache, page_table, lengths, q, tree=None, scale: float | None = None,
+                        stream=None, out=None):
+        """``softmax(scale q k^T) v`` of the new tokens' ``q`` [rows, heads, head_dim] (bfloat16 or float16) over
+        the cache, into which their keys and values are written already.  Each sees the tokens before the new
+        ones and, of the new ones, itself and those before it; or with ``tree`` [rows] int64, of at most 64
+        new tokens a sequence, those whose bit is set (bit j: new token j of the row's sequence).  Rows that see nothing give
+        zeros, and so do rows of q past the last sequence."""
+        handle, dtype = self._cached(plan, cache, page_table, lengths), q.dtype
+        code = _dtype_of(q, "q")
+        if code == _lib.SFE_F32:
+            raise InvalidModelOutput(f"q must be bfloat16 or float16, got {dtype}")
+        hq, _, _, ho = self._h
+        self._rows_of("q", q, dtype, plan.rows, plan.heads, plan.head_dim, hq)
+        tp = None
+        if tree is not None:
+            if tree.get_device() != self.device:
+                _wrong_device("tree", tree, self.device)
+            tp = _contiguous(tree, "tree", self._torch.int64, (plan.rows,))
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, cache.data, page_table, lengths, q, tree, out)
+        if out is None:
+            out = self._empty_like(q) if other is None else self._new(other, q)
+            ho.data, ho.row_stride, ho.head_stride = out.data_ptr(), plan.heads * plan.head_dim, plan.head_dim
+        else:
+            _same(out, q, "out")
+            if out.get_device() != self.device:
+                _wrong_device("out", out, self.device)
+            _heads(out, "out", q.shape, ho)
+        rc = self._lib.sfe_cache_attention(handle, cache.p, self._tokens_p, code, self._hp[0], tp,
+                                           plan.scale if scale is None else scale, self._hp[3], q.shape[0],
+                                           self._stream(stream))
+        if rc:
+            _check(rc)
+        return out
+
+    # -- steering of logits ----------------------------------------------------------------
+    def adjust_logits(self, logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None,
+                      allowed=None, states=None, stream=None, out=None):
+        """``logits`` [rows, vocab] steered before a choice.  A token that stands c > 0 times in its row's ``history``
+        [rows, most] int32 (its first ``lengths`` [rows] int32; tokens outside the vocabulary count for
+        nothing) has its logit divided by ``repetition``, or multiplied where it is not positive, then less
+        ``presence + frequency * c`` (numbers, or float32 [rows]); ``bias`` float32 [vocab] or [rows, vocab] is
+        added; tokens that the row's mask lacks get -inf: ``allowed`` int32 [masks, words] has token t's bit in bit t % 32 of
+        word t // 32, ``states`` [rows] int32 say which mask (outside [0, masks): none; without states, row r takes
+        mask r).  ``out`` may be ``logits``."""
+        torch, device, shape = self._torch, self.device, logits.shape
+        if len(shape) != 2:
+            raise InvalidModelOutput(f"logits must be [rows, vocab], got {list(shape)}")
+        rows, vocab = shape
+        if rows > MAX_INT32 or vocab > MAX_INT32:
+            raise InvalidModelOutput("rows and vocab must be below 2^31")
+
+        def table(name, t, dtype, columns):
+            """Rows with contiguous columns: address and stride."""
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
+            if t.dtype != dtype or t.dim() != 2 or (columns is not None and t.shape[1] != columns) or \
+                    (t.stride(1) != 1 and t.shape[1] > 1):
+                raise InvalidModelOutput(f"{name} must be {dtype} of [rows, {'columns' if columns is None else columns}] with "
+                                         f"contiguous rows, got {t.dtype} of {list(t.shape)}")
+            return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+        def each(name, t, dtype):
+            if t.get_device() != device:
+                _wrong_device(name, t, device)
+            return _contiguous(t, name, dtype, (rows,))
+        a = self._logits
+        a.dtype, a.rows, a.vocab = _dtype_of(logits, "logits"), rows, vocab
+        a.logits, a.logits_row = table("logits", logits, logits.dtype, vocab)
+        a.history = a.lengths = None
+        a.history_most = 0
+        if history is not None:
+            a.history, a.history_row = table("history", history, torch.int32, None)
+            if history.shape[0] != rows or history.shape[1] > MAX_INT32:
+                raise InvalidModelOutput(f"history must have {rows} rows, got {list(history.shape)}")
+            a.history_most = history.shape[1]
+            if lengths is not None:
+                a.lengths = each("lengths", lengths, torch.int32)
+            if history.shape[1] == 0:
+                a.history = a.lengths = None
+        elif lengths is not None:
+            raise InvalidModelOutput("lengths without a history")
+        given = []
+        for name, value in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+            tensor = isinstance(value, torch.Tensor)
+            given.append(value if tensor else None)
+            setattr(a, name, 1.0 if tensor else value)
+            setattr(a, {"frequency": "frequencies"}.get(name, name + "s"), each(name, value, self._f32) if tensor else None)
+        a.bias = None
+        if bias is not None:
+            if bias.dim() == 1:
+                a.bias, a.bias_row = self._weight("bias", bias, vocab), 0
+            else:
+                a.bias, a.bias_row = table("bias", bias, self._f32, vocab)
+                if bias.shape[0] != rows:
+                    raise InvalidModelOutput(f"bias must be [{vocab}] or [{rows}, {vocab}], got {list(bias.shape)}")
+        a.allowed = a.states = None
+        a.n_allowed = 0
+        if allowed is not None:
+            a.allowed, a.allowed_row = table("allowed", allowed, torch.int32, None)
+            if 32 * allowed.shape[1] < vocab or allowed.shape[0] > MAX_INT32 or (states is None and allowed.shape[0] != rows):
+                raise InvalidModelOutput(f"allowed must be [{'masks' if states is not None else rows}, {(vocab + 31) // 32}], "
+                                         f"got {list(allowed.shape)}")
+            a.n_allowed = allowed.shape[0]
+            if states is not None:
+                a.states = each("states", states, torch.int32)
+            if a.n_allowed == 0:  # (every row's state is outside)
+                a.allowed = a.states = None
+        elif states is not None:
+            raise InvalidModelOutput("states without masks")
+        other = None if stream is None else self._other(stream)
+        if other is not None:
+            self._held(other, logits, history, lengths, *given, bias, allowed, states, out)
+        if out is None:
+            out = self._empty_like(logits) if other is None else self._new(other, logits)
+            a.out, a.out_row = out.data_ptr(), vocab
+        else:
+            _same(out, logits, "out")
+            a.out, a.out_row = table("out", out, logits.dtype, vocab)
+        rc = self._lib.sfe_adjust_logits(self._fe._handle(), self._logits_p, self._stream(stream))
         if rc:
             _check(rc)
         return out

@@ -2,100 +2,673 @@
 //
 // For new token i of n of a sequence of L tokens, head h reading kv head h / group:
 // o_i = sum_j softmax_j(scale q_i . k_j) v_j over the context (j < L - n) and the new tokens that i sees:
-// those of its tree's bits, or without a tree itself and those before.  Codes of 8 bits enter the sums as they
-// are: a key's scale multiplies its score, a value's scale its weight.
+// those of its tree's bits, or without a tree itself and those before.  One pass over the keys with a running
+// reference exponent and sum, as in sfe_attn.hip.
+//
+// Codes of 8 bits enter the matrix products as they are (both 16-bit types hold them exactly): a key's scale
+// multiplies its scores, a value's scale its weight, in f32 before the weight's one rounding to 16
+// bits.  In f16, which lacks the range, weights are kept relative to the largest value scale so far.
+//
+// A wave takes steps of 32 keys through an LDS ring of its own, without a barrier: pages are looked up one step
+// ahead, rows go from memory into LDS directly, and what lies past a sequence's end or in no page
+// is read as zeros by the buffer's range.  Scores are S^T = K Q^T (a lane has one query's), which is the
+// operand order of O^T = V^T P^T once V's rows are paired by key in registers.  The order of channels in a
+// product is free, so lanes read whole chunks of K and of V.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "sfe_cache.hpp"
 #include "sfe_internal.hpp"
+#include "sfe_mat.hpp"
 
 namespace sfe {
 namespace {
 
-template <int TYPE>
-__device__ __forceinline__ float kept_value(const char* row, int d) {
-  if constexpr (TYPE == kCacheE4m3) return __builtin_amdgcn_cvt_f32_fp8((int)(uint8_t)row[d], 0);
-  else if constexpr (TYPE == kCacheInt8) return (float)(int8_t)row[d];
-  else if constexpr (TYPE == kCacheBf16) return (float)reinterpret_cast<const __bf16*>(row)[d];
-  else return (float)reinterpret_cast<const _Float16*>(row)[d];
+constexpr int kWaves = kCacheAttnWaves, kStep = 32, kRound = kCacheAttnRound;
+static_assert(kRound == kWaves * kStep, "a round is a step of each wave");
+
+__device__ __forceinline__ void load_lds_word(I4 buf, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf) : "memory");
+}
+__device__ __forceinline__ I4 buffer(uint64_t at, int bytes) {
+  I4 r;
+  r.x = __builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+  r.y = __builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu));
+  r.z = __builtin_amdgcn_readfirstlane(bytes);
+  r.w = kBufWord3;
+  return r;
+}
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t at) {
+  return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
 }
 
-// A wave a packed row: a lane takes a key's score, then two channels of the values' sum.
-template <typename T, int TYPE>
-__global__ __launch_bounds__(64) void sfe_cache_attn_kernel(CacheAttnArgs a, int64_t first) {
-  const CacheArgs& c = a.c;
-  const int64_t unit = first + blockIdx.x;
-  const int kvh = (int)(unit % c.kv_heads), lane = (int)threadIdx.x;
-  const CacheTile tile = c.tiles[unit / c.kv_heads];
-  const int length = c.lengths[tile.seq];
-  const int64_t part = (int64_t)Kept<TYPE>::kSize * c.dim << c.shift;
-  for (int r = tile.at; r < tile.at + tile.count; ++r) {
-    const int token = r / a.group, head = kvh * a.group + r - token * a.group;
-    const T* q = reinterpret_cast<const T*>(a.q.data + (tile.first + token) * a.q.row + head * a.q.head);
-    const int64_t context = (int64_t)length - tile.n, me = context + token;
-    const uint64_t bits = a.tree ? a.tree[tile.first + token] : 0;
-    float m = -INFINITY, l = 0.0f, o[2] = {0.0f, 0.0f};
-    const int64_t end = me < 0 ? 0 : (a.tree ? length : me + 1);
-    for (int64_t j0 = 0; j0 < end; j0 += 64) {
-      const int64_t j = j0 + lane, draft = j - context;
-      const int64_t page = j < end ? page_of(c, tile.seq, j) : -1;
-      const bool see = page >= 0 && (draft < 0 || !a.tree || (draft < 64 && (bits >> draft & 1)));
-      const char* record = c.data + (page * c.kv_heads + kvh) * c.record;
-      const int slot = (int)(j & ((1 << c.shift) - 1));
-      float s = -INFINITY, vs = 1.0f;
-      if (see) {
-        s = 0.0f;
-        for (int d = 0; d < c.dim; ++d) s += (float)q[d] * kept_value<TYPE>(record + (int64_t)Kept<TYPE>::kSize * slot * c.dim, d);
-        if (cache_coded(TYPE)) {
-          const float* scales = reinterpret_cast<const float*>(record + 2 * part);
-          s *= scales[slot];
-          vs = scales[(1 << c.shift) + slot];
-        }
-        s *= a.scale_log2;
-      }
-      float top = s;
-      for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-      const float nm = fmaxf(m, top);
-      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - nm);
-      m = nm;
-      const float p = see ? __builtin_amdgcn_exp2f(s - m) : 0.0f;
-      float sum = p;
-      for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-      l = l * f + sum;
-      o[0] *= f, o[1] *= f;
-      for (int i = 0; i < 64; ++i) {
-        if (!__shfl((int)see, i)) continue;
-        const float w = __shfl(p, i) * __shfl(vs, i);
-        const char* values = c.data + (__shfl(page, i) * c.kv_heads + kvh) * c.record + part +
-                             (int64_t)Kept<TYPE>::kSize * __shfl(slot, i) * c.dim;
-        for (int e = 0; e < 2; ++e)
-          if (lane + 64 * e < c.dim) o[e] += w * kept_value<TYPE>(values, lane + 64 * e);
+// Rows of a step in LDS: DP channels of E bytes, 16-byte chunks permuted by the row (as far as a row has them).
+template <int DP, int E>
+struct Ring {
+  static constexpr int kPitch = DP * E, kChunks = kPitch / 16;
+  static constexpr int kHalf = 16 * kPitch;                      // 16 rows of K, or of V
+  static constexpr int kScales = 4 * kHalf;                      // then 256 bytes of scales for each half
+  static constexpr int kBytes = kScales + (E == 1 ? 512 : 0);    // a step: K, V, scales
+  static constexpr int kStages = 2;
+  static constexpr int kLoads = 2 * (2 * (kHalf / 1024) + (E == 1 ? 1 : 0));  // of a step
+  static __device__ int swizzle(int row) { return kChunks == 16 ? row & 15 : (kChunks == 8 ? row & 7 : (row >> 1) & 3); }
+};
+
+typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+
+// Codes as 16-bit values, two a word.
+template <typename T, int TYPE, int WORD>
+__device__ __forceinline__ uint32_t pair_of(uint32_t x) {
+  if constexpr (TYPE == kCacheE4m3) {
+    if constexpr (std::is_same<T, Bf>::value)
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, WORD != 0));
+    else
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, WORD != 0));
+  } else {
+    const float a = (float)(int8_t)(x >> (16 * WORD)), b = (float)(int8_t)(x >> (16 * WORD + 8));
+    if constexpr (std::is_same<T, Bf>::value)  // (8 bits: the lower half of the f32 is zero)
+      return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+    else
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  }
+}
+
+// Operands of 16 keys' rows for all k steps of the first product: 32 channels each.
+template <typename T, int TYPE, int DP>
+__device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typename Mat<T>::V8 (&k)[DP / 32]) {
+  typedef typename Mat<T>::V8 V8;
+  if constexpr (Kept<TYPE>::kSize == 2) {
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) k[t] = __builtin_bit_cast(V8, lds_read<U4>(addr[t] + at));
+  } else {
+#pragma unroll
+    for (int t = 0; t < DP / 64; ++t) {
+      const U4 x = lds_read<U4>(addr[t] + at);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        U4 y;
+        y.x = pair_of<T, TYPE, 0>(x[2 * h]);
+        y.y = pair_of<T, TYPE, 1>(x[2 * h]);
+        y.z = pair_of<T, TYPE, 0>(x[2 * h + 1]);
+        y.w = pair_of<T, TYPE, 1>(x[2 * h + 1]);
+        k[2 * t + h] = __builtin_bit_cast(V8, y);
       }
     }
-    T* out = reinterpret_cast<T*>(const_cast<char*>(a.o.data) + (tile.first + token) * a.o.row + head * a.o.head);
-    for (int e = 0; e < 2; ++e)
-      if (lane + 64 * e < c.dim) out[lane + 64 * e] = (T)(l != 0.0f ? o[e] / l : 0.0f);
   }
+}
+
+// Operands of the second product: values of the lane's 8 keys (16 u + 4 quarter + i) in each of its channels.
+template <typename T, int TYPE, int DP>
+__device__ __forceinline__ void values_of(uint32_t (&addr)[4], uint32_t at, typename Mat<T>::V8 (&v)[DP / 16]) {
+  typedef typename Mat<T>::V8 V8;
+  constexpr int C = DP / 16, W = C / 2;  // a lane's channels, words of 16-bit pairs
+  constexpr int E = Kept<TYPE>::kSize, kPitch = DP * E;
+  uint32_t w[8][W];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t from = addr[i] + at + u * 16 * kPitch;
+      uint32_t* to = w[4 * u + i];
+      if constexpr (E == 2 && C == 8) {
+        const U4 x = lds_read<U4>(from);
+        to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+      } else if constexpr (E == 2) {
+        const U2 x = lds_read<U2>(from);
+        to[0] = x.x, to[1] = x.y;
+      } else if constexpr (C == 8) {
+        const U2 x = lds_read<U2>(from);
+        to[0] = pair_of<T, TYPE, 0>(x.x), to[1] = pair_of<T, TYPE, 1>(x.x);
+        to[2] = pair_of<T, TYPE, 0>(x.y), to[3] = pair_of<T, TYPE, 1>(x.y);
+      } else {
+        const uint32_t x = lds_read<uint32_t>(from);
+        to[0] = pair_of<T, TYPE, 0>(x), to[1] = pair_of<T, TYPE, 1>(x);
+      }
+    }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    U4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      y[e] = __builtin_amdgcn_perm(w[2 * e + 1][c / 2], w[2 * e][c / 2], c % 2 ? 0x07060302 : 0x05040100);
+    v[c] = __builtin_bit_cast(V8, y);
+  }
+}
+
+// The lowest n of 32 bits.
+__device__ __forceinline__ uint32_t low_bits(int64_t n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
+
+// What an item needs of its sequence's keys: those before `end`, in rounds.
+struct Span {
+  int64_t context;  // tokens before the new ones (negative: the first new tokens are none)
+  int end, rounds;
+};
+__device__ __forceinline__ Span span_of(const CacheAttnArgs& a, const CacheTile& t) {
+  Span s;
+  const int length = a.c.lengths[t.seq];
+  s.context = (int64_t)length - t.n;
+  int64_t end = length;
+  if (!a.tree) end = s.context + (t.at + t.count - 1) / a.group + 1;
+  const int64_t cap = (int64_t)a.c.table_pages << a.c.shift;
+  end = end < cap ? end : cap;
+  s.end = (int)(end < 0 ? 0 : end);
+  s.rounds = s.end > 0 ? (int)(((int64_t)s.end + kRound - 1) / kRound) : 1;
+  return s;
+}
+
+template <int CTRL, int MASK>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, MASK, 0xf, false);
+}
+// Inclusive sums over a wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x = dpp_add<0x111, 0xf>(x);  // from the lane 1, 2, 4 and 8 before, within 16
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // the row before's last lane, then that of the first two
+  x = dpp_add<0x143, 0xc>(x);
+  return x;
+}
+
+// Where the workgroup's share of all rounds begins: the item that holds round `at` and the rounds before that
+// item.  Units are (item, kv head), the heads of an item side by side.
+struct Start {
+  int total;           // rounds of all units
+  int item, before;    // rounds of the units before the item
+};
+__device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* lds, int* share, int least) {
+  const int t = (int)threadIdx.x, per = (a.c.n_tiles + 64 * kWaves - 1) / (64 * kWaves);
+  int mine = 0;
+  for (int i = t * per; i < min((t + 1) * per, a.c.n_tiles); ++i) mine += span_of(a, a.c.tiles[i]).rounds;
+  int sum = wave_scan(mine);
+  if ((t & 63) == 63) lds[t >> 6] = sum;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    if (v < (t >> 6)) sum += lds[v];
+    total += lds[v];
+  }
+  Start s;
+  s.total = total * a.c.kv_heads;
+  *share = max(least, (int)(((int64_t)s.total + gridDim.x - 1) / gridDim.x));
+  const int64_t at = (int64_t)w * *share;
+  int before = sum - mine;
+  if (at >= (int64_t)before * a.c.kv_heads && at < (int64_t)sum * a.c.kv_heads) {
+    int i = t * per;
+    for (;; ++i) {
+      const int r = span_of(a, a.c.tiles[i]).rounds;
+      if (at < (int64_t)(before + r) * a.c.kv_heads) break;
+      before += r;
+    }
+    lds[kWaves] = i;
+    lds[kWaves + 1] = before * a.c.kv_heads;
+  }
+  __syncthreads();
+  s.item = __builtin_amdgcn_readfirstlane(lds[kWaves]);
+  s.before = __builtin_amdgcn_readfirstlane(lds[kWaves + 1]);
+  return s;
+}
+
+// T: the queries' type; NR: tiles of 16 packed rows of an item.
+// WHOLE: a workgroup takes one unit, all of its rounds; otherwise an equal share of all rounds, of
+// which the first and last units may be cut: their parts go to a slot each and are joined by a second launch.
+template <typename T, int TYPE, int DP, int NR, bool WHOLE>
+__global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_kernel(CacheAttnArgs a, int64_t first) {
+  typedef Ring<DP, Kept<TYPE>::kSize> R;
+  typedef Mat<T> M;
+  typedef typename M::V8 V8;
+  typedef typename M::V2 V2;
+  constexpr bool kCoded = Kept<TYPE>::kSize == 1;
+  constexpr bool kRelative = kCoded && std::is_same<T, Hf>::value;
+  constexpr int E = Kept<TYPE>::kSize, C = DP / 16, S = R::kStages;
+  constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
+  constexpr int kRing = kWaves * S * R::kBytes, kJoin = 4 * (kWaves * 16 * kRowF + 2 * kWaves * 16);
+  __shared__ __align__(1024) char lds[kRing > kJoin ? kRing : kJoin];
+  __shared__ int lds_start[kWaves + 2];
+  const CacheArgs& c = a.c;
+  const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), quarter = lane >> 4;
+  const uint32_t base = lds_address(lds) + wave * S * R::kBytes;
+
+  // ---- addresses that stay
+  uint32_t k_addr[4], v_addr[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k_addr[i] = base + (lane & 15) * R::kPitch + 16 * (((4 * i + quarter) % R::kChunks) ^ R::swizzle(lane & 15));
+    const int row = 4 * quarter + i, byte = C * E * (lane & 15);
+    v_addr[i] = base + 2 * R::kHalf + row * R::kPitch + 16 * ((byte / 16) ^ R::swizzle(row)) + byte % 16;
+  }
+  // a lane's chunk of 16 rows in each load, its place in the record's rows or none
+  constexpr int kRowLoads = R::kHalf / 1024;
+  uint32_t from[kRowLoads];
+#pragma unroll
+  for (int i = 0; i < kRowLoads; ++i) {
+    const int row = (i * 64 + lane) / R::kChunks, chunk = ((i * 64 + lane) % R::kChunks) ^ R::swizzle(row);
+    from[i] = 16 * chunk < c.dim * E ? (uint32_t)(row * c.dim * E + 16 * chunk) : kOutside;
+  }
+  const int page_mask = (1 << c.shift) - 1;
+  const uint32_t part = (uint32_t)(c.dim * E) << c.shift;  // bytes of a record's K, and V
+
+  // ---- the workgroup's share
+  int64_t at, stop;  // rounds (WHOLE: of its one unit)
+  int item, before, share = 0, w = 0;
+  typedef const __attribute__((address_space(4))) CacheTile* Tiles;
+  const Tiles tiles = (Tiles)(uintptr_t)c.tiles;
+  CacheTile tile;
+  auto tile_at = [&](int i) {
+    const Tiles p = tiles + i;
+    tile.first = p->first, tile.seq = p->seq, tile.n = p->n, tile.at = p->at, tile.count = p->count;
+  };
+  int kvh0 = 0;
+  if (WHOLE) {
+    const int64_t unit = first + blockIdx.x;
+    item = (int)(unit / c.kv_heads);
+    kvh0 = (int)(unit - (int64_t)item * c.kv_heads);
+    at = before = 0;
+    stop = 1;
+  } else {
+    // consecutive workgroups go to the 8 XCDs in turn: each has a contiguous part of the shares
+    w = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
+    const Start s = start_of(a, w, lds_start, &share, a.least);
+    at = (int64_t)w * share;
+    stop = at + share < s.total ? at + share : s.total;
+    if (at >= stop) return;
+    item = s.item;
+    before = s.before;
+  }
+  while (at < stop) {
+    tile_at(__builtin_amdgcn_readfirstlane(item));
+    const Span sp = span_of(a, tile);
+    const int rounds = __builtin_amdgcn_readfirstlane(sp.rounds), end = __builtin_amdgcn_readfirstlane(sp.end);
+    const int64_t context = sp.context;
+    int kvh, r0, r1;
+    if (WHOLE) {
+      kvh = kvh0, r0 = 0, r1 = rounds;
+    } else {
+      const int in = (int)(at - before);
+      kvh = __builtin_amdgcn_readfirstlane((int)((unsigned)in / (unsigned)rounds));
+      r0 = in - kvh * rounds;
+      r1 = (int)(rounds - r0 < stop - at ? rounds : r0 + (stop - at));
+    }
+    const int32_t* pages = c.table + (int64_t)tile.seq * c.table_row;
+    typedef const __attribute__((address_space(4))) int32_t* Pages;
+    // the pages of a step's halves (-1: none)
+    auto look_up = [&](int r, int (&page)[2]) {
+      const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        page[h] = -1;
+        if (key + 16 * h < end) page[h] = ((Pages)(uintptr_t)pages)[(key + 16 * h) >> c.shift];
+      }
+    };
+    // a step's loads; the keys of either half that there are
+    auto load_step = [&](int r, int stage, const int (&page)[2]) {
+      const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+      int there = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool ok = page[h] >= 0 && page[h] < c.pages && key + 16 * h < end;
+        const int n = ok ? (end - key - 16 * h < 16 ? end - key - 16 * h : 16) : 0;
+        there |= n << (8 * h);
+        const uint64_t record = (uint64_t)(uintptr_t)c.data + (uint64_t)((int64_t)(ok ? page[h] : 0) * c.kv_heads + kvh) * (uint64_t)c.record;
+        const int slot = (key + 16 * h) & page_mask, bytes = n * c.dim * E;
+        const I4 kb = buffer(record + (uint32_t)(slot * c.dim * E), bytes);
+        const I4 vb = buffer(record + part + (uint32_t)(slot * c.dim * E), bytes);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * R::kBytes + h * R::kHalf);
+#pragma unroll
+        for (int i = 0; i < kRowLoads; ++i) load_lds(kb, from[i], to + i * 1024);
+#pragma unroll
+        for (int i = 0; i < kRowLoads; ++i) load_lds(vb, from[i], to + 2 * R::kHalf + i * 1024);
+        if (kCoded) {
+          const I4 sb = buffer(record + 2 * part + 4 * slot, n ? 4 * (page_mask + 1) + 4 * n : 0);
+          const int l = lane & 15;
+          const uint32_t off = lane < 32 && l < n ? (uint32_t)(4 * l + (lane < 16 ? 0 : 4 * (page_mask + 1))) : kOutside;
+          load_lds_word(sb, off, __builtin_amdgcn_readfirstlane(base + stage * R::kBytes + R::kScales + h * 256));
+        }
+      }
+      return there;
+    };
+    int page[2], there[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      look_up(r0 + s < r1 ? r0 + s : r1 - 1, page);
+      if (r0 + s >= r1) page[0] = page[1] = -1;
+      there[s] = load_step(r0 + s, s, page);
+    }
+    // ---- the queries, behind the first loads
+    const int total = tile.n * a.group;
+    V8 q[NR][DP / 32];
+    uint64_t bits[NR];
+    bool alive[NR];
+    int64_t me[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const int row = tile.at + 16 * n + (lane & 15), rc = row < total ? row : total - 1;
+      const int token = (int)((unsigned)rc / (unsigned)a.group), head = kvh * a.group + rc - token * a.group;
+      const char* p = a.q.data + (tile.first + token) * a.q.row + head * a.q.head;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        const int channel = E == 2 ? 32 * i + 8 * quarter : 64 * (i / 2) + 16 * quarter + 8 * (i % 2);
+        S8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (channel < c.dim) x = *reinterpret_cast<const S8*>(p + 2 * channel);
+        q[n][i] = __builtin_bit_cast(V8, x);
+      }
+      me[n] = context + token;
+      alive[n] = me[n] >= 0;
+      bits[n] = a.tree ? a.tree[tile.first + token] : 0;
+      if (tile.n < 64) bits[n] &= (1ull << tile.n) - 1;
+    }
+    look_up(r0 + S < r1 ? r0 + S : r1 - 1, page);
+    // (waited for here: a wait within the loop would be one for the loads into LDS too)
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) asm volatile("" : "+v"(q[n][i]));
+      asm volatile("" : "+v"(bits[n]));
+    }
+
+    F4 o[NR][C];
+    float m[NR], l[NR], top_scale[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      m[n] = kNever, l[n] = 0.0f, top_scale[n] = 0x1p-110f;
+#pragma unroll
+      for (int i = 0; i < C; ++i) o[n][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int stage = 0;
+    for (int r = r0; r < r1; ++r) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * R::kLoads) : "memory");
+      const uint32_t in = stage * R::kBytes;
+      const int64_t key = (int64_t)(r * kWaves + wave) * kStep;
+      const int now = there[0];
+      // ---- scores
+      F4 s[NR][2], ks[2], vs[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        V8 k[DP / 32];
+        keys_of<T, TYPE, DP>(k_addr, in + u * R::kHalf, k);
+        if (kCoded) {
+          ks[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 16 * quarter) * a.scale_log2;
+          vs[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 64 + 16 * quarter);
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          s[n][u] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i) s[n][u] = M::m16(k[i], q[n][i], s[n][u]);
+        }
+      }
+      V8 v[C];
+      values_of<T, TYPE, DP>(v_addr, in, v);
+      float top_value = 0.0f;  // (of the lane's keys)
+      if (kRelative)
+        top_value = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])),
+                          fmaxf(fmaxf(vs[1][0], vs[1][1]), fmaxf(vs[1][2], vs[1][3])));
+      // keys that some rows do not see
+      const bool uneven = key + kStep > context || now != 0x1010;
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        uint32_t see = ~0u;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][u][i] *= kCoded ? ks[u][i] : a.scale_log2;
+        if (uneven) {
+          see = a.tree ? low_bits(context - key) : low_bits(me[n] + 1 - key);
+          if (a.tree) {
+            const int64_t d = context - key;
+            if (d >= 0) see |= d < 32 ? (uint32_t)(bits[n] << d) : 0;
+            else see |= d > -64 ? (uint32_t)(bits[n] >> -d) : 0;
+          }
+          see &= low_bits(now & 0xff) | low_bits(now >> 8) << 16;
+          if (!alive[n]) see = 0;
+          see >>= 4 * quarter;  // the lane's keys are 16 u + 4 quarter + i
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][u][i] = (see >> (16 * u + i)) & 1 ? s[n][u][i] : -INFINITY;
+        }
+        float top = s[n][0][0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][u][i]);
+        if (__any(top > m[n] + M::kRise)) {
+          top = fmaxf(top, __shfl_xor(top, 16));
+          const float nm = fmaxf(m[n], max_halves(top) - M::kBelow);
+          const float f = exp2_fast(m[n] - nm);
+          m[n] = nm;
+          l[n] *= f;
+#pragma unroll
+          for (int i = 0; i < C; ++i) o[n][i] *= f;
+        }
+        if (kRelative) {
+          float top_seen = top_value;
+          if (uneven) {
+            top_seen = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) top_seen = (see >> (16 * u + i)) & 1 ? fmaxf(top_seen, vs[u][i]) : top_seen;
+          }
+          if (__any(top_seen > top_scale[n])) {
+            top_seen = max_halves(fmaxf(top_seen, __shfl_xor(top_seen, 16)));
+            // the power of two above it
+            const float up = fmaxf(top_scale[n], __uint_as_float((min(__float_as_uint(top_seen) >> 23, 252u) + 1) << 23));
+            const float f = top_scale[n] / up;
+            top_scale[n] = up;
+#pragma unroll
+            for (int i = 0; i < C; ++i) o[n][i] *= f;
+          }
+        }
+        const float relative = kRelative ? 1.0f / top_scale[n] : 1.0f;
+        V8 p;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            F2 x = {exp2_fast(s[n][u][i] - m[n]), exp2_fast(s[n][u][i + 1] - m[n])};
+            l[n] += x.x + x.y;
+            if (kCoded) {
+              x.x *= kRelative ? vs[u][i] * relative : vs[u][i], x.y *= kRelative ? vs[u][i + 1] * relative : vs[u][i + 1];
+              if (uneven) {  // (0 times a scale that is not finite)
+                x.x = (see >> (16 * u + i)) & 1 ? x.x : 0.0f;
+                x.y = (see >> (16 * u + i + 1)) & 1 ? x.y : 0.0f;
+              }
+            }
+            const V2 y = __builtin_convertvector(x, V2);
+            p[4 * u + i] = y.x;
+            p[4 * u + i + 1] = y.y;
+          }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          V8 x = v[i];
+          if (uneven && __any(nonfinite<T>(x) != 0)) {  // kept from the rows that do not see it as 0 * inf
+            S8 clean, up, down, seen;
+            split_nonfinite<T>(__builtin_bit_cast(S8, x), &clean, &up, &down);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) seen[j] = (see >> (16 * (j / 4) + j % 4)) & 1 ? M::kOne : 0;
+            const F4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            const F4 ups = M::m16(__builtin_bit_cast(V8, up), __builtin_bit_cast(V8, seen), zero);
+            const F4 downs = M::m16(__builtin_bit_cast(V8, down), __builtin_bit_cast(V8, seen), zero);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (ups[j] > 0.0f) o[n][i][j] += INFINITY;
+              if (downs[j] > 0.0f) o[n][i][j] -= INFINITY;
+            }
+            x = __builtin_bit_cast(V8, clean);
+          }
+          o[n][i] = M::m16(x, p, o[n][i]);
+        }
+      }
+      // ---- the buffer just read takes the step after those in flight
+#pragma unroll
+      for (int i = 0; i + 1 < S; ++i) there[i] = there[i + 1];
+      if (r + S >= r1) page[0] = page[1] = -1;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      there[S - 1] = load_step(r + S, stage, page);
+      look_up(r + S + 1 < r1 ? r + S + 1 : r1 - 1, page);
+      stage = stage + 1 == S ? 0 : stage + 1;
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      l[n] += __shfl_xor(l[n], 16);
+      l[n] = sum_halves(l[n]);
+      if (kRelative)
+#pragma unroll
+        for (int i = 0; i < C; ++i) o[n][i] *= top_scale[n];
+    }
+    // ---- the waves' results, added up through LDS, a tile of 16 rows at a time
+    const bool cut = !WHOLE && (r0 > 0 || r1 < rounds);
+    const int slot = 2 * w + (r1 < rounds);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    float* ow = reinterpret_cast<float*>(lds);                          // [wave][16][kRowF]
+    float2* ml = reinterpret_cast<float2*>(ow + kWaves * 16 * kRowF);   // [wave][16]
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      if (16 * n >= tile.count) break;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < C; i += 4)
+          *reinterpret_cast<F4*>(ow + (wave * 16 + (lane & 15)) * kRowF + C * (4 * quarter + j) + i) =
+              F4{o[n][i][j], o[n][i + 1][j], o[n][i + 2][j], o[n][i + 3][j]};
+      if (quarter == 0) ml[wave * 16 + lane] = make_float2(m[n], l[n]);
+      __syncthreads();
+      for (int e = t; e < 16 * (DP / 4); e += 64 * kWaves) {
+        const int row = e / (DP / 4), d = 4 * (e % (DP / 4));
+        float mm = kNever;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, ml[v * 16 + row].x);
+        F4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+          const float2 x = ml[v * 16 + row];
+          if (x.x == kNever && x.y == 0.0f) continue;  // (saw nothing)
+          const float f = exp2_fast(x.x - mm);
+          sum += x.y * f;
+          acc += *reinterpret_cast<const F4*>(ow + (v * 16 + row) * kRowF + d) * f;
+        }
+        const int rr = tile.at + 16 * n + row;
+        if (cut) {
+          const int64_t place = (int64_t)slot * (16 * NR) + 16 * n + row;
+          *reinterpret_cast<F4*>(a.part_o + place * DP + d) = acc;
+          if (d == 0) a.part_ml[place] = make_float2(mm, sum);
+        } else if (rr < total && d < c.dim) {
+          const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;  // (a row that sees nothing is zero)
+          const int token = (int)((unsigned)rr / (unsigned)a.group);
+          char* p = const_cast<char*>(a.o.data) + (tile.first + token) * a.o.row + (int64_t)(kvh * a.group + rr - token * a.group) * a.o.head;
+          const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};
+          const V2 f = __builtin_convertvector(x, V2), g = __builtin_convertvector(y, V2);
+          *reinterpret_cast<uint2*>(p + 2 * d) = make_uint2(__builtin_bit_cast(uint32_t, f), __builtin_bit_cast(uint32_t, g));
+        }
+      }
+    }
+    if (WHOLE) return;
+    if (t == 0 && r0 == 0) {
+      // what the join needs: the workgroup of the unit's first part, and how many parts
+      const int64_t last = (at + rounds - 1) / share;
+      a.units[(int64_t)item * c.kv_heads + kvh] = make_int2(w, cut ? (int)(last - w + 1) : 0);
+    }
+    __syncthreads();  // (the next unit's loads go where the results lie)
+    at += r1 - r0;
+    if (r1 == rounds && kvh == c.kv_heads - 1) {
+      ++item;
+      before += rounds * c.kv_heads;
+    }
+  }
+}
+
+// Parts of units that were cut, added up: a workgroup takes 4 rows of a unit, two teams every other part.
+template <typename T, int DP, int NR>
+__global__ __launch_bounds__(2 * DP) void sfe_cache_attn_join_kernel(CacheAttnArgs a, int64_t first) {
+  typedef typename Mat<T>::V2 V2;
+  constexpr int kLanes = DP / 4;  // of a row
+  __shared__ F4 half[4 * kLanes];
+  __shared__ float sums[4];
+  const int64_t block = first + blockIdx.x, unit = block / (4 * NR);
+  const int2 u = a.units[unit];
+  if (u.y == 0) return;
+  const int item = (int)(unit / a.c.kv_heads), kvh = (int)(unit - (int64_t)item * a.c.kv_heads);
+  const CacheTile tile = a.c.tiles[item];
+  const int t = (int)threadIdx.x, team = t / (4 * kLanes), in = t % (4 * kLanes), row4 = in / kLanes, d = 4 * (in % kLanes);
+  const int row = 4 * (int)(block - unit * (4 * NR)) + row4, rr = tile.at + row;
+  const bool there = row < tile.count && rr < tile.n * a.group;
+  float m = kNever;
+  // part p of the unit is its workgroup's last, but for the unit's last part
+  auto place = [&](int p) { return (int64_t)(2 * (u.x + p) + (p + 1 < u.y)) * (16 * NR) + row; };
+  F4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  float sum = 0.0f;
+  if (there) {
+    for (int p = 0; p < u.y; ++p) m = fmaxf(m, a.part_ml[place(p)].x);
+#pragma unroll 4
+    for (int p = team; p < u.y; p += 2) {
+      const float2 x = a.part_ml[place(p)];
+      const F4 v = *reinterpret_cast<const F4*>(a.part_o + place(p) * DP + d);
+      const float f = x.x == kNever && x.y == 0.0f ? 0.0f : exp2_fast(x.x - m);  // (a part that saw nothing: zeros)
+      sum += x.y * f;
+      acc += v * f;
+    }
+  }
+  if (team == 1) {
+    half[in] = acc;
+    if (d == 0) sums[row4] = sum;
+  }
+  __syncthreads();
+  if (team == 1 || !there || d >= a.c.dim) return;
+  acc += half[in];
+  sum += sums[row4];
+  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  const int token = (int)((unsigned)rr / (unsigned)a.group);
+  char* p = const_cast<char*>(a.o.data) + (tile.first + token) * a.o.row + (int64_t)(kvh * a.group + rr - token * a.group) * a.o.head;
+  const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};
+  const V2 f = __builtin_convertvector(x, V2), g = __builtin_convertvector(y, V2);
+  *reinterpret_cast<uint2*>(p + 2 * d) = make_uint2(__builtin_bit_cast(uint32_t, f), __builtin_bit_cast(uint32_t, g));
+}
+
+template <typename T, int TYPE, int DP, int NR>
+hipError_t run_rows(const CacheAttnArgs& a, hipStream_t stream) {
+  const int64_t units = (int64_t)a.c.n_tiles * a.c.kv_heads;
+  if (a.whole)
+    return for_launches(units, 64 * kWaves, [&](int64_t first, unsigned blocks) {
+      sfe_cache_attn_kernel<T, TYPE, DP, NR, true><<<dim3(blocks), dim3(64 * kWaves), 0, stream>>>(a, first);
+      return hipGetLastError();
+    });
+  sfe_cache_attn_kernel<T, TYPE, DP, NR, false><<<dim3((unsigned)a.shares), dim3(64 * kWaves), 0, stream>>>(a, 0);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  return for_launches(units * 4 * NR, 2 * DP, [&](int64_t first, unsigned blocks) {
+    sfe_cache_attn_join_kernel<T, DP, NR><<<dim3(blocks), dim3(2 * DP), 0, stream>>>(a, first);
+    return hipGetLastError();
+  });
 }
 
 template <typename T, int TYPE>
 hipError_t run(const CacheAttnArgs& a, hipStream_t stream) {
-  return for_launches((int64_t)a.c.n_tiles * a.c.kv_heads, 64, [&](int64_t first, unsigned blocks) {
-    sfe_cache_attn_kernel<T, TYPE><<<dim3(blocks), dim3(64), 0, stream>>>(a, first);
-    return hipGetLastError();
-  });
+  if (a.c.dim <= 64) {
+    if (a.tiles == 1) return run_rows<T, TYPE, 64, 1>(a, stream);
+    return a.tiles == 2 ? run_rows<T, TYPE, 64, 2>(a, stream) : run_rows<T, TYPE, 64, 4>(a, stream);
+  }
+  if (a.tiles == 1) return run_rows<T, TYPE, 128, 1>(a, stream);
+  return a.tiles == 2 ? run_rows<T, TYPE, 128, 2>(a, stream) : run_rows<T, TYPE, 128, 4>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_cache_attn(const CacheAttnArgs& a, int type, int dtype, hipStream_t stream) {
   switch (type) {
-    case kCacheBf16: return run<__bf16, kCacheBf16>(a, stream);
-    case kCacheF16: return run<_Float16, kCacheF16>(a, stream);
-    case kCacheE4m3: return dtype == kOpBf16 ? run<__bf16, kCacheE4m3>(a, stream) : run<_Float16, kCacheE4m3>(a, stream);
-    default: return dtype == kOpBf16 ? run<__bf16, kCacheInt8>(a, stream) : run<_Float16, kCacheInt8>(a, stream);
+    case kCacheBf16: return run<Bf, kCacheBf16>(a, stream);
+    case kCacheF16: return run<Hf, kCacheF16>(a, stream);
+    case kCacheE4m3: return dtype == kOpBf16 ? run<Bf, kCacheE4m3>(a, stream) : run<Hf, kCacheE4m3>(a, stream);
+    default: return dtype == kOpBf16 ? run<Bf, kCacheInt8>(a, stream) : run<Hf, kCacheInt8>(a, stream);
   }
 }
 

@@ -29,8 +29,8 @@ struct sfe_cache_plan : sfe::OpPlan {
   ~sfe_cache_plan() { sfe::op_drop(this); }
   int32_t n = 0, heads = 0, kv_heads = 0, dim = 0;
   int64_t rows = 0, longest = 0;  // new tokens, and those of the sequence with the most
-  int32_t n_tiles = 0, n_attn = 0;
-  size_t tiles = 0, attn = 0;  // offsets into buf
+  int32_t n_tiles = 0, n_attn = 0, attn_tiles = 1;  // attn_tiles: tiles of 16 packed rows of an attention's tile
+  size_t tiles = 0, attn = 0, part_o = 0, part_ml = 0, units = 0;  // offsets into buf
 };
 
 namespace {
@@ -250,6 +250,7 @@ int sfe_cache_plan_make(sfe_ctx* ctx, const int64_t* offsets, int32_t n, int32_t
     if ((rc = sfe::check_offsets("offsets", offsets, n))) return rc;
     if (offsets[0] != 0) return op_fail(SFE_INVALID_ARG, "offsets must begin at 0");
     if (offsets[n] > 1 << 24) return op_fail(SFE_INVALID_ARG, "more than 2^24 new tokens");
+    if (offsets[n] * (heads / kv_heads) > 1 << 28) return op_fail(SFE_INVALID_ARG, "more than 2^28 new tokens of grouped heads");
     if (!ctx) return op_fail(SFE_INVALID_ARG, "null context");
     auto plan = std::make_unique<sfe_cache_plan>();
     if ((rc = sfe::op_adopt(ctx, plan.get()))) return rc;
@@ -264,12 +265,15 @@ int sfe_cache_plan_make(sfe_ctx* ctx, const int64_t* offsets, int32_t n, int32_t
       return SFE_OK;
     }
     const int group = heads / kv_heads;
+    plan->attn_tiles = plan->longest * group <= 16 ? 1 : (plan->longest * group <= 32 ? 2 : 4);
+    const int rows = 16 * plan->attn_tiles;
     std::vector<sfe::CacheTile> tiles, attn;
     for (int32_t s = 0; s < n; ++s) {
       const int32_t m = (int32_t)(offsets[s + 1] - offsets[s]);
       for (int32_t at = 0; at < m; at += sfe::kCacheTileTokens)
         tiles.push_back({offsets[s], s, m, at, std::min(sfe::kCacheTileTokens, m - at)});
-      for (int32_t at = 0; at < m * group; at += 16) attn.push_back({offsets[s], s, m, at, std::min(16, m * group - at)});
+      for (int64_t at = 0; at < (int64_t)m * group; at += rows)
+        attn.push_back({offsets[s], s, m, (int32_t)at, (int32_t)std::min<int64_t>(rows, (int64_t)m * group - at)});
     }
     plan->n_tiles = (int32_t)tiles.size();
     plan->n_attn = (int32_t)attn.size();
@@ -277,7 +281,12 @@ int sfe_cache_plan_make(sfe_ctx* ctx, const int64_t* offsets, int32_t n, int32_t
     std::vector<char> table(plan->attn + attn.size() * sizeof(sfe::CacheTile));
     memcpy(table.data(), tiles.data(), tiles.size() * sizeof(sfe::CacheTile));
     memcpy(table.data() + plan->attn, attn.data(), attn.size() * sizeof(sfe::CacheTile));
-    if ((rc = sfe::op_upload(plan.get(), table.data(), table.size(), up(table.size()), static_cast<hipStream_t>(stream)))) return rc;
+    const size_t shares = (size_t)sfe::cache_attn_shares(sfe::op_cus(ctx));
+    plan->part_o = up(table.size());
+    plan->part_ml = plan->part_o + up(2 * shares * rows * sfe::cache_attn_dim(head_dim) * sizeof(float));
+    plan->units = plan->part_ml + up(2 * shares * rows * sizeof(float2));
+    const size_t room = plan->units + up(attn.size() * kv_heads * sizeof(int2));
+    if ((rc = sfe::op_upload(plan.get(), table.data(), table.size(), room, static_cast<hipStream_t>(stream)))) return rc;
     *out = plan.release();
     return SFE_OK;
   });
@@ -311,6 +320,12 @@ int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_
     if (tree && plan->longest > 64) return op_fail(SFE_INVALID_ARG, "a tree has at most 64 new tokens");
     if ((uintptr_t)tree % 8) return op_fail(SFE_INVALID_ARG, "tree must be aligned to 8 bytes");
     if (rows == 0) return SFE_OK;
+    const int64_t keys = (int64_t)tokens->table_pages * cache->page_size;
+    if (keys > sfe::kCacheAttnKeys) return op_fail(SFE_INVALID_ARG, "a page table of more than 2^30 tokens");
+    const int64_t rounds = std::max<int64_t>(1, (keys + sfe::kCacheAttnRound - 1) / sfe::kCacheAttnRound);
+    const int64_t units = (int64_t)plan->n_attn * plan->kv_heads;
+    if (units > (int64_t)1 << 30 || units * rounds > (int64_t)1 << 30)
+      return op_fail(SFE_INVALID_ARG, "batch too large: tiles of new tokens x kv_heads x tokens of a page table must be below 2^37");
     if ((rc = check_heads("q", q, plan->rows, 2, 16))) return rc;
     if ((rc = check_heads("out", out, rows, 2, 16))) return rc;
     if (!apart(*out, rows, plan->heads, plan->dim)) return op_fail(SFE_INVALID_ARG, "out: rows or heads overlap");
@@ -331,21 +346,29 @@ int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_
     x.a.o = tensor_of(out, 2);
     x.a.tree = tree;
     x.a.group = plan->heads / plan->kv_heads;
+    x.a.tiles = plan->attn_tiles;
+    x.a.whole = rounds <= 2;
+    x.a.least = 1;
     x.a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     x.plan = plan;
     x.type = cache->type;
     x.dtype = dtype;
     x.rows = rows;
     x.stream = static_cast<hipStream_t>(stream);
-    return sfe::op_call(plan->ctx, x.stream, "cache attention", [](void* arg, int) -> hipError_t {
+    return sfe::op_call(plan->ctx, x.stream, "cache attention", [](void* arg, int cus) -> hipError_t {
       Call& x = *static_cast<Call*>(arg);
       if (x.rows > x.plan->rows) {
         const hipError_t e = sfe::launch_attn_zero(x.a.o, x.plan->heads, x.plan->dim, 0, x.plan->rows, x.rows, x.stream);
         if (e != hipSuccess) return e;
       }
       if (x.plan->rows == 0) return hipSuccess;
-      x.a.c.tiles = reinterpret_cast<const sfe::CacheTile*>(static_cast<char*>(x.plan->buf) + x.plan->attn);
+      char* base = static_cast<char*>(x.plan->buf);
+      x.a.c.tiles = reinterpret_cast<const sfe::CacheTile*>(base + x.plan->attn);
       x.a.c.n_tiles = x.plan->n_attn;
+      x.a.part_o = reinterpret_cast<float*>(base + x.plan->part_o);
+      x.a.part_ml = reinterpret_cast<float2*>(base + x.plan->part_ml);
+      x.a.units = reinterpret_cast<int2*>(base + x.plan->units);
+      x.a.shares = sfe::cache_attn_shares(cus);
       return sfe::launch_cache_attn(x.a, x.type, x.dtype, x.stream);
     }, &x);
   });

@@ -54,11 +54,20 @@ hipError_t launch_cache_write(const CacheArgs& c, int type, const AttnTensor& k,
 hipError_t launch_cache_read(const CacheArgs& c, int type, const AttnTensor& k, const AttnTensor& v, int dtype, hipStream_t stream);
 
 // ---- attention of new tokens over the cache (sfe_cache_attn.hip) ---------------------------
+// A workgroup's waves, and the keys that they take together; tokens of a page table at most.
+constexpr int kCacheAttnWaves = 4, kCacheAttnRound = 128;
+constexpr int64_t kCacheAttnKeys = (int64_t)1 << 30;
+inline int cache_attn_dim(int dim) { return dim <= 64 ? 64 : 128; }  // padded
+inline int cache_attn_shares(int cus) { return 2 * ((cus + 7) / 8 * 8); }  // workgroups that share a call's rounds
 struct CacheAttnArgs {
-  CacheArgs c;
+  CacheArgs c;  // tiles: of 16 * tiles packed rows (token x head of a group)
   AttnTensor q, o;
   const uint64_t* tree;  // bit j of a row: it sees new token j of its sequence; null: its own and those before
-  int32_t group;
+  float* part_o;    // [2 * shares][tile row][padded dim]
+  float2* part_ml;  // [2 * shares][tile row]: (reference exponent, sum)
+  int2* units;      // [tile][kv head]: the share of its first part, and its parts (0: not cut)
+  int32_t group, tiles, shares, least;  // least: rounds of a share
+  bool whole;       // a workgroup takes a whole unit
   float scale_log2;  // scale * log2(e)
 };
 hipError_t launch_cache_attn(const CacheAttnArgs& a, int type, int dtype, hipStream_t stream);

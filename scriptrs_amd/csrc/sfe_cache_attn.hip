@@ -140,6 +140,38 @@ __device__ __forceinline__ void values_of(uint32_t (&addr)[4], uint32_t at, type
   }
 }
 
+// The lane's operand without its values that are not finite.
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::V8 finite_part(typename Mat<T>::V8 v) {
+  U4 w = __builtin_bit_cast(U4, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bad = ((w[i] & Mat<T>::kExp) + Mat<T>::kCarry) & 0x80008000u;
+    w[i] &= ~((bad >> 15) * 0xffffu);
+  }
+  return __builtin_bit_cast(typename Mat<T>::V8, w);
+}
+
+// Values of a row in LDS that are not finite, of the C channels that it has at `at`: bits of those that are +infinity or NaN,
+// and of those that are -infinity or NaN.
+template <int TYPE, int C>
+__device__ __forceinline__ void not_finite_bits(uint32_t at, uint32_t* up, uint32_t* down) {
+  *up = *down = 0;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    if constexpr (TYPE == kCacheE4m3) {
+      const uint32_t x = lds_read<uint8_t>(at + i);
+      if ((x & 0x7f) == 0x7f) *up |= 1u << i, *down |= 1u << i;
+    } else {
+      constexpr uint32_t e = TYPE == kCacheBf16 ? 0x7f80 : 0x7c00;
+      const uint32_t x = lds_read<uint16_t>(at + 2 * i);
+      const bool bad = (x & e) == e, nan = bad && (x & 0x7fff) != e;
+      if (nan || (bad && !(x & 0x8000))) *up |= 1u << i;
+      if (nan || (bad && (x & 0x8000))) *down |= 1u << i;
+    }
+  }
+}
+
 // The lowest n of 32 bits.
 __device__ __forceinline__ uint32_t low_bits(int64_t n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
 
@@ -220,12 +252,13 @@ __device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* ld
 // WHOLE: a workgroup takes one unit, all of its rounds; otherwise an equal share of all rounds, of
 // which the first and last units may be cut: their parts go to a slot each and are joined by a second launch.
 template <typename T, int TYPE, int DP, int NR, bool WHOLE>
-__global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_kernel(CacheAttnArgs a, int64_t first) {
+__global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 1 : 2) void sfe_cache_attn_kernel(CacheAttnArgs a, int64_t first) {
   typedef Ring<DP, Kept<TYPE>::kSize> R;
   typedef Mat<T> M;
   typedef typename M::V8 V8;
   typedef typename M::V2 V2;
   constexpr bool kCoded = Kept<TYPE>::kSize == 1;
+  constexpr bool kNotFinite = TYPE != kCacheInt8;  // the cache's type has infinities or NaN
   constexpr bool kRelative = kCoded && std::is_same<T, Hf>::value;
   constexpr int E = Kept<TYPE>::kSize, C = DP / 16, S = R::kStages;
   constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
@@ -375,8 +408,10 @@ __global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_k
 
     F4 o[NR][C];
     float m[NR], l[NR], top_scale[NR];
+    uint32_t ups[NR], downs[NR];  // results that get +infinity and -infinity in the end, bits C j + i of o[i][j]
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
+      ups[n] = downs[n] = 0;
       m[n] = kNever, l[n] = 0.0f, top_scale[n] = 0x1p-110f;
 #pragma unroll
       for (int i = 0; i < C; ++i) o[n][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -412,28 +447,63 @@ __global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_k
                           fmaxf(fmaxf(vs[1][0], vs[1][1]), fmaxf(vs[1][2], vs[1][3])));
       // keys that some rows do not see
       const bool uneven = key + kStep > context || now != 0x1010;
+      uint32_t see[NR];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) see[n] = ~0u;
+      if (uneven) {
+        const uint32_t there_bits = low_bits(now & 0xff) | low_bits(now >> 8) << 16;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          see[n] = low_bits(a.tree ? context - key : me[n] + 1 - key);
+          if (a.tree) {
+            const int64_t d = context - key;
+            if (d >= 0) see[n] |= d < 32 ? (uint32_t)(bits[n] << d) : 0;
+            else see[n] |= d > -64 ? (uint32_t)(bits[n] >> -d) : 0;
+          }
+          see[n] &= there_bits;
+          if (!alive[n]) see[n] = 0;
+        }
+        if constexpr (kNotFinite) {
+          // values that are not finite are kept from the rows that do not see them as 0 * inf: they are taken out, and
+          // remembered for the rows that do
+          uint32_t bad = 0;
+#pragma unroll
+          for (int i = 0; i < C; ++i) bad |= nonfinite<T>(v[i]);
+          if (__any(bad != 0)) {
+#pragma unroll 1
+            for (int row = 0; row < kStep; ++row) {
+              uint32_t up = 0, down = 0;
+#pragma unroll 1
+              for (int j = 0; j < 4; ++j) {
+                const int byte = C * E * (4 * quarter + j);
+                uint32_t u, d;
+                not_finite_bits<TYPE, C>(base + in + 2 * R::kHalf + row * R::kPitch + 16 * ((byte / 16) ^ R::swizzle(row & 15)) + byte % 16, &u, &d);
+                up |= u << (C * j), down |= d << (C * j);
+              }
+#pragma unroll
+              for (int n = 0; n < NR; ++n) {
+                const uint32_t mine = 0u - (see[n] >> row & 1);
+                ups[n] |= up & mine, downs[n] |= down & mine;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < C; ++i) v[i] = finite_part<T>(v[i]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) see[n] >>= 4 * quarter;  // the lane's keys are 16 u + 4 quarter + i
+      }
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        uint32_t see = ~0u;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[n][u][i] *= kCoded ? ks[u][i] : a.scale_log2;
-        if (uneven) {
-          see = a.tree ? low_bits(context - key) : low_bits(me[n] + 1 - key);
-          if (a.tree) {
-            const int64_t d = context - key;
-            if (d >= 0) see |= d < 32 ? (uint32_t)(bits[n] << d) : 0;
-            else see |= d > -64 ? (uint32_t)(bits[n] >> -d) : 0;
-          }
-          see &= low_bits(now & 0xff) | low_bits(now >> 8) << 16;
-          if (!alive[n]) see = 0;
-          see >>= 4 * quarter;  // the lane's keys are 16 u + 4 quarter + i
+        if (uneven)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][u][i] = (see >> (16 * u + i)) & 1 ? s[n][u][i] : -INFINITY;
-        }
+            for (int i = 0; i < 4; ++i) s[n][u][i] = (see[n] >> (16 * u + i)) & 1 ? s[n][u][i] : -INFINITY;
         float top = s[n][0][0];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -455,7 +525,7 @@ __global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_k
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) top_seen = (see >> (16 * u + i)) & 1 ? fmaxf(top_seen, vs[u][i]) : top_seen;
+              for (int i = 0; i < 4; ++i) top_seen = (see[n] >> (16 * u + i)) & 1 ? fmaxf(top_seen, vs[u][i]) : top_seen;
           }
           if (__any(top_seen > top_scale[n])) {
             top_seen = max_halves(fmaxf(top_seen, __shfl_xor(top_seen, 16)));
@@ -478,8 +548,8 @@ __global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_k
             if (kCoded) {
               x.x *= kRelative ? vs[u][i] * relative : vs[u][i], x.y *= kRelative ? vs[u][i + 1] * relative : vs[u][i + 1];
               if (uneven) {  // (0 times a scale that is not finite)
-                x.x = (see >> (16 * u + i)) & 1 ? x.x : 0.0f;
-                x.y = (see >> (16 * u + i + 1)) & 1 ? x.y : 0.0f;
+                x.x = (see[n] >> (16 * u + i)) & 1 ? x.x : 0.0f;
+                x.y = (see[n] >> (16 * u + i + 1)) & 1 ? x.y : 0.0f;
               }
             }
             const V2 y = __builtin_convertvector(x, V2);
@@ -487,25 +557,7 @@ __global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_k
             p[4 * u + i + 1] = y.y;
           }
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-          V8 x = v[i];
-          if (uneven && __any(nonfinite<T>(x) != 0)) {  // kept from the rows that do not see it as 0 * inf
-            S8 clean, up, down, seen;
-            split_nonfinite<T>(__builtin_bit_cast(S8, x), &clean, &up, &down);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) seen[j] = (see >> (16 * (j / 4) + j % 4)) & 1 ? M::kOne : 0;
-            const F4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-            const F4 ups = M::m16(__builtin_bit_cast(V8, up), __builtin_bit_cast(V8, seen), zero);
-            const F4 downs = M::m16(__builtin_bit_cast(V8, down), __builtin_bit_cast(V8, seen), zero);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (ups[j] > 0.0f) o[n][i][j] += INFINITY;
-              if (downs[j] > 0.0f) o[n][i][j] -= INFINITY;
-            }
-            x = __builtin_bit_cast(V8, clean);
-          }
-          o[n][i] = M::m16(x, p, o[n][i]);
-        }
+        for (int i = 0; i < C; ++i) o[n][i] = M::m16(v[i], p, o[n][i]);
       }
       // ---- the buffer just read takes the step after those in flight
 #pragma unroll
@@ -524,6 +576,17 @@ __global__ __launch_bounds__(64 * kWaves, NR == 4 ? 1 : 2) void sfe_cache_attn_k
 #pragma unroll
         for (int i = 0; i < C; ++i) o[n][i] *= top_scale[n];
     }
+    if constexpr (kNotFinite)
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+        if (__any((ups[n] | downs[n]) != 0))
+#pragma unroll
+          for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (ups[n] >> (C * j + i) & 1) o[n][i][j] += INFINITY;
+              if (downs[n] >> (C * j + i) & 1) o[n][i][j] -= INFINITY;
+            }
     // ---- the waves' results, added up through LDS, a tile of 16 rows at a time
     const bool cut = !WHOLE && (r0 > 0 || r1 < rounds);
     const int slot = 2 * w + (r1 < rounds);
@@ -654,11 +717,9 @@ hipError_t run_rows(const CacheAttnArgs& a, hipStream_t stream) {
 template <typename T, int TYPE>
 hipError_t run(const CacheAttnArgs& a, hipStream_t stream) {
   if (a.c.dim <= 64) {
-    if (a.tiles == 1) return run_rows<T, TYPE, 64, 1>(a, stream);
-    return a.tiles == 2 ? run_rows<T, TYPE, 64, 2>(a, stream) : run_rows<T, TYPE, 64, 4>(a, stream);
+    return a.tiles == 1 ? run_rows<T, TYPE, 64, 1>(a, stream) : run_rows<T, TYPE, 64, 2>(a, stream);
   }
-  if (a.tiles == 1) return run_rows<T, TYPE, 128, 1>(a, stream);
-  return a.tiles == 2 ? run_rows<T, TYPE, 128, 2>(a, stream) : run_rows<T, TYPE, 128, 4>(a, stream);
+  return a.tiles == 1 ? run_rows<T, TYPE, 128, 1>(a, stream) : run_rows<T, TYPE, 128, 2>(a, stream);
 }
 
 }  // namespace

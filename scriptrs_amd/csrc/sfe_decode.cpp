@@ -265,7 +265,7 @@ int sfe_cache_plan_make(sfe_ctx* ctx, const int64_t* offsets, int32_t n, int32_t
       return SFE_OK;
     }
     const int group = heads / kv_heads;
-    plan->attn_tiles = plan->longest * group <= 16 ? 1 : (plan->longest * group <= 32 ? 2 : 4);
+    plan->attn_tiles = plan->longest * group <= 16 ? 1 : 2;
     const int rows = 16 * plan->attn_tiles;
     std::vector<sfe::CacheTile> tiles, attn;
     for (int32_t s = 0; s < n; ++s) {

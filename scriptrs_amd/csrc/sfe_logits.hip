@@ -35,7 +35,7 @@ template <typename T, int N, int V, bool HISTORY, bool BIAS, bool MASK>
 __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int64_t first, int spans) {
   typedef Vec<T, N> Vector;
   constexpr int kSpan = kThreads * N * V;
-  __shared__ uint32_t counts[HISTORY ? kSpan : 1];
+  __shared__ __align__(16) uint32_t counts[HISTORY ? kSpan : 4];
   const int64_t block = first + blockIdx.x, r = block / spans;
   const int t = (int)threadIdx.x;
   const T* in = reinterpret_cast<const T*>(a.in) + r * a.in_row;
@@ -54,49 +54,96 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
       for (int i = 0; i < N; ++i) x[v].v[i] = at + i >= 0 && at + i < a.vocab ? in[at + i] : (T)0.0f;
     }
   }
-  float rep = 1.0f, presence = 0.0f, frequency = 0.0f;
-  if (HISTORY) {
-    for (int e = t; e < kSpan; e += kThreads) counts[e] = 0;
-    __syncthreads();
-    const int32_t* said = a.history + r * a.history_row;
-    int n = a.history_most;
-    if (a.lengths) n = min(n, a.lengths[r]);
-    for (int e = t; e < n; e += kThreads) {
-      const int32_t token = said[e], at = token - span0;
-      if (token >= 0 && token < a.vocab && at >= 0 && at < kSpan) atomicAdd(counts + at, 1u);
-    }
-    rep = a.repetitions ? a.repetitions[r] : a.repetition;
-    presence = a.presences ? a.presences[r] : a.presence;
-    frequency = a.frequencies ? a.frequencies[r] : a.frequency;
-    __syncthreads();
-  }
   const uint32_t* words = nullptr;
   if (MASK) {
     const int64_t state = a.states ? a.states[r] : r;
     if (state >= 0 && state < a.n_allowed) words = a.allowed + state * a.allowed_row;
   }
+  float bias[V][BIAS ? N : 1];
+  uint32_t bits[V];
+  if (BIAS) {
+    const float* from = a.bias + r * a.bias_row;
+    const bool whole = N > 1 && ((uintptr_t)from / 4 - before) % 4 == 0;  // vectors of 16 bytes
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int at = span0 + (v * kThreads + t) * N;
+      if (whole && at >= 0 && at + N <= a.vocab) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(from + at + i);
+          bias[v][i % N] = b.x, bias[v][(i + 1) % N] = b.y, bias[v][(i + 2) % N] = b.z, bias[v][(i + 3) % N] = b.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) bias[v][i] = at + i >= 0 && at + i < a.vocab ? from[at + i] : 0.0f;
+      }
+    }
+  }
+  if (MASK)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int at = span0 + (v * kThreads + t) * N;
+      bits[v] = ~0u;
+      if (words && at < a.vocab && at + N > 0) bits[v] = at >= 0 ? mask_bits(words, at, N, a.vocab) : words[0] << -at;
+    }
+  float rep = 1.0f, presence = 0.0f, frequency = 0.0f;
+  if (HISTORY) {
+    const int32_t* said = a.history + r * a.history_row;
+    int n = a.history_most;
+    if (a.lengths) n = min(n, a.lengths[r]);
+    rep = a.repetitions ? a.repetitions[r] : a.repetition;
+    presence = a.presences ? a.presences[r] : a.presence;
+    frequency = a.frequencies ? a.frequencies[r] : a.frequency;
+    constexpr int kAhead = 4;  // tokens of a thread in flight
+    int32_t token[kAhead];
+    auto tokens = [&](int e) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) token[i] = e + i * kThreads < n ? said[e + i * kThreads] : -1;
+    };
+    tokens(t);
+    for (int e = 4 * t; e < kSpan; e += 4 * kThreads) *reinterpret_cast<uint4*>(counts + e) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int e = t; e < n; e += kAhead * kThreads) {
+      int32_t now[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) now[i] = token[i];
+      tokens(e + kAhead * kThreads);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int at = now[i] - span0;
+        if (now[i] >= 0 && now[i] < a.vocab && at >= 0 && at < kSpan) atomicAdd(counts + at, 1u);
+      }
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int place = (v * kThreads + t) * N, at = span0 + place;
     if (at >= a.vocab || at + N <= 0) continue;
-    const bool whole = at >= 0 && at + N <= a.vocab;
-    const uint32_t bits = !MASK || !words ? ~0u : (at >= 0 ? mask_bits(words, at, N, a.vocab) : words[0] << -at);
+    float z[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = (float)x[v].v[i];
+    if (HISTORY) {
+      uint32_t c[N], any = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) c[i] = counts[place + i], any |= c[i];
+      if (any) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (c[i]) {
+            z[i] = z[i] > 0.0f ? z[i] / rep : z[i] * rep;
+            z[i] -= presence + frequency * (float)c[i];
+          }
+      }
+    }
     Vector y;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float z = (float)x[v].v[i];
-      if (HISTORY) {
-        const uint32_t c = counts[place + i];
-        if (c) {
-          z = z > 0.0f ? z / rep : z * rep;
-          z -= presence + frequency * (float)c;
-        }
-      }
-      if (BIAS && (whole || (at + i >= 0 && at + i < a.vocab))) z += a.bias[r * a.bias_row + at + i];
-      if (MASK) z = bits >> i & 1 ? z : -INFINITY;
-      y.v[i] = (T)z;
+      if (BIAS) z[i] += bias[v][i];
+      if (MASK) z[i] = bits[v] >> i & 1 ? z[i] : -INFINITY;
+      y.v[i] = (T)z[i];
     }
-    if (N > 1 && whole) {
+    if (N > 1 && at >= 0 && at + N <= a.vocab) {
       *reinterpret_cast<Vector*>(out + at) = y;
     } else {
 #pragma unroll

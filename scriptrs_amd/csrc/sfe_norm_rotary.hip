@@ -21,158 +21,188 @@ namespace sfe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTable = 4096;  // (cosine, sine) of a workgroup's rows and pairs
+constexpr int kTable = 4096;  // (cosine, sine) of a workgroup's rows and pairs at most
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
 
-// Sum over groups of `lanes` lanes, a power of two; every lane has it, of the same order.
-__device__ __forceinline__ float group_sum(float x, int lanes) {
-  if (lanes > 1) x += dpp<0xb1>(x);   // the other of 2
-  if (lanes > 2) x += dpp<0x4e>(x);   // the other two of 4
-  if (lanes > 4) x += dpp<0x141>(x);  // mirrored within 8
-  if (lanes > 8) x += dpp<0x140>(x);  // mirrored within 16
-  if (lanes > 16) x += __shfl_xor(x, 16);
-  if (lanes > 32) x += __shfl_xor(x, 32);
-  return x;
+// Sums of K values over groups of `lanes` lanes, a power of two; every lane has them, of the same order.
+template <int K>
+__device__ __forceinline__ void group_sums(float (&x)[K], int lanes) {
+  if (lanes > 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] += dpp<0xb1>(x[k]);  // the other of 2
+  if (lanes > 2)
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] += dpp<0x4e>(x[k]);  // the other two of 4
+  if (lanes > 4)
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] += dpp<0x141>(x[k]);  // mirrored within 8
+  if (lanes > 8)
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] += dpp<0x140>(x[k]);  // mirrored within 16
+  if (lanes > 16)
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] += __shfl_xor(x[k], 16);
+  if (lanes > 32)
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] += __shfl_xor(x[k], 32);
 }
 
-// A workgroup takes `heads` consecutive heads of the rows' q and k heads, laid end to end, K a
-// lane group.  N: channels of a vector; N = 1: a unit is a pair or a channel that does not turn, U of them a lane.
+// A workgroup takes K times `per` rows.  Places of a row: `lanes` for each of its heads, q's then k's; a thread
+// keeps its place in K rows (so that what depends on the place is computed once), all K loads
+// issued before the first store and before the rows' sines and cosines go into LDS.  Rows of more than 256 places
+// go in `chunks` workgroups.  N: channels of a vector; N = 1: a unit is a pair or a channel that does not
+// turn, U of them a lane.
 template <typename T, int N, bool INTERLEAVED, bool LAYER, int K, int U>
-__global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArgs a, int64_t first, int heads, int lanes,
-                                                                   int slots) {
+__global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArgs a, int64_t first, int places, int lanes,
+                                                                   int slots, int chunks, int per) {
   constexpr bool kOne = INTERLEAVED && N > 1;  // both channels of a pair in one vector
   constexpr int kPairs = kOne ? N / 2 : N;     // of a unit
   typedef Vec<T, N> V;
-  __shared__ float2 table[kTable];
-  __shared__ float weights[2][kNormRotaryMaxDim];
-  const int t = (int)threadIdx.x, pairs = a.rotary / 2, in_row = a.t[0].heads + a.t[1].heads;
-  const int groups = kThreads / lanes, group = t / lanes, lane = t - group * lanes;
-  // (workgroups count heads, rows of them: 64 bits)
-  const int64_t head0 = first + (int64_t)blockIdx.x * heads, row0 = head0 / in_row;
-  const int skip = (int)(head0 - row0 * in_row);
-  const int64_t left = a.rows * in_row - head0;
-  const int mine = left < heads ? (int)left : heads;
+  extern __shared__ float2 table[];
+  const int t = (int)threadIdx.x, pairs = a.rotary / 2;
+  const uint32_t group = blockIdx.x / (uint32_t)chunks, chunk = blockIdx.x - group * (uint32_t)chunks;
+  const int64_t row0 = first + (int64_t)group * K * per;
+  const int rows = (int)(a.rows - row0 < K * per ? a.rows - row0 : K * per);
+  const int in = per > 1 ? (int)((unsigned)t / (unsigned)places) : 0;  // row within a pass
+  const int place = per > 1 ? t - in * places : (int)chunk * (int)blockDim.x + t;
+  const bool mine = place < places && in < per;  // (all lanes of a head, or none)
+  const int head = (int)((unsigned)place / (unsigned)lanes), lane = place - head * lanes;
+  const bool second = head >= a.t[0].heads;
+  const int of = second ? head - a.t[0].heads : head;
+  const int64_t x_row = second ? a.t[1].x_row : a.t[0].x_row, y_row = second ? a.t[1].y_row : a.t[0].y_row;
+  const T* x = reinterpret_cast<const T*>(second ? a.t[1].x : a.t[0].x) + (row0 + in) * x_row + of * (second ? a.t[1].x_head : a.t[0].x_head);
+  T* y = reinterpret_cast<T*>(second ? a.t[1].y : a.t[0].y) + (row0 + in) * y_row + of * (second ? a.t[1].y_head : a.t[0].y_head);
+  const float* weight = second ? a.weight[1] : a.weight[0];
 
   V p[K][U], q[K][U];
-  bool second[K];
-  T* y[K];
-  int local[K];
+  float w0[U][N], w1[U][N];
+  int d0[U], d1[U];
+  bool turn[U];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int h = group + k * groups;
-    local[k] = -1;
-    if (h >= mine) continue;
-    const int r = (int)((unsigned)(skip + h) / (unsigned)in_row), head = skip + h - r * in_row;
-    local[k] = r;
-    second[k] = head >= a.t[0].heads;
-    const RotaryTensor& tn = a.t[second[k]];
-    const int of = second[k] ? head - a.t[0].heads : head;
-    const T* x = reinterpret_cast<const T*>(tn.x) + (row0 + r) * tn.x_row + of * tn.x_head;
-    y[k] = reinterpret_cast<T*>(tn.y) + (row0 + r) * tn.y_row + of * tn.y_head;
+  for (int u = 0; u < U; ++u) {
+    const int slot = lane + u * lanes;
+    turn[u] = slot < pairs / kPairs;
+    d0[u] = turn[u] ? slot * (INTERLEAVED ? 2 * kPairs : kPairs) : a.rotary + N * (slot - pairs / kPairs);
+    d1[u] = INTERLEAVED ? d0[u] + 1 : d0[u] + pairs;
+    if (slot >= slots || !mine) d0[u] = -1;  // (no channels)
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int slot = lane + u * lanes;
-      const bool turn = slot < pairs / kPairs;
-      const int d0 = turn ? slot * (INTERLEAVED ? 2 * kPairs : kPairs) : a.rotary + N * (slot - pairs / kPairs);
-      const int d1 = INTERLEAVED ? d0 + 1 : d0 + pairs;
       p[k][u] = q[k][u] = V{};
-      if (slot < slots) {
-        p[k][u] = *reinterpret_cast<const V*>(x + d0);
-        if (!kOne && turn) q[k][u] = *reinterpret_cast<const V*>(x + d1);
+      if (d0[u] >= 0 && in + k * per < rows) {
+        p[k][u] = *reinterpret_cast<const V*>(x + k * (int64_t)per * x_row + d0[u]);
+        if (!kOne && turn[u]) q[k][u] = *reinterpret_cast<const V*>(x + k * (int64_t)per * x_row + d1[u]);
       }
     }
-  }
-  // sines and cosines of the rows, and the weights, while the heads are on their way
-  const int rows = (int)((unsigned)(skip + mine - 1) / (unsigned)in_row) + 1;
-  for (int e = t; e < rows * pairs; e += kThreads) {
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w0[u][i] = weight && d0[u] >= 0 ? weight[d0[u] + i] : 1.0f;
+      w1[u][i] = weight && d0[u] >= 0 && turn[u] && !kOne ? weight[d1[u] + i] : 1.0f;
+    }
+  // sines and cosines of the rows, while the heads are on their way
+  for (int e = t; e < rows * pairs; e += (int)blockDim.x) {
     const int r = (int)((unsigned)e / (unsigned)pairs), i = e - r * pairs;
     float c, s;
     turn_cos_sin((uint32_t)(((uint64_t)(int64_t)a.positions[row0 + r] * a.step[i]) >> 32), &c, &s);
     table[e] = make_float2(a.magnitude * c, a.magnitude * s);
   }
-  for (int e = t; e < a.dim; e += kThreads) {
-    weights[0][e] = a.weight[0] ? a.weight[0][e] : 1.0f;
-    weights[1][e] = a.weight[1] ? a.weight[1][e] : 1.0f;
-  }
   __syncthreads();
+  if (!mine) return;
   const float over = 1.0f / (float)a.dim;
+  float e[K][U][N], f[K][U][N], sum[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    // (a group's lanes agree; those of a wave may not, and sums take all that are there)
-    float e[U][N], f[U][N], sum = 0.0f;
+    sum[k] = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        e[u][i] = local[k] < 0 ? 0.0f : (float)p[k][u].v[i];
-        f[u][i] = local[k] < 0 || kOne ? 0.0f : (float)q[k][u].v[i];
-        sum += e[u][i] + f[u][i];
+        e[k][u][i] = (float)p[k][u].v[i];
+        f[k][u][i] = kOne ? 0.0f : (float)q[k][u].v[i];
+        if (LAYER) sum[k] += kOne ? e[k][u][i] : e[k][u][i] + f[k][u][i];
       }
-    const float mean = LAYER ? group_sum(sum, lanes) * over : 0.0f;
-    float square = 0.0f;
+  }
+  if (LAYER) {
+    group_sums<K>(sum, lanes);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int slot = lane + u * lanes;
-      const bool in = slot < slots, turn = slot < pairs / kPairs;
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // (places that hold no channel stay zero)
+        const float mean = sum[k] * over, me = d0[u] >= 0 ? mean : 0.0f, mf = d0[u] >= 0 && turn[u] ? mean : 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          e[k][u][i] -= me;
+          if (!kOne) f[k][u][i] -= mf;
+        }
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    sum[k] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (LAYER) {  // (places that hold no channel stay zero)
-          e[u][i] = in ? e[u][i] - mean : 0.0f;
-          f[u][i] = in && turn && !kOne ? f[u][i] - mean : 0.0f;
-        }
-        square = __builtin_fmaf(e[u][i], e[u][i], square);
-        if (!kOne) square = __builtin_fmaf(f[u][i], f[u][i], square);
+        sum[k] = __builtin_fmaf(e[k][u][i], e[k][u][i], sum[k]);
+        if (!kOne) sum[k] = __builtin_fmaf(f[k][u][i], f[k][u][i], sum[k]);
       }
-    }
-    const float inv = 1.0f / sqrtf(group_sum(square, lanes) * over + a.eps);
-    if (local[k] < 0) continue;
-    const float* w = weights[second[k]];
+  }
+  group_sums<K>(sum, lanes);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (in + k * per >= rows) continue;
+    const float inv = 1.0f / sqrtf(sum[k] * over + a.eps);
+    T* yk = y + k * (int64_t)per * y_row;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int slot = lane + u * lanes;
-      if (slot >= slots) continue;
-      const bool turn = slot < pairs / kPairs;
-      const int d0 = turn ? slot * (INTERLEAVED ? 2 * kPairs : kPairs) : a.rotary + N * (slot - pairs / kPairs);
-      const int d1 = INTERLEAVED ? d0 + 1 : d0 + pairs;
+      if (d0[u] < 0) continue;
       V r, s;
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[u][i] *= inv * w[d0 + i];
-      if (!turn) {
+      for (int i = 0; i < N; ++i) e[k][u][i] *= inv * w0[u][i];
+      if (!turn[u]) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) r.v[i] = (T)e[u][i];
-        *reinterpret_cast<V*>(y[k] + d0) = r;
+        for (int i = 0; i < N; ++i) r.v[i] = (T)e[k][u][i];
+        *reinterpret_cast<V*>(yk + d0[u]) = r;
         continue;
       }
-      const float2* cs = table + local[k] * pairs + slot * kPairs;
+      const float2* cs = table + (in + k * per) * pairs + (lane + u * lanes) * kPairs;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        const float x0 = e[u][kOne ? (2 * i) % N : i];
-        const float x1 = kOne ? e[u][(2 * i + 1) % N] : f[u][i] * (inv * w[d1 + i]);
+        const float x0 = e[k][u][kOne ? (2 * i) % N : i];
+        const float x1 = kOne ? e[k][u][(2 * i + 1) % N] : f[k][u][i] * (inv * w1[u][i]);
         const T y0 = (T)__builtin_fmaf(x0, cs[i].x, -x1 * cs[i].y), y1 = (T)__builtin_fmaf(x1, cs[i].x, x0 * cs[i].y);
         r.v[kOne ? (2 * i) % N : i] = y0;
         if (kOne) r.v[(2 * i + 1) % N] = y1;
         else s.v[i] = y1;
       }
-      *reinterpret_cast<V*>(y[k] + d0) = r;
-      if (!kOne) *reinterpret_cast<V*>(y[k] + d1) = s;
+      *reinterpret_cast<V*>(yk + d0[u]) = r;
+      if (!kOne) *reinterpret_cast<V*>(yk + d1[u]) = s;
     }
   }
 }
 
 template <typename T, int N, bool INTERLEAVED, bool LAYER, int K, int U>
-hipError_t run_heads(const NormRotaryArgs& a, int lanes, int slots, hipStream_t stream) {
-  const int in_row = a.t[0].heads + a.t[1].heads, pairs = a.rotary / 2;
-  // as many heads as the lane groups take at K each, of rows that the table has room for
-  const int heads = (int)std::min<int64_t>(K * (kThreads / lanes), ((int64_t)(kTable / pairs) - 1) * in_row);
-  const int64_t total = a.rows * in_row, step = (int64_t)heads << 22;  // (launches of at most 2^22 workgroups)
-  for (int64_t first = 0; first < total; first += step) {
-    const int64_t n = std::min(step, total - first);
-    sfe_norm_rotary_kernel<T, N, INTERLEAVED, LAYER, K, U><<<dim3((unsigned)((n + heads - 1) / heads)), dim3(kThreads), 0, stream>>>(
-        a, first, heads, lanes, slots);
+hipError_t run_rows(const NormRotaryArgs& a, int lanes, int slots, hipStream_t stream) {
+  const int places = (a.t[0].heads + a.t[1].heads) * lanes, pairs = a.rotary / 2;
+  const int chunks = (places + kThreads - 1) / kThreads;
+  const int per = chunks > 1 ? 1 : std::max(1, std::min(kThreads / places, kTable / (K * pairs)));
+  // whole waves, as few as hold the places (a head's lanes never cross a chunk: both are powers of two of a wave)
+  const int threads = ((chunks > 1 ? (places + chunks - 1) / chunks : places * per) + 63) / 64 * 64;
+  const size_t lds = (size_t)K * per * pairs * sizeof(float2);
+  // (launches of at most 2^22 workgroups)
+  const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 22) / chunks) * K * per;
+  for (int64_t first = 0; first < a.rows; first += step) {
+    const int64_t rows = std::min(step, a.rows - first);
+    const unsigned blocks = (unsigned)((rows + K * per - 1) / (K * per) * chunks);
+    sfe_norm_rotary_kernel<T, N, INTERLEAVED, LAYER, K, U><<<dim3(blocks), dim3(threads), lds, stream>>>(a, first, places, lanes, slots, chunks, per);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -184,13 +214,13 @@ hipError_t run_units(const NormRotaryArgs& a, int slots, int cus, hipStream_t st
   int lanes = 1;
   while (lanes < slots && lanes < 64) lanes *= 2;
   if constexpr (N == 1) {
-    return run_heads<T, N, INTERLEAVED, LAYER, 1, kNormRotaryMaxDim / 64>(a, lanes, slots, stream);
+    return run_rows<T, N, INTERLEAVED, LAYER, 1, kNormRotaryMaxDim / 64>(a, lanes, slots, stream);
   } else {
-    // One head a lane group while the machine is not full at 4.
-    const int64_t heads = a.rows * (a.t[0].heads + a.t[1].heads);
-    const bool many = heads * lanes >= (int64_t)cus * 8 * kThreads * 4;
-    return many ? run_heads<T, N, INTERLEAVED, LAYER, 4, 1>(a, lanes, slots, stream)
-                : run_heads<T, N, INTERLEAVED, LAYER, 1, 1>(a, lanes, slots, stream);
+    // One row a thread while the machine is not full at 4.
+    const int64_t places = a.rows * (a.t[0].heads + a.t[1].heads) * lanes;
+    const bool many = places >= (int64_t)cus * 8 * kThreads * 4;
+    return many ? run_rows<T, N, INTERLEAVED, LAYER, 4, 1>(a, lanes, slots, stream)
+                : run_rows<T, N, INTERLEAVED, LAYER, 1, 1>(a, lanes, slots, stream);
   }
 }
 

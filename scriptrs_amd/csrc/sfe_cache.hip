@@ -47,12 +47,13 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t top, flo
   }
   top = max(top, 0x0f800000u);  // 2^-96
   *scale = __uint_as_float(top) / M;
-  const int e = (int)(top >> 23) - 127;
+  // M over the power of two of the largest (from 2^-96 up: no more than 2^105, no less than 2^-121)
+  const float c = __builtin_amdgcn_ldexpf(M, 127 - (int)(top >> 23));
   const float a = __uint_as_float((top & 0x7fffffu) | 0x3f800000u), r = 1.0f / a;
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float n = __builtin_amdgcn_ldexpf(x[i], -e) * M;
+    const float n = x[i] * c;
     const float guess = n * r;
     y[i] = __builtin_fmaf(__builtin_fmaf(-guess, a, n), r, guess);
   }
@@ -63,9 +64,11 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t top, flo
       int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
       w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], p, true);
     } else {
-      w[i] = 0;
+      // (1.5 * 2^23 more: the sum is rounded to a whole number, its low byte the code)
+      uint32_t b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[i] |= ((uint32_t)(int)__builtin_rintf(y[4 * i + j]) & 0xffu) << (8 * j);
+      for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(y[4 * i + j] + 12582912.0f);
+      w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), 0x05040100);
     }
   }
   return make_uint2(w[0], w[1]);
@@ -91,6 +94,7 @@ __device__ __forceinline__ float code_value(uint2 w, int i) {
 // channels each.
 struct Place {
   int64_t row;      // packed
+  int64_t token;    // of its sequence
   int64_t page;     // or -1
   int32_t slot, kvh;
   bool value, in;   // V; whether the lane has channels
@@ -103,9 +107,9 @@ __device__ __forceinline__ Place place_of(const CacheArgs& c, const CacheTile& t
   p.kvh = p.value ? part - c.kv_heads : part;
   p.in = token < tile.count && channel < c.dim;
   p.row = tile.first + tile.at + token;
-  const int64_t at = (int64_t)length - tile.n + tile.at + token;
-  p.page = p.in ? page_of(c, tile.seq, at) : -1;
-  p.slot = (int)(at & ((1 << c.shift) - 1));
+  p.token = (int64_t)length - tile.n + tile.at + token;
+  p.page = -1;
+  p.slot = (int)(p.token & ((1 << c.shift) - 1));
   return p;
 }
 template <int TYPE>
@@ -130,9 +134,12 @@ __global__ __launch_bounds__(kThreads) void sfe_cache_write_kernel(CacheArgs c, 
   for (int j = 0; j < kUnits; ++j) {
     p[j] = place_of(c, tile, unit0 + j * groups, channel, length);
     x[j] = Eight<T>{};
-    const AttnTensor& from = p[j].value ? v : k;
-    if (p[j].in) x[j] = *reinterpret_cast<const Eight<T>*>(from.data + p[j].row * from.row + p[j].kvh * from.head + (int64_t)sizeof(T) * channel);
+    const char* from = p[j].value ? v.data + p[j].row * v.row + p[j].kvh * v.head : k.data + p[j].row * k.row + p[j].kvh * k.head;
+    if (p[j].in) x[j] = *reinterpret_cast<const Eight<T>*>(from + (int64_t)sizeof(T) * channel);
   }
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j)
+    if (p[j].in) p[j].page = page_of(c, tile.seq, p[j].token);
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {
     float f[8];
@@ -173,7 +180,10 @@ __global__ __launch_bounds__(kThreads) void sfe_cache_read_kernel(CacheArgs c, A
   uint4 w[kUnits];
   float s[kUnits];
 #pragma unroll
-  for (int j = 0; j < kUnits; ++j) p[j] = place_of(c, tile, unit0 + j * groups, channel, length);
+  for (int j = 0; j < kUnits; ++j) {
+    p[j] = place_of(c, tile, unit0 + j * groups, channel, length);
+    if (p[j].in) p[j].page = page_of(c, tile.seq, p[j].token);
+  }
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {
     w[j] = make_uint4(0, 0, 0, 0);
@@ -202,8 +212,8 @@ __global__ __launch_bounds__(kThreads) void sfe_cache_read_kernel(CacheArgs c, A
 #pragma unroll
       for (int i = 0; i < 8; ++i) y.v[i] = (T)(float)x.v[i];
     }
-    const AttnTensor& to = p[j].value ? v : k;
-    *reinterpret_cast<Eight<T>*>(const_cast<char*>(to.data) + p[j].row * to.row + p[j].kvh * to.head + (int64_t)sizeof(T) * channel) = y;
+    const char* to = p[j].value ? v.data + p[j].row * v.row + p[j].kvh * v.head : k.data + p[j].row * k.row + p[j].kvh * k.head;
+    *reinterpret_cast<Eight<T>*>(const_cast<char*>(to) + (int64_t)sizeof(T) * channel) = y;
   }
 }
 

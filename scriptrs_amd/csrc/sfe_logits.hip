@@ -29,13 +29,17 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int t, int 
   return bits;
 }
 
+// Waits for the workgroup's LDS accesses, not for its loads.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // N: elements of a vector (16 bytes, or one); V: vectors of a thread.  Vectors begin at multiples of 16 bytes:
 // the first of a row may begin up to N - 1 elements before it.
-template <typename T, int N, int V, bool HISTORY, bool BIAS, bool MASK>
+// H: bytes of a count, 0 without a history.
+template <typename T, int N, int V, int H, bool BIAS, bool MASK>
 __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int64_t first, int spans) {
   typedef Vec<T, N> Vector;
   constexpr int kSpan = kThreads * N * V;
-  __shared__ __align__(16) uint32_t counts[HISTORY ? kSpan : 4];
+  __shared__ __align__(16) uint32_t counts[H ? kSpan * H / 4 : 4];
   const int64_t block = first + blockIdx.x, r = block / spans;
   const int t = (int)threadIdx.x;
   const T* in = reinterpret_cast<const T*>(a.in) + r * a.in_row;
@@ -43,6 +47,23 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
   const int before = N > 1 ? (int)((uintptr_t)in / sizeof(T) % N) : 0;
   const int span0 = (int)(block - r * spans) * kSpan - before;  // first token of the span
 
+  // ---- all loads, those of the history first
+  int n = 0;
+  float rep = 1.0f, over = 1.0f, presence = 0.0f, frequency = 0.0f;
+  const int32_t* said = a.history + (H ? r * a.history_row : 0);
+  constexpr int kAhead = 4;  // tokens of a thread in flight
+  int32_t token[kAhead];
+  auto tokens = [&](int e) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) token[i] = e + i * kThreads < a.history_most ? said[e + i * kThreads] : -1;
+  };
+  if (H) {
+    tokens(t);
+    n = a.lengths ? min(a.lengths[r], a.history_most) : a.history_most;
+    rep = a.repetitions ? a.repetitions[r] : a.repetition;
+    presence = a.presences ? a.presences[r] : a.presence;
+    frequency = a.frequencies ? a.frequencies[r] : a.frequency;
+  }
   Vector x[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -86,35 +107,26 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
       bits[v] = ~0u;
       if (words && at < a.vocab && at + N > 0) bits[v] = at >= 0 ? mask_bits(words, at, N, a.vocab) : words[0] << -at;
     }
-  float rep = 1.0f, presence = 0.0f, frequency = 0.0f;
-  if (HISTORY) {
-    const int32_t* said = a.history + r * a.history_row;
-    int n = a.history_most;
-    if (a.lengths) n = min(n, a.lengths[r]);
-    rep = a.repetitions ? a.repetitions[r] : a.repetition;
-    presence = a.presences ? a.presences[r] : a.presence;
-    frequency = a.frequencies ? a.frequencies[r] : a.frequency;
-    constexpr int kAhead = 4;  // tokens of a thread in flight
-    int32_t token[kAhead];
-    auto tokens = [&](int e) {
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) token[i] = e + i * kThreads < n ? said[e + i * kThreads] : -1;
-    };
-    tokens(t);
-    for (int e = 4 * t; e < kSpan; e += 4 * kThreads) *reinterpret_cast<uint4*>(counts + e) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    for (int e = t; e < n; e += kAhead * kThreads) {
+  // ---- the history's tokens of the span, counted in LDS
+  if (H) {
+    for (int e = 4 * t; e < kSpan * H / 4; e += 4 * kThreads) *reinterpret_cast<uint4*>(counts + e) = make_uint4(0, 0, 0, 0);
+    over = 1.0f / rep;
+    lds_barrier();
+    for (int e = t; e < n;) {
       int32_t now[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) now[i] = token[i];
-      tokens(e + kAhead * kThreads);
+      for (int i = 0; i < kAhead; ++i) now[i] = e + i * kThreads < n ? token[i] : -1;
+      e += kAhead * kThreads;
+      tokens(e);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int at = now[i] - span0;
-        if (now[i] >= 0 && now[i] < a.vocab && at >= 0 && at < kSpan) atomicAdd(counts + at, 1u);
+        if (now[i] < 0 || now[i] >= a.vocab || at < 0 || at >= kSpan) continue;
+        if (H == 2) atomicAdd(counts + at / 2, at & 1 ? 0x10000u : 1u);
+        else atomicAdd(counts + at, 1u);
       }
     }
-    __syncthreads();
+    lds_barrier();
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -123,24 +135,33 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
     float z[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) z[i] = (float)x[v].v[i];
-    if (HISTORY) {
-      uint32_t c[N], any = 0;
+    if (H) {
+      constexpr int kWords = N * H < 4 ? 1 : N * H / 4;
+      uint32_t c[kWords], any = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) c[i] = counts[place + i], any |= c[i];
+      for (int i = 0; i < kWords; ++i) c[i] = counts[place * H / 4 + i], any |= c[i];
+      if (N == 1 && H == 2) any = c[0] = place & 1 ? c[0] >> 16 : c[0] & 0xffffu;
       if (any) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (c[i]) {
-            z[i] = z[i] > 0.0f ? z[i] / rep : z[i] * rep;
-            z[i] -= presence + frequency * (float)c[i];
-          }
+        for (int i = 0; i < N; ++i) {
+          const uint32_t count = H == 2 ? (i % 2 ? c[i / 2] >> 16 : c[i / 2] & 0xffffu) : c[i];
+          // the quotient by its reciprocal, corrected by the remainder (none of an infinity)
+          float y = z[i] * over;
+          const float left = __builtin_fmaf(-y, rep, z[i]);
+          y = left == left ? __builtin_fmaf(left, over, y) : y;
+          y = (z[i] > 0.0f ? y : z[i] * rep) - (presence + frequency * (float)count);
+          z[i] = count ? y : z[i];
+        }
       }
     }
     Vector y;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (BIAS) z[i] += bias[v][i];
-      if (MASK) z[i] = bits[v] >> i & 1 ? z[i] : -INFINITY;
+      if (MASK) {  // (as whole numbers: two operations)
+        const uint32_t m = (uint32_t)((int32_t)(bits[v] << (31 - i)) >> 31);
+        z[i] = __uint_as_float((__float_as_uint(z[i]) & m) | (0xff800000u & ~m));
+      }
       y.v[i] = (T)z[i];
     }
     if (N > 1 && at >= 0 && at + N <= a.vocab) {
@@ -153,29 +174,27 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
   }
 }
 
-template <typename T, int N, int V, bool HISTORY, bool BIAS, bool MASK>
+template <typename T, int N, int V, int H, bool BIAS, bool MASK>
 hipError_t run(const LogitsArgs& a, hipStream_t stream) {
   constexpr int kSpan = kThreads * N * V;
   const int spans = (int)(((int64_t)a.vocab + (N - 1) + kSpan - 1) / kSpan);
   return for_launches((int64_t)a.rows * spans, kThreads, [&](int64_t first, unsigned blocks) {
-    sfe_logits_kernel<T, N, V, HISTORY, BIAS, MASK><<<dim3(blocks), dim3(kThreads), 0, stream>>>(a, first, spans);
+    sfe_logits_kernel<T, N, V, H, BIAS, MASK><<<dim3(blocks), dim3(kThreads), 0, stream>>>(a, first, spans);
     return hipGetLastError();
   });
 }
 
-template <typename T, int N, int V>
+template <typename T, int N, int V, int H>
 hipError_t run_what(const LogitsArgs& a, hipStream_t stream) {
-  const int what = (a.history ? 4 : 0) | (a.bias ? 2 : 0) | (a.allowed ? 1 : 0);
-  switch (what) {
-    case 0: return run<T, N, V, false, false, false>(a, stream);
-    case 1: return run<T, N, V, false, false, true>(a, stream);
-    case 2: return run<T, N, V, false, true, false>(a, stream);
-    case 3: return run<T, N, V, false, true, true>(a, stream);
-    case 4: return run<T, N, V, true, false, false>(a, stream);
-    case 5: return run<T, N, V, true, false, true>(a, stream);
-    case 6: return run<T, N, V, true, true, false>(a, stream);
-    default: return run<T, N, V, true, true, true>(a, stream);
-  }
+  if (a.bias) return a.allowed ? run<T, N, V, H, true, true>(a, stream) : run<T, N, V, H, true, false>(a, stream);
+  return a.allowed ? run<T, N, V, H, false, true>(a, stream) : run<T, N, V, H, false, false>(a, stream);
+}
+
+template <typename T, int N, int V>
+hipError_t run_history(const LogitsArgs& a, hipStream_t stream) {
+  if (!a.history) return run_what<T, N, V, 0>(a, stream);
+  // counts of 16 bits where they hold a whole history
+  return a.history_most < 65536 ? run_what<T, N, V, 2>(a, stream) : run_what<T, N, V, 4>(a, stream);
 }
 
 template <typename T>
@@ -183,7 +202,7 @@ hipError_t run_type(const LogitsArgs& a, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
   // vectors where a row's input and output lie alike
   const bool alike = (uintptr_t)a.in % 16 == (uintptr_t)a.out % 16 && (a.in_row - a.out_row) % N == 0;
-  return alike ? run_what<T, N, 4>(a, stream) : run_what<T, 1, 4>(a, stream);
+  return alike ? run_history<T, N, 4>(a, stream) : run_history<T, 1, 4>(a, stream);
 }
 
 }  // namespace

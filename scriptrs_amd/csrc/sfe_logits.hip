@@ -186,7 +186,8 @@ hipError_t run(const LogitsArgs& a, hipStream_t stream) {
 
 template <typename T, int N, int V, int H>
 hipError_t run_what(const LogitsArgs& a, hipStream_t stream) {
-  if (a.bias) return a.allowed ? run<T, N, V, H, true, true>(a, stream) : run<T, N, V, H, true, false>(a, stream);
+  // (half the vectors where biases take as many registers again)
+  if (a.bias) return a.allowed ? run<T, N, V / 2, H, true, true>(a, stream) : run<T, N, V / 2, H, true, false>(a, stream);
   return a.allowed ? run<T, N, V, H, false, true>(a, stream) : run<T, N, V, H, false, false>(a, stream);
 }
 

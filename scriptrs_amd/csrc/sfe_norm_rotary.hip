@@ -54,8 +54,8 @@ __device__ __forceinline__ void group_sums(float (&x)[K], int lanes) {
 // A workgroup takes K times `per` rows.  Places of a row: `lanes` for each of its heads, q's then k's; a thread
 // keeps its place in K rows (so that what depends on the place is computed once), all K loads
 // issued before the first store and before the rows' sines and cosines go into LDS.  Rows of more than 256 places
-// go in `chunks` workgroups.  N: channels of a vector; N = 1: a unit is a pair or a channel that does not
-// turn, U of them a lane.
+// go in `chunks` workgroups.  N: channels of a vector; a lane's unit is one or two vectors (two of those that do not
+// turn as well), N = 1: one or two channels, U units a lane.
 template <typename T, int N, bool INTERLEAVED, bool LAYER, int K, int U>
 __global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArgs a, int64_t first, int places, int lanes,
                                                                    int slots, int chunks, int per) {
@@ -81,15 +81,26 @@ __global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArg
   V p[K][U], q[K][U];
   float w0[U][N], w1[U][N];
   int d0[U], d1[U];
-  bool turn[U];
+  bool turn[U], both[U];  // (both: the second vector is there too)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int slot = lane + u * lanes;
-    turn[u] = slot < pairs / kPairs;
-    d0[u] = turn[u] ? slot * (INTERLEAVED ? 2 * kPairs : kPairs) : a.rotary + N * (slot - pairs / kPairs);
-    d1[u] = INTERLEAVED ? d0[u] + 1 : d0[u] + pairs;
+    const int slot = lane + u * lanes, rest = slot - pairs / kPairs;
+    turn[u] = rest < 0;
+    d0[u] = turn[u] ? slot * (INTERLEAVED ? 2 * kPairs : kPairs) : a.rotary + (kOne ? N : 2 * N) * rest;
+    d1[u] = turn[u] ? (INTERLEAVED ? d0[u] + 1 : d0[u] + pairs) : d0[u] + N;
     if (slot >= slots || !mine) d0[u] = -1;  // (no channels)
+    both[u] = !kOne && d0[u] >= 0 && d1[u] < a.dim;
   }
+  // what the table and the products need is asked for first, so that waiting for it is not waiting for the heads
+  const int my_row = (int)((unsigned)t / (unsigned)pairs);
+  const int32_t position = t < rows * pairs ? a.positions[row0 + my_row] : 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w0[u][i] = weight && d0[u] >= 0 ? weight[d0[u] + i] : 1.0f;
+      w1[u][i] = weight && both[u] ? weight[d1[u] + i] : 1.0f;
+    }
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -97,24 +108,22 @@ __global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArg
       p[k][u] = q[k][u] = V{};
       if (d0[u] >= 0 && in + k * per < rows) {
         p[k][u] = *reinterpret_cast<const V*>(x + k * (int64_t)per * x_row + d0[u]);
-        if (!kOne && turn[u]) q[k][u] = *reinterpret_cast<const V*>(x + k * (int64_t)per * x_row + d1[u]);
+        if (!kOne && both[u]) q[k][u] = *reinterpret_cast<const V*>(x + k * (int64_t)per * x_row + d1[u]);
       }
     }
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      w0[u][i] = weight && d0[u] >= 0 ? weight[d0[u] + i] : 1.0f;
-      w1[u][i] = weight && d0[u] >= 0 && turn[u] && !kOne ? weight[d1[u] + i] : 1.0f;
-    }
   // sines and cosines of the rows, while the heads are on their way
-  for (int e = t; e < rows * pairs; e += (int)blockDim.x) {
-    const int r = (int)((unsigned)e / (unsigned)pairs), i = e - r * pairs;
+  auto turned = [&](int e, int r, int32_t at) {
     float c, s;
-    turn_cos_sin((uint32_t)(((uint64_t)(int64_t)a.positions[row0 + r] * a.step[i]) >> 32), &c, &s);
+    turn_cos_sin((uint32_t)(((uint64_t)(int64_t)at * a.step[e - r * pairs]) >> 32), &c, &s);
     table[e] = make_float2(a.magnitude * c, a.magnitude * s);
+  };
+  if (t < rows * pairs) turned(t, my_row, position);
+  for (int e = t + (int)blockDim.x; e < rows * pairs; e += (int)blockDim.x) {
+    const int r = (int)((unsigned)e / (unsigned)pairs);
+    turned(e, r, a.positions[row0 + r]);
   }
-  __syncthreads();
+  // (the workgroup's LDS is waited for, and not its loads)
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   if (!mine) return;
   const float over = 1.0f / (float)a.dim;
   float e[K][U][N], f[K][U][N], sum[K];
@@ -136,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArg
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int u = 0; u < U; ++u) {  // (places that hold no channel stay zero)
-        const float mean = sum[k] * over, me = d0[u] >= 0 ? mean : 0.0f, mf = d0[u] >= 0 && turn[u] ? mean : 0.0f;
+        const float mean = sum[k] * over, me = d0[u] >= 0 ? mean : 0.0f, mf = both[u] ? mean : 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           e[k][u][i] -= me;
@@ -169,8 +178,9 @@ __global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArg
       for (int i = 0; i < N; ++i) e[k][u][i] *= inv * w0[u][i];
       if (!turn[u]) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) r.v[i] = (T)e[k][u][i];
+        for (int i = 0; i < N; ++i) r.v[i] = (T)e[k][u][i], s.v[i] = (T)(f[k][u][i] * (inv * w1[u][i]));
         *reinterpret_cast<V*>(yk + d0[u]) = r;
+        if (both[u]) *reinterpret_cast<V*>(yk + d1[u]) = s;
         continue;
       }
       const float2* cs = table + (in + k * per) * pairs + (lane + u * lanes) * kPairs;
@@ -237,8 +247,9 @@ bool vectors(const NormRotaryArgs& a) {
 
 template <typename T, int N, bool INTERLEAVED>
 int slots_of(const NormRotaryArgs& a) {
-  const int pairs = INTERLEAVED && N > 1 ? N / 2 : N;
-  return a.rotary / 2 / pairs + (a.dim - a.rotary) / N;
+  const bool one = INTERLEAVED && N > 1;
+  const int pairs = one ? N / 2 : N, copied = one ? N : 2 * N;
+  return a.rotary / 2 / pairs + (a.dim - a.rotary + copied - 1) / copied;
 }
 
 template <typename T, bool INTERLEAVED, bool LAYER>

@@ -41,6 +41,8 @@ __device__ __forceinline__ I4 buffer(uint64_t at, int bytes) {
   r.w = kBufWord3;
   return r;
 }
+// Waits for the workgroup's LDS accesses, not for its loads.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <typename V>
 __device__ __forceinline__ V lds_read(uint32_t at) {
   return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
@@ -53,7 +55,6 @@ struct Ring {
   static constexpr int kHalf = 16 * kPitch;                      // 16 rows of K, or of V
   static constexpr int kScales = 4 * kHalf;                      // then 256 bytes of scales for each half
   static constexpr int kBytes = kScales + (E == 1 ? 512 : 0);    // a step: K, V, scales
-  static constexpr int kStages = 2;
   static constexpr int kLoads = 2 * (2 * (kHalf / 1024) + (E == 1 ? 1 : 0));  // of a step
   static __device__ int swizzle(int row) { return kChunks == 16 ? row & 15 : (kChunks == 8 ? row & 7 : (row >> 1) & 3); }
 };
@@ -173,23 +174,23 @@ __device__ __forceinline__ void not_finite_bits(uint32_t at, uint32_t* up, uint3
 }
 
 // The lowest n of 32 bits.
-__device__ __forceinline__ uint32_t low_bits(int64_t n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
 
 // What an item needs of its sequence's keys: those before `end`, in rounds.
 struct Span {
-  int64_t context;  // tokens before the new ones (negative: the first new tokens are none)
+  int context;  // tokens before the new ones (negative: the first new tokens are none)
   int end, rounds;
 };
 __device__ __forceinline__ Span span_of(const CacheAttnArgs& a, const CacheTile& t) {
   Span s;
   const int length = a.c.lengths[t.seq];
-  s.context = (int64_t)length - t.n;
-  int64_t end = length;
+  s.context = (length > 0 ? length : 0) - t.n;
+  int end = s.context + t.n;
   if (!a.tree) end = s.context + (t.at + t.count - 1) / a.group + 1;
-  const int64_t cap = (int64_t)a.c.table_pages << a.c.shift;
+  const int cap = a.c.table_pages << a.c.shift;
   end = end < cap ? end : cap;
-  s.end = (int)(end < 0 ? 0 : end);
-  s.rounds = s.end > 0 ? (int)(((int64_t)s.end + kRound - 1) / kRound) : 1;
+  s.end = end < 0 ? 0 : end;
+  s.rounds = s.end > 0 ? (s.end - 1) / kRound + 1 : 1;
   return s;
 }
 
@@ -251,6 +252,7 @@ __device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* ld
 // T: the queries' type; NR: tiles of 16 packed rows of an item.
 // WHOLE: a workgroup takes one unit, all of its rounds; otherwise an equal share of all rounds, of
 // which the first and last units may be cut: their parts go to a slot each and are joined by a second launch.
+// The first loads of a share's next unit are in flight while the waves add their results of one up.
 template <typename T, int TYPE, int DP, int NR, bool WHOLE>
 __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 1 : 2) void sfe_cache_attn_kernel(CacheAttnArgs a, int64_t first) {
   typedef Ring<DP, Kept<TYPE>::kSize> R;
@@ -260,14 +262,16 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   constexpr bool kCoded = Kept<TYPE>::kSize == 1;
   constexpr bool kNotFinite = TYPE != kCacheInt8;  // the cache's type has infinities or NaN
   constexpr bool kRelative = kCoded && std::is_same<T, Hf>::value;
-  constexpr int E = Kept<TYPE>::kSize, C = DP / 16, S = R::kStages;
+  constexpr int E = Kept<TYPE>::kSize, C = DP / 16;
   constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
-  constexpr int kRing = kWaves * S * R::kBytes, kJoin = 4 * (kWaves * 16 * kRowF + 2 * kWaves * 16);
-  __shared__ __align__(1024) char lds[kRing > kJoin ? kRing : kJoin];
+  constexpr int kStage = kWaves * R::kBytes;  // two stages, each of all waves
+  __shared__ __align__(1024) char lds[2 * kStage];
   __shared__ int lds_start[kWaves + 2];
+  // the waves' results go where the second stage is
+  static_assert(4 * (kWaves * 16 * kRowF + 2 * kWaves * 16) <= kStage, "results fit a stage");
   const CacheArgs& c = a.c;
   const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), quarter = lane >> 4;
-  const uint32_t base = lds_address(lds) + wave * S * R::kBytes;
+  const uint32_t base = lds_address(lds) + wave * R::kBytes;
 
   // ---- addresses that stay
   uint32_t k_addr[4], v_addr[4];
@@ -289,121 +293,123 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   const uint32_t part = (uint32_t)(c.dim * E) << c.shift;  // bytes of a record's K, and V
 
   // ---- the workgroup's share
-  int64_t at, stop;  // rounds (WHOLE: of its one unit)
-  int item, before, share = 0, w = 0;
-  typedef const __attribute__((address_space(4))) CacheTile* Tiles;
-  const Tiles tiles = (Tiles)(uintptr_t)c.tiles;
-  CacheTile tile;
-  auto tile_at = [&](int i) {
-    const Tiles p = tiles + i;
+  int at = 0, stop = 1;  // rounds (WHOLE: one unit)
+  int before = 0, share = 0, w = 0;
+  // a unit, and the rounds of it that are the workgroup's
+  struct Unit {
+    int64_t first;
+    int seq, n, at, count, total;
+    int item, kvh, rounds, end, context, r0, r1;
+  } u;
+  auto unit_of = [&](int item, int kvh) {  // (but its rounds)
+    typedef const __attribute__((address_space(4))) CacheTile* Tiles;
+    const Tiles p = (Tiles)(uintptr_t)c.tiles + __builtin_amdgcn_readfirstlane(item);
+    CacheTile tile;
     tile.first = p->first, tile.seq = p->seq, tile.n = p->n, tile.at = p->at, tile.count = p->count;
+    const Span s = span_of(a, tile);
+    Unit x;
+    x.first = tile.first, x.seq = tile.seq, x.n = tile.n, x.at = tile.at, x.count = tile.count, x.total = tile.n * a.group;
+    x.item = item, x.kvh = kvh;
+    x.rounds = __builtin_amdgcn_readfirstlane(s.rounds), x.end = __builtin_amdgcn_readfirstlane(s.end);
+    x.context = __builtin_amdgcn_readfirstlane(s.context);
+    x.r0 = 0, x.r1 = x.rounds;
+    return x;
   };
-  int kvh0 = 0;
   if (WHOLE) {
     const int64_t unit = first + blockIdx.x;
-    item = (int)(unit / c.kv_heads);
-    kvh0 = (int)(unit - (int64_t)item * c.kv_heads);
-    at = before = 0;
-    stop = 1;
+    const int item = (int)(unit / c.kv_heads);
+    u = unit_of(item, (int)(unit - (int64_t)item * c.kv_heads));
   } else {
     // consecutive workgroups go to the 8 XCDs in turn: each has a contiguous part of the shares
     w = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
     const Start s = start_of(a, w, lds_start, &share, a.least);
-    at = (int64_t)w * share;
+    if ((int64_t)w * share >= s.total) return;
+    at = w * share;
     stop = at + share < s.total ? at + share : s.total;
-    if (at >= stop) return;
-    item = s.item;
     before = s.before;
+    u = unit_of(s.item, 0);
+    u.kvh = (int)((unsigned)(at - before) / (unsigned)u.rounds);
+    u.r0 = at - before - u.kvh * u.rounds;
+    u.r1 = u.rounds - u.r0 < stop - at ? u.rounds : u.r0 + (stop - at);
   }
-  while (at < stop) {
-    tile_at(__builtin_amdgcn_readfirstlane(item));
-    const Span sp = span_of(a, tile);
-    const int rounds = __builtin_amdgcn_readfirstlane(sp.rounds), end = __builtin_amdgcn_readfirstlane(sp.end);
-    const int64_t context = sp.context;
-    int kvh, r0, r1;
-    if (WHOLE) {
-      kvh = kvh0, r0 = 0, r1 = rounds;
-    } else {
-      const int in = (int)(at - before);
-      kvh = __builtin_amdgcn_readfirstlane((int)((unsigned)in / (unsigned)rounds));
-      r0 = in - kvh * rounds;
-      r1 = (int)(rounds - r0 < stop - at ? rounds : r0 + (stop - at));
-    }
-    const int32_t* pages = c.table + (int64_t)tile.seq * c.table_row;
+
+  // the pages of a step's halves (-1: none)
+  auto look_up = [&](const Unit& x, int r, int (&page)[2]) {
     typedef const __attribute__((address_space(4))) int32_t* Pages;
-    // the pages of a step's halves (-1: none)
-    auto look_up = [&](int r, int (&page)[2]) {
-      const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+    const Pages pages = (Pages)(uintptr_t)c.table + (int64_t)x.seq * c.table_row;
+    const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        page[h] = -1;
-        if (key + 16 * h < end) page[h] = ((Pages)(uintptr_t)pages)[(key + 16 * h) >> c.shift];
-      }
-    };
-    // a step's loads; the keys of either half that there are
-    auto load_step = [&](int r, int stage, const int (&page)[2]) {
-      const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
-      int there = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool ok = page[h] >= 0 && page[h] < c.pages && key + 16 * h < end;
-        const int n = ok ? (end - key - 16 * h < 16 ? end - key - 16 * h : 16) : 0;
-        there |= n << (8 * h);
-        const uint64_t record = (uint64_t)(uintptr_t)c.data + (uint64_t)((int64_t)(ok ? page[h] : 0) * c.kv_heads + kvh) * (uint64_t)c.record;
-        const int slot = (key + 16 * h) & page_mask, bytes = n * c.dim * E;
-        const I4 kb = buffer(record + (uint32_t)(slot * c.dim * E), bytes);
-        const I4 vb = buffer(record + part + (uint32_t)(slot * c.dim * E), bytes);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * R::kBytes + h * R::kHalf);
-#pragma unroll
-        for (int i = 0; i < kRowLoads; ++i) load_lds(kb, from[i], to + i * 1024);
-#pragma unroll
-        for (int i = 0; i < kRowLoads; ++i) load_lds(vb, from[i], to + 2 * R::kHalf + i * 1024);
-        if (kCoded) {
-          const I4 sb = buffer(record + 2 * part + 4 * slot, n ? 4 * (page_mask + 1) + 4 * n : 0);
-          const int l = lane & 15;
-          const uint32_t off = lane < 32 && l < n ? (uint32_t)(4 * l + (lane < 16 ? 0 : 4 * (page_mask + 1))) : kOutside;
-          load_lds_word(sb, off, __builtin_amdgcn_readfirstlane(base + stage * R::kBytes + R::kScales + h * 256));
-        }
-      }
-      return there;
-    };
-    int page[2], there[S];
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      look_up(r0 + s < r1 ? r0 + s : r1 - 1, page);
-      if (r0 + s >= r1) page[0] = page[1] = -1;
-      there[s] = load_step(r0 + s, s, page);
+    for (int h = 0; h < 2; ++h) {
+      page[h] = -1;
+      if (r < x.r1 && key + 16 * h < x.end) page[h] = pages[(key + 16 * h) >> c.shift];
     }
-    // ---- the queries, behind the first loads
-    const int total = tile.n * a.group;
-    V8 q[NR][DP / 32];
-    uint64_t bits[NR];
-    bool alive[NR];
-    int64_t me[NR];
+  };
+  // a step's loads; returns the keys of either half that there are
+  auto load_step = [&](const Unit& x, int r, int stage, const int (&page)[2]) {
+    const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+    int there = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool ok = page[h] >= 0 && page[h] < c.pages;
+      const int left = x.end - key - 16 * h, n = ok ? (left < 16 ? left : 16) : 0;
+      there |= n << (8 * h);
+      const uint64_t record = (uint64_t)(uintptr_t)c.data + (uint64_t)((int64_t)(ok ? page[h] : 0) * c.kv_heads + x.kvh) * (uint64_t)c.record;
+      const int slot = (key + 16 * h) & page_mask, bytes = n * c.dim * E;
+      const I4 kb = buffer(record + (uint32_t)(slot * c.dim * E), bytes);
+      const I4 vb = buffer(record + part + (uint32_t)(slot * c.dim * E), bytes);
+      const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * kStage + h * R::kHalf);
+#pragma unroll
+      for (int i = 0; i < kRowLoads; ++i) load_lds(kb, from[i], to + i * 1024);
+#pragma unroll
+      for (int i = 0; i < kRowLoads; ++i) load_lds(vb, from[i], to + 2 * R::kHalf + i * 1024);
+      if (kCoded) {
+        const I4 sb = buffer(record + 2 * part + 4 * slot, n ? 4 * (page_mask + 1) + 4 * n : 0);
+        const int l = lane & 15;
+        const uint32_t off = lane < 32 && l < n ? (uint32_t)(4 * l + (lane < 16 ? 0 : 4 * (page_mask + 1))) : kOutside;
+        load_lds_word(sb, off, __builtin_amdgcn_readfirstlane(base + stage * kStage + R::kScales + h * 256));
+      }
+    }
+    return there;
+  };
+  V8 q[NR][DP / 32];
+  uint64_t bits[NR];
+  int me[NR];  // the row's own place
+  auto load_queries = [&](const Unit& x) {
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const int row = tile.at + 16 * n + (lane & 15), rc = row < total ? row : total - 1;
-      const int token = (int)((unsigned)rc / (unsigned)a.group), head = kvh * a.group + rc - token * a.group;
-      const char* p = a.q.data + (tile.first + token) * a.q.row + head * a.q.head;
+      const int row = x.at + 16 * n + (lane & 15), rc = row < x.total ? row : x.total - 1;
+      const int token = (int)((unsigned)rc / (unsigned)a.group), head = x.kvh * a.group + rc - token * a.group;
+      const char* p = a.q.data + (x.first + token) * a.q.row + head * a.q.head;
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
         const int channel = E == 2 ? 32 * i + 8 * quarter : 64 * (i / 2) + 16 * quarter + 8 * (i % 2);
-        S8 x = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (channel < c.dim) x = *reinterpret_cast<const S8*>(p + 2 * channel);
-        q[n][i] = __builtin_bit_cast(V8, x);
+        S8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (channel < c.dim) v = *reinterpret_cast<const S8*>(p + 2 * channel);
+        q[n][i] = __builtin_bit_cast(V8, v);
       }
-      me[n] = context + token;
-      alive[n] = me[n] >= 0;
-      bits[n] = a.tree ? a.tree[tile.first + token] : 0;
-      if (tile.n < 64) bits[n] &= (1ull << tile.n) - 1;
+      me[n] = x.context + token;
+      bits[n] = a.tree ? a.tree[x.first + token] : 0;
     }
-    look_up(r0 + S < r1 ? r0 + S : r1 - 1, page);
-    // (waited for here: a wait within the loop would be one for the loads into LDS too)
+  };
+  int page[2], page_next[2], there, there_next = 0;
+  look_up(u, u.r0, page);
+  look_up(u, u.r0 + 1, page_next);
+  there = load_step(u, u.r0, 0, page);
+  load_queries(u);
+
+  for (;;) {
+    const int context = u.context, r0 = u.r0, r1 = u.r1;
+    // the queries and the first step, waited for here: a wait for the queries within the loop would be one for its loads into LDS
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) asm volatile("" : "+v"(q[n][i]));
+      if (u.n < 64) bits[n] &= (1ull << u.n) - 1;
       asm volatile("" : "+v"(bits[n]));
+    }
+    if (r0 + 1 < r1) {
+      there_next = load_step(u, r0 + 1, 1, page_next);
+      look_up(u, r0 + 2, page);
     }
 
     F4 o[NR][C];
@@ -416,12 +422,13 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
       for (int i = 0; i < C; ++i) o[n][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    int stage = 0;
+    uint32_t in = 0;  // the step's stage
     for (int r = r0; r < r1; ++r) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * R::kLoads) : "memory");
-      const uint32_t in = stage * R::kBytes;
-      const int64_t key = (int64_t)(r * kWaves + wave) * kStep;
-      const int now = there[0];
+      if (r + 1 < r1)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R::kLoads) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const int key = (r * kWaves + wave) * kStep, now = there;
       // ---- scores
       F4 s[NR][2], ks[2], vs[2];
 #pragma unroll
@@ -456,12 +463,12 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         for (int n = 0; n < NR; ++n) {
           see[n] = low_bits(a.tree ? context - key : me[n] + 1 - key);
           if (a.tree) {
-            const int64_t d = context - key;
+            const int d = context - key;
             if (d >= 0) see[n] |= d < 32 ? (uint32_t)(bits[n] << d) : 0;
             else see[n] |= d > -64 ? (uint32_t)(bits[n] >> -d) : 0;
           }
           see[n] &= there_bits;
-          if (!alive[n]) see[n] = 0;
+          if (me[n] < 0) see[n] = 0;
         }
         if constexpr (kNotFinite) {
           // values that are not finite are kept from the rows that do not see them as 0 * inf: they are taken out, and
@@ -559,14 +566,14 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
         for (int i = 0; i < C; ++i) o[n][i] = M::m16(v[i], p, o[n][i]);
       }
-      // ---- the buffer just read takes the step after those in flight
-#pragma unroll
-      for (int i = 0; i + 1 < S; ++i) there[i] = there[i + 1];
-      if (r + S >= r1) page[0] = page[1] = -1;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      there[S - 1] = load_step(r + S, stage, page);
-      look_up(r + S + 1 < r1 ? r + S + 1 : r1 - 1, page);
-      stage = stage + 1 == S ? 0 : stage + 1;
+      // ---- the buffer just read takes the step after the next
+      there = there_next;
+      if (r + 2 < r1) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        there_next = load_step(u, r + 2, in ? 1 : 0, page);
+        look_up(u, r + 3, page);
+      }
+      in ^= kStage;
     }
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -587,16 +594,34 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
               if (ups[n] >> (C * j + i) & 1) o[n][i][j] += INFINITY;
               if (downs[n] >> (C * j + i) & 1) o[n][i][j] -= INFINITY;
             }
+    // ---- the next unit's first loads
+    const Unit done = u;
+    at += r1 - r0;
+    const bool more = !WHOLE && at < stop;
+    if (more) {
+      if (done.kvh == c.kv_heads - 1) {
+        before += done.rounds * c.kv_heads;
+        u = unit_of(done.item + 1, 0);
+      } else {
+        u.kvh = done.kvh + 1;
+      }
+      u.r0 = 0;
+      u.r1 = u.rounds < stop - at ? u.rounds : stop - at;
+      look_up(u, 0, page);
+      look_up(u, 1, page_next);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      there = load_step(u, 0, 0, page);
+      load_queries(u);
+    }
     // ---- the waves' results, added up through LDS, a tile of 16 rows at a time
-    const bool cut = !WHOLE && (r0 > 0 || r1 < rounds);
-    const int slot = 2 * w + (r1 < rounds);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    float* ow = reinterpret_cast<float*>(lds);                          // [wave][16][kRowF]
+    const bool cut = !WHOLE && (r0 > 0 || r1 < done.rounds);
+    const int slot = 2 * w + (r1 < done.rounds);
+    float* ow = reinterpret_cast<float*>(lds + kStage);                 // [wave][16][kRowF]
     float2* ml = reinterpret_cast<float2*>(ow + kWaves * 16 * kRowF);   // [wave][16]
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      if (16 * n >= tile.count) break;
-      __syncthreads();
+      if (16 * n >= done.count) break;
+      lds_barrier();
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -604,9 +629,10 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
           *reinterpret_cast<F4*>(ow + (wave * 16 + (lane & 15)) * kRowF + C * (4 * quarter + j) + i) =
               F4{o[n][i][j], o[n][i + 1][j], o[n][i + 2][j], o[n][i + 3][j]};
       if (quarter == 0) ml[wave * 16 + lane] = make_float2(m[n], l[n]);
-      __syncthreads();
+      lds_barrier();
       for (int e = t; e < 16 * (DP / 4); e += 64 * kWaves) {
         const int row = e / (DP / 4), d = 4 * (e % (DP / 4));
+        if (16 * n + row >= done.count || d >= c.dim) continue;
         float mm = kNever;
 #pragma unroll
         for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, ml[v * 16 + row].x);
@@ -620,15 +646,15 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
           sum += x.y * f;
           acc += *reinterpret_cast<const F4*>(ow + (v * 16 + row) * kRowF + d) * f;
         }
-        const int rr = tile.at + 16 * n + row;
+        const int rr = done.at + 16 * n + row;
         if (cut) {
           const int64_t place = (int64_t)slot * (16 * NR) + 16 * n + row;
           *reinterpret_cast<F4*>(a.part_o + place * DP + d) = acc;
           if (d == 0) a.part_ml[place] = make_float2(mm, sum);
-        } else if (rr < total && d < c.dim) {
+        } else {
           const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;  // (a row that sees nothing is zero)
           const int token = (int)((unsigned)rr / (unsigned)a.group);
-          char* p = const_cast<char*>(a.o.data) + (tile.first + token) * a.o.row + (int64_t)(kvh * a.group + rr - token * a.group) * a.o.head;
+          char* p = const_cast<char*>(a.o.data) + (done.first + token) * a.o.row + (int64_t)(done.kvh * a.group + rr - token * a.group) * a.o.head;
           const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};
           const V2 f = __builtin_convertvector(x, V2), g = __builtin_convertvector(y, V2);
           *reinterpret_cast<uint2*>(p + 2 * d) = make_uint2(__builtin_bit_cast(uint32_t, f), __builtin_bit_cast(uint32_t, g));
@@ -638,59 +664,64 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     if (WHOLE) return;
     if (t == 0 && r0 == 0) {
       // what the join needs: the workgroup of the unit's first part, and how many parts
-      const int64_t last = (at + rounds - 1) / share;
-      a.units[(int64_t)item * c.kv_heads + kvh] = make_int2(w, cut ? (int)(last - w + 1) : 0);
+      const int last = (at - (r1 - r0) + done.rounds - 1) / share;
+      a.units[(int64_t)done.item * c.kv_heads + done.kvh] = make_int2(w, cut ? last - w + 1 : 0);
     }
-    __syncthreads();  // (the next unit's loads go where the results lie)
-    at += r1 - r0;
-    if (r1 == rounds && kvh == c.kv_heads - 1) {
-      ++item;
-      before += rounds * c.kv_heads;
-    }
+    if (!more) return;
+    lds_barrier();  // (the second stage is the loads' again)
   }
 }
 
-// Parts of units that were cut, added up: a workgroup takes 4 rows of a unit, two teams every other part.
+// Parts of units that were cut, added up: a workgroup takes 4 rows of a unit, each of its teams every
+// kTeams-th part with a reference exponent of its own.
 template <typename T, int DP, int NR>
-__global__ __launch_bounds__(2 * DP) void sfe_cache_attn_join_kernel(CacheAttnArgs a, int64_t first) {
+__global__ __launch_bounds__(512) void sfe_cache_attn_join_kernel(CacheAttnArgs a, int64_t first, int groups) {
   typedef typename Mat<T>::V2 V2;
-  constexpr int kLanes = DP / 4;  // of a row
-  __shared__ F4 half[4 * kLanes];
-  __shared__ float sums[4];
-  const int64_t block = first + blockIdx.x, unit = block / (4 * NR);
+  constexpr int kLanes = DP / 4, kTeams = 512 / (4 * kLanes);  // lanes of a row
+  __shared__ F4 sums[kTeams][4 * kLanes];
+  __shared__ float2 ml[kTeams][4];
+  const int64_t block = first + blockIdx.x, unit = block / groups;
   const int2 u = a.units[unit];
   if (u.y == 0) return;
   const int item = (int)(unit / a.c.kv_heads), kvh = (int)(unit - (int64_t)item * a.c.kv_heads);
   const CacheTile tile = a.c.tiles[item];
   const int t = (int)threadIdx.x, team = t / (4 * kLanes), in = t % (4 * kLanes), row4 = in / kLanes, d = 4 * (in % kLanes);
-  const int row = 4 * (int)(block - unit * (4 * NR)) + row4, rr = tile.at + row;
-  const bool there = row < tile.count && rr < tile.n * a.group;
-  float m = kNever;
+  const int row = 4 * (int)(block - unit * groups) + row4;
+  const bool there = row < tile.count && d < a.c.dim;
   // part p of the unit is its workgroup's last, but for the unit's last part
   auto place = [&](int p) { return (int64_t)(2 * (u.x + p) + (p + 1 < u.y)) * (16 * NR) + row; };
   F4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  float sum = 0.0f;
-  if (there) {
-    for (int p = 0; p < u.y; ++p) m = fmaxf(m, a.part_ml[place(p)].x);
+  float sum = 0.0f, m = kNever;
+  if (there)
 #pragma unroll 4
-    for (int p = team; p < u.y; p += 2) {
+    for (int p = team; p < u.y; p += kTeams) {
       const float2 x = a.part_ml[place(p)];
       const F4 v = *reinterpret_cast<const F4*>(a.part_o + place(p) * DP + d);
-      const float f = x.x == kNever && x.y == 0.0f ? 0.0f : exp2_fast(x.x - m);  // (a part that saw nothing: zeros)
-      sum += x.y * f;
-      acc += v * f;
+      if (x.x == kNever && x.y == 0.0f) continue;  // (saw nothing)
+      const float nm = fmaxf(m, x.x), f = exp2_fast(m - nm), g = exp2_fast(x.x - nm);
+      m = nm;
+      sum = sum * f + x.y * g;
+      acc = acc * f + v * g;
     }
-  }
-  if (team == 1) {
-    half[in] = acc;
-    if (d == 0) sums[row4] = sum;
-  }
+  sums[team][in] = acc;
+  if (d == 0) ml[team][row4] = make_float2(m, sum);
   __syncthreads();
-  if (team == 1 || !there || d >= a.c.dim) return;
-  acc += half[in];
-  sum += sums[row4];
+  if (team > 0 || !there) return;
+  float top = kNever;
+#pragma unroll
+  for (int v = 0; v < kTeams; ++v) top = fmaxf(top, ml[v][row4].x);
+  acc = F4{0.0f, 0.0f, 0.0f, 0.0f};
+  sum = 0.0f;
+#pragma unroll
+  for (int v = 0; v < kTeams; ++v) {
+    const float2 x = ml[v][row4];
+    if (x.x == kNever && x.y == 0.0f) continue;
+    const float f = exp2_fast(x.x - top);
+    sum += x.y * f;
+    acc += sums[v][in] * f;
+  }
   const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-  const int token = (int)((unsigned)rr / (unsigned)a.group);
+  const int rr = tile.at + row, token = (int)((unsigned)rr / (unsigned)a.group);
   char* p = const_cast<char*>(a.o.data) + (tile.first + token) * a.o.row + (int64_t)(kvh * a.group + rr - token * a.group) * a.o.head;
   const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};
   const V2 f = __builtin_convertvector(x, V2), g = __builtin_convertvector(y, V2);
@@ -708,8 +739,9 @@ hipError_t run_rows(const CacheAttnArgs& a, hipStream_t stream) {
   sfe_cache_attn_kernel<T, TYPE, DP, NR, false><<<dim3((unsigned)a.shares), dim3(64 * kWaves), 0, stream>>>(a, 0);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  return for_launches(units * 4 * NR, 2 * DP, [&](int64_t first, unsigned blocks) {
-    sfe_cache_attn_join_kernel<T, DP, NR><<<dim3(blocks), dim3(2 * DP), 0, stream>>>(a, first);
+  const int groups = (a.rows + 3) / 4;
+  return for_launches(units * groups, 512, [&](int64_t first, unsigned blocks) {
+    sfe_cache_attn_join_kernel<T, DP, NR><<<dim3(blocks), dim3(512), 0, stream>>>(a, first, groups);
     return hipGetLastError();
   });
 }

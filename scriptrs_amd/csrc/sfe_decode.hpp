@@ -66,7 +66,7 @@ struct CacheAttnArgs {
   float* part_o;    // [2 * shares][tile row][padded dim]
   float2* part_ml;  // [2 * shares][tile row]: (reference exponent, sum)
   int2* units;      // [tile][kv head]: the share of its first part, and its parts (0: not cut)
-  int32_t group, tiles, shares, least;  // least: rounds of a share
+  int32_t group, tiles, rows, shares, least;  // rows: of a tile at most; least: rounds of a share
   bool whole;       // a workgroup takes a whole unit
   float scale_log2;  // scale * log2(e)
 };

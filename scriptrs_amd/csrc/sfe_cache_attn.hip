@@ -62,27 +62,34 @@ struct Ring {
 typedef uint32_t U2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
-// Codes as 16-bit values, two a word.
+// Two e4m3 codes as 16-bit values.
 template <typename T, int TYPE, int WORD>
 __device__ __forceinline__ uint32_t pair_of(uint32_t x) {
-  if constexpr (TYPE == kCacheE4m3) {
-    if constexpr (std::is_same<T, Bf>::value)
-      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, WORD != 0));
-    else
-      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, WORD != 0));
-  } else {
-    const float a = (float)(int8_t)(x >> (16 * WORD)), b = (float)(int8_t)(x >> (16 * WORD + 8));
-    if constexpr (std::is_same<T, Bf>::value)  // (8 bits: the lower half of the f32 is zero)
-      return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
-    else
-      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-  }
+  if constexpr (std::is_same<T, Bf>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, WORD != 0));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, WORD != 0));
 }
+// An int8 code of each of two words as 16-bit values.
+template <typename T, int BYTE>
+__device__ __forceinline__ uint32_t whole_pair(uint32_t x, uint32_t y) {
+  const float a = (float)(int8_t)(x >> (8 * BYTE)), b = (float)(int8_t)(y >> (8 * BYTE));
+  if constexpr (std::is_same<T, Bf>::value)  // (8 bits: the lower half of the f32 is zero)
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+
+// The type of the first product.  int8 codes become f16 in one operation a pair: the code plus 128 as the
+// low bits of 1024, so that a key's channels are 1152 more than its codes, which the product starts less of.
+template <typename T, int TYPE>
+using Scored = typename std::conditional<TYPE == kCacheInt8, Hf, T>::type;
+constexpr float kCodeOffset = 1152.0f;
 
 // Operands of 16 keys' rows for all k steps of the first product: 32 channels each.
 template <typename T, int TYPE, int DP>
-__device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typename Mat<T>::V8 (&k)[DP / 32]) {
-  typedef typename Mat<T>::V8 V8;
+__device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typename Mat<Scored<T, TYPE>>::V8 (&k)[DP / 32]) {
+  typedef typename Mat<Scored<T, TYPE>>::V8 V8;
   if constexpr (Kept<TYPE>::kSize == 2) {
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) k[t] = __builtin_bit_cast(V8, lds_read<U4>(addr[t] + at));
@@ -93,10 +100,19 @@ __device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typena
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         U4 y;
-        y.x = pair_of<T, TYPE, 0>(x[2 * h]);
-        y.y = pair_of<T, TYPE, 1>(x[2 * h]);
-        y.z = pair_of<T, TYPE, 0>(x[2 * h + 1]);
-        y.w = pair_of<T, TYPE, 1>(x[2 * h + 1]);
+        if constexpr (TYPE == kCacheInt8) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t w = x[2 * h + i] ^ 0x80808080u;
+            y[2 * i] = __builtin_amdgcn_perm(0x64646464u, w, 0x04010400);
+            y[2 * i + 1] = __builtin_amdgcn_perm(0x64646464u, w, 0x04030402);
+          }
+        } else {
+          y.x = pair_of<T, TYPE, 0>(x[2 * h]);
+          y.y = pair_of<T, TYPE, 1>(x[2 * h]);
+          y.z = pair_of<T, TYPE, 0>(x[2 * h + 1]);
+          y.w = pair_of<T, TYPE, 1>(x[2 * h + 1]);
+        }
         k[2 * t + h] = __builtin_bit_cast(V8, y);
       }
     }
@@ -107,38 +123,51 @@ __device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typena
 template <typename T, int TYPE, int DP>
 __device__ __forceinline__ void values_of(uint32_t (&addr)[4], uint32_t at, typename Mat<T>::V8 (&v)[DP / 16]) {
   typedef typename Mat<T>::V8 V8;
-  constexpr int C = DP / 16, W = C / 2;  // a lane's channels, words of 16-bit pairs
+  constexpr int C = DP / 16;  // a lane's channels
   constexpr int E = Kept<TYPE>::kSize, kPitch = DP * E;
-  uint32_t w[8][W];
+  constexpr int W = C * E / 4;  // words of a row's channels
+  uint32_t raw[8][W];
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t from = addr[i] + at + u * 16 * kPitch;
-      uint32_t* to = w[4 * u + i];
-      if constexpr (E == 2 && C == 8) {
-        const U4 x = lds_read<U4>(from);
-        to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
-      } else if constexpr (E == 2) {
-        const U2 x = lds_read<U2>(from);
-        to[0] = x.x, to[1] = x.y;
-      } else if constexpr (C == 8) {
-        const U2 x = lds_read<U2>(from);
-        to[0] = pair_of<T, TYPE, 0>(x.x), to[1] = pair_of<T, TYPE, 1>(x.x);
-        to[2] = pair_of<T, TYPE, 0>(x.y), to[3] = pair_of<T, TYPE, 1>(x.y);
-      } else {
-        const uint32_t x = lds_read<uint32_t>(from);
-        to[0] = pair_of<T, TYPE, 0>(x), to[1] = pair_of<T, TYPE, 1>(x);
-      }
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t from = addr[e % 4] + at + (e / 4) * 16 * kPitch;
+    if constexpr (W == 4) {
+      const U4 x = lds_read<U4>(from);
+      raw[e][0] = x.x, raw[e][1] = x.y, raw[e][2] = x.z, raw[e][3] = x.w;
+    } else if constexpr (W == 2) {
+      const U2 x = lds_read<U2>(from);
+      raw[e][0] = x.x, raw[e][1] = x.y;
+    } else {
+      raw[e][0] = lds_read<uint32_t>(from);
     }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    U4 y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      y[e] = __builtin_amdgcn_perm(w[2 * e + 1][c / 2], w[2 * e][c / 2], c % 2 ? 0x07060302 : 0x05040100);
-    v[c] = __builtin_bit_cast(V8, y);
   }
+  U4 y[C];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (TYPE == kCacheInt8) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        y[4 * w][e] = whole_pair<T, 0>(raw[2 * e][w], raw[2 * e + 1][w]);
+        y[4 * w + 1][e] = whole_pair<T, 1>(raw[2 * e][w], raw[2 * e + 1][w]);
+        y[4 * w + 2][e] = whole_pair<T, 2>(raw[2 * e][w], raw[2 * e + 1][w]);
+        y[4 * w + 3][e] = whole_pair<T, 3>(raw[2 * e][w], raw[2 * e + 1][w]);
+      }
+    } else {
+      uint32_t a[C / 2], b[C / 2];  // channels by twos of either row
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if constexpr (E == 2) {
+          a[w] = raw[2 * e][w], b[w] = raw[2 * e + 1][w];
+        } else {
+          a[2 * w] = pair_of<T, TYPE, 0>(raw[2 * e][w]), a[2 * w + 1] = pair_of<T, TYPE, 1>(raw[2 * e][w]);
+          b[2 * w] = pair_of<T, TYPE, 0>(raw[2 * e + 1][w]), b[2 * w + 1] = pair_of<T, TYPE, 1>(raw[2 * e + 1][w]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) y[c][e] = __builtin_amdgcn_perm(b[c / 2], a[c / 2], c % 2 ? 0x07060302 : 0x05040100);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) v[c] = __builtin_bit_cast(V8, y[c]);
 }
 
 // The lane's operand without its values that are not finite.
@@ -260,7 +289,10 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   typedef typename M::V8 V8;
   typedef typename M::V2 V2;
   constexpr bool kCoded = Kept<TYPE>::kSize == 1;
-  constexpr bool kNotFinite = TYPE != kCacheInt8;  // the cache's type has infinities or NaN
+  constexpr bool kWhole = TYPE == kCacheInt8;
+  constexpr bool kNotFinite = !kWhole;  // the cache's type has infinities or NaN
+  typedef Mat<Scored<T, TYPE>> QM;
+  typedef typename QM::V8 Q8;
   constexpr bool kRelative = kCoded && std::is_same<T, Hf>::value;
   constexpr int E = Kept<TYPE>::kSize, C = DP / 16;
   constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
@@ -281,12 +313,12 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     const int row = 4 * quarter + i, byte = C * E * (lane & 15);
     v_addr[i] = base + 2 * R::kHalf + row * R::kPitch + 16 * ((byte / 16) ^ R::swizzle(row)) + byte % 16;
   }
-  // a lane's chunk of 16 rows in each load, its place in the record's rows or none
+  // a lane's chunk of 32 rows in each load, its place in the record's rows or none
   constexpr int kRowLoads = R::kHalf / 1024;
-  uint32_t from[kRowLoads];
+  uint32_t from[2 * kRowLoads];
 #pragma unroll
-  for (int i = 0; i < kRowLoads; ++i) {
-    const int row = (i * 64 + lane) / R::kChunks, chunk = ((i * 64 + lane) % R::kChunks) ^ R::swizzle(row);
+  for (int i = 0; i < 2 * kRowLoads; ++i) {
+    const int row = (i * 64 + lane) / R::kChunks, chunk = ((i * 64 + lane) % R::kChunks) ^ R::swizzle(row & 15);
     from[i] = 16 * chunk < c.dim * E ? (uint32_t)(row * c.dim * E + 16 * chunk) : kOutside;
   }
   const int page_mask = (1 << c.shift) - 1;
@@ -338,40 +370,53 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     typedef const __attribute__((address_space(4))) int32_t* Pages;
     const Pages pages = (Pages)(uintptr_t)c.table + (int64_t)x.seq * c.table_row;
     const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+    page[0] = page[1] = -1;
+    if (r < x.r1 && key < x.end) page[0] = pages[key >> c.shift];
+    if (c.shift == 4 && r < x.r1 && key + 16 < x.end) page[1] = pages[(key + 16) >> c.shift];
+  };
+  // loads of 16 or 32 rows of a page that begin with token `key`, n of which there are, into a stage's half h and on
+  auto load_rows = [&](const Unit& x, int key, int n, int page, int stage, int h, auto halves_) {
+    constexpr int kHalves = decltype(halves_)::value;
+    const uint64_t record = (uint64_t)(uintptr_t)c.data + (uint64_t)((int64_t)page * c.kv_heads + x.kvh) * (uint64_t)c.record;
+    const int slot = key & page_mask, bytes = n * c.dim * E;
+    const I4 kb = buffer(record + (uint32_t)(slot * c.dim * E), bytes);
+    const I4 vb = buffer(record + part + (uint32_t)(slot * c.dim * E), bytes);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * kStage + h * R::kHalf);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      page[h] = -1;
-      if (r < x.r1 && key + 16 * h < x.end) page[h] = pages[(key + 16 * h) >> c.shift];
+    for (int i = 0; i < kHalves * kRowLoads; ++i) load_lds(kb, from[i], to + i * 1024);
+#pragma unroll
+    for (int i = 0; i < kHalves * kRowLoads; ++i) load_lds(vb, from[i], to + 2 * R::kHalf + i * 1024);
+    if (kCoded) {
+      // 16 scales of K, 16 of V, and the same of the second half
+      const I4 sb = buffer(record + 2 * part + 4 * slot, n ? 4 * (page_mask + 1) + 4 * n : 0);
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i) {
+        const int l = (lane & 15) + 16 * i;
+        const uint32_t off = lane < 32 && l < n ? (uint32_t)(4 * l + (lane < 16 ? 0 : 4 * (page_mask + 1))) : kOutside;
+        load_lds_word(sb, off, __builtin_amdgcn_readfirstlane(base + stage * kStage + R::kScales + (h + i) * 256));
+      }
     }
   };
   // a step's loads; returns the keys of either half that there are
   auto load_step = [&](const Unit& x, int r, int stage, const int (&page)[2]) {
     const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+    if (c.shift > 4) {
+      const bool ok = page[0] >= 0 && page[0] < c.pages;
+      const int left = x.end - key, n = ok ? (left < 32 ? left : 32) : 0;
+      load_rows(x, key, n, ok ? page[0] : 0, stage, 0, std::integral_constant<int, 2>());
+      return n <= 16 ? n : 16 | (n - 16) << 8;
+    }
     int there = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bool ok = page[h] >= 0 && page[h] < c.pages;
       const int left = x.end - key - 16 * h, n = ok ? (left < 16 ? left : 16) : 0;
+      load_rows(x, key + 16 * h, n, ok ? page[h] : 0, stage, h, std::integral_constant<int, 1>());
       there |= n << (8 * h);
-      const uint64_t record = (uint64_t)(uintptr_t)c.data + (uint64_t)((int64_t)(ok ? page[h] : 0) * c.kv_heads + x.kvh) * (uint64_t)c.record;
-      const int slot = (key + 16 * h) & page_mask, bytes = n * c.dim * E;
-      const I4 kb = buffer(record + (uint32_t)(slot * c.dim * E), bytes);
-      const I4 vb = buffer(record + part + (uint32_t)(slot * c.dim * E), bytes);
-      const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * kStage + h * R::kHalf);
-#pragma unroll
-      for (int i = 0; i < kRowLoads; ++i) load_lds(kb, from[i], to + i * 1024);
-#pragma unroll
-      for (int i = 0; i < kRowLoads; ++i) load_lds(vb, from[i], to + 2 * R::kHalf + i * 1024);
-      if (kCoded) {
-        const I4 sb = buffer(record + 2 * part + 4 * slot, n ? 4 * (page_mask + 1) + 4 * n : 0);
-        const int l = lane & 15;
-        const uint32_t off = lane < 32 && l < n ? (uint32_t)(4 * l + (lane < 16 ? 0 : 4 * (page_mask + 1))) : kOutside;
-        load_lds_word(sb, off, __builtin_amdgcn_readfirstlane(base + stage * kStage + R::kScales + h * 256));
-      }
     }
     return there;
   };
-  V8 q[NR][DP / 32];
+  S8 q[NR][DP / 32];
   uint64_t bits[NR];
   int me[NR];  // the row's own place
   auto load_queries = [&](const Unit& x) {
@@ -385,7 +430,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         const int channel = E == 2 ? 32 * i + 8 * quarter : 64 * (i / 2) + 16 * quarter + 8 * (i % 2);
         S8 v = {0, 0, 0, 0, 0, 0, 0, 0};
         if (channel < c.dim) v = *reinterpret_cast<const S8*>(p + 2 * channel);
-        q[n][i] = __builtin_bit_cast(V8, v);
+        q[n][i] = v;
       }
       me[n] = x.context + token;
       bits[n] = a.tree ? a.tree[x.first + token] : 0;
@@ -411,6 +456,45 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       there_next = load_step(u, r0 + 1, 1, page_next);
       look_up(u, r0 + 2, page);
     }
+    float scale = a.scale_log2, start[NR];  // start: what the rows' scores begin at
+#pragma unroll
+    for (int n = 0; n < NR; ++n) start[n] = 0.0f;
+    if constexpr (kWhole) {
+      if constexpr (std::is_same<T, Bf>::value) {
+        // queries in f16: all by one power of two that takes the largest finite one to 2^14 (the least that f16 holds is
+        // 2^-38 of it: what is lost is far below the scores' own rounding)
+        uint32_t top = 0;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t x = (uint16_t)q[n][i][j] & 0x7f80u;
+              top = max(top, x == 0x7f80u ? 0u : x);
+            }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        const int e = top ? (int)(top >> 7) : 127;
+        scale = __builtin_amdgcn_ldexpf(scale, e - 141);
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              q[n][i][j] = __builtin_bit_cast(short, (Hf)__builtin_amdgcn_ldexpf(__uint_as_float((uint32_t)(uint16_t)q[n][i][j] << 16), 141 - e));
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) start[n] += (float)__builtin_bit_cast(Hf, (short)q[n][i][j]);
+        start[n] += __shfl_xor(start[n], 16);
+        start[n] = -kCodeOffset * sum_halves(start[n]);
+      }
+    }
 
     F4 o[NR][C];
     float m[NR], l[NR], top_scale[NR];
@@ -433,17 +517,17 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       F4 s[NR][2], ks[2], vs[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        V8 k[DP / 32];
+        Q8 k[DP / 32];
         keys_of<T, TYPE, DP>(k_addr, in + u * R::kHalf, k);
         if (kCoded) {
-          ks[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 16 * quarter) * a.scale_log2;
+          ks[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 16 * quarter) * scale;
           vs[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 64 + 16 * quarter);
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          s[n][u] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+          s[n][u] = F4{start[n], start[n], start[n], start[n]};
 #pragma unroll
-          for (int i = 0; i < DP / 32; ++i) s[n][u] = M::m16(k[i], q[n][i], s[n][u]);
+          for (int i = 0; i < DP / 32; ++i) s[n][u] = QM::m16(k[i], __builtin_bit_cast(Q8, q[n][i]), s[n][u]);
         }
       }
       V8 v[C];
@@ -475,7 +559,11 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
           // remembered for the rows that do
           uint32_t bad = 0;
 #pragma unroll
-          for (int i = 0; i < C; ++i) bad |= nonfinite<T>(v[i]);
+          for (int i = 0; i < C; ++i) {
+            U4 x = __builtin_bit_cast(U4, v[i]);
+            asm volatile("" : "+v"(x));  // (or it would be looked at in every step)
+            bad |= nonfinite<T>(__builtin_bit_cast(V8, x));
+          }
           if (__any(bad != 0)) {
 #pragma unroll 1
             for (int row = 0; row < kStep; ++row) {
@@ -505,7 +593,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][u][i] *= kCoded ? ks[u][i] : a.scale_log2;
+          for (int i = 0; i < 4; ++i) s[n][u][i] *= kCoded ? ks[u][i] : scale;
         if (uneven)
 #pragma unroll
           for (int u = 0; u < 2; ++u)

@@ -27,8 +27,7 @@
 namespace sfe {
 namespace {
 
-constexpr int kWaves = kCacheAttnWaves, kStep = 32, kRound = kCacheAttnRound;
-static_assert(kRound == kWaves * kStep, "a round is a step of each wave");
+constexpr int kWaves = kCacheAttnWaves, kStep = kCacheAttnStep;
 
 __device__ __forceinline__ void load_lds_word(I4 buf, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf) : "memory");
@@ -210,7 +209,8 @@ struct Span {
   int context;  // tokens before the new ones (negative: the first new tokens are none)
   int end, rounds;
 };
-__device__ __forceinline__ Span span_of(const CacheAttnArgs& a, const CacheTile& t) {
+// round: keys of one.
+__device__ __forceinline__ Span span_of(const CacheAttnArgs& a, const CacheTile& t, int round) {
   Span s;
   const int length = a.c.lengths[t.seq];
   s.context = (length > 0 ? length : 0) - t.n;
@@ -219,7 +219,7 @@ __device__ __forceinline__ Span span_of(const CacheAttnArgs& a, const CacheTile&
   const int cap = a.c.table_pages << a.c.shift;
   end = end < cap ? end : cap;
   s.end = end < 0 ? 0 : end;
-  s.rounds = s.end > 0 ? (s.end - 1) / kRound + 1 : 1;
+  s.rounds = s.end > 0 ? (s.end - 1) / round + 1 : 1;
   return s;
 }
 
@@ -244,10 +244,10 @@ struct Start {
   int total;           // rounds of all units
   int item, before;    // rounds of the units before the item
 };
-__device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* lds, int* share, int least) {
+__device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* lds, int* share, int round) {
   const int t = (int)threadIdx.x, per = (a.c.n_tiles + 64 * kWaves - 1) / (64 * kWaves);
   int mine = 0;
-  for (int i = t * per; i < min((t + 1) * per, a.c.n_tiles); ++i) mine += span_of(a, a.c.tiles[i]).rounds;
+  for (int i = t * per; i < min((t + 1) * per, a.c.n_tiles); ++i) mine += span_of(a, a.c.tiles[i], round).rounds;
   int sum = wave_scan(mine);
   if ((t & 63) == 63) lds[t >> 6] = sum;
   __syncthreads();
@@ -259,13 +259,13 @@ __device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* ld
   }
   Start s;
   s.total = total * a.c.kv_heads;
-  *share = max(least, (int)(((int64_t)s.total + gridDim.x - 1) / gridDim.x));
+  *share = max(a.least, (int)(((int64_t)s.total + gridDim.x - 1) / gridDim.x));
   const int64_t at = (int64_t)w * *share;
   int before = sum - mine;
   if (at >= (int64_t)before * a.c.kv_heads && at < (int64_t)sum * a.c.kv_heads) {
     int i = t * per;
     for (;; ++i) {
-      const int r = span_of(a, a.c.tiles[i]).rounds;
+      const int r = span_of(a, a.c.tiles[i], round).rounds;
       if (at < (int64_t)(before + r) * a.c.kv_heads) break;
       before += r;
     }
@@ -278,11 +278,12 @@ __device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* ld
   return s;
 }
 
-// T: the queries' type; NR: tiles of 16 packed rows of an item.
+// T: the queries' type; NR: tiles of 16 packed rows of a wave.  SHARE waves read the same steps, each for rows of its own,
+// from a ring of three stages that they fill together, with one barrier a step; the others take other steps.
 // WHOLE: a workgroup takes one unit, all of its rounds; otherwise an equal share of all rounds, of
 // which the first and last units may be cut: their parts go to a slot each and are joined by a second launch.
 // The first loads of a share's next unit are in flight while the waves add their results of one up.
-template <typename T, int TYPE, int DP, int NR, bool WHOLE>
+template <typename T, int TYPE, int DP, int NR, int SHARE, bool WHOLE>
 __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 1 : 2) void sfe_cache_attn_kernel(CacheAttnArgs a, int64_t first) {
   typedef Ring<DP, Kept<TYPE>::kSize> R;
   typedef Mat<T> M;
@@ -296,14 +297,16 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   constexpr bool kRelative = kCoded && std::is_same<T, Hf>::value;
   constexpr int E = Kept<TYPE>::kSize, C = DP / 16;
   constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
-  constexpr int kStage = kWaves * R::kBytes;  // two stages, each of all waves
-  __shared__ __align__(1024) char lds[2 * kStage];
+  constexpr int kGroups = kWaves / SHARE, kRound = kGroups * kStep;  // waves by steps; keys of a round
+  constexpr int kStages = SHARE > 1 ? 3 : 2, kStage = kGroups * R::kBytes;
+  // the waves' results go behind the first stage
+  constexpr int kResults = 4 * (kWaves * 16 * kRowF + 2 * kWaves * 16), kRest = (kStages - 1) * kStage;
+  __shared__ __align__(1024) char lds[kStage + (kRest > kResults ? kRest : kResults)];
   __shared__ int lds_start[kWaves + 2];
-  // the waves' results go where the second stage is
-  static_assert(4 * (kWaves * 16 * kRowF + 2 * kWaves * 16) <= kStage, "results fit a stage");
   const CacheArgs& c = a.c;
   const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), quarter = lane >> 4;
-  const uint32_t base = lds_address(lds) + wave * R::kBytes;
+  const int group = wave / SHARE, member = wave % SHARE;
+  const uint32_t base = lds_address(lds) + group * R::kBytes;
 
   // ---- addresses that stay
   uint32_t k_addr[4], v_addr[4];
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     const Tiles p = (Tiles)(uintptr_t)c.tiles + __builtin_amdgcn_readfirstlane(item);
     CacheTile tile;
     tile.first = p->first, tile.seq = p->seq, tile.n = p->n, tile.at = p->at, tile.count = p->count;
-    const Span s = span_of(a, tile);
+    const Span s = span_of(a, tile, kRound);
     Unit x;
     x.first = tile.first, x.seq = tile.seq, x.n = tile.n, x.at = tile.at, x.count = tile.count, x.total = tile.n * a.group;
     x.item = item, x.kvh = kvh;
@@ -354,7 +357,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   } else {
     // consecutive workgroups go to the 8 XCDs in turn: each has a contiguous part of the shares
     w = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
-    const Start s = start_of(a, w, lds_start, &share, a.least);
+    const Start s = start_of(a, w, lds_start, &share, kRound);
     if ((int64_t)w * share >= s.total) return;
     at = w * share;
     stop = at + share < s.total ? at + share : s.total;
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   auto look_up = [&](const Unit& x, int r, int (&page)[2]) {
     typedef const __attribute__((address_space(4))) int32_t* Pages;
     const Pages pages = (Pages)(uintptr_t)c.table + (int64_t)x.seq * c.table_row;
-    const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+    const int key = __builtin_amdgcn_readfirstlane((r * kGroups + group) * kStep);
     page[0] = page[1] = -1;
     if (r < x.r1 && key < x.end) page[0] = pages[key >> c.shift];
     if (c.shift == 4 && r < x.r1 && key + 16 < x.end) page[1] = pages[(key + 16) >> c.shift];
@@ -382,15 +385,20 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     const I4 kb = buffer(record + (uint32_t)(slot * c.dim * E), bytes);
     const I4 vb = buffer(record + part + (uint32_t)(slot * c.dim * E), bytes);
     const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * kStage + h * R::kHalf);
+    // (of waves that share a step: two take a half of K and of V each, four half a half)
 #pragma unroll
-    for (int i = 0; i < kHalves * kRowLoads; ++i) load_lds(kb, from[i], to + i * 1024);
+    for (int i = 0; i < kHalves * kRowLoads; ++i)
+      if (SHARE == 1 || (SHARE == 2 ? member == 0 : member == (h * kRowLoads + i) / kRowLoads)) load_lds(kb, from[i], to + i * 1024);
 #pragma unroll
-    for (int i = 0; i < kHalves * kRowLoads; ++i) load_lds(vb, from[i], to + 2 * R::kHalf + i * 1024);
+    for (int i = 0; i < kHalves * kRowLoads; ++i)
+      if (SHARE == 1 || (SHARE == 2 ? member == 1 : member == 2 + (h * kRowLoads + i) / kRowLoads))
+        load_lds(vb, from[i], to + 2 * R::kHalf + i * 1024);
     if (kCoded) {
       // 16 scales of K, 16 of V, and the same of the second half
       const I4 sb = buffer(record + 2 * part + 4 * slot, n ? 4 * (page_mask + 1) + 4 * n : 0);
 #pragma unroll
       for (int i = 0; i < kHalves; ++i) {
+        if (SHARE > 1 && member != h + i) continue;
         const int l = (lane & 15) + 16 * i;
         const uint32_t off = lane < 32 && l < n ? (uint32_t)(4 * l + (lane < 16 ? 0 : 4 * (page_mask + 1))) : kOutside;
         load_lds_word(sb, off, __builtin_amdgcn_readfirstlane(base + stage * kStage + R::kScales + (h + i) * 256));
@@ -399,7 +407,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   };
   // a step's loads; returns the keys of either half that there are
   auto load_step = [&](const Unit& x, int r, int stage, const int (&page)[2]) {
-    const int key = __builtin_amdgcn_readfirstlane((r * kWaves + wave) * kStep);
+    const int key = __builtin_amdgcn_readfirstlane((r * kGroups + group) * kStep);
     if (c.shift > 4) {
       const bool ok = page[0] >= 0 && page[0] < c.pages;
       const int left = x.end - key, n = ok ? (left < 32 ? left : 32) : 0;
@@ -422,7 +430,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   auto load_queries = [&](const Unit& x) {
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const int row = x.at + 16 * n + (lane & 15), rc = row < x.total ? row : x.total - 1;
+      const int row = x.at + 16 * (NR * member + n) + (lane & 15), rc = row < x.total ? row : x.total - 1;
       const int token = (int)((unsigned)rc / (unsigned)a.group), head = x.kvh * a.group + rc - token * a.group;
       const char* p = a.q.data + (x.first + token) * a.q.row + head * a.q.head;
 #pragma unroll
@@ -436,7 +444,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       bits[n] = a.tree ? a.tree[x.first + token] : 0;
     }
   };
-  int page[2], page_next[2], there, there_next = 0;
+  int page[2], page_next[2], there, there_next = 0, there_after = 0;
   look_up(u, u.r0, page);
   look_up(u, u.r0 + 1, page_next);
   there = load_step(u, u.r0, 0, page);
@@ -508,11 +516,25 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     }
     uint32_t in = 0;  // the step's stage
     for (int r = r0; r < r1; ++r) {
-      if (r + 1 < r1)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R::kLoads) : "memory");
-      else
+      // the step's loads of this wave, but not those of the next
+      constexpr int kMine = 4 * kRowLoads / SHARE;
+      if (r + 1 >= r1)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      const int key = (r * kWaves + wave) * kStep, now = there;
+      else if (SHARE == 1)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R::kLoads) : "memory");
+      else if (kCoded && member < 2)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kMine + 1) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kMine) : "memory");
+      if (SHARE > 1) {
+        // everyone's loads of the step are there, and nobody reads the one before, whose stage takes the step after the next
+        lds_barrier();
+        if (r + 2 < r1) {
+          there_after = load_step(u, r + 2, in == 0 ? 2 : (in == kStage ? 0 : 1), page);
+          look_up(u, r + 3, page);
+        }
+      }
+      const int key = (r * kGroups + group) * kStep, now = there;
       // ---- scores
       F4 s[NR][2], ks[2], vs[2];
 #pragma unroll
@@ -654,14 +676,19 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
         for (int i = 0; i < C; ++i) o[n][i] = M::m16(v[i], p, o[n][i]);
       }
-      // ---- the buffer just read takes the step after the next
       there = there_next;
-      if (r + 2 < r1) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        there_next = load_step(u, r + 2, in ? 1 : 0, page);
-        look_up(u, r + 3, page);
+      if (SHARE > 1) {
+        there_next = there_after;
+        in = in == 2 * kStage ? 0 : in + kStage;
+      } else {
+        // the buffer just read takes the step after the next
+        if (r + 2 < r1) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          there_next = load_step(u, r + 2, in ? 1 : 0, page);
+          look_up(u, r + 3, page);
+        }
+        in ^= kStage;
       }
-      in ^= kStage;
     }
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -687,6 +714,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     at += r1 - r0;
     const bool more = !WHOLE && at < stop;
     if (more) {
+      if (SHARE > 1) lds_barrier();  // (a member may still read the first stage)
       if (done.kvh == c.kv_heads - 1) {
         before += done.rounds * c.kv_heads;
         u = unit_of(done.item + 1, 0);
@@ -718,25 +746,27 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
               F4{o[n][i][j], o[n][i + 1][j], o[n][i + 2][j], o[n][i + 3][j]};
       if (quarter == 0) ml[wave * 16 + lane] = make_float2(m[n], l[n]);
       lds_barrier();
-      for (int e = t; e < 16 * (DP / 4); e += 64 * kWaves) {
-        const int row = e / (DP / 4), d = 4 * (e % (DP / 4));
-        if (16 * n + row >= done.count || d >= c.dim) continue;
+      for (int e = t; e < SHARE * 16 * (DP / 4); e += 64 * kWaves) {
+        const int of = e / (16 * (DP / 4)), row16 = e / (DP / 4) % 16, d = 4 * (e % (DP / 4));  // (of: the member)
+        const int row = 16 * (NR * of + n) + row16;
+        if (row >= done.count || d >= c.dim) continue;
         float mm = kNever;
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, ml[v * 16 + row].x);
+        for (int v = 0; v < kGroups; ++v) mm = fmaxf(mm, ml[(v * SHARE + of) * 16 + row16].x);
         F4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) {
-          const float2 x = ml[v * 16 + row];
+        for (int v = 0; v < kGroups; ++v) {
+          const int from = (v * SHARE + of) * 16 + row16;
+          const float2 x = ml[from];
           if (x.x == kNever && x.y == 0.0f) continue;  // (saw nothing)
           const float f = exp2_fast(x.x - mm);
           sum += x.y * f;
-          acc += *reinterpret_cast<const F4*>(ow + (v * 16 + row) * kRowF + d) * f;
+          acc += *reinterpret_cast<const F4*>(ow + from * kRowF + d) * f;
         }
-        const int rr = done.at + 16 * n + row;
+        const int rr = done.at + row;
         if (cut) {
-          const int64_t place = (int64_t)slot * (16 * NR) + 16 * n + row;
+          const int64_t place = (int64_t)slot * (16 * NR * SHARE) + row;
           *reinterpret_cast<F4*>(a.part_o + place * DP + d) = acc;
           if (d == 0) a.part_ml[place] = make_float2(mm, sum);
         } else {
@@ -762,7 +792,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 
 // Parts of units that were cut, added up: a workgroup takes 4 rows of a unit, each of its teams every
 // kTeams-th part with a reference exponent of its own.
-template <typename T, int DP, int NR>
+template <typename T, int DP>
 __global__ __launch_bounds__(512) void sfe_cache_attn_join_kernel(CacheAttnArgs a, int64_t first, int groups) {
   typedef typename Mat<T>::V2 V2;
   constexpr int kLanes = DP / 4, kTeams = 512 / (4 * kLanes);  // lanes of a row
@@ -777,7 +807,7 @@ __global__ __launch_bounds__(512) void sfe_cache_attn_join_kernel(CacheAttnArgs 
   const int row = 4 * (int)(block - unit * groups) + row4;
   const bool there = row < tile.count && d < a.c.dim;
   // part p of the unit is its workgroup's last, but for the unit's last part
-  auto place = [&](int p) { return (int64_t)(2 * (u.x + p) + (p + 1 < u.y)) * (16 * NR) + row; };
+  auto place = [&](int p) { return (int64_t)(2 * (u.x + p) + (p + 1 < u.y)) * (16 * a.tiles) + row; };
   F4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   float sum = 0.0f, m = kNever;
   if (there)
@@ -816,30 +846,37 @@ __global__ __launch_bounds__(512) void sfe_cache_attn_join_kernel(CacheAttnArgs 
   *reinterpret_cast<uint2*>(p + 2 * d) = make_uint2(__builtin_bit_cast(uint32_t, f), __builtin_bit_cast(uint32_t, g));
 }
 
-template <typename T, int TYPE, int DP, int NR>
+template <typename T, int TYPE, int DP, int NR, int SHARE>
 hipError_t run_rows(const CacheAttnArgs& a, hipStream_t stream) {
   const int64_t units = (int64_t)a.c.n_tiles * a.c.kv_heads;
   if (a.whole)
     return for_launches(units, 64 * kWaves, [&](int64_t first, unsigned blocks) {
-      sfe_cache_attn_kernel<T, TYPE, DP, NR, true><<<dim3(blocks), dim3(64 * kWaves), 0, stream>>>(a, first);
+      sfe_cache_attn_kernel<T, TYPE, DP, NR, SHARE, true><<<dim3(blocks), dim3(64 * kWaves), 0, stream>>>(a, first);
       return hipGetLastError();
     });
-  sfe_cache_attn_kernel<T, TYPE, DP, NR, false><<<dim3((unsigned)a.shares), dim3(64 * kWaves), 0, stream>>>(a, 0);
+  sfe_cache_attn_kernel<T, TYPE, DP, NR, SHARE, false><<<dim3((unsigned)a.shares), dim3(64 * kWaves), 0, stream>>>(a, 0);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int groups = (a.rows + 3) / 4;
   return for_launches(units * groups, 512, [&](int64_t first, unsigned blocks) {
-    sfe_cache_attn_join_kernel<T, DP, NR><<<dim3(blocks), dim3(512), 0, stream>>>(a, first, groups);
+    sfe_cache_attn_join_kernel<T, DP><<<dim3(blocks), dim3(512), 0, stream>>>(a, first, groups);
     return hipGetLastError();
   });
 }
 
+template <typename T, int TYPE, int DP>
+hipError_t run_tiles(const CacheAttnArgs& a, hipStream_t stream) {
+  switch (a.tiles) {
+    case 1: return run_rows<T, TYPE, DP, 1, 1>(a, stream);
+    case 2: return run_rows<T, TYPE, DP, 2, 1>(a, stream);
+    case 4: return run_rows<T, TYPE, DP, 2, 2>(a, stream);
+    default: return run_rows<T, TYPE, DP, 2, 4>(a, stream);
+  }
+}
+
 template <typename T, int TYPE>
 hipError_t run(const CacheAttnArgs& a, hipStream_t stream) {
-  if (a.c.dim <= 64) {
-    return a.tiles == 1 ? run_rows<T, TYPE, 64, 1>(a, stream) : run_rows<T, TYPE, 64, 2>(a, stream);
-  }
-  return a.tiles == 1 ? run_rows<T, TYPE, 128, 1>(a, stream) : run_rows<T, TYPE, 128, 2>(a, stream);
+  return a.c.dim <= 64 ? run_tiles<T, TYPE, 64>(a, stream) : run_tiles<T, TYPE, 128>(a, stream);
 }
 
 }  // namespace

@@ -265,7 +265,7 @@ int sfe_cache_plan_make(sfe_ctx* ctx, const int64_t* offsets, int32_t n, int32_t
       return SFE_OK;
     }
     const int group = heads / kv_heads;
-    plan->attn_tiles = plan->longest * group <= 16 ? 1 : 2;
+    plan->attn_tiles = sfe::cache_attn_tiles(plan->longest * group);
     const int rows = 16 * plan->attn_tiles;
     std::vector<sfe::CacheTile> tiles, attn;
     for (int32_t s = 0; s < n; ++s) {
@@ -322,10 +322,10 @@ int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_
     if (rows == 0) return SFE_OK;
     const int64_t keys = (int64_t)tokens->table_pages * cache->page_size;
     if (keys > sfe::kCacheAttnKeys) return op_fail(SFE_INVALID_ARG, "a page table of more than 2^30 tokens");
-    const int64_t rounds = std::max<int64_t>(1, (keys + sfe::kCacheAttnRound - 1) / sfe::kCacheAttnRound);
+    const int64_t rounds = std::max<int64_t>(1, (keys + sfe::cache_attn_round(plan->attn_tiles) - 1) / sfe::cache_attn_round(plan->attn_tiles));
     const int64_t units = (int64_t)plan->n_attn * plan->kv_heads;
     if (units > (int64_t)1 << 30 || units * rounds > (int64_t)1 << 30)
-      return op_fail(SFE_INVALID_ARG, "batch too large: tiles of new tokens x kv_heads x tokens of a page table must be below 2^37");
+      return op_fail(SFE_INVALID_ARG, "batch too large: tiles of new tokens x kv_heads x tokens of a page table must be below 2^35");
     if ((rc = check_heads("q", q, plan->rows, 2, 16))) return rc;
     if ((rc = check_heads("out", out, rows, 2, 16))) return rc;
     if (!apart(*out, rows, plan->heads, plan->dim)) return op_fail(SFE_INVALID_ARG, "out: rows or heads overlap");

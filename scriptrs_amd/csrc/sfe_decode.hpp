@@ -54,9 +54,13 @@ hipError_t launch_cache_write(const CacheArgs& c, int type, const AttnTensor& k,
 hipError_t launch_cache_read(const CacheArgs& c, int type, const AttnTensor& k, const AttnTensor& v, int dtype, hipStream_t stream);
 
 // ---- attention of new tokens over the cache (sfe_cache_attn.hip) ---------------------------
-// A workgroup's waves, and the keys that they take together; tokens of a page table at most.
-constexpr int kCacheAttnWaves = 4, kCacheAttnRound = 128;
+// A workgroup's waves, and the keys of a wave's step; tokens of a page table at most.
+constexpr int kCacheAttnWaves = 4, kCacheAttnStep = 32;
 constexpr int64_t kCacheAttnKeys = (int64_t)1 << 30;
+// Tiles of 16 packed rows of a workgroup: 1 or 2 in each wave, all of whose waves take other keys; 4 and 8, of which two
+// and four waves read the same keys.
+inline int cache_attn_tiles(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 8)); }
+inline int cache_attn_round(int tiles) { return kCacheAttnStep * kCacheAttnWaves / (tiles <= 2 ? 1 : tiles / 2); }  // keys
 inline int cache_attn_dim(int dim) { return dim <= 64 ? 64 : 128; }  // padded
 inline int cache_attn_shares(int cus) { return 2 * ((cus + 7) / 8 * 8); }  // workgroups that share a call's rounds
 struct CacheAttnArgs {

@@ -259,7 +259,7 @@ __device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* ld
   }
   Start s;
   s.total = total * a.c.kv_heads;
-  *share = max(a.least, (int)(((int64_t)s.total + gridDim.x - 1) / gridDim.x));
+  *share = (int)(((int64_t)s.total + gridDim.x - 1) / gridDim.x);
   const int64_t at = (int64_t)w * *share;
   int before = sum - mine;
   if (at >= (int64_t)before * a.c.kv_heads && at < (int64_t)sum * a.c.kv_heads) {
@@ -799,10 +799,10 @@ __global__ __launch_bounds__(512) void sfe_cache_attn_join_kernel(CacheAttnArgs 
   __shared__ F4 sums[kTeams][4 * kLanes];
   __shared__ float2 ml[kTeams][4];
   const int64_t block = first + blockIdx.x, unit = block / groups;
-  const int2 u = a.units[unit];
-  if (u.y == 0) return;
   const int item = (int)(unit / a.c.kv_heads), kvh = (int)(unit - (int64_t)item * a.c.kv_heads);
+  const int2 u = a.units[unit];
   const CacheTile tile = a.c.tiles[item];
+  if (u.y == 0) return;
   const int t = (int)threadIdx.x, team = t / (4 * kLanes), in = t % (4 * kLanes), row4 = in / kLanes, d = 4 * (in % kLanes);
   const int row = 4 * (int)(block - unit * groups) + row4;
   const bool there = row < tile.count && d < a.c.dim;

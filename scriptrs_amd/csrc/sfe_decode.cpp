@@ -348,8 +348,7 @@ int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_
     x.a.group = plan->heads / plan->kv_heads;
     x.a.tiles = plan->attn_tiles;
     x.a.rows = (int32_t)std::min<int64_t>(16 * plan->attn_tiles, plan->longest * x.a.group);
-    x.a.whole = rounds <= 2;
-    x.a.least = 1;
+    x.a.whole = sfe::cache_attn_whole(units, keys, plan->attn_tiles, sfe::cache_coded(cache->type) ? 1 : 2);
     x.a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     x.plan = plan;
     x.type = cache->type;

@@ -3,6 +3,8 @@
 // logits): what their entry points (sfe_decode.cpp) share with their kernels.
 #pragma once
 
+#include <algorithm>
+
 #include "sfe_ops.hpp"
 
 namespace sfe {
@@ -61,6 +63,18 @@ constexpr int64_t kCacheAttnKeys = (int64_t)1 << 30;
 // and four waves read the same keys.
 inline int cache_attn_tiles(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 8)); }
 inline int cache_attn_round(int tiles) { return kCacheAttnStep * kCacheAttnWaves / (tiles <= 2 ? 1 : tiles / 2); }  // keys
+// Whether each workgroup takes a whole unit (a tile and kv head), or an equal share of all units' rounds, which are then
+// joined by a second launch.  A unit alone takes 0.9 us a round, 1.2 of shared steps; shares cost 5 us more, and divide what
+// the device takes for all of it.  That is counted for a third of the table's tokens (`keys`), since lengths differ.  Measured, 16/4
+// heads of 128 in e4m3, one token of n sequences over l tokens, whole / shares: n 1, l 600 8.9 / 10.3 us, 1,200
+// 13.7 / 11.9; n 32, 1,200 15.4 / 18.0, 4,800 44.7 / 36.8; n 64 of 600 to 4,800 44.2 / 34.5; n 128, 2,400 54.9 / 58.1, of 300 to
+// 2,400 33.6 / 34.5.  16 tokens: n 1, 600 20.4 / 16.7; n 32, 600 21.0 / 32.3, 2,400 58.6 / 44.4; n 128, 2,400 85.9 / 88.4.
+// Past 4,096 tokens one long sequence among short ones would keep the others waiting.
+inline bool cache_attn_whole(int64_t units, int64_t keys, int tiles, int esize) {
+  const double rounds = (double)std::max<int64_t>(1, (keys + cache_attn_round(tiles) - 1) / cache_attn_round(tiles));
+  const double alone = tiles <= 2 ? 0.92 : 1.24, all = std::max(0.0024 * esize, 0.002 * std::min(tiles, 4));
+  return keys <= 4096 && alone * rounds <= 5.0 + all * (double)units * rounds;
+}
 inline int cache_attn_dim(int dim) { return dim <= 64 ? 64 : 128; }  // padded
 inline int cache_attn_shares(int cus) { return 2 * ((cus + 7) / 8 * 8); }  // workgroups that share a call's rounds
 struct CacheAttnArgs {
@@ -70,7 +84,7 @@ struct CacheAttnArgs {
   float* part_o;    // [2 * shares][tile row][padded dim]
   float2* part_ml;  // [2 * shares][tile row]: (reference exponent, sum)
   int2* units;      // [tile][kv head]: the share of its first part, and its parts (0: not cut)
-  int32_t group, tiles, rows, shares, least;  // rows: of a tile at most; least: rounds of a share
+  int32_t group, tiles, rows, shares;  // rows: of a tile at most
   bool whole;       // a workgroup takes a whole unit
   float scale_log2;  // scale * log2(e)
 };

@@ -37,7 +37,7 @@ struct Kept<kCacheInt8> {
 
 // The page of a sequence's token, or -1 where the cache has none: before its first, past the
 // table, or in a page that is none of the cache's.
-__device__ __forceinline__ int64_t page_of(const CacheArgs& c, int seq, int64_t token) {
+__host__ __device__ __forceinline__ int64_t page_of(const CacheArgs& c, int seq, int64_t token) {
   const int64_t column = token >> c.shift;
   if (token < 0 || column >= c.table_pages) return -1;
   const int32_t page = c.table[seq * c.table_row + column];

@@ -17,7 +17,7 @@ namespace sfe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 4;  // of a thread
+constexpr int kTokens = 4;  // of a thread
 
 template <typename T>
 struct alignas(16) Eight {
@@ -90,107 +90,119 @@ __device__ __forceinline__ float code_value(uint2 w, int i) {
   }
 }
 
-// What a thread does of a tile: a unit is a row of a token, one of K and V, and a kv head, of `lanes` lanes of 8
-// channels each.
-struct Place {
-  int64_t row;      // packed
-  int64_t token;    // of its sequence
-  int64_t page;     // or -1
-  int32_t slot, kvh;
-  bool value, in;   // V; whether the lane has channels
+// A workgroup's part of a tile, and a thread's place in its tokens' rows: `lanes` lanes of 8 channels for each of the K and V
+// heads, laid end to end.  A thread keeps its place in kTokens tokens, so that what depends on the place is
+// computed once; where a tile's tokens lie (16 of them, in two pages at most) is scalar.
+struct Shape {
+  int places, lanes, per, by_place, by_token;  // per: tokens of a pass; by_...: workgroups of a tile
 };
-__device__ __forceinline__ Place place_of(const CacheArgs& c, const CacheTile& tile, int unit, int channel, int length) {
-  Place p;
-  const int both = 2 * c.kv_heads;
-  const int token = (int)((unsigned)unit / (unsigned)both), part = unit - token * both;
-  p.value = part >= c.kv_heads;
-  p.kvh = p.value ? part - c.kv_heads : part;
-  p.in = token < tile.count && channel < c.dim;
-  p.row = tile.first + tile.at + token;
-  p.token = (int64_t)length - tile.n + tile.at + token;
-  p.page = -1;
-  p.slot = (int)(p.token & ((1 << c.shift) - 1));
-  return p;
-}
-template <int TYPE>
-__device__ __forceinline__ char* codes_at(const CacheArgs& c, const Place& p, int channel, float** scale) {
-  char* record = c.data + (p.page * c.kv_heads + p.kvh) * c.record;
-  const int64_t part = (int64_t)Kept<TYPE>::kSize * c.dim << c.shift;
-  *scale = reinterpret_cast<float*>(record + 2 * part) + ((int64_t)p.value << c.shift) + p.slot;
-  return record + (p.value ? part : 0) + (int64_t)Kept<TYPE>::kSize * (p.slot * c.dim + channel);
+struct Part {
+  CacheTile tile;
+  int position;           // of the tile's first token
+  int64_t page[2];        // that it is in, and the next
+  int token, kvh, channel;
+  bool value, in;         // V; whether the thread has channels
+  __device__ __forceinline__ Part(const CacheArgs& c, const Shape& s, int64_t block) {
+    typedef const __attribute__((address_space(4))) CacheTile* Tiles;
+    const int of_tile = s.by_place * s.by_token, t = (int)threadIdx.x;
+    const int64_t at = block / of_tile;
+    const int rest = (int)(block - at * of_tile), chunk = rest / s.by_token;
+    const Tiles p = (Tiles)(uintptr_t)c.tiles + at;
+    tile.first = p->first, tile.seq = p->seq, tile.n = p->n, tile.at = p->at, tile.count = p->count;
+    const int length = c.lengths[tile.seq];
+    position = __builtin_amdgcn_readfirstlane(max(length, 0) - tile.n + tile.at);
+    const int pass = s.per > 1 ? (int)((unsigned)t / (unsigned)s.places) : 0;
+    const int place = s.per > 1 ? t - pass * s.places : chunk * kThreads + t;
+    token = (rest - chunk * s.by_token) * kTokens * s.per + pass;
+    const int head = (int)((unsigned)place / (unsigned)s.lanes);
+    channel = 8 * (place - head * s.lanes);
+    value = head >= c.kv_heads;
+    kvh = value ? head - c.kv_heads : head;
+    in = place < s.places && pass < s.per && channel < c.dim;
+  }
+  __device__ __forceinline__ void look_up(const CacheArgs& c) {
+    const int64_t from = (position >> c.shift) * ((int64_t)1 << c.shift);
+    page[0] = page_of(c, tile.seq, position < 0 ? -1 : position);
+    page[1] = page_of(c, tile.seq, from + (1 << c.shift));
+  }
+  // The codes of token i's place and its scale; null where the cache has none.
+  template <int TYPE>
+  __device__ __forceinline__ char* codes_at(const CacheArgs& c, int i, float** scale) const {
+    const int64_t at = (int64_t)position + i, next = (at >> c.shift) != (position >> c.shift);
+    const int64_t in_page = next ? page[1] : page[0];
+    if (in_page < 0) return nullptr;
+    const int slot = (int)(at & ((1 << c.shift) - 1)), part = Kept<TYPE>::kSize * c.dim << c.shift;
+    char* record = c.data + (in_page * c.kv_heads + kvh) * c.record;
+    *scale = reinterpret_cast<float*>(record + 2 * part + (value ? 4 << c.shift : 0)) + slot;
+    return record + (value ? part : 0) + Kept<TYPE>::kSize * (slot * c.dim + channel);
+  }
+};
+template <typename T>
+__device__ __forceinline__ const char* row_at(const Part& p, const AttnTensor& k, const AttnTensor& v, int64_t* row) {
+  *row = p.value ? v.row : k.row;
+  return (p.value ? v.data : k.data) + (p.tile.first + p.tile.at) * *row + p.kvh * (p.value ? v.head : k.head) + (int64_t)sizeof(T) * p.channel;
 }
 
 template <typename T, int TYPE>
-__global__ __launch_bounds__(kThreads) void sfe_cache_write_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first, int chunks,
-                                                                   int lanes) {
-  const int64_t block = first + blockIdx.x, at_tile = block / chunks;
-  const CacheTile tile = c.tiles[at_tile];
-  const int length = c.lengths[tile.seq];
-  const int groups = kThreads / lanes, group = (int)threadIdx.x / lanes, channel = 8 * ((int)threadIdx.x - group * lanes);
-  const int unit0 = (int)(block - at_tile * chunks) * kUnits * groups + group;
-  Place p[kUnits];
-  Eight<T> x[kUnits];
+__global__ __launch_bounds__(kThreads) void sfe_cache_write_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first, Shape shape) {
+  Part p(c, shape, first + blockIdx.x);
+  int64_t row;
+  const char* from = row_at<T>(p, k, v, &row);
+  Eight<T> x[kTokens];
 #pragma unroll
-  for (int j = 0; j < kUnits; ++j) {
-    p[j] = place_of(c, tile, unit0 + j * groups, channel, length);
+  for (int j = 0; j < kTokens; ++j) {
+    const int i = p.token + j * shape.per;
     x[j] = Eight<T>{};
-    const char* from = p[j].value ? v.data + p[j].row * v.row + p[j].kvh * v.head : k.data + p[j].row * k.row + p[j].kvh * k.head;
-    if (p[j].in) x[j] = *reinterpret_cast<const Eight<T>*>(from + (int64_t)sizeof(T) * channel);
+    if (p.in && i < p.tile.count) x[j] = *reinterpret_cast<const Eight<T>*>(from + i * row);
   }
+  p.look_up(c);
 #pragma unroll
-  for (int j = 0; j < kUnits; ++j)
-    if (p[j].in) p[j].page = page_of(c, tile.seq, p[j].token);
-#pragma unroll
-  for (int j = 0; j < kUnits; ++j) {
+  for (int j = 0; j < kTokens; ++j) {
+    const int i = p.token + j * shape.per;
     float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)x[j].v[i];
+    for (int e = 0; e < 8; ++e) f[e] = (float)x[j].v[e];
     float* scale;
-    if constexpr (TYPE == kCacheE4m3 || TYPE == kCacheInt8) {
-      uint32_t top = 0;  // (magnitudes order as their bits do, infinity and NaN last)
+    uint32_t top = 0;  // (magnitudes order as their bits do, infinity and NaN last)
+    if constexpr (Kept<TYPE>::kSize == 1) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-      top = group_max(top, lanes);
-      if (p[j].page < 0) continue;
-      char* to = codes_at<TYPE>(c, p[j], channel, &scale);
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+      top = group_max(top, shape.lanes);
+    }
+    if (!p.in || i >= p.tile.count) continue;
+    char* to = p.codes_at<TYPE>(c, i, &scale);
+    if (!to) continue;
+    if constexpr (Kept<TYPE>::kSize == 1) {
       float s;
       *reinterpret_cast<uint2*>(to) = codes_of<TYPE>(f, top, &s);
-      if (channel == 0) *scale = s;
+      if (p.channel == 0) *scale = s;
     } else {
-      if (p[j].page < 0) continue;
-      char* to = codes_at<TYPE>(c, p[j], channel, &scale);
       typedef typename std::conditional<TYPE == kCacheBf16, __bf16, _Float16>::type O;
       Eight<O> y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y.v[i] = (O)f[i];
+      for (int e = 0; e < 8; ++e) y.v[e] = (O)f[e];
       *reinterpret_cast<Eight<O>*>(to) = y;
     }
   }
 }
 
 template <typename T, int TYPE>
-__global__ __launch_bounds__(kThreads) void sfe_cache_read_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first, int chunks,
-                                                                  int lanes) {
-  const int64_t block = first + blockIdx.x, at_tile = block / chunks;
-  const CacheTile tile = c.tiles[at_tile];
-  const int length = c.lengths[tile.seq];
-  const int groups = kThreads / lanes, group = (int)threadIdx.x / lanes, channel = 8 * ((int)threadIdx.x - group * lanes);
-  const int unit0 = (int)(block - at_tile * chunks) * kUnits * groups + group;
-  Place p[kUnits];
-  uint4 w[kUnits];
-  float s[kUnits];
+__global__ __launch_bounds__(kThreads) void sfe_cache_read_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first, Shape shape) {
+  Part p(c, shape, first + blockIdx.x);
+  p.look_up(c);
+  int64_t row;
+  char* to = const_cast<char*>(row_at<T>(p, k, v, &row));
+  uint4 w[kTokens];
+  float s[kTokens];
 #pragma unroll
-  for (int j = 0; j < kUnits; ++j) {
-    p[j] = place_of(c, tile, unit0 + j * groups, channel, length);
-    if (p[j].in) p[j].page = page_of(c, tile.seq, p[j].token);
-  }
-#pragma unroll
-  for (int j = 0; j < kUnits; ++j) {
+  for (int j = 0; j < kTokens; ++j) {
+    const int i = p.token + j * shape.per;
     w[j] = make_uint4(0, 0, 0, 0);
     s[j] = 0.0f;
-    if (p[j].page < 0) continue;
+    if (!p.in || i >= p.tile.count) continue;
     float* scale;
-    const char* from = codes_at<TYPE>(c, p[j], channel, &scale);
+    const char* from = p.codes_at<TYPE>(c, i, &scale);
+    if (!from) continue;
     if constexpr (Kept<TYPE>::kSize == 1) {
       const uint2 x = *reinterpret_cast<const uint2*>(from);
       w[j].x = x.x, w[j].y = x.y;
@@ -200,32 +212,35 @@ __global__ __launch_bounds__(kThreads) void sfe_cache_read_kernel(CacheArgs c, A
     }
   }
 #pragma unroll
-  for (int j = 0; j < kUnits; ++j) {
-    if (!p[j].in) continue;
+  for (int j = 0; j < kTokens; ++j) {
+    const int i = p.token + j * shape.per;
+    if (!p.in || i >= p.tile.count) continue;
     Eight<T> y;
     if constexpr (Kept<TYPE>::kSize == 1) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y.v[i] = (T)(code_value<TYPE>(make_uint2(w[j].x, w[j].y), i) * s[j]);
+      for (int e = 0; e < 8; ++e) y.v[e] = (T)(code_value<TYPE>(make_uint2(w[j].x, w[j].y), e) * s[j]);
     } else {
       typedef typename std::conditional<TYPE == kCacheBf16, __bf16, _Float16>::type O;
       const Eight<O> x = __builtin_bit_cast(Eight<O>, w[j]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y.v[i] = (T)(float)x.v[i];
+      for (int e = 0; e < 8; ++e) y.v[e] = (T)(float)x.v[e];
     }
-    const char* to = p[j].value ? v.data + p[j].row * v.row + p[j].kvh * v.head : k.data + p[j].row * k.row + p[j].kvh * k.head;
-    *reinterpret_cast<Eight<T>*>(const_cast<char*>(to) + (int64_t)sizeof(T) * channel) = y;
+    *reinterpret_cast<Eight<T>*>(to + i * row) = y;
   }
 }
 
 template <typename T, int TYPE, bool WRITE>
 hipError_t run(const CacheArgs& c, const AttnTensor& k, const AttnTensor& v, hipStream_t stream) {
-  int lanes = 2;
-  while (8 * lanes < c.dim) lanes *= 2;
-  const int units = kCacheTileTokens * 2 * c.kv_heads, each = kUnits * (kThreads / lanes);
-  const int chunks = (units + each - 1) / each;
-  return for_launches((int64_t)c.n_tiles * chunks, kThreads, [&](int64_t first, unsigned blocks) {
-    if (WRITE) sfe_cache_write_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, first, chunks, lanes);
-    else sfe_cache_read_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, first, chunks, lanes);
+  Shape s;
+  s.lanes = 2;
+  while (8 * s.lanes < c.dim) s.lanes *= 2;
+  s.places = 2 * c.kv_heads * s.lanes;
+  s.by_place = (s.places + kThreads - 1) / kThreads;
+  s.per = s.by_place > 1 ? 1 : kThreads / s.places;
+  s.by_token = (c.most + kTokens * s.per - 1) / (kTokens * s.per);
+  return for_launches((int64_t)c.n_tiles * s.by_place * s.by_token, kThreads, [&](int64_t first, unsigned blocks) {
+    if (WRITE) sfe_cache_write_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, first, s);
+    else sfe_cache_read_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, first, s);
     return hipGetLastError();
   });
 }

@@ -125,6 +125,7 @@ int move(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache_tokens* t
     Call& x = *static_cast<Call*>(arg);
     x.c.tiles = reinterpret_cast<const sfe::CacheTile*>(static_cast<char*>(x.plan->buf) + x.plan->tiles);
     x.c.n_tiles = x.plan->n_tiles;
+    x.c.most = (int32_t)std::min<int64_t>(sfe::kCacheTileTokens, x.plan->longest);
     return x.write ? sfe::launch_cache_write(x.c, x.type, x.k, x.v, x.dtype, x.stream)
                    : sfe::launch_cache_read(x.c, x.type, x.k, x.v, x.dtype, x.stream);
   }, &x);

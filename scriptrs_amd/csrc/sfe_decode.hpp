@@ -50,7 +50,7 @@ struct CacheArgs {
   const int32_t* lengths;
   const CacheTile* tiles;
   int64_t table_row;
-  int32_t n_tiles, table_pages, shift, kv_heads, dim;  // shift: log2 of the page's size
+  int32_t n_tiles, most, table_pages, shift, kv_heads, dim;  // most: tokens of a tile; shift: log2 of the page's size
 };
 hipError_t launch_cache_write(const CacheArgs& c, int type, const AttnTensor& k, const AttnTensor& v, int dtype, hipStream_t stream);
 hipError_t launch_cache_read(const CacheArgs& c, int type, const AttnTensor& k, const AttnTensor& v, int dtype, hipStream_t stream);

@@ -191,7 +191,7 @@ class ModelOps:
 
     def __init__(self, device: int = 0, extractor: ParakeetFeatureExtractor | None = None):
         import torch
-        self._torch, self._f32 = torch, torch.float32
+        self._torch, self._f32, self._int32 = torch, torch.float32, torch.int32
         _DTYPES.update({torch.float32: _lib.SFE_F32, torch.bfloat16: _lib.SFE_BF16, torch.float16: _lib.SFE_F16})
         # (0.6 us less than new_empty)
         self._empty_like = functools.partial(torch.empty_like, memory_format=torch.contiguous_format)
@@ -607,30 +607,32 @@ class ModelOps:
 
     def _cached(self, plan: CachePlan, cache: KvCache, page_table, lengths):
         """Checks what a call over a cache has in common and writes the tokens' places into their struct."""
-        handle, device, int32 = plan._handle, self.device, self._torch.int32
+        handle, device, int32 = plan._handle, self.device, self._int32
         if handle is None:
             raise InvalidModelOutput("the plan is closed")
         if plan._ops is not self:
             raise InvalidModelOutput("the plan belongs to another ModelOps")
-        for name, t in (("the cache", cache.data), ("page_table", page_table), ("lengths", lengths)):
-            if t.get_device() != device:
-                _wrong_device(name, t, device)
-        n, shape = plan.sequences, page_table.shape
-        if page_table.dtype != int32 or len(shape) != 2 or shape[0] != n or shape[1] > MAX_INT32 or \
-                (page_table.stride(1) != 1 and shape[1] > 1):
-            raise InvalidModelOutput(f"page_table must be an int32 tensor of [{n}, pages] with contiguous rows, got "
-                                     f"{page_table.dtype} of {list(shape)}")
-        t = self._tokens
-        t.lengths = _contiguous(lengths, "lengths", int32, (n,))
-        t.page_table, t.table_pages = page_table.data_ptr(), shape[1]
-        t.table_stride = page_table.stride(0) if n > 1 else shape[1]
+        if cache.data.get_device() != device or page_table.get_device() != device or lengths.get_device() != device:
+            for name, t in (("the cache", cache.data), ("page_table", page_table), ("lengths", lengths)):
+                if t.get_device() != device:
+                    _wrong_device(name, t, device)
+        n, shape, t = plan.sequences, page_table.shape, self._tokens
+        if page_table.dtype != int32 or len(shape) != 2 or shape[0] != n or shape[1] > MAX_INT32:
+            raise InvalidModelOutput(f"page_table must be an int32 tensor of [{n}, pages], got {page_table.dtype} of {list(shape)}")
+        row, column = page_table.stride()
+        if column != 1 and shape[1] > 1:
+            raise InvalidModelOutput("page_table must have contiguous rows")
+        if lengths.dtype != int32 or lengths.shape != (n,) or not lengths.is_contiguous():
+            raise InvalidModelOutput(f"lengths must be a contiguous int32 tensor of [{n}], got {lengths.dtype} of {list(lengths.shape)}")
+        t.lengths, t.page_table, t.table_pages = lengths.data_ptr(), page_table.data_ptr(), shape[1]
+        t.table_stride = row if n > 1 else shape[1]
         return handle
 
     def _rows_of(self, name, t, dtype, rows, heads, dim, h) -> None:
         if t.get_device() != self.device:
             _wrong_device(name, t, self.device)
         shape = t.shape
-        if t.dtype != dtype or len(shape) != 3 or shape[0] < rows or shape[1:] != (heads, dim):
+        if t.dtype != dtype or len(shape) != 3 or shape[0] < rows or shape[1] != heads or shape[2] != dim:
             raise InvalidModelOutput(f"{name} must be {dtype} of [{rows}, {heads}, {dim}], got {t.dtype} of {list(shape)}")
         _heads(t, name, shape, h)
 
@@ -661,14 +663,14 @@ class ModelOps:
         hk, hv = self._h[1], self._h[2]
         other = None if stream is None else self._other(stream)
         if out is None:
-            shape, dtype = (plan.rows, plan.kv_heads, plan.head_dim), dtype or torch.bfloat16
+            shape, dtype = (2, plan.rows, plan.kv_heads, plan.head_dim), dtype or torch.bfloat16
             if other is None:
-                k, v = (torch.empty(shape, dtype=dtype, device=cache.data.device) for _ in range(2))
+                both = torch.empty(shape, dtype=dtype, device=cache.data.device)
             else:
                 with torch.cuda.stream(other):
-                    k, v = (torch.empty(shape, dtype=dtype, device=cache.data.device) for _ in range(2))
-                for t in (k, v):
-                    t.record_stream(torch.cuda.current_stream(self.device))
+                    both = torch.empty(shape, dtype=dtype, device=cache.data.device)
+                both.record_stream(torch.cuda.current_stream(self.device))
+            k, v = both.unbind(0)
         else:
             k, v = out
             if dtype is not None and k.dtype != dtype:

@@ -79,16 +79,17 @@ __device__ __forceinline__ uint32_t whole_pair(uint32_t x, uint32_t y) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
 
-// The type of the first product.  int8 codes become f16 in one operation a pair: the code plus 128 as the
-// low bits of 1024, so that a key's channels are 1152 more than its codes, which the product starts less of.
+// The type that both products are in: f16 for codes, whose weights then keep 11 bits also where the queries are bf16.
 template <typename T, int TYPE>
-using Scored = typename std::conditional<TYPE == kCacheInt8, Hf, T>::type;
+using Product = typename std::conditional<Kept<TYPE>::kSize == 1, Hf, T>::type;
+// int8 codes become f16 in one operation a pair for the first product: the code plus 128 as the low bits
+// of 1024, so that a key's channels are 1152 more than its codes, which the product starts less of.
 constexpr float kCodeOffset = 1152.0f;
 
 // Operands of 16 keys' rows for all k steps of the first product: 32 channels each.
 template <typename T, int TYPE, int DP>
-__device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typename Mat<Scored<T, TYPE>>::V8 (&k)[DP / 32]) {
-  typedef typename Mat<Scored<T, TYPE>>::V8 V8;
+__device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typename Mat<T>::V8 (&k)[DP / 32]) {
+  typedef typename Mat<T>::V8 V8;
   if constexpr (Kept<TYPE>::kSize == 2) {
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) k[t] = __builtin_bit_cast(V8, lds_read<U4>(addr[t] + at));
@@ -286,15 +287,16 @@ __device__ __forceinline__ Start start_of(const CacheAttnArgs& a, int w, int* ld
 template <typename T, int TYPE, int DP, int NR, int SHARE, bool WHOLE>
 __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 1 : 2) void sfe_cache_attn_kernel(CacheAttnArgs a, int64_t first) {
   typedef Ring<DP, Kept<TYPE>::kSize> R;
-  typedef Mat<T> M;
+  typedef Product<T, TYPE> W;
+  typedef Mat<W> M;
   typedef typename M::V8 V8;
   typedef typename M::V2 V2;
+  typedef typename Mat<T>::V2 O2;
   constexpr bool kCoded = Kept<TYPE>::kSize == 1;
+  constexpr bool kSplit = kCoded && std::is_same<T, Hf>::value;  // a weight is two 16-bit numbers
+  constexpr bool kConverted = !std::is_same<T, W>::value;           // queries are bf16, products f16
   constexpr bool kWhole = TYPE == kCacheInt8;
   constexpr bool kNotFinite = !kWhole;  // the cache's type has infinities or NaN
-  typedef Mat<Scored<T, TYPE>> QM;
-  typedef typename QM::V8 Q8;
-  constexpr bool kRelative = kCoded && std::is_same<T, Hf>::value;
   constexpr int E = Kept<TYPE>::kSize, C = DP / 16;
   constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
   constexpr int kGroups = kWaves / SHARE, kRound = kGroups * kStep;  // waves by steps; keys of a round
@@ -464,35 +466,34 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       there_next = load_step(u, r0 + 1, 1, page_next);
       look_up(u, r0 + 2, page);
     }
-    float scale = a.scale_log2, start[NR];  // start: what the rows' scores begin at
+    float start[NR], unit[NR];  // what the rows' scores begin at, and the power of two that is their unit
 #pragma unroll
-    for (int n = 0; n < NR; ++n) start[n] = 0.0f;
-    if constexpr (kWhole) {
-      if constexpr (std::is_same<T, Bf>::value) {
-        // queries in f16: all by one power of two that takes the largest finite one to 2^14 (the least that f16 holds is
-        // 2^-38 of it: what is lost is far below the scores' own rounding)
+    for (int n = 0; n < NR; ++n) {
+      start[n] = 0.0f, unit[n] = 1.0f;
+      if constexpr (kConverted) {
+        // bf16 queries in f16, each row by a power of two of its own that takes its largest finite one to 2^14 (the least
+        // that f16 holds is 2^-38 of it: what is lost is far below the scores' own rounding)
         uint32_t top = 0;
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
+        for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-          for (int i = 0; i < DP / 32; ++i)
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t x = (uint16_t)q[n][i][j] & 0x7f80u;
+            top = max(top, x == 0x7f80u ? 0u : x);
+          }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        // (below 2^-100 as if they were that: their scores are zero to any sum)
+        const int e = max((int)(top >> 7), 27);
+        unit[n] = __uint_as_float((uint32_t)(e - 14) << 23);  // 2^(e - 141)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t x = (uint16_t)q[n][i][j] & 0x7f80u;
-              top = max(top, x == 0x7f80u ? 0u : x);
-            }
+        for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        const int e = top ? (int)(top >> 7) : 127;
-        scale = __builtin_amdgcn_ldexpf(scale, e - 141);
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              q[n][i][j] = __builtin_bit_cast(short, (Hf)__builtin_amdgcn_ldexpf(__uint_as_float((uint32_t)(uint16_t)q[n][i][j] << 16), 141 - e));
+          for (int j = 0; j < 8; ++j)
+            q[n][i][j] = __builtin_bit_cast(short, (Hf)__builtin_amdgcn_ldexpf(__uint_as_float((uint32_t)(uint16_t)q[n][i][j] << 16), 141 - e));
       }
+    }
+    if constexpr (kWhole) {
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
 #pragma unroll
@@ -539,23 +540,23 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       F4 s[NR][2], ks[2], vs[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        Q8 k[DP / 32];
-        keys_of<T, TYPE, DP>(k_addr, in + u * R::kHalf, k);
+        V8 k[DP / 32];
+        keys_of<W, TYPE, DP>(k_addr, in + u * R::kHalf, k);
         if (kCoded) {
-          ks[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 16 * quarter) * scale;
+          ks[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 16 * quarter) * a.scale_log2;
           vs[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 64 + 16 * quarter);
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
           s[n][u] = F4{start[n], start[n], start[n], start[n]};
 #pragma unroll
-          for (int i = 0; i < DP / 32; ++i) s[n][u] = QM::m16(k[i], __builtin_bit_cast(Q8, q[n][i]), s[n][u]);
+          for (int i = 0; i < DP / 32; ++i) s[n][u] = M::m16(k[i], __builtin_bit_cast(V8, q[n][i]), s[n][u]);
         }
       }
       V8 v[C];
-      values_of<T, TYPE, DP>(v_addr, in, v);
+      values_of<W, TYPE, DP>(v_addr, in, v);
       float top_value = 0.0f;  // (of the lane's keys)
-      if (kRelative)
+      if (kCoded)
         top_value = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])),
                           fmaxf(fmaxf(vs[1][0], vs[1][1]), fmaxf(vs[1][2], vs[1][3])));
       // keys that some rows do not see
@@ -584,7 +585,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
           for (int i = 0; i < C; ++i) {
             U4 x = __builtin_bit_cast(U4, v[i]);
             asm volatile("" : "+v"(x));  // (or it would be looked at in every step)
-            bad |= nonfinite<T>(__builtin_bit_cast(V8, x));
+            bad |= nonfinite<W>(__builtin_bit_cast(V8, x));
           }
           if (__any(bad != 0)) {
 #pragma unroll 1
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
               }
             }
 #pragma unroll
-            for (int i = 0; i < C; ++i) v[i] = finite_part<T>(v[i]);
+            for (int i = 0; i < C; ++i) v[i] = finite_part<W>(v[i]);
           }
         }
 #pragma unroll
@@ -615,7 +616,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][u][i] *= kCoded ? ks[u][i] : scale;
+          for (int i = 0; i < 4; ++i) s[n][u][i] *= kCoded ? ks[u][i] : a.scale_log2;
         if (uneven)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -626,6 +627,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][u][i]);
+        if (kConverted) top *= unit[n];
         if (__any(top > m[n] + M::kRise)) {
           top = fmaxf(top, __shfl_xor(top, 16));
           const float nm = fmaxf(m[n], max_halves(top) - M::kBelow);
@@ -635,7 +637,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
           for (int i = 0; i < C; ++i) o[n][i] *= f;
         }
-        if (kRelative) {
+        if (kCoded) {
           float top_seen = top_value;
           if (uneven) {
             top_seen = 0.0f;
@@ -654,16 +656,18 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
             for (int i = 0; i < C; ++i) o[n][i] *= f;
           }
         }
-        const float relative = kRelative ? 1.0f / top_scale[n] : 1.0f;
-        V8 p;
+        const float relative = __uint_as_float(0x7f000000u - __float_as_uint(top_scale[n]));  // (of a power of two)
+        V8 p, rest;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
-            F2 x = {exp2_fast(s[n][u][i] - m[n]), exp2_fast(s[n][u][i + 1] - m[n])};
+            // (the unit is a power of two: nothing is lost in the product)
+            F2 x = {exp2_fast(kConverted ? __builtin_fmaf(s[n][u][i], unit[n], -m[n]) : s[n][u][i] - m[n]),
+                    exp2_fast(kConverted ? __builtin_fmaf(s[n][u][i + 1], unit[n], -m[n]) : s[n][u][i + 1] - m[n])};
             l[n] += x.x + x.y;
             if (kCoded) {
-              x.x *= kRelative ? vs[u][i] * relative : vs[u][i], x.y *= kRelative ? vs[u][i + 1] * relative : vs[u][i + 1];
+              x.x *= vs[u][i] * relative, x.y *= vs[u][i + 1] * relative;
               if (uneven) {  // (0 times a scale that is not finite)
                 x.x = (see[n] >> (16 * u + i)) & 1 ? x.x : 0.0f;
                 x.y = (see[n] >> (16 * u + i + 1)) & 1 ? x.y : 0.0f;
@@ -672,9 +676,18 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
             const V2 y = __builtin_convertvector(x, V2);
             p[4 * u + i] = y.x;
             p[4 * u + i + 1] = y.y;
+            if (kSplit) {
+              const F2 d = {x.x - (float)y.x, x.y - (float)y.y};
+              const V2 z = __builtin_convertvector(d, V2);
+              rest[4 * u + i] = z.x;
+              rest[4 * u + i + 1] = z.y;
+            }
           }
 #pragma unroll
         for (int i = 0; i < C; ++i) o[n][i] = M::m16(v[i], p, o[n][i]);
+        if (kSplit)
+#pragma unroll
+          for (int i = 0; i < C; ++i) o[n][i] = M::m16(v[i], rest, o[n][i]);
       }
       there = there_next;
       if (SHARE > 1) {
@@ -694,7 +707,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     for (int n = 0; n < NR; ++n) {
       l[n] += __shfl_xor(l[n], 16);
       l[n] = sum_halves(l[n]);
-      if (kRelative)
+      if (kCoded)
 #pragma unroll
         for (int i = 0; i < C; ++i) o[n][i] *= top_scale[n];
     }
@@ -774,7 +787,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
           const int token = (int)((unsigned)rr / (unsigned)a.group);
           char* p = const_cast<char*>(a.o.data) + (done.first + token) * a.o.row + (int64_t)(done.kvh * a.group + rr - token * a.group) * a.o.head;
           const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};
-          const V2 f = __builtin_convertvector(x, V2), g = __builtin_convertvector(y, V2);
+          const O2 f = __builtin_convertvector(x, O2), g = __builtin_convertvector(y, O2);
           *reinterpret_cast<uint2*>(p + 2 * d) = make_uint2(__builtin_bit_cast(uint32_t, f), __builtin_bit_cast(uint32_t, g));
         }
       }

@@ -576,6 +576,34 @@ def test_hidden_values_that_are_not_finite(ops, kind, dtype):
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
+def test_rows_do_not_touch_each_other(ops, kind, dtype):
+    """Queries that are not finite, far larger or far smaller than others leave the others' results as they are."""
+    import torch
+    from scriptrs_amd import KvCache
+    K, D = 2, 64
+    for m in (2, 20):
+        n = 150 + m
+        cache = KvCache(11, 16, K, D, dtype=kind)
+        table, length = torch.arange(11, device="cuda", dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32, device="cuda")
+        kv = torch.randn(n, 2 * K, D, device="cuda", generator=gen(m)).to(torch_dtype(dtype))
+        ops.cache_write(ops.cache_plan([0, n], K, K, D), cache, table, length, kv[:, :K], kv[:, K:])
+        plan = ops.cache_plan([0, m], 4, K, D)
+        q = torch.randn(m, 4, D, device="cuda", generator=gen(m + 1)).to(torch_dtype(dtype))
+        want = ops.cache_attention(plan, cache, table, length, q)
+        for value in (math.nan, math.inf, 60000.0 if dtype == "f16" else 3e38, 1e-7 if dtype == "f16" else 1e-38):
+            other = q.clone()
+            other[1, 2] = value
+            got = ops.cache_attention(plan, cache, table, length, other)
+            keep = torch.ones(m, 4, dtype=torch.bool, device="cuda")
+            keep[1, 2] = False
+            assert torch.equal(got[keep], want[keep]), (m, value)
+            if abs(value) < 1e-3:  # (all scores alike)
+                mean = quantised(kv[:150 + 2, K:], kind).double().mean(0)[1]
+                size = quantised(kv[:150 + 2, K:], kind).double().abs().mean(0)[1]
+                within(got[1, 2], mean, (2 * U[dtype] + 2.0 ** -13) * size)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
 def test_scores_and_values_far_from_one(ops, kind, dtype):
     run_attention(ops, [200, 700], [1, 2], 4, 2, 64, 32, kind, dtype, scale=1e-6)
     run_attention(ops, [200, 700], [1, 2], 4, 2, 64, 32, kind, dtype, values=2e-4)

@@ -473,24 +473,32 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       if constexpr (kConverted) {
         // bf16 queries in f16, each row by a power of two of its own that takes its largest finite one to 2^14 (the least
         // that f16 holds is 2^-38 of it: what is lost is far below the scores' own rounding)
-        uint32_t top = 0;
+        uint32_t top = 0;  // (exponents of two queries at a time, those of infinities and NaN left out)
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
+        for (int i = 0; i < DP / 32; ++i) {
+          const U4 w = __builtin_bit_cast(U4, q[n][i]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t x = (uint16_t)q[n][i][j] & 0x7f80u;
-            top = max(top, x == 0x7f80u ? 0u : x);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = w[j] & 0x7f80u, hi = (w[j] >> 16) & 0x7f80u;
+            top = max(top, max(lo == 0x7f80u ? 0u : lo, hi == 0x7f80u ? 0u : hi));
           }
+        }
         top = max(top, (uint32_t)__shfl_xor((int)top, 16));
         top = max(top, (uint32_t)__shfl_xor((int)top, 32));
         // (below 2^-100 as if they were that: their scores are zero to any sum)
         const int e = max((int)(top >> 7), 27);
         unit[n] = __uint_as_float((uint32_t)(e - 14) << 23);  // 2^(e - 141)
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
+        for (int i = 0; i < DP / 32; ++i) {
+          U4 w = __builtin_bit_cast(U4, q[n][i]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            q[n][i][j] = __builtin_bit_cast(short, (Hf)__builtin_amdgcn_ldexpf(__uint_as_float((uint32_t)(uint16_t)q[n][i][j] << 16), 141 - e));
+          for (int j = 0; j < 4; ++j) {
+            const F2 y = {__builtin_amdgcn_ldexpf(__uint_as_float(w[j] << 16), 141 - e),
+                          __builtin_amdgcn_ldexpf(__uint_as_float(w[j] & 0xffff0000u), 141 - e)};
+            w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, Mat<Hf>::V2));
+          }
+          q[n][i] = __builtin_bit_cast(S8, w);
+        }
       }
     }
     if constexpr (kWhole) {
@@ -657,32 +665,32 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
           }
         }
         const float relative = __uint_as_float(0x7f000000u - __float_as_uint(top_scale[n]));  // (of a power of two)
+        float x[8];  // (the unit is a power of two: nothing is lost in the product)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = s[n][e / 4][e % 4];
+          x[e] = exp2_fast(kConverted ? __builtin_fmaf(y, unit[n], -m[n]) : y - m[n]);
+        }
+        l[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        if (kCoded) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= vs[e / 4][e % 4] * relative;
+          if (uneven)  // (0 times a scale that is not finite)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (see[n] >> (16 * (e / 4) + e % 4)) & 1 ? x[e] : 0.0f;
+        }
         V8 p, rest;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            // (the unit is a power of two: nothing is lost in the product)
-            F2 x = {exp2_fast(kConverted ? __builtin_fmaf(s[n][u][i], unit[n], -m[n]) : s[n][u][i] - m[n]),
-                    exp2_fast(kConverted ? __builtin_fmaf(s[n][u][i + 1], unit[n], -m[n]) : s[n][u][i + 1] - m[n])};
-            l[n] += x.x + x.y;
-            if (kCoded) {
-              x.x *= vs[u][i] * relative, x.y *= vs[u][i + 1] * relative;
-              if (uneven) {  // (0 times a scale that is not finite)
-                x.x = (see[n] >> (16 * u + i)) & 1 ? x.x : 0.0f;
-                x.y = (see[n] >> (16 * u + i + 1)) & 1 ? x.y : 0.0f;
-              }
-            }
-            const V2 y = __builtin_convertvector(x, V2);
-            p[4 * u + i] = y.x;
-            p[4 * u + i + 1] = y.y;
-            if (kSplit) {
-              const F2 d = {x.x - (float)y.x, x.y - (float)y.y};
-              const V2 z = __builtin_convertvector(d, V2);
-              rest[4 * u + i] = z.x;
-              rest[4 * u + i + 1] = z.y;
-            }
+        for (int e = 0; e < 8; e += 2) {
+          const F2 y = {x[e], x[e + 1]};
+          const V2 z = __builtin_convertvector(y, V2);
+          p[e] = z.x, p[e + 1] = z.y;
+          if (kSplit) {
+            const F2 d = {x[e] - (float)z.x, x[e + 1] - (float)z.y};
+            const V2 f = __builtin_convertvector(d, V2);
+            rest[e] = f.x, rest[e + 1] = f.y;
           }
+        }
 #pragma unroll
         for (int i = 0; i < C; ++i) o[n][i] = M::m16(v[i], p, o[n][i]);
         if (kSplit)

@@ -813,10 +813,10 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 
 // Parts of units that were cut, added up: a workgroup takes 4 rows of a unit, each of its teams every
 // kTeams-th part with a reference exponent of its own.
-template <typename T, int DP>
-__global__ __launch_bounds__(512) void sfe_cache_attn_join_kernel(CacheAttnArgs a, int64_t first, int groups) {
+template <typename T, int DP, int THREADS>
+__global__ __launch_bounds__(THREADS) void sfe_cache_attn_join_kernel(CacheAttnArgs a, int64_t first, int groups) {
   typedef typename Mat<T>::V2 V2;
-  constexpr int kLanes = DP / 4, kTeams = 512 / (4 * kLanes);  // lanes of a row
+  constexpr int kLanes = DP / 4, kTeams = THREADS / (4 * kLanes);  // lanes of a row
   __shared__ F4 sums[kTeams][4 * kLanes];
   __shared__ float2 ml[kTeams][4];
   const int64_t block = first + blockIdx.x, unit = block / groups;
@@ -879,8 +879,12 @@ hipError_t run_rows(const CacheAttnArgs& a, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int groups = (a.rows + 3) / 4;
+  // (a unit has about shares / units + 1 parts: few of them take half the waves.  256 units of 64 rows: 11.8 us with 512
+  // threads, 10.1 with 256; 16 units in 34 parts: 6.7 and 9.3)
+  const bool few = 4 * units >= a.shares;
   return for_launches(units * groups, 512, [&](int64_t first, unsigned blocks) {
-    sfe_cache_attn_join_kernel<T, DP><<<dim3(blocks), dim3(512), 0, stream>>>(a, first, groups);
+    if (few) sfe_cache_attn_join_kernel<T, DP, 256><<<dim3(blocks), dim3(256), 0, stream>>>(a, first, groups);
+    else sfe_cache_attn_join_kernel<T, DP, 512><<<dim3(blocks), dim3(512), 0, stream>>>(a, first, groups);
     return hipGetLastError();
   });
 }

@@ -325,7 +325,8 @@ int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_
     if (keys > sfe::kCacheAttnKeys) return op_fail(SFE_INVALID_ARG, "a page table of more than 2^30 tokens");
     const int64_t rounds = std::max<int64_t>(1, (keys + sfe::cache_attn_round(plan->attn_tiles) - 1) / sfe::cache_attn_round(plan->attn_tiles));
     const int64_t units = (int64_t)plan->n_attn * plan->kv_heads;
-    if (units > (int64_t)1 << 30 || units * rounds > (int64_t)1 << 30)
+    const bool whole = sfe::cache_attn_whole(units, keys, plan->attn_tiles, sfe::cache_coded(cache->type) ? 1 : 2);
+    if (!whole && units * rounds > (int64_t)1 << 30)
       return op_fail(SFE_INVALID_ARG, "batch too large: tiles of new tokens x kv_heads x tokens of a page table must be below 2^35");
     if ((rc = check_heads("q", q, plan->rows, 2, 16))) return rc;
     if ((rc = check_heads("out", out, rows, 2, 16))) return rc;
@@ -349,7 +350,7 @@ int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_
     x.a.group = plan->heads / plan->kv_heads;
     x.a.tiles = plan->attn_tiles;
     x.a.rows = (int32_t)std::min<int64_t>(16 * plan->attn_tiles, plan->longest * x.a.group);
-    x.a.whole = sfe::cache_attn_whole(units, keys, plan->attn_tiles, sfe::cache_coded(cache->type) ? 1 : 2);
+    x.a.whole = whole;
     x.a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     x.plan = plan;
     x.type = cache->type;

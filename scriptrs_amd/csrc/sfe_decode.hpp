@@ -69,11 +69,16 @@ inline int cache_attn_round(int tiles) { return kCacheAttnStep * kCacheAttnWaves
 // heads of 128 in e4m3, one token of n sequences over l tokens, whole / shares: n 1, l 600 8.9 / 10.3 us, 1,200
 // 13.7 / 11.9; n 32, 1,200 15.4 / 18.0, 4,800 44.7 / 36.8; n 64 of 600 to 4,800 44.2 / 34.5; n 128, 2,400 54.9 / 58.1, of 300 to
 // 2,400 33.6 / 34.5.  16 tokens: n 1, 600 20.4 / 16.7; n 32, 600 21.0 / 32.3, 2,400 58.6 / 44.4; n 128, 2,400 85.9 / 88.4.
-// Past 4,096 tokens one long sequence among short ones would keep the others waiting.
+// Past 4,096 tokens one long sequence among short ones would keep the others waiting, but shares have every unit's length
+// to look through: with thousands of units they are whole as long as that costs more than the longest unit alone can.
+// n 512 of 600 in a table of 5,000, 16 kv_heads 111 / 148, one of them of 60,000 tokens (and its table) 512 / 177; n 20,000 of
+// 200 285 / 550; runs of new tokens: 64 of 1,024 over 6,000 6,495 / 9,769, one of 40,000 21,486 / 29,039, one of 16,384
+// over 32,768 12,153 / 12,138.
 inline bool cache_attn_whole(int64_t units, int64_t keys, int tiles, int esize) {
   const double rounds = (double)std::max<int64_t>(1, (keys + cache_attn_round(tiles) - 1) / cache_attn_round(tiles));
   const double alone = tiles <= 2 ? 0.92 : 1.24, all = std::max(0.0024 * esize, 0.002 * std::min(tiles, 4));
-  return keys <= 4096 && alone * rounds <= 5.0 + all * (double)units * rounds;
+  if (keys > 4096) return units >= 8192 && alone * rounds <= 5.0 + (tiles <= 2 ? 0.0045 : 0.2) * (double)units;
+  return alone * rounds <= 5.0 + all * (double)units * rounds;
 }
 inline int cache_attn_dim(int dim) { return dim <= 64 ? 64 : 128; }  // padded
 inline int cache_attn_shares(int cus) { return 2 * ((cus + 7) / 8 * 8); }  // workgroups that share a call's rounds

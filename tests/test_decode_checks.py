@@ -290,4 +290,5 @@ def test_tiles_and_shares(checks):
     assert [L.stub_attn_tiles(n) for n in (1, 16, 17, 32, 33, 64, 65, 1 << 24)] == [1, 1, 2, 2, 4, 4, 8, 8]
     assert [L.stub_attn_round(n) for n in (1, 2, 4, 8)] == [128, 128, 64, 32]
     assert L.stub_attn_whole(4, 128, 1, 1) and L.stub_attn_whole(1024, 1875, 1, 1) and L.stub_attn_whole(4, 600, 1, 1)
-    assert not L.stub_attn_whole(4, 1200, 1, 1) and not L.stub_attn_whole(1 << 20, 5000, 1, 1)
+    assert not L.stub_attn_whole(4, 1200, 1, 1) and not L.stub_attn_whole(4096, 5000, 1, 1) and L.stub_attn_whole(8192, 5000, 1, 1)
+    assert not L.stub_attn_whole(8192, 60000, 1, 1) and L.stub_attn_whole(8192, 40000, 8, 1)

@@ -532,6 +532,37 @@ def test_long_sequences_are_cut(ops):
     run_attention(ops, [4097, 2900], [16, 16], 4, 1, 64, 32, "bf16", tree=random_tree(16, np.random.RandomState(1)) * 2)
 
 
+def test_long_runs_of_new_tokens(ops):
+    """A prompt's second chunk: many tiles of 128 rows, whole and in shares."""
+    run_attention(ops, [900], [600], 8, 2, 64, 32, "int8")
+    run_attention(ops, [5000, 10], [40, 3], 8, 2, 128, 64, "e4m3", columns=400)
+    run_attention(ops, [150] * 40, [140] * 40, 8, 8, 32, 16, "bf16", columns=1000)
+
+
+def test_caches_past_4_gib(ops):
+    """Pages whose places pass 32 bits."""
+    import torch
+    from scriptrs_amd import KvCache
+    K, D, page, n = 8, 128, 64, 150
+    for kind in ("bf16", "int8"):
+        pages = (5 << 30) // (K * (2 * page * D * (2 if kind == "bf16" else 1)))
+        cache = KvCache(pages, page, K, D, dtype=kind)
+        assert cache.data.numel() > 1 << 32
+        table = torch.tensor([[pages - 1, 0, pages - 2]], dtype=torch.int32, device="cuda")
+        length = torch.tensor([n], dtype=torch.int32, device="cuda")
+        kv = torch.randn(n, 2 * K, D, device="cuda", generator=gen(1)).bfloat16()
+        whole = ops.cache_plan([0, n], K, K, D)
+        ops.cache_write(whole, cache, table, length, kv[:, :K], kv[:, K:])
+        k, v = ops.cache_read(whole, cache, table, length, dtype=torch.float32)
+        kq, vq = quantised(kv[:, :K], kind), quantised(kv[:, K:], kind)
+        assert torch.equal(k.cpu(), kq) and torch.equal(v.cpu(), vq)
+        q = torch.randn(1, 2 * K, D, device="cuda", generator=gen(2)).bfloat16()
+        got = ops.cache_attention(ops.cache_plan([0, 1], 2 * K, K, D), cache, table, length, q)
+        want, size = attended(q.cpu(), kq, vq, torch.ones(1, n, dtype=torch.bool), D ** -0.5)
+        within(got, want, (2 * U["bf16"] + 2.0 ** -13) * size)
+        del cache
+
+
 @pytest.mark.parametrize("kind,dtype", KINDS)
 def test_hidden_values_that_are_not_finite(ops, kind, dtype):
     """NaN and infinities of drafts that a row does not see reach nothing; those that it sees do."""

@@ -2,9 +2,15 @@
 //
 // New token i of n of a sequence of `length` tokens is at length - n + i, in the page that the sequence's
 // table names; a record (one kv head of a page) holds its tokens' K rows, V rows and scales
-// together (sfe_decode.hpp).  The quotient x M / a is rounded correctly before it is rounded to a
-// code (x M is exact for 16-bit x after a power of two is taken off a, one division's remainder
-// corrects it), so that values halfway between two codes go to the even one.
+// together (sfe_decode.hpp).
+//
+// Codes are x M / a to the nearest, halves to the even one, a the row's largest magnitude.  Let x, a of 16 bits be
+// whole numbers below 2^11 times powers of two.  A point p halfway between two codes (5 bits in e4m3, 8 in int8) differs from
+// x M / a by nothing, or by 2^-19 of it at least: x M and p a are whole numbers below 2^19 times powers of two.  A product
+// of x and M times a's reciprocal is off by 4 of 24 bits' last steps at most (reciprocal 2, two roundings 1 each): rounded to
+// multiples of 16 of them it is p itself where it should be, and on the right side of p elsewhere (12 of
+// them away at least).  For x of 32 bits the quotient is rounded correctly first: x M is exact up to its one
+// rounding after a power of two is taken off a, and one division's remainder corrects it.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -37,25 +43,34 @@ __device__ __forceinline__ uint32_t group_max(uint32_t x, int lanes) {
   return x;
 }
 
-// 8 codes of x, top the bits of the row's largest magnitude; *scale: the row's.
-template <int TYPE>
+// 8 codes of x, values of T; top the bits of the row's largest magnitude; *scale: the row's.
+template <typename T, int TYPE>
 __device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t top, float* scale) {
-  constexpr float M = Kept<TYPE>::kTop;
+  constexpr float M = Kept<TYPE>::kTop, kPart = 1.0f / M;
   if (top >= 0x7f800000u) {
     *scale = __uint_as_float(0x7fc00000u);
     return make_uint2(0, 0);
   }
   top = max(top, 0x0f800000u);  // 2^-96
-  *scale = __uint_as_float(top) / M;
+  // (quotients by a reciprocal, corrected by their remainders)
+  const float most = __uint_as_float(top), part = most * kPart;
+  *scale = __builtin_fmaf(__builtin_fmaf(-part, M, most), kPart, part);
   // M over the power of two of the largest (from 2^-96 up: no more than 2^105, no less than 2^-121)
   const float c = __builtin_amdgcn_ldexpf(M, 127 - (int)(top >> 23));
-  const float a = __uint_as_float((top & 0x7fffffu) | 0x3f800000u), r = 1.0f / a;
+  const float a = __uint_as_float((top & 0x7fffffu) | 0x3f800000u);
   float y[8];
+  if constexpr (sizeof(T) == 2) {
+    const float m = c * __builtin_amdgcn_rcpf(a);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float n = x[i] * c;
-    const float guess = n * r;
-    y[i] = __builtin_fmaf(__builtin_fmaf(-guess, a, n), r, guess);
+    for (int i = 0; i < 8; ++i) y[i] = __uint_as_float((__float_as_uint(x[i] * m) + 8u) & ~15u);
+  } else {
+    const float r = 1.0f / a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float n = x[i] * c;
+      const float guess = n * r;
+      y[i] = __builtin_fmaf(__builtin_fmaf(-guess, a, n), r, guess);
+    }
   }
   uint32_t w[2];
 #pragma unroll
@@ -72,6 +87,29 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t top, flo
     }
   }
   return make_uint2(w[0], w[1]);
+}
+
+// The bits of the largest magnitude of 8 values as f32 (magnitudes order as their bits do, infinity and NaN last).
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const Eight<T>& x) {
+  if constexpr (sizeof(T) == 2) {
+    typedef unsigned short Pair __attribute__((ext_vector_type(2)));
+    const uint4 w = __builtin_bit_cast(uint4, x);
+    auto bits = [](uint32_t v) { return __builtin_bit_cast(Pair, v & 0x7fff7fffu); };
+    const Pair m = __builtin_elementwise_max(__builtin_elementwise_max(bits(w.x), bits(w.y)),
+                                             __builtin_elementwise_max(bits(w.z), bits(w.w)));
+    return max((uint32_t)m.x, (uint32_t)m.y);
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x.v[e]) & 0x7fffffffu);
+    return top;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t top) {
+  if constexpr (sizeof(T) == 2) return __float_as_uint((float)__builtin_bit_cast(T, (unsigned short)top));
+  else return top;
 }
 
 // Value of code i of 8.
@@ -100,14 +138,15 @@ struct Part {
   CacheTile tile;
   int position;           // of the tile's first token
   int64_t page[2];        // that it is in, and the next
+  char* record[2];        // of the thread's kv head in them
   int token, kvh, channel;
   bool value, in;         // V; whether the thread has channels
-  __device__ __forceinline__ Part(const CacheArgs& c, const Shape& s, int64_t block) {
+  __device__ __forceinline__ Part(const CacheArgs& c, const Shape& s, int64_t first_tile, uint32_t first) {
     typedef const __attribute__((address_space(4))) CacheTile* Tiles;
     const int of_tile = s.by_place * s.by_token, t = (int)threadIdx.x;
-    const int64_t at = block / of_tile;
-    const int rest = (int)(block - at * of_tile), chunk = rest / s.by_token;
-    const Tiles p = (Tiles)(uintptr_t)c.tiles + at;
+    const uint32_t block = first + blockIdx.x, at = block / (uint32_t)of_tile;
+    const int rest = (int)(block - at * of_tile), chunk = (int)((uint32_t)rest / (uint32_t)s.by_token);
+    const Tiles p = (Tiles)(uintptr_t)c.tiles + (first_tile + at);
     tile.first = p->first, tile.seq = p->seq, tile.n = p->n, tile.at = p->at, tile.count = p->count;
     const int length = c.lengths[tile.seq];
     position = __builtin_amdgcn_readfirstlane(max(length, 0) - tile.n + tile.at);
@@ -124,17 +163,18 @@ struct Part {
     const int64_t from = (position >> c.shift) * ((int64_t)1 << c.shift);
     page[0] = page_of(c, tile.seq, position < 0 ? -1 : position);
     page[1] = page_of(c, tile.seq, from + (1 << c.shift));
+    const int64_t in_page = kvh * c.record;
+    for (int i = 0; i < 2; ++i) record[i] = c.data + page[i] * c.kv_heads * c.record + in_page;
   }
   // The codes of token i's place and its scale; null where the cache has none.
   template <int TYPE>
   __device__ __forceinline__ char* codes_at(const CacheArgs& c, int i, float** scale) const {
-    const int64_t at = (int64_t)position + i, next = (at >> c.shift) != (position >> c.shift);
-    const int64_t in_page = next ? page[1] : page[0];
-    if (in_page < 0) return nullptr;
-    const int slot = (int)(at & ((1 << c.shift) - 1)), part = Kept<TYPE>::kSize * c.dim << c.shift;
-    char* record = c.data + (in_page * c.kv_heads + kvh) * c.record;
-    *scale = reinterpret_cast<float*>(record + 2 * part + (value ? 4 << c.shift : 0)) + slot;
-    return record + (value ? part : 0) + Kept<TYPE>::kSize * (slot * c.dim + channel);
+    const int at = (position & ((1 << c.shift) - 1)) + i, next = at >> c.shift;
+    if ((next ? page[1] : page[0]) < 0) return nullptr;
+    const int slot = at & ((1 << c.shift) - 1), part = Kept<TYPE>::kSize * c.dim << c.shift;
+    char* in = next ? record[1] : record[0];
+    *scale = reinterpret_cast<float*>(in + (uint32_t)(2 * part + (value ? 4 << c.shift : 0) + 4 * slot));
+    return in + (uint32_t)((value ? part : 0) + Kept<TYPE>::kSize * (slot * c.dim + channel));
   }
 };
 template <typename T>
@@ -144,8 +184,8 @@ __device__ __forceinline__ const char* row_at(const Part& p, const AttnTensor& k
 }
 
 template <typename T, int TYPE>
-__global__ __launch_bounds__(kThreads) void sfe_cache_write_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first, Shape shape) {
-  Part p(c, shape, first + blockIdx.x);
+__global__ __launch_bounds__(kThreads) void sfe_cache_write_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first_tile, uint32_t first, Shape shape) {
+  Part p(c, shape, first_tile, first);
   int64_t row;
   const char* from = row_at<T>(p, k, v, &row);
   Eight<T> x[kTokens];
@@ -163,18 +203,14 @@ __global__ __launch_bounds__(kThreads) void sfe_cache_write_kernel(CacheArgs c, 
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = (float)x[j].v[e];
     float* scale;
-    uint32_t top = 0;  // (magnitudes order as their bits do, infinity and NaN last)
-    if constexpr (Kept<TYPE>::kSize == 1) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-      top = group_max(top, shape.lanes);
-    }
+    uint32_t top = 0;
+    if constexpr (Kept<TYPE>::kSize == 1) top = top_bits<T>(group_max(top_of(x[j]), shape.lanes));
     if (!p.in || i >= p.tile.count) continue;
     char* to = p.codes_at<TYPE>(c, i, &scale);
     if (!to) continue;
     if constexpr (Kept<TYPE>::kSize == 1) {
       float s;
-      *reinterpret_cast<uint2*>(to) = codes_of<TYPE>(f, top, &s);
+      *reinterpret_cast<uint2*>(to) = codes_of<T, TYPE>(f, top, &s);
       if (p.channel == 0) *scale = s;
     } else {
       typedef typename std::conditional<TYPE == kCacheBf16, __bf16, _Float16>::type O;
@@ -187,8 +223,8 @@ __global__ __launch_bounds__(kThreads) void sfe_cache_write_kernel(CacheArgs c, 
 }
 
 template <typename T, int TYPE>
-__global__ __launch_bounds__(kThreads) void sfe_cache_read_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first, Shape shape) {
-  Part p(c, shape, first + blockIdx.x);
+__global__ __launch_bounds__(kThreads) void sfe_cache_read_kernel(CacheArgs c, AttnTensor k, AttnTensor v, int64_t first_tile, uint32_t first, Shape shape) {
+  Part p(c, shape, first_tile, first);
   p.look_up(c);
   int64_t row;
   char* to = const_cast<char*>(row_at<T>(p, k, v, &row));
@@ -238,9 +274,12 @@ hipError_t run(const CacheArgs& c, const AttnTensor& k, const AttnTensor& v, hip
   s.by_place = (s.places + kThreads - 1) / kThreads;
   s.per = s.by_place > 1 ? 1 : kThreads / s.places;
   s.by_token = (c.most + kTokens * s.per - 1) / (kTokens * s.per);
-  return for_launches((int64_t)c.n_tiles * s.by_place * s.by_token, kThreads, [&](int64_t first, unsigned blocks) {
-    if (WRITE) sfe_cache_write_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, first, s);
-    else sfe_cache_read_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, first, s);
+  const int of_tile = s.by_place * s.by_token;
+  return for_launches((int64_t)c.n_tiles * of_tile, kThreads, [&](int64_t at, unsigned blocks) {
+    const int64_t tile = at / of_tile;
+    const uint32_t first = (uint32_t)(at % of_tile);
+    if (WRITE) sfe_cache_write_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, tile, first, s);
+    else sfe_cache_read_kernel<T, TYPE><<<dim3(blocks), dim3(kThreads), 0, stream>>>(c, k, v, tile, first, s);
     return hipGetLastError();
   });
 }

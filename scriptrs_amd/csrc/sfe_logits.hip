@@ -36,16 +36,17 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // the first of a row may begin up to N - 1 elements before it.
 // H: bytes of a count, 0 without a history.
 template <typename T, int N, int V, int H, bool BIAS, bool MASK>
-__global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int64_t first, int spans) {
+__global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int64_t first_row, uint32_t first_span, uint32_t spans) {
   typedef Vec<T, N> Vector;
   constexpr int kSpan = kThreads * N * V;
   __shared__ __align__(16) uint32_t counts[H ? kSpan * H / 4 : 4];
-  const int64_t block = first + blockIdx.x, r = block / spans;
+  const uint32_t block = first_span + blockIdx.x, of_first = block / spans;
+  const int64_t r = first_row + of_first;
   const int t = (int)threadIdx.x;
   const T* in = reinterpret_cast<const T*>(a.in) + r * a.in_row;
   T* out = reinterpret_cast<T*>(a.out) + r * a.out_row;
   const int before = N > 1 ? (int)((uintptr_t)in / sizeof(T) % N) : 0;
-  const int span0 = (int)(block - r * spans) * kSpan - before;  // first token of the span
+  const int span0 = (int)(block - of_first * spans) * kSpan - before;  // first token of the span
 
   // ---- all loads, those of the history first
   int n = 0;
@@ -112,16 +113,18 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
     for (int e = 4 * t; e < kSpan * H / 4; e += 4 * kThreads) *reinterpret_cast<uint4*>(counts + e) = make_uint4(0, 0, 0, 0);
     over = 1.0f / rep;
     lds_barrier();
+    const int low = max(span0, 0);
+    const uint32_t tokens_here = (uint32_t)(min(span0 + kSpan, a.vocab) - low);
     for (int e = t; e < n;) {
-      int32_t now[kAhead];
+      uint32_t now[kAhead];  // (from the span's first token on; a token that does not count is past its end)
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) now[i] = e + i * kThreads < n ? token[i] : -1;
+      for (int i = 0; i < kAhead; ++i) now[i] = e + i * kThreads < n ? (uint32_t)token[i] - (uint32_t)low : ~0u;
       e += kAhead * kThreads;
       tokens(e);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int at = now[i] - span0;
-        if (now[i] < 0 || now[i] >= a.vocab || at < 0 || at >= kSpan) continue;
+        if (now[i] >= tokens_here) continue;
+        const int at = (int)now[i] + low - span0;
         if (H == 2) atomicAdd(counts + at / 2, at & 1 ? 0x10000u : 1u);
         else atomicAdd(counts + at, 1u);
       }
@@ -145,11 +148,18 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const uint32_t count = H == 2 ? (i % 2 ? c[i / 2] >> 16 : c[i / 2] & 0xffffu) : c[i];
-          // the quotient by its reciprocal, corrected by the remainder (none of an infinity)
-          float y = z[i] * over;
-          const float left = __builtin_fmaf(-y, rep, z[i]);
-          y = left == left ? __builtin_fmaf(left, over, y) : y;
-          y = (z[i] > 0.0f ? y : z[i] * rep) - (presence + frequency * (float)count);
+          float y;
+          if constexpr (sizeof(T) == 2) {
+            // (off by 1.5 steps of f32 before the one rounding to 16 bits)
+            y = z[i] * (z[i] > 0.0f ? over : rep);
+          } else {
+            // the quotient by its reciprocal, corrected by the remainder (none of an infinity)
+            y = z[i] * over;
+            const float left = __builtin_fmaf(-y, rep, z[i]);
+            y = left == left ? __builtin_fmaf(left, over, y) : y;
+            y = z[i] > 0.0f ? y : z[i] * rep;
+          }
+          y -= presence + frequency * (float)count;
           z[i] = count ? y : z[i];
         }
       }
@@ -179,7 +189,7 @@ hipError_t run(const LogitsArgs& a, hipStream_t stream) {
   constexpr int kSpan = kThreads * N * V;
   const int spans = (int)(((int64_t)a.vocab + (N - 1) + kSpan - 1) / kSpan);
   return for_launches((int64_t)a.rows * spans, kThreads, [&](int64_t first, unsigned blocks) {
-    sfe_logits_kernel<T, N, V, H, BIAS, MASK><<<dim3(blocks), dim3(kThreads), 0, stream>>>(a, first, spans);
+    sfe_logits_kernel<T, N, V, H, BIAS, MASK><<<dim3(blocks), dim3(kThreads), 0, stream>>>(a, first / spans, (uint32_t)(first % spans), (uint32_t)spans);
     return hipGetLastError();
   });
 }

@@ -51,6 +51,12 @@ __device__ __forceinline__ void group_sums(float (&x)[K], int lanes) {
     for (int k = 0; k < K; ++k) x[k] += __shfl_xor(x[k], 32);
 }
 
+// 1 / sqrt(x), to a step of f32 (x tiny: of 2^64 x).
+__device__ __forceinline__ float over_root(float x) {
+  const bool tiny = x < 0x1p-96f;
+  return __builtin_amdgcn_rsqf(tiny ? x * 0x1p64f : x) * (tiny ? 0x1p32f : 1.0f);
+}
+
 // A workgroup takes K times `per` rows.  Places of a row: `lanes` for each of its heads, q's then k's; a thread
 // keeps its place in K rows (so that what depends on the place is computed once), all K loads
 // issued before the first store and before the rows' sines and cosines go into LDS.  Rows of more than 256 places
@@ -168,7 +174,7 @@ __global__ __launch_bounds__(kThreads) void sfe_norm_rotary_kernel(NormRotaryArg
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if (in + k * per >= rows) continue;
-    const float inv = 1.0f / sqrtf(sum[k] * over + a.eps);
+    const float inv = over_root(sum[k] * over + a.eps);
     T* yk = y + k * (int64_t)per * y_row;
 #pragma unroll
     for (int u = 0; u < U; ++u) {

@@ -494,7 +494,7 @@ typedef struct sfe_logits {
   const void* logits;
   void* out;
   int64_t logits_row, out_row; /* strides in elements */
-  /* Tokens said before, history_most of each row (or the first lengths[r] of them); those outside
+  /* Tokens said before, history_most of each row (at most 2^30; or the first lengths[r] of them); those outside
    * [0, vocab) count for nothing.  NULL: none. */
   const int32_t* history;
   int64_t history_row;

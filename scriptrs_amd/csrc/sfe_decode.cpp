@@ -384,7 +384,8 @@ int sfe_adjust_logits(sfe_ctx* ctx, const sfe_logits* l, void* stream) {
     if (!known_dtype(l->dtype)) return op_fail(SFE_INVALID_ARG, "dtype must be SFE_F32, SFE_BF16 or SFE_F16");
     if (l->rows < 0) return op_fail(SFE_INVALID_ARG, "negative number of rows");
     if (l->vocab <= 0 || l->vocab > (1 << 24)) return op_fail(SFE_INVALID_ARG, "vocab must be in [1, 2^24]");
-    if (l->history && l->history_most < 0) return op_fail(SFE_INVALID_ARG, "negative history_most");
+    if (l->history && (l->history_most < 0 || l->history_most > 1 << 30))
+      return op_fail(SFE_INVALID_ARG, "history_most must be in [0, 2^30]");
     if (!l->history && l->lengths) return op_fail(SFE_INVALID_ARG, "lengths without a history");
     if (!l->repetitions && (!(l->repetition > 0.0f) || !isfinite(l->repetition)))
       return op_fail(SFE_INVALID_ARG, "repetition must be positive and finite");

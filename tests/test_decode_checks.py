@@ -252,6 +252,7 @@ def test_logits(checks):
     refused(L, call(history=None), "lengths without")
     refused(L, call(allowed=None), "states without")
     refused(L, call(history_most=-1), "history_most")
+    refused(L, call(history_most=(1 << 30) + 1), "history_most")
     refused(L, call(n_allowed=-1), "n_allowed")
     for value in (0.0, -1.0, float("inf"), float("nan")):
         refused(L, call(repetition=value), "repetition")

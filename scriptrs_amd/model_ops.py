@@ -131,7 +131,7 @@ class KvCache:
     ``dtype``: "bf16" or "f16", or 8 bits with a scale for each token and kv head, "e4m3" or "int8".
     ``data``, uint8 of [pages, kv_heads, record], holds all of it, zeros at first (or the caller's own
     contiguous tensor): a page is ``data[p]``, so that pages can be copied, and beams reordered, as
-    any other state.  ``page_size`` is a power of two from 16 to 1024, ``head_dim`` a
+    any other state, in place.  ``page_size`` is a power of two from 16 to 1024, ``head_dim`` a
     multiple of 16, at most 128."""
 
     TYPES = {"bf16": 1, "f16": 2, "e4m3": 3, "int8": 4}
@@ -152,10 +152,15 @@ class KvCache:
         if data is None:
             data = torch.zeros(shape, dtype=torch.uint8, device=torch.device("cuda", device))
         _contiguous(data, "data", torch.uint8, shape)
-        self.data, self.dtype = data, dtype
+        self._data, self.dtype = data, dtype
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
         self.c = SfeCache(data.data_ptr(), pages, page_size, kv_heads, head_dim, self.TYPES[dtype])
         self.p = ctypes.byref(self.c)
+
+    @property
+    def data(self):
+        """The cache's memory: written in place (another tensor is another ``KvCache``)."""
+        return self._data
 
 
 class CachePlan:

@@ -539,6 +539,13 @@ def test_long_runs_of_new_tokens(ops):
     run_attention(ops, [150] * 40, [140] * 40, 8, 8, 32, 16, "bf16", columns=1000)
 
 
+def test_a_cache_keeps_its_memory():
+    from scriptrs_amd import KvCache
+    cache = KvCache(2, 16, 1, 16)
+    with pytest.raises(AttributeError):
+        cache.data = cache.data.clone()
+
+
 def test_caches_past_4_gib(ops):
     """Pages whose places pass 32 bits."""
     import torch

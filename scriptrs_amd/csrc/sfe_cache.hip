@@ -4,6 +4,12 @@
 // table names; a record (one kv head of a page) holds its tokens' K rows, V rows and scales
 // together (sfe_decode.hpp).
 //
+// Bound by memory: every element is read and written once, a workgroup's rows lie next to each other in both.  Written, 205,000
+// tokens of 4 heads of 128 from bf16 to e4m3: 636 MB in 137 us (4.6 TB/s; bf16 to bf16 5.2), 256 clips of 13-251 tokens of 8 heads
+// of 64 in f16 18.5 us and read back 12.7 (5.7 and 8 TB/s, part of it in the last-level cache); 8 prompts of 700-8,192
+// tokens in int8 read in 36 us (5.3 TB/s).  A thread keeps its place in four tokens (clips written and read 37 us with a
+// token a thread, 31 with four and codes by one product).
+//
 // Codes are x M / a to the nearest, halves to the even one, a the row's largest magnitude.  Let x, a of 16 bits be
 // whole numbers below 2^11 times powers of two.  A point p halfway between two codes (5 bits in e4m3, 8 in int8) differs from
 // x M / a by nothing, or by 2^-19 of it at least: x M and p a are whole numbers below 2^19 times powers of two.  A product

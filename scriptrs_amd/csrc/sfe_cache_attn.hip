@@ -3,17 +3,32 @@
 // For new token i of n of a sequence of L tokens, head h reading kv head h / group:
 // o_i = sum_j softmax_j(scale q_i . k_j) v_j over the context (j < L - n) and the new tokens that i sees:
 // those of its tree's bits, or without a tree itself and those before.  One pass over the keys with a running
-// reference exponent and sum, as in sfe_attn.hip.
+// reference exponent and sum in f32, as in sfe_attn.hip: a step's maximum m' replaces m only when it is kRise above it, and
+// o and l are then multiplied by 2^(m - m').
 //
-// Codes of 8 bits enter the matrix products as they are (both 16-bit types hold them exactly): a key's scale
-// multiplies its scores, a value's scale its weight, in f32 before the weight's one rounding to 16
-// bits.  In f16, which lacks the range, weights are kept relative to the largest value scale so far.
+// Rows of a unit (a kv head and up to 128 of a sequence's token x head of the group) are the columns of both matrix products,
+// so that a group's heads share the reads of their kv head: S^T = K Q^T leaves a lane with one query's scores of the 8
+// keys that O^T = V^T P^T takes from it, once V's rows are paired by key in registers.  The order of channels in a product
+// is free, so lanes read whole chunks of K and of V.
 //
-// A wave takes steps of 32 keys through an LDS ring of its own, without a barrier: pages are looked up one step
-// ahead, rows go from memory into LDS directly, and what lies past a sequence's end or in no page
-// is read as zeros by the buffer's range.  Scores are S^T = K Q^T (a lane has one query's), which is the
-// operand order of O^T = V^T P^T once V's rows are paired by key in registers.  The order of channels in a
-// product is free, so lanes read whole chunks of K and of V.
+// Codes of 8 bits are f16 in both products, which holds them exactly: a key's scale multiplies its scores, a value's
+// scale its weight, in f32.  Weights are kept relative to a power of two above the largest value scale so far, since f16
+// lacks their range, and rounded once to 11 bits; where the queries are f16 (and outputs have 11 bits too) to 22, as two
+// numbers.  bf16 queries become f16 by a power of two of their own row.  16-bit caches multiply in their own type, weights
+// rounded once to it.
+//
+// A step is 32 keys.  Pages are looked up a step ahead; rows go from memory into LDS directly, and what lies past a
+// sequence's end or in no page is read as zeros by the buffer's range, so that nothing is read outside a record.  Up to 32 rows
+// a workgroup's four waves take steps of their own, through rings of two stages of their own, without a barrier in the
+// loop; of 64 and 128 rows two and four waves read the same steps from a ring of three, with one barrier a step (codes are then
+// converted once for 32 rows a wave; 64 rows a wave took 180 us where this takes 83, since its accumulators left the
+// registers that the products write).
+//
+// What bounds it: one token a sequence, memory and the trip of a unit (256 x 126-1,500 tokens, 16/4 heads of 128 in e4m3:
+// 152 MB in 40 us, 3.8 TB/s; 2 x 5 tokens over 45,000, 8 heads of 64 in f16: 184 MB in 36 us, 5.1 TB/s, and 7 of the
+// join); trees, vector instructions beside the matrix cores (32 x 16 over 700-8,192, 32/8 heads of 128 in int8: 204 MB in 77
+// us and 10 of the join; 61% of the CUs' time issues vector instructions, 16% of it products).  A step of 32 keys and 32 rows
+// takes 451 of them: conversions of both operands' codes, two products a weight for its scale, exponentials and maxima.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -6,6 +6,11 @@
 // are f32, the variance from the deviations; the result is rounded once, where a norm and a rotary
 // pass behind it would round twice.
 //
+// Bound by memory: each element is read and written once.  52,640 rows of 8 + 8 heads of 128 in bf16, 96 channels turned, layer
+// norms: 431 MB in 106 us, 4.1 TB/s, where the turn alone (sfe_rotary.hip) runs at the copy's 4.9-5.1; vector instructions
+// take 62% of the CUs' time.  Four rows a thread: 2 121, 8 117 us and more, 1 172 (what depends on the place is computed once, and
+// there is enough in flight).  64 rows of 16 + 4 heads: 4.4 us, the launch and one trip.
+//
 // A head is a group of lanes, a power of two; a lane holds the channels that turn together (half: two vectors
 // R / 2 apart, interleaved: one vector of whole pairs), so that sums are exchanges within the
 // group and a turn is within a lane.

@@ -6,7 +6,7 @@
 // In f32, rounded once.
 //
 // Bound by memory and, with histories, by the vector instructions of their penalties (71% of the CUs' time): 512 rows of 128,000 in
-// bf16 with histories of up to 1,500, biases and a grammar, 266 MB in 64 us (4.2 TB/s), 183 before all
+// bf16 with histories of up to 1,500, biases and a grammar, 266 MB in 62 us (4.3 TB/s), 183 before all
 // loads were in flight together; 64 rows in f16 with histories of up to 8,192 13 us, the history's scan by each span the rest.
 //
 // One pass over the logits: a workgroup takes a span of one row's tokens, has all of its
@@ -24,14 +24,6 @@ namespace sfe {
 namespace {
 
 constexpr int kThreads = 256;
-
-// The mask bits of n <= 32 tokens from t on.
-__device__ __forceinline__ uint32_t mask_bits(const uint32_t* words, int t, int n, int vocab) {
-  const int w = t >> 5, shift = t & 31;
-  uint32_t bits = words[w] >> shift;
-  if (shift && shift + n > 32 && 32 * (w + 1) < vocab) bits |= words[w + 1] << (32 - shift);
-  return bits;
-}
 
 // Waits for the workgroup's LDS accesses, not for its loads.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -86,7 +78,7 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
     if (state >= 0 && state < a.n_allowed) words = a.allowed + state * a.allowed_row;
   }
   float bias[V][BIAS ? N : 1];
-  uint32_t bits[V];
+  uint32_t low_word[V], high_word[V];  // of the mask: that of a vector's first token and the next
   if (BIAS) {
     const float* from = a.bias + r * a.bias_row;
     const bool whole = N > 1 && ((uintptr_t)from / 4 - before) % 4 == 0;  // vectors of 16 bytes
@@ -109,8 +101,12 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int at = span0 + (v * kThreads + t) * N;
-      bits[v] = ~0u;
-      if (words && at < a.vocab && at + N > 0) bits[v] = at >= 0 ? mask_bits(words, at, N, a.vocab) : words[0] << -at;
+      const int w = at >> 5;
+      low_word[v] = high_word[v] = ~0u;
+      if (words && at < a.vocab) {
+        low_word[v] = w >= 0 ? words[w] : 0;
+        if (before && 32 * (w + 1) < a.vocab) high_word[v] = words[w + 1];  // (else a vector's bits are in one)
+      }
     }
   // ---- the history's tokens of the span, counted in LDS
   if (H) {
@@ -169,11 +165,12 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
       }
     }
     Vector y;
+    const uint32_t bits = MASK ? __builtin_amdgcn_alignbit(high_word[v], low_word[v], at & 31) : 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (BIAS) z[i] += bias[v][i];
       if (MASK) {  // (as whole numbers: two operations)
-        const uint32_t m = (uint32_t)((int32_t)(bits[v] << (31 - i)) >> 31);
+        const uint32_t m = (uint32_t)((int32_t)(bits << (31 - i)) >> 31);
         z[i] = __uint_as_float((__float_as_uint(z[i]) & m) | (0xff800000u & ~m));
       }
       y.v[i] = (T)z[i];
@@ -217,8 +214,8 @@ hipError_t run_type(const LogitsArgs& a, hipStream_t stream) {
   // vectors where a row's input and output lie alike
   const bool alike = (uintptr_t)a.in % 16 == (uintptr_t)a.out % 16 && (a.in_row - a.out_row) % N == 0;
   // Spans of 4,096 tokens, 8,192 where a long history is read by every one of them and no biases take
-  // registers.  512 rows of 128,000 in bf16 with histories of up to 1,500: 4,096 62 us with a grammar, 68 with biases too; 8,192
-  // 67 and 82; 2,048 75 with both.  64 rows with histories of up to 8,192: 14.0 and 12.7.
+  // registers.  512 rows of 128,000 in bf16 with histories of up to 1,500: 4,096 58 us with a grammar, 62 with biases too; 8,192
+  // 59 and 69; 2,048 62 and 71.  64 rows with histories of up to 8,192: 14.0 and 12.7.
   constexpr int V = 4096 / (kThreads * N);
   if (!alike) return run_history<T, 1, 4>(a, stream);
   if (a.history && a.history_most > 4096 && !a.bias) return run_history<T, N, 2 * V>(a, stream);

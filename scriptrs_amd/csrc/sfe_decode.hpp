@@ -96,6 +96,28 @@ struct CacheAttnArgs {
 hipError_t launch_cache_attn(const CacheAttnArgs& a, int type, int dtype, hipStream_t stream);
 
 // ---- steering of logits (sfe_logits.hip) -----------------------------------------------------
+// A row's tokens in spans, a workgroup each: vectors of n lie at multiples of their size, so that the first span
+// begins `before` tokens (less than n) before the row.  There are as many spans as the row with the most before
+// it needs: of another row the last one may begin at the vocabulary's end or past it, and has no tokens.
+constexpr int logits_spans(int vocab, int n, int span) { return (int)(((int64_t)vocab + (n - 1) + span - 1) / span); }
+struct LogitsSpan {
+  int32_t first;    // token of its first place
+  int32_t low;      // first token of the row that it has
+  uint32_t tokens;  // that it has
+  // The place of a token, or -1 where the span has no such.
+  __host__ __device__ int32_t place(int32_t token) const {
+    const uint32_t at = (uint32_t)token - (uint32_t)low;
+    return at < tokens ? (int32_t)at + low - first : -1;
+  }
+};
+__host__ __device__ inline LogitsSpan logits_span(int number, int span, int before, int vocab) {
+  LogitsSpan s;
+  s.first = number * span - before;
+  s.low = s.first > 0 ? s.first : 0;
+  const int end = s.first + span < vocab ? s.first + span : vocab;
+  s.tokens = end > s.low ? (uint32_t)(end - s.low) : 0u;
+  return s;
+}
 struct LogitsArgs {
   const char* in;
   char* out;

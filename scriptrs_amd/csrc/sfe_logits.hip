@@ -42,7 +42,9 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
   const T* in = reinterpret_cast<const T*>(a.in) + r * a.in_row;
   T* out = reinterpret_cast<T*>(a.out) + r * a.out_row;
   const int before = N > 1 ? (int)((uintptr_t)in / sizeof(T) % N) : 0;
-  const int span0 = (int)(block - of_first * spans) * kSpan - before;  // first token of the span
+  const LogitsSpan span = logits_span((int)(block - of_first * spans), kSpan, before, a.vocab);
+  if (span.tokens == 0) return;  // (the workgroup's: past the row's end)
+  const int span0 = span.first;
 
   // ---- all loads, those of the history first
   int n = 0;
@@ -113,20 +115,17 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
     for (int e = 4 * t; e < kSpan * H / 4; e += 4 * kThreads) *reinterpret_cast<uint4*>(counts + e) = make_uint4(0, 0, 0, 0);
     over = 1.0f / rep;
     lds_barrier();
-    const int low = max(span0, 0);
-    const uint32_t tokens_here = (uint32_t)(min(span0 + kSpan, a.vocab) - low);
     for (int e = t; e < n;) {
-      uint32_t now[kAhead];  // (from the span's first token on; a token that does not count is past its end)
+      int32_t now[kAhead];  // places in the span, or -1
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) now[i] = e + i * kThreads < n ? (uint32_t)token[i] - (uint32_t)low : ~0u;
+      for (int i = 0; i < kAhead; ++i) now[i] = e + i * kThreads < n ? span.place(token[i]) : -1;
       e += kAhead * kThreads;
       tokens(e);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        if (now[i] >= tokens_here) continue;
-        const int at = (int)now[i] + low - span0;
-        if (H == 2) atomicAdd(counts + at / 2, at & 1 ? 0x10000u : 1u);
-        else atomicAdd(counts + at, 1u);
+        if (now[i] < 0) continue;
+        if (H == 2) atomicAdd(counts + now[i] / 2, now[i] & 1 ? 0x10000u : 1u);
+        else atomicAdd(counts + now[i], 1u);
       }
     }
     lds_barrier();
@@ -188,7 +187,7 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
 template <typename T, int N, int V, int H, bool BIAS, bool MASK>
 hipError_t run(const LogitsArgs& a, hipStream_t stream) {
   constexpr int kSpan = kThreads * N * V;
-  const int spans = (int)(((int64_t)a.vocab + (N - 1) + kSpan - 1) / kSpan);
+  const int spans = logits_spans(a.vocab, N, kSpan);
   return for_launches((int64_t)a.rows * spans, kThreads, [&](int64_t first, unsigned blocks) {
     sfe_logits_kernel<T, N, V, H, BIAS, MASK><<<dim3(blocks), dim3(kThreads), 0, stream>>>(a, first / spans, (uint32_t)(first % spans), (uint32_t)spans);
     return hipGetLastError();

@@ -1,0 +1,32 @@
+"""Steered logits where their kernel's forms meet, against 64 bits: vocabularies next to a span's end, and histories at
+which the spans and the counts change."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+from test_gpu_decode import U, gen, ops, steered, torch_dtype, within  # noqa: E402, F401
+
+
+def close(got, want, dtype):
+    """Values below 64: up to 6 roundings in f32, and the output's own."""
+    import torch
+    finite = torch.where(torch.isfinite(want), want.abs(), torch.zeros_like(want))
+    within(got, want, U[dtype] * finite + 6 * 2.0 ** -24 * 64)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [*range(4088, 4098), 8183, 8185, 8186, 8189, 8190, 8191, 8192, 12_287])
+def test_vocabularies_next_to_a_span_s_end(ops, vocab, dtype):  # noqa: F811
+    """A row's last span has one token, a few or none, by where the row begins."""
+    import torch
+    rows, at = 3, 5
+    wide = (3 * torch.randn(rows, vocab + 9, device="cuda", generator=gen(vocab))).to(torch_dtype(dtype))
+    history = torch.randint(-2, vocab + 2, (rows, 400), device="cuda", generator=gen(1)).int()
+    history[:, 300:] = vocab - 1 - history[:, 300:].abs() % 8
+    for x in (wide[:, :vocab].contiguous(), wide[:, at:at + vocab]):
+        close(ops.adjust_logits(x, history=history, repetition=1.25, frequency=0.03125),
+              steered(x, history, None, 1.25, 0.0, 0.03125, None, None, None), dtype)
+    out = torch.full_like(wide, 9.0)
+    ops.adjust_logits(wide[:, at:at + vocab], history=history, presence=0.5, out=out[:, at:at + vocab])
+    assert torch.equal(out[:, at:at + vocab], ops.adjust_logits(wide[:, at:at + vocab].contiguous(), history=history, presence=0.5))
+    assert (out[:, :at] == 9.0).all() and (out[:, at + vocab:] == 9.0).all()

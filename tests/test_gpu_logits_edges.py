@@ -30,3 +30,25 @@ def test_vocabularies_next_to_a_span_s_end(ops, vocab, dtype):  # noqa: F811
     ops.adjust_logits(wide[:, at:at + vocab], history=history, presence=0.5, out=out[:, at:at + vocab])
     assert torch.equal(out[:, at:at + vocab], ops.adjust_logits(wide[:, at:at + vocab].contiguous(), history=history, presence=0.5))
     assert (out[:, :at] == 9.0).all() and (out[:, at + vocab:] == 9.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("most", [4096, 4097, 65_535, 65_536])
+@pytest.mark.parametrize("bias", [False, True])
+def test_long_histories(ops, most, bias, dtype):  # noqa: F811
+    """Spans of 4,096 and 8,192 tokens, counts of 16 and 32 bits: a row that says one token throughout beside rows
+    whose tokens are the neighbours of it, and rows of any tokens over all spans."""
+    import torch
+    vocab, rows = 20_011, 4
+    g = gen(most)
+    logits = (3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(torch_dtype(dtype))
+    history = torch.randint(-2, vocab + 2, (rows, most), device="cuda", generator=g).int()
+    history[0] = 8191                            # one token, a span's last
+    history[1, 1::2], history[1, ::2] = 8192, 8193
+    history[2, :most - 1], history[2, most - 1] = 12_288, 12_289
+    lengths = torch.tensor([most, most, most + 5, most - 1], dtype=torch.int32, device="cuda")
+    args = dict(history=history, lengths=lengths, repetition=1.25, presence=0.5, frequency=2.0 ** -13,
+                bias=torch.randn(vocab, device="cuda", generator=g) if bias else None, allowed=None, states=None)
+    want = steered(logits, **args)
+    assert want.abs().max() < 64
+    close(ops.adjust_logits(logits, **args), want, dtype)

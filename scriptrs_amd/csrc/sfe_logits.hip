@@ -152,10 +152,11 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
             // (off by 1.5 steps of f32 before the one rounding to 16 bits)
             y = z[i] * (z[i] > 0.0f ? over : rep);
           } else {
-            // the quotient by its reciprocal, corrected by the remainder (none of an infinity)
+            // the quotient by its reciprocal, corrected by the remainder; where that is past the largest number,
+            // by a division (the quotient may be it yet, and an infinity has no remainder)
             y = z[i] * over;
-            const float left = __builtin_fmaf(-y, rep, z[i]);
-            y = left == left ? __builtin_fmaf(left, over, y) : y;
+            if (__builtin_isfinite(y)) y = __builtin_fmaf(__builtin_fmaf(-y, rep, z[i]), over, y);
+            else y = z[i] / rep;
             y = z[i] > 0.0f ? y : z[i] * rep;
           }
           y -= presence + frequency * (float)count;

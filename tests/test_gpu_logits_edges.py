@@ -52,3 +52,28 @@ def test_long_histories(ops, most, bias, dtype):  # noqa: F811
     want = steered(logits, **args)
     assert want.abs().max() < 64
     close(ops.adjust_logits(logits, **args), want, dtype)
+
+
+@pytest.mark.parametrize("each", [False, True])
+def test_quotients_that_overflow(ops, each):  # noqa: F811
+    """f32 logits over a repetition below one: infinite where the quotient is past f32's largest, and the quotient up to it."""
+    import numpy as np
+    import torch
+    big = float(np.finfo(np.float32).max)
+    values = [big, 3e38, 1.7014118e38, np.float32(big) / 2, 1e38, 1.0, 0.0, -1.0, -3e38, -big, float("inf"), -float("inf"), 1e-45, 2.0 ** -130]
+    for repetition in (0.5, 0.3, 0.7, 0.9999999, 1e-20, 2.0 ** -126, 1.5, 1e20, 3e38):
+        rep = np.float32(repetition)
+        with np.errstate(over="ignore", invalid="ignore", under="ignore"):
+            edge = np.float32(big) * rep  # (quotients next to the largest number)
+            x = np.array(values + [np.nextafter(edge, s * np.float32(np.inf)) for s in (1, -1)] + [edge], np.float32)
+            want = np.where(x > 0, x / rep, x * rep)
+        logits = torch.from_numpy(np.stack([x, x])).cuda()
+        history = torch.arange(len(x), dtype=torch.int32, device="cuda").repeat(2, 1)
+        got = ops.adjust_logits(logits, history=history, repetition=torch.full((2,), repetition, device="cuda") if each else repetition)
+        for row in got.cpu().numpy():
+            same = (row == want) | (np.isnan(row) & np.isnan(want))
+            # (a quotient is right to a step, below the normal numbers to the least step)
+            finite = np.isfinite(row) & np.isfinite(want)
+            err = np.abs(np.where(finite, row, 0.0).astype(np.float64) - np.where(finite, want, 0.0))
+            close_by = finite & (err <= 2.0 ** -23 * np.abs(want) + 2.0 ** -149)
+            assert (same | close_by).all(), (repetition, x[~(same | close_by)], row[~(same | close_by)], want[~(same | close_by)])

@@ -335,7 +335,7 @@ int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_
     const Rows others[] = {rows_of("q", *q, plan->rows, plan->heads, plan->dim, 2), call.memory, call.table, call.lengths,
                            Rows("tree", tree, tree ? 1 : 0, 0, plan->rows * 8)};
     for (const Rows& o : others)
-      if (plan->rows > 0 && share(mine, o)) return op_fail(SFE_INVALID_ARG, std::string("out overlaps ") + o.name);
+      if (share(mine, o)) return op_fail(SFE_INVALID_ARG, std::string("out overlaps ") + o.name);
     struct Call {
       sfe::CacheAttnArgs a;
       const sfe_cache_plan* plan;

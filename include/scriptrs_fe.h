@@ -499,7 +499,7 @@ typedef struct sfe_logits {
   const int32_t* history;
   int64_t history_row;
   const int32_t* lengths;
-  /* Of all rows, or of each (f32 [rows]) where the pointer is not NULL.  repetition is positive. */
+  /* Of all rows, or of each (f32 [rows]) where the pointer is not NULL.  repetition is at least 2^-126. */
   float repetition, presence, frequency;
   const float *repetitions, *presences, *frequencies;
   const float* bias; /* f32, rows bias_row apart (0: one for all rows); NULL: none */

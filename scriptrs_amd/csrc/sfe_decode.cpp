@@ -387,8 +387,9 @@ int sfe_adjust_logits(sfe_ctx* ctx, const sfe_logits* l, void* stream) {
     if (l->history && (l->history_most < 0 || l->history_most > 1 << 30))
       return op_fail(SFE_INVALID_ARG, "history_most must be in [0, 2^30]");
     if (!l->history && l->lengths) return op_fail(SFE_INVALID_ARG, "lengths without a history");
-    if (!l->repetitions && (!(l->repetition > 0.0f) || !isfinite(l->repetition)))
-      return op_fail(SFE_INVALID_ARG, "repetition must be positive and finite");
+    // (below f32's normal numbers its reciprocal, which quotients are products with, is infinite)
+    if (!l->repetitions && (!(l->repetition >= 0x1p-126f) || !isfinite(l->repetition)))
+      return op_fail(SFE_INVALID_ARG, "repetition must be finite and at least 2^-126");
     if ((!l->presences && !isfinite(l->presence)) || (!l->frequencies && !isfinite(l->frequency)))
       return op_fail(SFE_INVALID_ARG, "presence and frequency must be finite");
     if (l->allowed && l->n_allowed < 0) return op_fail(SFE_INVALID_ARG, "negative n_allowed");

@@ -731,7 +731,7 @@ class ModelOps:
                       allowed=None, states=None, stream=None, out=None):
         """``logits`` [rows, vocab] steered before a choice.  A token that stands c > 0 times in its row's ``history``
         [rows, most] int32 (its first ``lengths`` [rows] int32; tokens outside the vocabulary count for
-        nothing) has its logit divided by ``repetition``, or multiplied where it is not positive, then less
+        nothing) has its logit divided by ``repetition`` (at least 2^-126), or multiplied where it is not positive, then less
         ``presence + frequency * c`` (numbers, or float32 [rows]); ``bias`` float32 [vocab] or [rows, vocab] is
         added; tokens that the row's mask lacks get -inf: ``allowed`` int32 [masks, words] has token t's bit in bit t % 32 of
         word t // 32, ``states`` [rows] int32 say which mask (outside [0, masks): none; without states, row r takes

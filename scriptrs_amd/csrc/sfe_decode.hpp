@@ -104,11 +104,8 @@ struct LogitsSpan {
   int32_t first;    // token of its first place
   int32_t low;      // first token of the row that it has
   uint32_t tokens;  // that it has
-  // The place of a token, or -1 where the span has no such.
-  __host__ __device__ int32_t place(int32_t token) const {
-    const uint32_t at = (uint32_t)token - (uint32_t)low;
-    return at < tokens ? (int32_t)at + low - first : -1;
-  }
+  __host__ __device__ bool has(int32_t token) const { return (uint32_t)token - (uint32_t)low < tokens; }
+  __host__ __device__ int32_t place(int32_t token) const { return token - first; }  // (of a token that it has)
 };
 __host__ __device__ inline LogitsSpan logits_span(int number, int span, int before, int vocab) {
   LogitsSpan s;

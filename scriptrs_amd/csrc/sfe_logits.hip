@@ -43,7 +43,6 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
   T* out = reinterpret_cast<T*>(a.out) + r * a.out_row;
   const int before = N > 1 ? (int)((uintptr_t)in / sizeof(T) % N) : 0;
   const LogitsSpan span = logits_span((int)(block - of_first * spans), kSpan, before, a.vocab);
-  if (span.tokens == 0) return;  // (the workgroup's: past the row's end)
   const int span0 = span.first;
 
   // ---- all loads, those of the history first
@@ -116,16 +115,17 @@ __global__ __launch_bounds__(kThreads) void sfe_logits_kernel(LogitsArgs a, int6
     over = 1.0f / rep;
     lds_barrier();
     for (int e = t; e < n;) {
-      int32_t now[kAhead];  // places in the span, or -1
+      int32_t now[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) now[i] = e + i * kThreads < n ? span.place(token[i]) : -1;
+      for (int i = 0; i < kAhead; ++i) now[i] = e + i * kThreads < n ? token[i] : -1;
       e += kAhead * kThreads;
       tokens(e);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        if (now[i] < 0) continue;
-        if (H == 2) atomicAdd(counts + now[i] / 2, now[i] & 1 ? 0x10000u : 1u);
-        else atomicAdd(counts + now[i], 1u);
+        if (!span.has(now[i])) continue;
+        const int at = span.place(now[i]);
+        if (H == 2) atomicAdd(counts + at / 2, at & 1 ? 0x10000u : 1u);
+        else atomicAdd(counts + at, 1u);
       }
     }
     lds_barrier();

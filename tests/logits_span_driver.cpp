@@ -21,7 +21,7 @@ int check(int vocab, int n, int span, int before) {
     for (int64_t around : near)
       for (int64_t token = around - 9; token <= around + 9; ++token) {
         if (token < -2147483647 - 1 || token > 2147483647) continue;
-        const int at = s.place((int32_t)token);
+        const int at = s.has((int32_t)token) ? s.place((int32_t)token) : -1;
         const bool mine = token >= 0 && token < vocab && token >= s.first && token < (int64_t)s.first + span;
         if (at != (mine ? (int)(token - s.first) : -1)) {
           std::printf("vocab %d, vectors of %d, span %d of %d, %d before: token %lld at %d\n", vocab, n, i, span, before, (long long)token, at);

@@ -12,9 +12,10 @@
 // is free, so lanes read whole chunks of K and of V.
 //
 // Codes of 8 bits are f16 in both products, which holds them exactly: a key's scale multiplies its scores, a value's
-// scale its weight, in f32.  Weights are kept relative to a power of two above the largest value scale so far, since f16
-// lacks their range, and rounded once to 11 bits; where the queries are f16 (and outputs have 11 bits too) to 22, as two
-// numbers.  bf16 queries become f16 by a power of two of their own row.  16-bit caches multiply in their own type, weights
+// scale its weight, in f32.  Weights times value scales are kept relative to a power of two, since f16 lacks their range: it
+// goes down with the weights and up with the largest product seen, so that a token's scale counts only as far as its weight does.
+// They are rounded once to 11 bits, or where the queries are f16 (and outputs have 11 bits too) to 22, as two numbers; to
+// multiples of 2^-28 of a row's largest where that is more.  bf16 queries become f16 by a power of two of their own row.  16-bit caches multiply in their own type, weights
 // rounded once to it.
 //
 // A step is 32 keys.  Pages are looked up a step ahead; rows go from memory into LDS directly, and what lies past a
@@ -220,6 +221,11 @@ __device__ __forceinline__ void not_finite_bits(uint32_t at, uint32_t* up, uint3
 // The lowest n of 32 bits.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); }
 
+// The least unit of weights times value scales (a weight of 2^-8 times the least scale has it).
+constexpr float kLeastUnit = 0x1p-120f;
+// 1 over a power of two.
+__device__ __forceinline__ float over_power(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+
 // What an item needs of its sequence's keys: those before `end`, in rounds.
 struct Span {
   int context;  // tokens before the new ones (negative: the first new tokens are none)
@@ -312,6 +318,8 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   constexpr bool kConverted = !std::is_same<T, W>::value;           // queries are bf16, products f16
   constexpr bool kWhole = TYPE == kCacheInt8;
   constexpr bool kNotFinite = !kWhole;  // the cache's type has infinities or NaN
+  // (weights of codes are at most 1, and fit f16 by a unit of their own)
+  constexpr float kRise = kCoded ? 0.0f : M::kRise, kBelow = kCoded ? -8.0f : M::kBelow;
   constexpr int E = Kept<TYPE>::kSize, C = DP / 16;
   constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
   constexpr int kGroups = kWaves / SHARE, kRound = kGroups * kStep;  // waves by steps; keys of a round
@@ -529,12 +537,12 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     }
 
     F4 o[NR][C];
-    float m[NR], l[NR], top_scale[NR];
+    float m[NR], l[NR], unit_w[NR];  // unit_w: what weights times value scales are kept in (a power of two)
     uint32_t ups[NR], downs[NR];  // results that get +infinity and -infinity in the end, bits C j + i of o[i][j]
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       ups[n] = downs[n] = 0;
-      m[n] = kNever, l[n] = 0.0f, top_scale[n] = 0x1p-110f;
+      m[n] = kNever, l[n] = 0.0f, unit_w[n] = kLeastUnit;
 #pragma unroll
       for (int i = 0; i < C; ++i) o[n][i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -651,35 +659,22 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][u][i]);
         if (kConverted) top *= unit[n];
-        if (__any(top > m[n] + M::kRise)) {
-          top = fmaxf(top, __shfl_xor(top, 16));
-          const float nm = fmaxf(m[n], max_halves(top) - M::kBelow);
-          const float f = exp2_fast(m[n] - nm);
+        if (__any(top > m[n] + kRise)) {
+          top = max_halves(fmaxf(top, __shfl_xor(top, 16)));
+          // (whole numbers where weights have a unit: it goes down by powers of two)
+          const float nm = fmaxf(m[n], kCoded ? ceilf(top) - kBelow : top - kBelow);
+          float f = exp2_fast(m[n] - nm);
           m[n] = nm;
           l[n] *= f;
-#pragma unroll
-          for (int i = 0; i < C; ++i) o[n][i] *= f;
-        }
-        if (kCoded) {
-          float top_seen = top_value;
-          if (uneven) {
-            top_seen = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) top_seen = (see[n] >> (16 * u + i)) & 1 ? fmaxf(top_seen, vs[u][i]) : top_seen;
+          if (kCoded) {
+            const float down = unit_w[n] * f;
+            unit_w[n] = fmaxf(down, kLeastUnit);
+            f = down * over_power(unit_w[n]);  // (1 but at the least unit)
           }
-          if (__any(top_seen > top_scale[n])) {
-            top_seen = max_halves(fmaxf(top_seen, __shfl_xor(top_seen, 16)));
-            // the power of two above it
-            const float up = fmaxf(top_scale[n], __uint_as_float((min(__float_as_uint(top_seen) >> 23, 252u) + 1) << 23));
-            const float f = top_scale[n] / up;
-            top_scale[n] = up;
+          if (!kCoded || __any(f != 1.0f))
 #pragma unroll
             for (int i = 0; i < C; ++i) o[n][i] *= f;
-          }
         }
-        const float relative = __uint_as_float(0x7f000000u - __float_as_uint(top_scale[n]));  // (of a power of two)
         float x[8];  // (the unit is a power of two: nothing is lost in the product)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -689,7 +684,25 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         l[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         if (kCoded) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= vs[e / 4][e % 4] * relative;
+          for (int e = 0; e < 8; ++e) x[e] *= vs[e / 4][e % 4];
+          // weights are at most 1: up to this scale none times it passes 2^15 units
+          if (__any(top_value > unit_w[n] * 0x1p15f)) {
+            float most = 0.0f;  // (of seen keys: the others' weights are zero, or not numbers times a scale that is not finite)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, x[e]);
+            most = max_halves(fmaxf(most, __shfl_xor(most, 16)));
+            if (__any(most > unit_w[n] * 0x1p7f)) {
+              // the largest becomes 2^4 to 2^5 units, so that ordinary scales do not come here again
+              const float to = most > unit_w[n] * 0x1p7f ? __uint_as_float((min(__float_as_uint(most) >> 23, 250u) - 4) << 23) : unit_w[n];
+              const float f = unit_w[n] * over_power(to);
+              unit_w[n] = to;
+#pragma unroll
+              for (int i = 0; i < C; ++i) o[n][i] *= f;
+            }
+          }
+          const float relative = over_power(unit_w[n]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= relative;
           if (uneven)  // (0 times a scale that is not finite)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = (see[n] >> (16 * (e / 4) + e % 4)) & 1 ? x[e] : 0.0f;
@@ -732,7 +745,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       l[n] = sum_halves(l[n]);
       if (kCoded)
 #pragma unroll
-        for (int i = 0; i < C; ++i) o[n][i] *= top_scale[n];
+        for (int i = 0; i < C; ++i) o[n][i] *= unit_w[n];
     }
     if constexpr (kNotFinite)
 #pragma unroll

@@ -1,0 +1,54 @@
+"""Attention over a paged cache at the ends of what its types hold, against 64 bits: value scales far apart."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+from test_gpu_decode import KINDS, TOP, U, attended, gen, ops, quantised, torch_dtype, within  # noqa: E402, F401
+
+CODED = [x for x in KINDS if x[0] in TOP]
+
+
+def filled(ops, k, v, kind, page=16):  # noqa: F811
+    """A cache of one sequence's k, v [tokens, kv_heads, dim], its page table and length."""
+    import torch
+    from scriptrs_amd import KvCache
+    n, K, D = k.shape
+    cache = KvCache(-(-n // page), page, K, D, dtype=kind)
+    table = torch.arange(cache.pages, device="cuda", dtype=torch.int32).flip(0)[None].contiguous()
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    ops.cache_write(ops.cache_plan([0, n], K, K, D), cache, table, length, k, v)
+    return cache, table, length
+
+
+def attend(ops, q, held, K, scale=None, tree=None):  # noqa: F811
+    rows, H, D = q.shape
+    return ops.cache_attention(ops.cache_plan([0, rows], H, K, D), *held, q, tree=tree, scale=scale)
+
+
+@pytest.mark.parametrize("kind,dtype", CODED)
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("ratio", [2.0 ** 20, 2.0 ** 26, 2.0 ** 30, 2.0 ** 60])
+def test_a_large_value_of_next_to_no_weight(ops, ratio, rising, kind, dtype):  # noqa: F811
+    """A token that a row sees with a weight of e^-60 of the rest, and values far above theirs: what the others' weights add up
+    to keeps its bits, wherever the token is.  rising: the others' scores rise by 80 on the way, so that the first of them weigh as
+    little."""
+    import torch
+    n, D = 256, 64
+    g = gen(3)
+    q = torch.randint(0, 2, (1, 2, D), device="cuda", generator=g).mul_(2).sub_(1).to(torch_dtype(dtype))
+    q[0, 1] = q[0, 0]
+    k = torch.randn(n, 1, D, device="cuda", generator=g)
+    if rising:
+        k += q[:, :1].float() * (torch.arange(n, device="cuda") * (80.0 / n / math.sqrt(D)))[:, None, None]
+    v = torch.randn(n, 1, D, device="cuda", generator=g)
+    for at in (0, 1, 40, 250, n - 1):
+        far, large = k.clone(), v.clone()
+        far[at, 0] = -60.0 / math.sqrt(D) * q[0, 0].float()
+        large[at] *= ratio
+        got = attend(ops, q, filled(ops, far, large, kind), 1)
+        want, size = attended(q.cpu(), quantised(far, kind), quantised(large, kind), torch.ones(1, n, dtype=torch.bool), D ** -0.5)
+        assert size.max() < 8
+        # (two roundings to 16 bits, and f32's)
+        within(got, want, (2 * U[dtype] + 2.0 ** -13) * size)

@@ -225,6 +225,34 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >=
 constexpr float kLeastUnit = 0x1p-120f;
 // 1 over a power of two.
 __device__ __forceinline__ float over_power(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+// The power of two from x on, within 2^-126 and 2^126.  A result is kept divided by that of its sum of weights, so that it is no
+// larger than the values that it is a mean of.
+__device__ __forceinline__ float power_from(float x) {
+  return __uint_as_float(min(max((__float_as_uint(x) + 0x7fffffu) & 0x7f800000u, 0x00800000u), 0x7e800000u));
+}
+// Results of the same row, each with its reference exponent and sum of weights, as one.
+template <int N>
+struct Joined {
+  float weight[N];  // of each: 0 of one that saw nothing
+  float m = kNever, sum = 0.0f;
+  __device__ __forceinline__ Joined(const float2 (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i].x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float f = x[i].x == kNever && x[i].y == 0.0f ? 0.0f : exp2_fast(x[i].x - m);
+      sum += x[i].y * f;
+      weight[i] = f * power_from(x[i].y);
+    }
+    const float over = over_power(power_from(sum));
+#pragma unroll
+    for (int i = 0; i < N; ++i) weight[i] *= over;
+  }
+  // What makes the sum of weighted results the row's (zero of a row that sees nothing).
+  __device__ __forceinline__ float last() const {
+    return sum > 0.0f || sum != sum ? 1.0f / (sum * over_power(power_from(sum))) : 0.0f;
+  }
+};
 
 // What an item needs of its sequence's keys: those before `end`, in rounds.
 struct Span {
@@ -743,9 +771,12 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
     for (int n = 0; n < NR; ++n) {
       l[n] += __shfl_xor(l[n], 16);
       l[n] = sum_halves(l[n]);
-      if (kCoded)
+      const float over = over_power(power_from(l[n]));
 #pragma unroll
-        for (int i = 0; i < C; ++i) o[n][i] *= unit_w[n];
+      for (int i = 0; i < C; ++i) {
+        o[n][i] *= over;
+        if (kCoded) o[n][i] *= unit_w[n];
+      }
     }
     if constexpr (kNotFinite)
 #pragma unroll
@@ -799,27 +830,21 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         const int of = e / (16 * (DP / 4)), row16 = e / (DP / 4) % 16, d = 4 * (e % (DP / 4));  // (of: the member)
         const int row = 16 * (NR * of + n) + row16;
         if (row >= done.count || d >= c.dim) continue;
-        float mm = kNever;
+        float2 each[kGroups];
 #pragma unroll
-        for (int v = 0; v < kGroups; ++v) mm = fmaxf(mm, ml[(v * SHARE + of) * 16 + row16].x);
+        for (int v = 0; v < kGroups; ++v) each[v] = ml[(v * SHARE + of) * 16 + row16];
+        const Joined<kGroups> joined(each);
         F4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kGroups; ++v) {
-          const int from = (v * SHARE + of) * 16 + row16;
-          const float2 x = ml[from];
-          if (x.x == kNever && x.y == 0.0f) continue;  // (saw nothing)
-          const float f = exp2_fast(x.x - mm);
-          sum += x.y * f;
-          acc += *reinterpret_cast<const F4*>(ow + from * kRowF + d) * f;
-        }
+        for (int v = 0; v < kGroups; ++v)
+          acc += *reinterpret_cast<const F4*>(ow + ((v * SHARE + of) * 16 + row16) * kRowF + d) * joined.weight[v];
         const int rr = done.at + row;
         if (cut) {
           const int64_t place = (int64_t)slot * (16 * NR * SHARE) + row;
           *reinterpret_cast<F4*>(a.part_o + place * DP + d) = acc;
-          if (d == 0) a.part_ml[place] = make_float2(mm, sum);
+          if (d == 0) a.part_ml[place] = make_float2(joined.m, joined.sum);
         } else {
-          const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;  // (a row that sees nothing is zero)
+          const float inv = joined.last();
           const int token = (int)((unsigned)rr / (unsigned)a.group);
           char* p = const_cast<char*>(a.o.data) + (done.first + token) * a.o.row + (int64_t)(done.kvh * a.group + rr - token * a.group) * a.o.head;
           const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};
@@ -864,30 +889,24 @@ __global__ __launch_bounds__(THREADS) void sfe_cache_attn_join_kernel(CacheAttnA
     for (int p = team; p < u.y; p += kTeams) {
       const float2 x = a.part_ml[place(p)];
       const F4 v = *reinterpret_cast<const F4*>(a.part_o + place(p) * DP + d);
-      if (x.x == kNever && x.y == 0.0f) continue;  // (saw nothing)
-      const float nm = fmaxf(m, x.x), f = exp2_fast(m - nm), g = exp2_fast(x.x - nm);
-      m = nm;
-      sum = sum * f + x.y * g;
-      acc = acc * f + v * g;
+      const float2 both[2] = {make_float2(m, sum), x};
+      const Joined<2> joined(both);
+      m = joined.m;
+      sum = joined.sum;
+      acc = acc * joined.weight[0] + v * joined.weight[1];
     }
   sums[team][in] = acc;
   if (d == 0) ml[team][row4] = make_float2(m, sum);
   __syncthreads();
   if (team > 0 || !there) return;
-  float top = kNever;
+  float2 each[kTeams];
 #pragma unroll
-  for (int v = 0; v < kTeams; ++v) top = fmaxf(top, ml[v][row4].x);
+  for (int v = 0; v < kTeams; ++v) each[v] = ml[v][row4];
+  const Joined<kTeams> joined(each);
   acc = F4{0.0f, 0.0f, 0.0f, 0.0f};
-  sum = 0.0f;
 #pragma unroll
-  for (int v = 0; v < kTeams; ++v) {
-    const float2 x = ml[v][row4];
-    if (x.x == kNever && x.y == 0.0f) continue;
-    const float f = exp2_fast(x.x - top);
-    sum += x.y * f;
-    acc += sums[v][in] * f;
-  }
-  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  for (int v = 0; v < kTeams; ++v) acc += sums[v][in] * joined.weight[v];
+  const float inv = joined.last();
   const int rr = tile.at + row, token = (int)((unsigned)rr / (unsigned)a.group);
   char* p = const_cast<char*>(a.o.data) + (tile.first + token) * a.o.row + (int64_t)(kvh * a.group + rr - token * a.group) * a.o.head;
   const F2 x = {acc.x * inv, acc.y * inv}, y = {acc.z * inv, acc.w * inv};

@@ -1,4 +1,5 @@
-"""Attention over a paged cache at the ends of what its types hold, against 64 bits: value scales far apart."""
+"""Attention over a paged cache at the ends of what its types hold, against 64 bits: value scales far apart and the
+largest values."""
 import math
 
 import pytest
@@ -27,6 +28,12 @@ def attend(ops, q, held, K, scale=None, tree=None):  # noqa: F811
     return ops.cache_attention(ops.cache_plan([0, rows], H, K, D), *held, q, tree=tree, scale=scale)
 
 
+def chain(rows, n):
+    """What each of the last `rows` of n tokens sees."""
+    import torch
+    return torch.arange(n)[None] <= torch.arange(n - rows, n)[:, None]
+
+
 @pytest.mark.parametrize("kind,dtype", CODED)
 @pytest.mark.parametrize("rising", [False, True])
 @pytest.mark.parametrize("ratio", [2.0 ** 20, 2.0 ** 26, 2.0 ** 30, 2.0 ** 60])
@@ -52,3 +59,19 @@ def test_a_large_value_of_next_to_no_weight(ops, ratio, rising, kind, dtype):  #
         assert size.max() < 8
         # (two roundings to 16 bits, and f32's)
         within(got, want, (2 * U[dtype] + 2.0 ** -13) * size)
+
+
+@pytest.mark.parametrize("kind", sorted(TOP))
+@pytest.mark.parametrize("n,rows", [(1000, 1), (1000, 3), (700, 40), (20_000, 2)])
+def test_the_largest_values(ops, n, rows, kind):  # noqa: F811
+    """Means of values up to the largest of bf16 are no larger than they are, however many: no sum on the way is infinite."""
+    import torch
+    D = 64
+    g = gen(4)
+    v = ((0.5 + 0.5 * torch.rand(n, 2, D, device="cuda", generator=g)) * 3.3e38).bfloat16()
+    v[..., ::2] *= -1
+    q = (0.1 * torch.randn(rows, 4, D, device="cuda", generator=g)).bfloat16()
+    k = torch.randn(n, 2, D, device="cuda", generator=g).bfloat16()
+    got = attend(ops, q, filled(ops, k, v, kind), 2)
+    want, size = attended(q.cpu(), quantised(k, kind), quantised(v, kind), chain(rows, n), D ** -0.5)
+    within(got, want, (2 * U["bf16"] + 2.0 ** -13) * size)

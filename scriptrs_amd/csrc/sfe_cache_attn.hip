@@ -346,8 +346,10 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   constexpr bool kConverted = !std::is_same<T, W>::value;           // queries are bf16, products f16
   constexpr bool kWhole = TYPE == kCacheInt8;
   constexpr bool kNotFinite = !kWhole;  // the cache's type has infinities or NaN
-  // (weights of codes are at most 1, and fit f16 by a unit of their own)
-  constexpr float kRise = kCoded ? 0.0f : M::kRise, kBelow = kCoded ? -8.0f : M::kBelow;
+  // Weights of codes are at most 1, and fit f16 by a unit of their own.  Those over bf16 are at most 2^-16, so that a wave's sums over
+  // its keys do not pass the largest value where their mean does not (2^16 keys of 3e38).
+  constexpr float kRise = kCoded ? 0.0f : (TYPE == kCacheBf16 ? -16.0f : M::kRise);
+  constexpr float kBelow = kCoded ? -8.0f : (TYPE == kCacheBf16 ? -24.0f : M::kBelow);
   constexpr int E = Kept<TYPE>::kSize, C = DP / 16;
   constexpr int kRowF = DP + 4;  // floats of a result's row in LDS (4 of padding)
   constexpr int kGroups = kWaves / SHARE, kRound = kGroups * kStep;  // waves by steps; keys of a round

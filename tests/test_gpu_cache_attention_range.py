@@ -61,7 +61,7 @@ def test_a_large_value_of_next_to_no_weight(ops, ratio, rising, kind, dtype):  #
         within(got, want, (2 * U[dtype] + 2.0 ** -13) * size)
 
 
-@pytest.mark.parametrize("kind", sorted(TOP))
+@pytest.mark.parametrize("kind", ["bf16", *sorted(TOP)])
 @pytest.mark.parametrize("n,rows", [(1000, 1), (1000, 3), (700, 40), (20_000, 2)])
 def test_the_largest_values(ops, n, rows, kind):  # noqa: F811
     """Means of values up to the largest of bf16 are no larger than they are, however many: no sum on the way is infinite."""
@@ -75,3 +75,34 @@ def test_the_largest_values(ops, n, rows, kind):  # noqa: F811
     got = attend(ops, q, filled(ops, k, v, kind), 2)
     want, size = attended(q.cpu(), quantised(k, kind), quantised(v, kind), chain(rows, n), D ** -0.5)
     within(got, want, (2 * U["bf16"] + 2.0 ** -13) * size)
+
+
+@pytest.mark.parametrize("kind", ["bf16", *sorted(TOP)])
+def test_small_values(ops, kind):  # noqa: F811
+    """Values down to 2^-90 keep their bits, alone and behind large weights."""
+    import torch
+    n, D = 700, 64
+    g = gen(7)
+    k, v = torch.randn(n, 2, D, device="cuda", generator=g).bfloat16(), torch.randn(n, 2, D, device="cuda", generator=g) * 2.0 ** -90
+    v = (v.sign() * v.abs().clamp(min=2.0 ** -94)).bfloat16()
+    for gain in (0.1, 8.0):
+        q = (gain * torch.randn(3, 4, D, device="cuda", generator=g)).bfloat16()
+        got = attend(ops, q, filled(ops, k, v, kind), 2)
+        want, size = attended(q.cpu(), quantised(k, kind), quantised(v, kind), chain(3, n), D ** -0.5)
+        # (gain 8: scores of up to 40, whose f32 error is 2^-24 of the sum of 64 products' magnitudes)
+        within(got, want, (2 * U["bf16"] + 2.0 ** -13) * size)
+
+
+@pytest.mark.parametrize("kind", ["bf16", *sorted(TOP)])
+def test_the_largest_values_of_many_sequences(ops, kind):  # noqa: F811
+    """As above, each workgroup over all of a sequence's 4,000 tokens."""
+    import torch
+    n, seqs, D = 4000, 300, 64
+    g = gen(8)
+    k, v = torch.randn(n, 1, D, device="cuda", generator=g).bfloat16(), torch.full((n, 1, D), 3e38, device="cuda").bfloat16()
+    cache, table, length = filled(ops, k, v, kind)
+    q = (0.1 * torch.randn(seqs, 2, D, device="cuda", generator=g)).bfloat16()
+    plan = ops.cache_plan(list(range(seqs + 1)), 2, 1, D)
+    got = ops.cache_attention(plan, cache, table.expand(seqs, -1), length.expand(seqs).contiguous(), q)
+    want = quantised(v[:1], kind).double().expand(seqs, 2, D)
+    within(got, want, (2 * U["bf16"] + 2.0 ** -13) * want.abs())

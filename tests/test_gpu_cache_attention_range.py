@@ -1,5 +1,5 @@
-"""Attention over a paged cache at the ends of what its types hold, against 64 bits: value scales far apart and the
-largest values."""
+"""Attention over a paged cache at the ends of what its types hold, against 64 bits: value scales far apart, the
+largest values, scores past f32."""
 import math
 
 import pytest
@@ -106,3 +106,29 @@ def test_the_largest_values_of_many_sequences(ops, kind):  # noqa: F811
     got = ops.cache_attention(plan, cache, table.expand(seqs, -1), length.expand(seqs).contiguous(), q)
     want = quantised(v[:1], kind).double().expand(seqs, 2, D)
     within(got, want, (2 * U["bf16"] + 2.0 ** -13) * want.abs())
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+def test_scores_past_f32(ops, kind, dtype):  # noqa: F811
+    """A row whose scores are infinite in f32 is NaN, and not zeros as of a row that sees nothing; others keep theirs.  bf16: queries of
+    1e36 and keys of 1e4, whose 64 products of either sign add up to 1e40; f16: 6e4 and 1e4 make 1e9, and the scale 1e39."""
+    import torch
+    n, D = 200, 64
+    g = gen(5)
+    kv = torch.randn(n, 2, D, device="cuda", generator=g)
+    kv[:, 0] *= 1e4
+    kv = kv.to(torch_dtype(dtype))
+    held = filled(ops, kv[:, :1], kv[:, 1:], kind)
+    scale = 1e30 if dtype == "f16" else None
+    for m in (2, 20):
+        q = torch.randn(m, 2, D, device="cuda", generator=g).to(torch_dtype(dtype))
+        want = attend(ops, q, held, 1, scale=scale)
+        large = q.clone()
+        large[1, 1] = 60000.0 if dtype == "f16" else 1e36
+        got = attend(ops, large, held, 1, scale=scale)
+        keep = torch.ones(m, 2, dtype=torch.bool, device="cuda")
+        keep[1, 1] = False
+        assert torch.equal(got[keep], want[keep])
+        assert got[1, 1].isnan().all()
+        if kind in TOP:  # (codes' products stay in range: a scale that brings their sum back does)
+            assert attend(ops, large, held, 1, scale=1e-9 if dtype == "bf16" else 1.0)[1, 1].isfinite().all()

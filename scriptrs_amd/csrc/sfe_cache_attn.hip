@@ -709,7 +709,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float y = s[n][e / 4][e % 4];
-          x[e] = exp2_fast(kConverted ? __builtin_fmaf(y, unit[n], -m[n]) : y - m[n]);
+          x[e] = exp2_fast(kConverted ? __builtin_fmaf(y, unit[n], -m[n]) : rounded_less(y, m[n]));
         }
         l[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         if (kCoded) {

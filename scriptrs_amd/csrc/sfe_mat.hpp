@@ -66,6 +66,13 @@ __device__ __forceinline__ float scaled_less(float s, float c, float m) {
   return x - m;
 }
 
+// a - b, where a is a rounded product already (never one fused operation with it: the reference b of a row of large scores is
+// such a product, and an exact one less it would be off by its rounding).
+__device__ __forceinline__ float rounded_less(float a, float b) {
+#pragma clang fp contract(off)
+  return a - b;
+}
+
 // The larger (sum) of this lane's value and that of the lane 32 away.
 __device__ __forceinline__ float max_halves(float x) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

@@ -1,5 +1,5 @@
 """Attention over a paged cache at the ends of what its types hold, against 64 bits: value scales far apart, the
-largest values, scores past f32."""
+largest values, scores far from one and past f32."""
 import math
 
 import pytest
@@ -132,3 +132,32 @@ def test_scores_past_f32(ops, kind, dtype):  # noqa: F811
         assert got[1, 1].isnan().all()
         if kind in TOP:  # (codes' products stay in range: a scale that brings their sum back does)
             assert attend(ops, large, held, 1, scale=1e-9 if dtype == "bf16" else 1.0)[1, 1].isfinite().all()
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("scale", [2.0 ** 20, 1e25, 1e30])
+def test_scores_far_past_one(ops, scale, kind, dtype):  # noqa: F811
+    """Whole numbers as keys and queries, which every type holds (the largest magnitude is the largest code): scores are exact up to the
+    scale, differ by a scale at least, and so a row is the mean of its best keys' values."""
+    import torch
+    n, D = 300, 64
+    rng = torch.Generator().manual_seed(6)
+    k = torch.randint(-4, 5, (n, 1, D), generator=rng).float() * 16
+    k[..., 0] = TOP.get(kind, 448.0)
+    if kind == "int8":
+        k[..., 1:] /= 8
+    k[200:220] = k[30:50]  # (ties)
+    v = torch.randn(n, 1, D, generator=rng)
+    for m in (1, 20):
+        q = torch.randint(-2, 3, (m, 2, D), generator=rng).to(torch_dtype(dtype))
+        held = filled(ops, k.cuda(), v.cuda(), kind)
+        got = attend(ops, q.cuda(), held, 1, scale=scale)
+        kq, vq, see = quantised(k, kind), quantised(v, kind).double(), chain(m, n)
+        assert torch.equal(kq, k)
+        want, size = torch.zeros(m, 2, D, dtype=torch.float64), torch.zeros(m, 2, D, dtype=torch.float64)
+        for i in range(m):
+            for h in range(2):
+                s = torch.where(see[i], k[:, 0].double() @ q[i, h].double(), torch.tensor(-math.inf, dtype=torch.float64))
+                best = vq[s == s.max(), 0]
+                want[i, h], size[i, h] = best.mean(0), best.abs().mean(0)
+        within(got, want, (2 * U[dtype] + 2.0 ** -13) * size)

@@ -77,22 +77,16 @@ struct Ring {
 typedef uint32_t U2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
-// Two e4m3 codes as 16-bit values.
-template <typename T, int TYPE, int WORD>
+// Two e4m3 codes in f16.
+template <int WORD>
 __device__ __forceinline__ uint32_t pair_of(uint32_t x) {
-  if constexpr (std::is_same<T, Bf>::value)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, WORD != 0));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, WORD != 0));
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, WORD != 0));
 }
-// An int8 code of each of two words as 16-bit values.
-template <typename T, int BYTE>
+// An int8 code of each of two words in f16.
+template <int BYTE>
 __device__ __forceinline__ uint32_t whole_pair(uint32_t x, uint32_t y) {
   const float a = (float)(int8_t)(x >> (8 * BYTE)), b = (float)(int8_t)(y >> (8 * BYTE));
-  if constexpr (std::is_same<T, Bf>::value)  // (8 bits: the lower half of the f32 is zero)
-    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
 
 // The type that both products are in: f16 for codes, whose weights then keep 11 bits also where the queries are bf16.
@@ -124,10 +118,10 @@ __device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typena
             y[2 * i + 1] = __builtin_amdgcn_perm(0x64646464u, w, 0x04030402);
           }
         } else {
-          y.x = pair_of<T, TYPE, 0>(x[2 * h]);
-          y.y = pair_of<T, TYPE, 1>(x[2 * h]);
-          y.z = pair_of<T, TYPE, 0>(x[2 * h + 1]);
-          y.w = pair_of<T, TYPE, 1>(x[2 * h + 1]);
+          y.x = pair_of<0>(x[2 * h]);
+          y.y = pair_of<1>(x[2 * h]);
+          y.z = pair_of<0>(x[2 * h + 1]);
+          y.w = pair_of<1>(x[2 * h + 1]);
         }
         k[2 * t + h] = __builtin_bit_cast(V8, y);
       }
@@ -162,10 +156,10 @@ __device__ __forceinline__ void values_of(uint32_t (&addr)[4], uint32_t at, type
     if constexpr (TYPE == kCacheInt8) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        y[4 * w][e] = whole_pair<T, 0>(raw[2 * e][w], raw[2 * e + 1][w]);
-        y[4 * w + 1][e] = whole_pair<T, 1>(raw[2 * e][w], raw[2 * e + 1][w]);
-        y[4 * w + 2][e] = whole_pair<T, 2>(raw[2 * e][w], raw[2 * e + 1][w]);
-        y[4 * w + 3][e] = whole_pair<T, 3>(raw[2 * e][w], raw[2 * e + 1][w]);
+        y[4 * w][e] = whole_pair<0>(raw[2 * e][w], raw[2 * e + 1][w]);
+        y[4 * w + 1][e] = whole_pair<1>(raw[2 * e][w], raw[2 * e + 1][w]);
+        y[4 * w + 2][e] = whole_pair<2>(raw[2 * e][w], raw[2 * e + 1][w]);
+        y[4 * w + 3][e] = whole_pair<3>(raw[2 * e][w], raw[2 * e + 1][w]);
       }
     } else {
       uint32_t a[C / 2], b[C / 2];  // channels by twos of either row
@@ -174,8 +168,8 @@ __device__ __forceinline__ void values_of(uint32_t (&addr)[4], uint32_t at, type
         if constexpr (E == 2) {
           a[w] = raw[2 * e][w], b[w] = raw[2 * e + 1][w];
         } else {
-          a[2 * w] = pair_of<T, TYPE, 0>(raw[2 * e][w]), a[2 * w + 1] = pair_of<T, TYPE, 1>(raw[2 * e][w]);
-          b[2 * w] = pair_of<T, TYPE, 0>(raw[2 * e + 1][w]), b[2 * w + 1] = pair_of<T, TYPE, 1>(raw[2 * e + 1][w]);
+          a[2 * w] = pair_of<0>(raw[2 * e][w]), a[2 * w + 1] = pair_of<1>(raw[2 * e][w]);
+          b[2 * w] = pair_of<0>(raw[2 * e + 1][w]), b[2 * w + 1] = pair_of<1>(raw[2 * e + 1][w]);
         }
       }
 #pragma unroll

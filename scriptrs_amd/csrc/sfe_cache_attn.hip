@@ -92,9 +92,15 @@ __device__ __forceinline__ uint32_t whole_pair(uint32_t x, uint32_t y) {
 // The type that both products are in: f16 for codes, whose weights then keep 11 bits also where the queries are bf16.
 template <typename T, int TYPE>
 using Product = typename std::conditional<Kept<TYPE>::kSize == 1, Hf, T>::type;
-// int8 codes become f16 in one operation a pair for the first product: the code plus 128 as the low bits
-// of 1024, so that a key's channels are 1152 more than its codes, which the product starts less of.
-constexpr float kCodeOffset = 1152.0f;
+// Codes 2 WORD and 2 WORD + 1 of four int8 codes and 128 each: the low bits of 1024 in f16, of which 1152 are taken off.  (1152 times the
+// queries' sum taken off the product instead is an operation a pair less, and 4% of an output where queries of 1,000 meet keys
+// of one channel.)
+template <int WORD>
+__device__ __forceinline__ uint32_t offset_pair(uint32_t x) {
+  typedef Mat<Hf>::V2 V2;
+  const V2 more = __builtin_bit_cast(V2, __builtin_amdgcn_perm(0x64646464u, x, WORD ? 0x04030402 : 0x04010400));
+  return __builtin_bit_cast(uint32_t, more - V2{(Hf)1152.0f, (Hf)1152.0f});
+}
 
 // Operands of 16 keys' rows for all k steps of the first product: 32 channels each.
 template <typename T, int TYPE, int DP>
@@ -114,8 +120,8 @@ __device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typena
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t w = x[2 * h + i] ^ 0x80808080u;
-            y[2 * i] = __builtin_amdgcn_perm(0x64646464u, w, 0x04010400);
-            y[2 * i + 1] = __builtin_amdgcn_perm(0x64646464u, w, 0x04030402);
+            y[2 * i] = offset_pair<0>(w);
+            y[2 * i + 1] = offset_pair<1>(w);
           }
         } else {
           y.x = pair_of<0>(x[2 * h]);
@@ -338,8 +344,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   constexpr bool kCoded = Kept<TYPE>::kSize == 1;
   constexpr bool kSplit = kCoded && std::is_same<T, Hf>::value;  // a weight is two 16-bit numbers
   constexpr bool kConverted = !std::is_same<T, W>::value;           // queries are bf16, products f16
-  constexpr bool kWhole = TYPE == kCacheInt8;
-  constexpr bool kNotFinite = !kWhole;  // the cache's type has infinities or NaN
+  constexpr bool kNotFinite = TYPE != kCacheInt8;  // the cache's type has infinities or NaN
   // Weights of codes are at most 1, and fit f16 by a unit of their own.  Those over bf16 are at most 2^-16, so that a wave's sums over
   // its keys do not pass the largest value where their mean does not (2^16 keys of 3e38).
   constexpr float kRise = kCoded ? 0.0f : (TYPE == kCacheBf16 ? -16.0f : M::kRise);
@@ -513,10 +518,10 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       there_next = load_step(u, r0 + 1, 1, page_next);
       look_up(u, r0 + 2, page);
     }
-    float start[NR], unit[NR];  // what the rows' scores begin at, and the power of two that is their unit
+    float unit[NR];  // the power of two that is the unit of a row's scores
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      start[n] = 0.0f, unit[n] = 1.0f;
+      unit[n] = 1.0f;
       if constexpr (kConverted) {
         // bf16 queries in f16, each row by a power of two of its own that takes its largest finite one to 2^14 (the least
         // that f16 holds is 2^-38 of it: what is lost is far below the scores' own rounding)
@@ -548,18 +553,6 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         }
       }
     }
-    if constexpr (kWhole) {
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) start[n] += (float)__builtin_bit_cast(Hf, (short)q[n][i][j]);
-        start[n] += __shfl_xor(start[n], 16);
-        start[n] = -kCodeOffset * sum_halves(start[n]);
-      }
-    }
-
     F4 o[NR][C];
     float m[NR], l[NR], unit_w[NR];  // unit_w: what weights times value scales are kept in (a power of two)
     uint32_t ups[NR], downs[NR];  // results that get +infinity and -infinity in the end, bits C j + i of o[i][j]
@@ -603,7 +596,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          s[n][u] = F4{start[n], start[n], start[n], start[n]};
+          s[n][u] = F4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int i = 0; i < DP / 32; ++i) s[n][u] = M::m16(k[i], __builtin_bit_cast(V8, q[n][i]), s[n][u]);
         }

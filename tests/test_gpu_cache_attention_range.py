@@ -161,3 +161,24 @@ def test_scores_far_past_one(ops, scale, kind, dtype):  # noqa: F811
                 best = vq[s == s.max(), 0]
                 want[i, h], size[i, h] = best.mean(0), best.abs().mean(0)
         within(got, want, (2 * U[dtype] + 2.0 ** -13) * size)
+
+
+@pytest.mark.parametrize("kind", sorted(TOP))
+def test_scores_of_large_queries_and_few_channels(ops, kind):  # noqa: F811
+    """Keys of one channel, queries that are all large: a score has the bits of its one product, whatever the channels without a
+    part in it.  Scores of 1,000 that differ by a few: 3 roundings of f32 (product, key's scale, scale of the logarithm) of 1,445 each."""
+    import torch
+    n, D = 6, 128
+    rng = torch.Generator().manual_seed(9)
+    k, v = torch.zeros(n, 1, D), torch.randn(n, 1, D, generator=rng)
+    k[torch.arange(n), 0, torch.arange(n) * 20 + 3] = 1.0
+    for m in (1, 20):
+        q = 1000 + 0.5 * torch.randint(0, 6, (m, 2, D), generator=rng)
+        held = filled(ops, k.cuda(), v.cuda(), kind)
+        got = ops.cache_attention(ops.cache_plan([0, m], 2, 1, D), held[0], held[1], held[2], q.half().cuda(),
+                                  tree=torch.full((m,), (1 << m) - 1 if m > 1 else 1, dtype=torch.int64, device="cuda"), scale=1.0)
+        see = torch.ones(m, n, dtype=torch.bool)
+        if m > n:  # (new tokens before the first are none, and see nothing)
+            see[:m - n] = False
+        want, size = attended(q, k, quantised(v, kind), see, 1.0)
+        within(got, want, (2 * U["f16"] + 2.0 ** -13 + 2 * 3 * 2.0 ** -24 * 1445) * size)

@@ -11,12 +11,11 @@
 // keys that O^T = V^T P^T takes from it, once V's rows are paired by key in registers.  The order of channels in a product
 // is free, so lanes read whole chunks of K and of V.
 //
-// Codes of 8 bits are f16 in both products, which holds them exactly: a key's scale multiplies its scores, a value's
-// scale its weight, in f32.  Weights times value scales are kept relative to a power of two, since f16 lacks their range: it
+// Codes of 8 bits are of the queries' type in the first product and f16 in the second, both of which hold them exactly: a key's scale
+// multiplies its scores, a value's scale its weight, in f32.  Weights times value scales are kept relative to a power of two, since f16 lacks their range: it
 // goes down with the weights and up with the largest product seen, so that a token's scale counts only as far as its weight does.
 // They are rounded once to 11 bits, or where the queries are f16 (and outputs have 11 bits too) to 22, as two numbers; to
-// multiples of 2^-28 of a row's largest where that is more.  bf16 queries become f16 by a power of two of their own row.  16-bit caches multiply in their own type, weights
-// rounded once to it.
+// multiples of 2^-28 of a row's largest where that is more.  16-bit caches multiply in their own type, weights rounded once to it.
 //
 // A step is 32 keys.  Pages are looked up a step ahead; rows go from memory into LDS directly, and what lies past a
 // sequence's end or in no page is read as zeros by the buffer's range, so that nothing is read outside a record.  Up to 32 rows
@@ -77,30 +76,36 @@ struct Ring {
 typedef uint32_t U2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
-// Two e4m3 codes in f16.
-template <int WORD>
+// Two e4m3 codes as 16-bit values.
+template <typename T, int WORD>
 __device__ __forceinline__ uint32_t pair_of(uint32_t x) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, WORD != 0));
+  if constexpr (std::is_same<T, Bf>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, WORD != 0));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, WORD != 0));
 }
-// An int8 code of each of two words in f16.
-template <int BYTE>
-__device__ __forceinline__ uint32_t whole_pair(uint32_t x, uint32_t y) {
-  const float a = (float)(int8_t)(x >> (8 * BYTE)), b = (float)(int8_t)(y >> (8 * BYTE));
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+// Two int8 codes as 16-bit values.
+template <typename T>
+__device__ __forceinline__ uint32_t whole_pair(int8_t x, int8_t y) {
+  const float a = (float)x, b = (float)y;
+  if constexpr (std::is_same<T, Bf>::value)  // (8 bits: the lower half of the f32 is zero)
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
-
-// The type that both products are in: f16 for codes, whose weights then keep 11 bits also where the queries are bf16.
-template <typename T, int TYPE>
-using Product = typename std::conditional<Kept<TYPE>::kSize == 1, Hf, T>::type;
-// Codes 2 WORD and 2 WORD + 1 of four int8 codes and 128 each: the low bits of 1024 in f16, of which 1152 are taken off.  (1152 times the
-// queries' sum taken off the product instead is an operation a pair less, and 4% of an output where queries of 1,000 meet keys
-// of one channel.)
+// Codes 2 WORD and 2 WORD + 1 of four int8 codes in f16: with 128 more they are the low bits of 1024, of which 1152 are taken
+// off.  (1152 times the queries' sum taken off the product instead is an operation a pair less, and 4% of an output where
+// queries of 1,000 meet keys of one channel.)
 template <int WORD>
 __device__ __forceinline__ uint32_t offset_pair(uint32_t x) {
   typedef Mat<Hf>::V2 V2;
-  const V2 more = __builtin_bit_cast(V2, __builtin_amdgcn_perm(0x64646464u, x, WORD ? 0x04030402 : 0x04010400));
+  const V2 more = __builtin_bit_cast(V2, __builtin_amdgcn_perm(0x64646464u, x ^ 0x80808080u, WORD ? 0x04030402 : 0x04010400));
   return __builtin_bit_cast(uint32_t, more - V2{(Hf)1152.0f, (Hf)1152.0f});
 }
+
+// The type that the second product is in: f16 for codes, whose weights then keep 11 bits also where the queries are bf16.
+template <typename T, int TYPE>
+using Product = typename std::conditional<Kept<TYPE>::kSize == 1, Hf, T>::type;
 
 // Operands of 16 keys' rows for all k steps of the first product: 32 channels each.
 template <typename T, int TYPE, int DP>
@@ -119,15 +124,20 @@ __device__ __forceinline__ void keys_of(uint32_t (&addr)[4], uint32_t at, typena
         if constexpr (TYPE == kCacheInt8) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t w = x[2 * h + i] ^ 0x80808080u;
-            y[2 * i] = offset_pair<0>(w);
-            y[2 * i + 1] = offset_pair<1>(w);
+            const uint32_t w = x[2 * h + i];
+            if constexpr (std::is_same<T, Bf>::value) {
+              y[2 * i] = whole_pair<T>((int8_t)w, (int8_t)(w >> 8));
+              y[2 * i + 1] = whole_pair<T>((int8_t)(w >> 16), (int8_t)(w >> 24));
+            } else {
+              y[2 * i] = offset_pair<0>(w);
+              y[2 * i + 1] = offset_pair<1>(w);
+            }
           }
         } else {
-          y.x = pair_of<0>(x[2 * h]);
-          y.y = pair_of<1>(x[2 * h]);
-          y.z = pair_of<0>(x[2 * h + 1]);
-          y.w = pair_of<1>(x[2 * h + 1]);
+          y.x = pair_of<T, 0>(x[2 * h]);
+          y.y = pair_of<T, 1>(x[2 * h]);
+          y.z = pair_of<T, 0>(x[2 * h + 1]);
+          y.w = pair_of<T, 1>(x[2 * h + 1]);
         }
         k[2 * t + h] = __builtin_bit_cast(V8, y);
       }
@@ -162,10 +172,9 @@ __device__ __forceinline__ void values_of(uint32_t (&addr)[4], uint32_t at, type
     if constexpr (TYPE == kCacheInt8) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        y[4 * w][e] = whole_pair<0>(raw[2 * e][w], raw[2 * e + 1][w]);
-        y[4 * w + 1][e] = whole_pair<1>(raw[2 * e][w], raw[2 * e + 1][w]);
-        y[4 * w + 2][e] = whole_pair<2>(raw[2 * e][w], raw[2 * e + 1][w]);
-        y[4 * w + 3][e] = whole_pair<3>(raw[2 * e][w], raw[2 * e + 1][w]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          y[4 * w + i][e] = whole_pair<T>((int8_t)(raw[2 * e][w] >> 8 * i), (int8_t)(raw[2 * e + 1][w] >> 8 * i));
       }
     } else {
       uint32_t a[C / 2], b[C / 2];  // channels by twos of either row
@@ -174,8 +183,8 @@ __device__ __forceinline__ void values_of(uint32_t (&addr)[4], uint32_t at, type
         if constexpr (E == 2) {
           a[w] = raw[2 * e][w], b[w] = raw[2 * e + 1][w];
         } else {
-          a[2 * w] = pair_of<0>(raw[2 * e][w]), a[2 * w + 1] = pair_of<1>(raw[2 * e][w]);
-          b[2 * w] = pair_of<0>(raw[2 * e + 1][w]), b[2 * w + 1] = pair_of<1>(raw[2 * e + 1][w]);
+          a[2 * w] = pair_of<T, 0>(raw[2 * e][w]), a[2 * w + 1] = pair_of<T, 1>(raw[2 * e][w]);
+          b[2 * w] = pair_of<T, 0>(raw[2 * e + 1][w]), b[2 * w + 1] = pair_of<T, 1>(raw[2 * e + 1][w]);
         }
       }
 #pragma unroll
@@ -342,8 +351,8 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
   typedef typename M::V2 V2;
   typedef typename Mat<T>::V2 O2;
   constexpr bool kCoded = Kept<TYPE>::kSize == 1;
+  constexpr bool kFar = kCoded && std::is_same<T, Bf>::value;     // products of queries and codes may pass f32 where scores do not
   constexpr bool kSplit = kCoded && std::is_same<T, Hf>::value;  // a weight is two 16-bit numbers
-  constexpr bool kConverted = !std::is_same<T, W>::value;           // queries are bf16, products f16
   constexpr bool kNotFinite = TYPE != kCacheInt8;  // the cache's type has infinities or NaN
   // Weights of codes are at most 1, and fit f16 by a unit of their own.  Those over bf16 are at most 2^-16, so that a wave's sums over
   // its keys do not pass the largest value where their mean does not (2^16 keys of 3e38).
@@ -518,13 +527,12 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       there_next = load_step(u, r0 + 1, 1, page_next);
       look_up(u, r0 + 2, page);
     }
-    float unit[NR];  // the power of two that is the unit of a row's scores
+    // rows of queries past 2^73 are taken down to it; the power of two is their scores' unit
+    float unit[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       unit[n] = 1.0f;
-      if constexpr (kConverted) {
-        // bf16 queries in f16, each row by a power of two of its own that takes its largest finite one to 2^14 (the least
-        // that f16 holds is 2^-38 of it: what is lost is far below the scores' own rounding)
+      if constexpr (kFar) {
         uint32_t top = 0;  // (exponents of two queries at a time, those of infinities and NaN left out)
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i) {
@@ -535,24 +543,26 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
             top = max(top, max(lo == 0x7f80u ? 0u : lo, hi == 0x7f80u ? 0u : hi));
           }
         }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-        // (below 2^-100 as if they were that: their scores are zero to any sum)
-        const int e = max((int)(top >> 7), 27);
-        unit[n] = __uint_as_float((uint32_t)(e - 14) << 23);  // 2^(e - 141)
+        if (__any(top > 200u << 7)) {
+          top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+          top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+          const int down = max((int)(top >> 7) - 200, 0);
+          unit[n] = __uint_as_float((uint32_t)(127 + down) << 23);
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-          U4 w = __builtin_bit_cast(U4, q[n][i]);
+          for (int i = 0; i < DP / 32; ++i) {
+            U4 w = __builtin_bit_cast(U4, q[n][i]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const F2 y = {__builtin_amdgcn_ldexpf(__uint_as_float(w[j] << 16), 141 - e),
-                          __builtin_amdgcn_ldexpf(__uint_as_float(w[j] & 0xffff0000u), 141 - e)};
-            w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, Mat<Hf>::V2));
+            for (int j = 0; j < 4; ++j) {
+              const F2 y = {__builtin_amdgcn_ldexpf(__uint_as_float(w[j] << 16), -down),
+                            __builtin_amdgcn_ldexpf(__uint_as_float(w[j] & 0xffff0000u), -down)};
+              w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, Mat<Bf>::V2));
+            }
+            q[n][i] = __builtin_bit_cast(S8, w);
           }
-          q[n][i] = __builtin_bit_cast(S8, w);
         }
       }
     }
+
     F4 o[NR][C];
     float m[NR], l[NR], unit_w[NR];  // unit_w: what weights times value scales are kept in (a power of two)
     uint32_t ups[NR], downs[NR];  // results that get +infinity and -infinity in the end, bits C j + i of o[i][j]
@@ -588,8 +598,8 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
       F4 s[NR][2], ks[2], vs[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        V8 k[DP / 32];
-        keys_of<W, TYPE, DP>(k_addr, in + u * R::kHalf, k);
+        typename Mat<T>::V8 k[DP / 32];
+        keys_of<T, TYPE, DP>(k_addr, in + u * R::kHalf, k);
         if (kCoded) {
           ks[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 16 * quarter) * a.scale_log2;
           vs[u] = lds_read<F4>(base + in + R::kScales + u * 256 + 64 + 16 * quarter);
@@ -598,7 +608,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         for (int n = 0; n < NR; ++n) {
           s[n][u] = F4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int i = 0; i < DP / 32; ++i) s[n][u] = M::m16(k[i], __builtin_bit_cast(V8, q[n][i]), s[n][u]);
+          for (int i = 0; i < DP / 32; ++i) s[n][u] = Mat<T>::m16(k[i], __builtin_bit_cast(typename Mat<T>::V8, q[n][i]), s[n][u]);
         }
       }
       V8 v[C];
@@ -675,7 +685,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][u][i]);
-        if (kConverted) top *= unit[n];
+        if (kFar) top *= unit[n];
         if (__any(top > m[n] + kRise)) {
           top = max_halves(fmaxf(top, __shfl_xor(top, 16)));
           // (whole numbers where weights have a unit: it goes down by powers of two)
@@ -696,7 +706,7 @@ __global__ __launch_bounds__(64 * kWaves, Kept<TYPE>::kSize == 2 && DP == 128 ? 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float y = s[n][e / 4][e % 4];
-          x[e] = exp2_fast(kConverted ? __builtin_fmaf(y, unit[n], -m[n]) : rounded_less(y, m[n]));
+          x[e] = exp2_fast(kFar ? __builtin_fmaf(y, unit[n], -m[n]) : rounded_less(y, m[n]));
         }
         l[n] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         if (kCoded) {

@@ -182,3 +182,23 @@ def test_scores_of_large_queries_and_few_channels(ops, kind):  # noqa: F811
             see[:m - n] = False
         want, size = attended(q, k, quantised(v, kind), see, 1.0)
         within(got, want, (2 * U["f16"] + 2.0 ** -13 + 2 * 3 * 2.0 ** -24 * 1445) * size)
+
+
+@pytest.mark.parametrize("kind", ["bf16", *sorted(TOP)])
+@pytest.mark.parametrize("large", [1e13, 1e30])
+def test_queries_of_very_different_channels(ops, large, kind):  # noqa: F811
+    """A channel of the queries far above the others, where all keys are zero, takes nothing from the others' part in the scores."""
+    import torch
+    n, D = 150, 64
+    g = gen(10)
+    k, v = (torch.randn(n, 1, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    k[..., 5] = 0.0
+    held = filled(ops, k, v, kind)
+    for m in (1, 20):
+        q = torch.randn(m, 2, D, device="cuda", generator=g).bfloat16()
+        want = attend(ops, q, held, 1)
+        q[..., 5] = large
+        got = attend(ops, q, held, 1)
+        assert torch.equal(got, want)
+        exact, size = attended(q.cpu(), quantised(k, kind), quantised(v, kind), chain(m, n), D ** -0.5)
+        within(got, exact, (2 * U["bf16"] + 2.0 ** -13) * size)

@@ -422,7 +422,7 @@ int sfe_norm_rotary(sfe_ctx* ctx, const sfe_rotary_table* table, int32_t norm, f
  * V [page_size][head_dim], and for the types of 8 bits f32 scales, K [page_size] and V [page_size].
  * SFE_CACHE_E4M3 and SFE_CACHE_INT8 keep a token's channels of one kv head as codes and one scale:
  * with a their largest magnitude (at least 2^-96) and M 448 or 127, code = x M / a rounded to the
- * type (halves to even), scale = a / M, and a code stands for code * scale.  Channels that are not all finite
+ * type (halves to even; of f32 channels x M is rounded to f32 first), scale = a / M, and a code stands for code * scale.  Channels that are not all finite
  * read as NaN, all of them.  page_size is a power of two from 16 to 1024, head_dim a multiple of 16, at
  * most 128. */
 typedef enum sfe_cache_type {
@@ -454,7 +454,9 @@ typedef struct sfe_cache_tokens {
 
 /* The new tokens of n sequences, packed: those of sequence s are the rows [offsets[s], offsets[s + 1])
  * (host array of n + 1 from 0 on; none is fine), its last tokens.  heads: of the queries (a multiple of kv_heads).
- * Made, shared, captured and freed as an sfe_attn_plan is. */
+ * Made, shared, captured and freed as an sfe_attn_plan is.  It holds room for the parts of an attention's results, by the most
+ * rows (new tokens x heads of a group) of a sequence: on 256 CUs 8 MB for up to 16 rows, 17 for 32, 34 for 64, 68 for more
+ * (half of that for heads of up to 64). */
 typedef struct sfe_cache_plan sfe_cache_plan;
 int sfe_cache_plan_make(sfe_ctx* ctx, const int64_t* offsets, int32_t n, int32_t heads, int32_t kv_heads,
                         int32_t head_dim, void* stream, sfe_cache_plan** out);
@@ -466,7 +468,7 @@ void sfe_cache_plan_free(sfe_cache_plan* plan);
 int sfe_cache_write(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache_tokens* tokens, int32_t dtype,
                     const sfe_heads* k, const sfe_heads* v, void* stream);
 
-/* Reads the plan's tokens back into k, v, rounded once to dtype.  Of a plan whose new tokens are
+/* Reads the plan's tokens back into k, v: of codes code * scale in f32, then rounded to dtype.  Of a plan whose new tokens are
  * all of each sequence's, the whole sequences, as sfe_attention takes them. */
 int sfe_cache_read(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache_tokens* tokens, int32_t dtype,
                    const sfe_heads* k, const sfe_heads* v, void* stream);
@@ -476,8 +478,9 @@ int sfe_cache_read(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache
  *   out_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens before the new ones and the new
  * tokens that i sees, zero where there is none.  tree NULL: itself and those before it.  tree [offsets[n]]: bit j
  * of row i is set where i sees new token j of its sequence (of at most 64; bits past its last are ignored).
- * What is not seen contributes nothing, whatever its values.  dtype: SFE_BF16 or SFE_F16, a cache of 16
- * bits has the same.  q and out are 16-byte aligned (data and strides); out must not overlap q, the cache or the tree.
+ * What is not seen contributes nothing, whatever its values.  Scores and sums are f32.  Weights are rounded to the type of a cache of
+ * 16 bits; over codes, weight * scale of a value to 11 bits (22 where dtype is SFE_F16), and not finer than 2^-28 of a row's
+ * largest.  dtype: SFE_BF16 or SFE_F16, a cache of 16 bits has the same.  q and out are 16-byte aligned (data and strides); out must not overlap q, the cache or the tree.
  * rows: rows of out, at least offsets[n]; those past the last sequence are zeroed. */
 int sfe_cache_attention(sfe_cache_plan* plan, const sfe_cache* cache, const sfe_cache_tokens* tokens, int32_t dtype,
                         const sfe_heads* q, const uint64_t* tree, float scale, const sfe_heads* out, int64_t rows,

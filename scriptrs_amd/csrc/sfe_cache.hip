@@ -5,7 +5,7 @@
 // together (sfe_decode.hpp).
 //
 // Bound by memory: every element is read and written once, a workgroup's rows lie next to each other in both.  Written, 205,000
-// tokens of 4 heads of 128 from bf16 to e4m3: 636 MB in 137 us (4.6 TB/s; bf16 to bf16 5.2), 256 clips of 13-251 tokens of 8 heads
+// tokens of 4 heads of 128 from bf16 to e4m3: 636 MB in 135 us (4.7 TB/s; bf16 to bf16 5.2), read back 128 (5.0; 5.4), 256 clips of 13-251 tokens of 8 heads
 // of 64 in f16 18.5 us and read back 12.7 (5.7 and 8 TB/s, part of it in the last-level cache); 8 prompts of 700-8,192
 // tokens in int8 read in 36 us (5.3 TB/s).  A thread keeps its place in four tokens (clips written and read 37 us with a
 // token a thread, 31 with four and codes by one product).

@@ -11,24 +11,26 @@
 // keys that O^T = V^T P^T takes from it, once V's rows are paired by key in registers.  The order of channels in a product
 // is free, so lanes read whole chunks of K and of V.
 //
-// Codes of 8 bits are of the queries' type in the first product and f16 in the second, both of which hold them exactly: a key's scale
-// multiplies its scores, a value's scale its weight, in f32.  Weights times value scales are kept relative to a power of two, since f16 lacks their range: it
-// goes down with the weights and up with the largest product seen, so that a token's scale counts only as far as its weight does.
-// They are rounded once to 11 bits, or where the queries are f16 (and outputs have 11 bits too) to 22, as two numbers; to
-// multiples of 2^-28 of a row's largest where that is more.  16-bit caches multiply in their own type, weights rounded once to it.
+// Codes of 8 bits are of the queries' type in the first product and f16 in the second, both of which hold them exactly: a
+// key's scale multiplies its scores, a value's scale its weight, in f32.  Weights times value scales are kept relative to a power of
+// two, since f16 lacks their range: it goes down with the weights and up with the largest product seen, so that a token's
+// scale counts only as far as its weight does.  They are rounded once to 11 bits, or where the queries are f16 (and outputs have 11
+// bits too) to 22, as two numbers; to multiples of 2^-28 of a row's largest where that is more.  16-bit caches multiply in their
+// own type, weights rounded once to it.
 //
 // A step is 32 keys.  Pages are looked up a step ahead; rows go from memory into LDS directly, and what lies past a
 // sequence's end or in no page is read as zeros by the buffer's range, so that nothing is read outside a record.  Up to 32 rows
 // a workgroup's four waves take steps of their own, through rings of two stages of their own, without a barrier in the
 // loop; of 64 and 128 rows two and four waves read the same steps from a ring of three, with one barrier a step (codes are then
-// converted once for 32 rows a wave; 64 rows a wave took 180 us where this takes 83, since its accumulators left the
+// converted once for 32 rows a wave; 64 rows a wave took 180 us where this takes 84, since its accumulators left the
 // registers that the products write).
 //
 // What bounds it: one token a sequence, memory and the trip of a unit (256 x 126-1,500 tokens, 16/4 heads of 128 in e4m3:
-// 152 MB in 40 us, 3.8 TB/s; 2 x 5 tokens over 45,000, 8 heads of 64 in f16: 184 MB in 36 us, 5.1 TB/s, and 7 of the
-// join); trees, vector instructions beside the matrix cores (32 x 16 over 700-8,192, 32/8 heads of 128 in int8: 204 MB in 77
-// us and 10 of the join; 61% of the CUs' time issues vector instructions, 16% of it products).  A step of 32 keys and 32 rows
-// takes 451 of them: conversions of both operands' codes, two products a weight for its scale, exponentials and maxima.
+// 152 MB in 40 us, 3.8 TB/s; 2 x 5 tokens over 45,000, 8 heads of 64 in f16: 184 MB in 35 us, 5.2 TB/s, and 5 of the
+// join); trees, vector instructions beside the matrix cores (32 x 16 over 700-8,192, 32/8 heads of 128 in int8: 204 MB in 76
+// us and 9 of the join; 63% of the CUs' time issues vector instructions, 15% of it products).  A step of 32 keys and 32 rows takes
+// about 450 of them: conversions of both operands' codes (by both waves of a pair, the same), two products a weight for its
+// scale, exponentials and maxima.  Runs of hundreds of tokens are bound by the same: 380-670 TFLOP/s where long products reach 1,352.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -925,8 +927,8 @@ hipError_t run_rows(const CacheAttnArgs& a, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int groups = (a.rows + 3) / 4;
-  // (a unit has about shares / units + 1 parts: few of them take half the waves.  256 units of 64 rows: 11.8 us with 512
-  // threads, 10.1 with 256; 16 units in 34 parts: 6.7 and 9.3)
+  // (a unit has about shares / units + 1 parts: few of them take half the waves.  256 units of 64 rows: 11.5 us with 512
+  // threads, 9.0 with 256; 16 units in 34 parts: 4.7 and 5.0)
   const bool few = 4 * units >= a.shares;
   return for_launches(units * groups, 512, [&](int64_t first, unsigned blocks) {
     if (few) sfe_cache_attn_join_kernel<T, DP, 256><<<dim3(blocks), dim3(256), 0, stream>>>(a, first, groups);

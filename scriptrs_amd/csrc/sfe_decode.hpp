@@ -65,15 +65,17 @@ inline int cache_attn_tiles(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 
 inline int cache_attn_round(int tiles) { return kCacheAttnStep * kCacheAttnWaves / (tiles <= 2 ? 1 : tiles / 2); }  // keys
 // Whether each workgroup takes a whole unit (a tile and kv head), or an equal share of all units' rounds, which are then
 // joined by a second launch.  A unit alone takes 0.9 us a round, 1.2 of shared steps; shares cost 5 us more, and divide what
-// the device takes for all of it.  That is counted for a third of the table's tokens (`keys`), since lengths differ.  Measured, 16/4
-// heads of 128 in e4m3, one token of n sequences over l tokens, whole / shares: n 1, l 600 8.9 / 10.3 us, 1,200
-// 13.7 / 11.9; n 32, 1,200 15.4 / 18.0, 4,800 44.7 / 36.8; n 64 of 600 to 4,800 44.2 / 34.5; n 128, 2,400 54.9 / 58.1, of 300 to
-// 2,400 33.6 / 34.5.  16 tokens: n 1, 600 20.4 / 16.7; n 32, 600 21.0 / 32.3, 2,400 58.6 / 44.4; n 128, 2,400 85.9 / 88.4.
+// the device takes for all of it.  That is counted for a third of the table's tokens (`keys`), since lengths differ.  Measured (a
+// call of ten in a graph), 16/4 heads of 128 in e4m3, one token of n sequences over l tokens, whole / shares: n 1, l 600
+// 10.1 / 10.8 us, 1,200 15.2 / 12.6; n 32, 1,200 16.6 / 20.8, 4,800 46.2 / 37.9; n 64 of 600 to 4,800 47.1 / 41.6; n 128, 2,400
+// 59.5 / 61.1, of 300 to 2,400 36.3 / 42.7; n 256 of 126 to 1,500 42.0 / 54.8.  16 tokens: n 1, 600 22.2 / 18.6; n 32, 600
+// 23.7 / 34.9, 2,400 63.4 / 47.9; n 128, 2,400 98.5 / 100.2.  In bf16, one token: n 1, 600 10.0 / 10.0, 1,200 15.1 / 15.5; n 32, 1,200
+// 18.1 / 28.5, 4,800 63.6 / 62.2; n 128, 2,400 114 / 118; n 256 of 126 to 1,500 82 / 92.
 // Past 4,096 tokens one long sequence among short ones would keep the others waiting, but shares have every unit's length
 // to look through: with thousands of units they are whole as long as that costs more than the longest unit alone can.
-// n 512 of 600 in a table of 5,000, 16 kv_heads 111 / 148, one of them of 60,000 tokens (and its table) 512 / 177; n 20,000 of
-// 200 285 / 550; runs of new tokens: 64 of 1,024 over 6,000 6,495 / 9,769, one of 40,000 21,486 / 29,039, one of 16,384
-// over 32,768 12,153 / 12,138.
+// Heads of 64: n 512 of 600 in a table of 5,000, 16 kv_heads 120 / 153, one of them of 60,000 tokens (and its table) 499 / 188; n
+// 20,000 of 200 306 / 549; runs of new tokens: 64 of 1,024 over 6,000 6,265 / 9,309, one of 40,000 18,855 / 26,452, one of 16,384
+// over 32,768 7,977 / 11,225 (4,096 units, which the rule shares).
 inline bool cache_attn_whole(int64_t units, int64_t keys, int tiles, int esize) {
   const double rounds = (double)std::max<int64_t>(1, (keys + cache_attn_round(tiles) - 1) / cache_attn_round(tiles));
   const double alone = tiles <= 2 ? 0.92 : 1.24, all = std::max(0.0024 * esize, 0.002 * std::min(tiles, 4));

@@ -5,8 +5,8 @@
 //   z += bias[t]; a token that the row's mask lacks: z = -inf.
 // In f32, rounded once.
 //
-// Bound by memory and, with histories, by the vector instructions of their penalties (81% of the CUs' time): 512 rows of 128,000 in
-// bf16 with histories of up to 1,500, biases and a grammar, 266 MB in 62 us (4.3 TB/s), 183 before all
+// Bound by memory and, with histories, by the vector instructions of their penalties (82% of the CUs' time): 512 rows of 128,000 in
+// bf16 with histories of up to 1,500, biases and a grammar, 266 MB in 60 us (4.4 TB/s), 183 before all
 // loads were in flight together; 64 rows in f16 with histories of up to 8,192 13 us, the history's scan by each span the rest.
 //
 // One pass over the logits: a workgroup takes a span of one row's tokens, has all of its

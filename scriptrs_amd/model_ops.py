@@ -661,7 +661,7 @@ class ModelOps:
 
     def cache_read(self, plan: CachePlan, cache: KvCache, page_table, lengths, dtype=None, stream=None, out=None):
         """The plan's tokens out of the cache, ``(k, v)`` of [rows, kv_heads, head_dim] in ``dtype`` (bfloat16
-        without; float32 or float16), rounded once; ``out``: the two tensors to write.  With a plan of whole sequences (its new tokens
+        without; float32 or float16): code * scale in float32, then rounded; ``out``: the two tensors to write.  With a plan of whole sequences (its new tokens
         are all of each) these are the keys and values that ``attention`` takes.  Tokens in no place are zeros."""
         torch = self._torch
         handle = self._cached(plan, cache, page_table, lengths)
